@@ -336,3 +336,21 @@ def gemm_sparse24(A_packed, E, B, C=None, stream=None):
     check(_sp().kebab_gemm_sparse24(_dtype_code(B), A_packed.data_ptr(), E.data_ptr(), B.data_ptr(), C.data_ptr(),
                                     M, N, K, _stream_ptr(stream)))
     return C
+
+
+# ----------------------------------------------------------------------------- language-model operators
+# Mixture-of-experts and 8-bit integer operators; their modules import torch,
+# so they are loaded on first use.
+_OPERATORS = {"quantize_i8": "int8", "gemm_i8": "int8", "gemm_grouped_i8": "int8", "linear_i8": "int8",
+              "linear_grouped_i8": "int8", "Routing": "experts", "route": "experts", "route_backward": "experts",
+              "dispatch": "experts", "combine": "experts", "combine_backward": "experts", "gemm_grouped": "experts",
+              "gemm_grouped_dw": "experts"}
+
+
+def __getattr__(name):
+    if name not in _OPERATORS:
+        raise AttributeError("module %r has no attribute %r" % (__name__, name))
+    import importlib
+    f = getattr(importlib.import_module("." + _OPERATORS[name], __name__), name)
+    globals()[name] = f
+    return f

@@ -1,0 +1,189 @@
+"""Operators of a mixture-of-experts layer (C ABI: include/kebab/experts.h).
+
+    routing = route(logits, k)                       # weights, experts, plan
+    xs = dispatch(x, routing.slots)                  # tokens to expert order
+    ys = gemm_grouped(xs, W, routing.offsets)        # ys[r] = xs[r] W_e
+    y = combine(ys, routing.slots, routing.weights)  # back to tokens
+
+Tokens are rows and matrices are row-major torch tensors. Nothing is copied to
+the host: the ragged sizes stay on the device in `offsets`. All calls are
+asynchronous on `stream` (default: torch's current stream) and raise KebabError
+on a refusal. kebab_b200.moe has the same as differentiable functions.
+"""
+from typing import NamedTuple
+
+import torch
+
+from ._call import CODES, bad, call, dense, on, pitch, stacked, tensor
+
+_FLOATS = (torch.float16, torch.bfloat16)
+_ANY = (torch.float16, torch.bfloat16, torch.float32)
+_F32, _I32 = (torch.float32,), (torch.int32,)
+_ONE_BLOCK, _BLOCKS = 128, 148  # kebab_route_workspace
+
+
+class Routing(NamedTuple):
+    """Of T tokens over E experts: weights [T, k] float32, experts [T, k]
+    int32, offsets [E + 1] int32 (choices of lower experts), slots [T, k] int32
+    (places of the choices sorted by expert)."""
+    weights: torch.Tensor
+    experts: torch.Tensor
+    offsets: torch.Tensor
+    slots: torch.Tensor
+
+
+def route(logits, k, renormalize=True, stream=None):
+    """Top-k routing of logits [T, E] (F16, BF16 or F32): the k largest logits
+    of each token (equal ones: the lower expert first), with the softmax over
+    them (renormalize) or over all E as weights, and the sort by expert."""
+    dev = tensor("route", "logits", logits, 2, _ANY)
+    T, E = logits.shape
+    with on(dev, stream):
+        at = logits.device
+        weights = torch.empty((T, k), dtype=torch.float32, device=at)
+        # One allocation: experts, slots, offsets and the workspace.
+        n, work = T * k, 0 if T <= _ONE_BLOCK else _BLOCKS * E
+        ints = torch.empty((2 * n + E + 1 + work,), dtype=torch.int32, device=at)
+        experts, slots, offsets = ints[:n].view(T, k), ints[n:2 * n].view(T, k), ints[2 * n:2 * n + E + 1]
+        p = ints.data_ptr()
+        call("kebab_route", CODES[logits.dtype], logits.data_ptr(), pitch(logits), T, E, k, 1 if renormalize else 0,
+             weights.data_ptr(), p, p + 8 * n, p + 4 * n, p + 8 * n + 4 * E + 4 if work else None, 4 * work)
+    return Routing(weights, experts, offsets, slots)
+
+
+def route_backward(logits, routing, dweights, renormalize=True, stream=None):
+    """Gradient of the logits (of their type) from the weights' [T, k]."""
+    what = "route_backward"
+    dev = tensor(what, "logits", logits, 2, _ANY)
+    T, E = logits.shape
+    k = routing.experts.shape[-1]
+    dense(what, "routing.weights", routing.weights, (T, k), _F32, dev)
+    dense(what, "routing.experts", routing.experts, (T, k), _I32, dev)
+    dense(what, "dweights", dweights, (T, k), _F32, dev)
+    with on(dev, stream):
+        d = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
+        call("kebab_route_backward", CODES[logits.dtype], logits.data_ptr(), pitch(logits), T, E, k,
+             1 if renormalize else 0, routing.weights.data_ptr(), routing.experts.data_ptr(), dweights.data_ptr(),
+             d.data_ptr(), E)
+    return d
+
+
+def _slots(what, slots, T, dev):
+    tensor(what, "slots", slots, 2, _I32, dev)
+    k = slots.shape[1]
+    dense(what, "slots", slots, (T, k), _I32, dev)
+    return k
+
+
+def dispatch(x, slots, rows=None, stream=None):
+    """xs[slots[t, j]] = x[t]: x [T, H] -> xs [rows, H] (default T * k rows). A
+    slot outside [0, rows) is a dropped choice; rows that no slot names are
+    not written."""
+    what = "dispatch"
+    dev = tensor(what, "x", x, 2, _FLOATS)
+    T, H = x.shape
+    k = _slots(what, slots, T, dev)
+    rows = T * k if rows is None else rows
+    with on(dev, stream):
+        xs = torch.empty((rows, H), dtype=x.dtype, device=x.device)
+        call("kebab_expert_dispatch", CODES[x.dtype], x.data_ptr(), pitch(x), slots.data_ptr(), xs.data_ptr(), H, T, k,
+             rows, H)
+    return xs
+
+
+def combine(ys, slots, weights=None, stream=None):
+    """y[t] = sum_j weights[t, j] ys[slots[t, j]] -> [T, H]; without weights
+    the plain sum, which is the gradient of dispatch."""
+    what = "combine"
+    dev = tensor(what, "ys", ys, 2, _FLOATS)
+    R, H = ys.shape
+    T = slots.shape[0]
+    k = _slots(what, slots, T, dev)
+    if weights is not None:
+        dense(what, "weights", weights, (T, k), _F32, dev)
+    with on(dev, stream):
+        y = torch.empty((T, H), dtype=ys.dtype, device=ys.device)
+        call("kebab_expert_combine", CODES[ys.dtype], ys.data_ptr(), pitch(ys), slots.data_ptr(),
+             None if weights is None else weights.data_ptr(), y.data_ptr(), H, T, k, R, H)
+    return y
+
+
+def combine_backward(dy, ys, slots, weights, stream=None):
+    """Gradients of combine -> (dys [R, H], dweights [T, k] float32). Rows of
+    dys that no slot names are not written."""
+    what = "combine_backward"
+    dev = tensor(what, "dy", dy, 2, _FLOATS)
+    T, H = dy.shape
+    tensor(what, "ys", ys, 2, (dy.dtype,), dev)
+    R = ys.shape[0]
+    if ys.shape[1] != H:
+        raise bad("combine_backward: dy has rows of %d, ys of %d" % (H, ys.shape[1]))
+    k = _slots(what, slots, T, dev)
+    dense(what, "weights", weights, (T, k), _F32, dev)
+    with on(dev, stream):
+        dys = torch.empty((R, H), dtype=dy.dtype, device=dy.device)
+        dweights = torch.empty((T, k), dtype=torch.float32, device=dy.device)
+        call("kebab_expert_combine_backward", CODES[dy.dtype], dy.data_ptr(), pitch(dy), ys.data_ptr(), pitch(ys),
+             slots.data_ptr(), weights.data_ptr(), dys.data_ptr(), H, dweights.data_ptr(), T, k, R, H)
+    return dys, dweights
+
+
+def _mode(what, opmode):
+    m = opmode.upper() if isinstance(opmode, str) else opmode
+    if m not in ("RC", "RR"):
+        raise bad("%s: opmode must be RC or RR, got %s" % (what, opmode))
+    return m
+
+
+def gemm_grouped(X, W, offsets, Y=None, opmode="RC", stream=None):
+    """Y[r] = X[r] W_e for the rows offsets[e] <= r < offsets[e + 1] of expert
+    e: X [R, K], offsets [E + 1] (int32, on the device), W [E, N, K] ("RC": the
+    K x N matrices column-major) or [E, K, N] ("RR"); Y [R, N]. Rows of no
+    expert are not written. The gradient of X is
+    gemm_grouped(dY, W, offsets, opmode=the other)."""
+    what = "gemm_grouped"
+    m = _mode(what, opmode)
+    dev = tensor(what, "X", X, 2, _FLOATS)
+    R, K = X.shape
+    tensor(what, "W", W, 3, (X.dtype,), dev)
+    E = W.shape[0]
+    N, Kw = (W.shape[1], W.shape[2]) if m == "RC" else (W.shape[2], W.shape[1])
+    if Kw != K:
+        raise bad("gemm_grouped: inner dimensions differ: X has %d, W %d" % (K, Kw))
+    dense(what, "offsets", offsets, (E + 1,), _I32, dev)
+    with on(dev, stream):
+        if Y is None:
+            Y = torch.empty((R, N), dtype=X.dtype, device=X.device)
+        else:
+            tensor(what, "Y", Y, 2, (X.dtype,), dev)
+            if tuple(Y.shape) != (R, N):
+                raise bad("gemm_grouped: Y must be [%d, %d], got %s" % (R, N, tuple(Y.shape)))
+        call("kebab_gemm_grouped", CODES[X.dtype], X.data_ptr(), pitch(X), W.data_ptr(), *stacked(W), Y.data_ptr(),
+             pitch(Y), offsets.data_ptr(), E, R, N, K, m.encode())
+    return Y
+
+
+def gemm_grouped_dw(X, dY, offsets, dW=None, opmode="RC", stream=None):
+    """The gradient of W: dW[e] = the sum over the expert's rows of dY[r, n]
+    X[r, k], [E, N, K] ("RC") or [E, K, N] ("RR"); zeros for an expert without
+    rows."""
+    what = "gemm_grouped_dw"
+    m = _mode(what, opmode)
+    dev = tensor(what, "X", X, 2, _FLOATS)
+    R, K = X.shape
+    tensor(what, "dY", dY, 2, (X.dtype,), dev)
+    if dY.shape[0] != R:
+        raise bad("gemm_grouped_dw: X has %d rows, dY %d" % (R, dY.shape[0]))
+    N = dY.shape[1]
+    tensor(what, "offsets", offsets, 1, _I32, dev)
+    E = offsets.shape[0] - 1
+    dense(what, "offsets", offsets, (E + 1,), _I32, dev)
+    shape = (E, N, K) if m == "RC" else (E, K, N)
+    with on(dev, stream):
+        if dW is None:
+            dW = torch.empty(shape, dtype=X.dtype, device=X.device)
+        else:
+            dense(what, "dW", dW, shape, (X.dtype,), dev)
+        call("kebab_gemm_grouped_dw", CODES[X.dtype], X.data_ptr(), pitch(X), dY.data_ptr(), pitch(dY), dW.data_ptr(),
+             offsets.data_ptr(), E, R, N, K, m.encode())
+    return dW
