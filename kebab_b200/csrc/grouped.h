@@ -42,6 +42,9 @@ __device__ __forceinline__ void group_range(const int32_t* offsets, int e, int R
 }
 
 int launch_grouped_simt(const GroupedProblem& p);
+int launch_grouped_umma(const GroupedProblem& p);
+// Whether TMA can address X and W (and dY): the others take the CUDA cores.
+bool grouped_tma_ok(const GroupedProblem& p);
 
 // Runs the body of a C entry point; an exception (host memory) becomes a status.
 template <typename F>

@@ -46,7 +46,11 @@ int parse_mode(const char* what, const char* opmode, bool* kn) {
   return fail(KEBAB_EINVAL, std::string(what) + ": opmode must be RC or RR, got " + m);
 }
 
-int run(const GroupedProblem& p) { return launch_grouped_simt(p); }
+int run(const GroupedProblem& p) {
+  // dw without rows has no operand for a tensor map; it only writes zeros.
+  if (p.R > 0 && grouped_tma_ok(p)) return launch_grouped_umma(p);
+  return launch_grouped_simt(p);
+}
 
 int run_i8(const char* what, int out, const int8_t* q, int64_t ldq, const float* scale, const int8_t* Wq, int64_t ldw,
            int64_t w_stride, const float* w_scale, const void* bias, void* Y, int64_t ldy, const int32_t* offsets,

@@ -43,6 +43,14 @@ int make_tmap_2d(CUtensorMap* out, const void* base, int dtype, uint64_t rows, u
 int make_tmap_2d_sw(CUtensorMap* out, const void* base, int dtype, uint64_t rows, uint64_t cols, uint64_t ld,
                     uint32_t box_rows, uint32_t box_cols, int swizzle_bytes);
 
+// Tensor map of `rank` (2 or 3) dimensions, innermost first: type KEBAB_F16,
+// KEBAB_BF16 or TMAP_U8, extents and box in elements, strides of dimensions
+// 1.. in bytes (multiples of 16; the base 16-byte aligned), swizzle 0, 32, 64
+// or 128 bytes.
+constexpr int TMAP_U8 = 100;
+int make_tmap(CUtensorMap* out, const void* base, int type, int rank, const uint64_t* dims, const uint64_t* strides,
+              const uint32_t* box, int swizzle_bytes);
+
 // Stream-K workspace of the calling (device, stream): `ws_bytes` of FP32
 // partials and `flags` uint32 flags (zeroed once, when allocated), plus the
 // epoch this launch must write into the flags (one more than the last).
