@@ -14,7 +14,7 @@ from typing import NamedTuple
 
 import torch
 
-from ._call import CODES, bad, call, dense, on, pitch, stacked, tensor
+from ._call import CODES, bad, call, dense, elsewhere, on, pitch, stacked, tensor
 
 _FLOATS = (torch.float16, torch.bfloat16)
 _ANY = (torch.float16, torch.bfloat16, torch.float32)
@@ -37,17 +37,20 @@ def route(logits, k, renormalize=True, stream=None):
     of each token (equal ones: the lower expert first), with the softmax over
     them (renormalize) or over all E as weights, and the sort by expert."""
     dev = tensor("route", "logits", logits, 2, _ANY)
+    if elsewhere(dev, stream):
+        with on(dev, stream):
+            return route(logits, k, renormalize)
     T, E = logits.shape
-    with on(dev, stream):
-        at = logits.device
-        weights = torch.empty((T, k), dtype=torch.float32, device=at)
-        # One allocation: experts, slots, offsets and the workspace.
-        n, work = T * k, 0 if T <= _ONE_BLOCK else _BLOCKS * E
-        ints = torch.empty((2 * n + E + 1 + work,), dtype=torch.int32, device=at)
-        experts, slots, offsets = ints[:n].view(T, k), ints[n:2 * n].view(T, k), ints[2 * n:2 * n + E + 1]
-        p = ints.data_ptr()
-        call("kebab_route", CODES[logits.dtype], logits.data_ptr(), pitch(logits), T, E, k, 1 if renormalize else 0,
-             weights.data_ptr(), p, p + 8 * n, p + 4 * n, p + 8 * n + 4 * E + 4 if work else None, 4 * work)
+    if not 1 <= k <= E:
+        raise bad("route: k = %s is not in 1..%d" % (k, E))
+    weights = logits.new_empty((T, k), dtype=torch.float32)
+    experts, slots = logits.new_empty((2, T, k), dtype=torch.int32).unbind(0)
+    offsets = logits.new_empty((E + 1,), dtype=torch.int32)
+    size = 0 if T <= _ONE_BLOCK else 4 * _BLOCKS * E
+    ws = logits.new_empty((size,), dtype=torch.uint8) if size else None
+    call("kebab_route", dev, CODES[logits.dtype], logits.data_ptr(), pitch(logits), T, E, k, 1 if renormalize else 0,
+         weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(), slots.data_ptr(), ws.data_ptr() if size else None,
+         size)
     return Routing(weights, experts, offsets, slots)
 
 
@@ -60,15 +63,17 @@ def route_backward(logits, routing, dweights, renormalize=True, stream=None):
     dense(what, "routing.weights", routing.weights, (T, k), _F32, dev)
     dense(what, "routing.experts", routing.experts, (T, k), _I32, dev)
     dense(what, "dweights", dweights, (T, k), _F32, dev)
-    with on(dev, stream):
-        d = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
-        call("kebab_route_backward", CODES[logits.dtype], logits.data_ptr(), pitch(logits), T, E, k,
-             1 if renormalize else 0, routing.weights.data_ptr(), routing.experts.data_ptr(), dweights.data_ptr(),
-             d.data_ptr(), E)
+    if elsewhere(dev, stream):
+        with on(dev, stream):
+            return route_backward(logits, routing, dweights, renormalize)
+    d = logits.new_empty((T, E))
+    call("kebab_route_backward", dev, CODES[logits.dtype], logits.data_ptr(), pitch(logits), T, E, k,
+         1 if renormalize else 0, routing.weights.data_ptr(), routing.experts.data_ptr(), dweights.data_ptr(),
+         d.data_ptr(), E)
     return d
 
 
-def _slots(what, slots, T, dev):
+def _check_slots(what, slots, T, dev):
     tensor(what, "slots", slots, 2, _I32, dev)
     k = slots.shape[1]
     dense(what, "slots", slots, (T, k), _I32, dev)
@@ -82,12 +87,14 @@ def dispatch(x, slots, rows=None, stream=None):
     what = "dispatch"
     dev = tensor(what, "x", x, 2, _FLOATS)
     T, H = x.shape
-    k = _slots(what, slots, T, dev)
+    k = _check_slots(what, slots, T, dev)
+    if elsewhere(dev, stream):
+        with on(dev, stream):
+            return dispatch(x, slots, rows)
     rows = T * k if rows is None else rows
-    with on(dev, stream):
-        xs = torch.empty((rows, H), dtype=x.dtype, device=x.device)
-        call("kebab_expert_dispatch", CODES[x.dtype], x.data_ptr(), pitch(x), slots.data_ptr(), xs.data_ptr(), H, T, k,
-             rows, H)
+    xs = x.new_empty((rows, H))
+    call("kebab_expert_dispatch", dev, CODES[x.dtype], x.data_ptr(), pitch(x), slots.data_ptr(), xs.data_ptr(), H, T, k,
+         rows, H)
     return xs
 
 
@@ -97,14 +104,17 @@ def combine(ys, slots, weights=None, stream=None):
     what = "combine"
     dev = tensor(what, "ys", ys, 2, _FLOATS)
     R, H = ys.shape
+    tensor(what, "slots", slots, 2, _I32, dev)
     T = slots.shape[0]
-    k = _slots(what, slots, T, dev)
+    k = _check_slots(what, slots, T, dev)
     if weights is not None:
         dense(what, "weights", weights, (T, k), _F32, dev)
-    with on(dev, stream):
-        y = torch.empty((T, H), dtype=ys.dtype, device=ys.device)
-        call("kebab_expert_combine", CODES[ys.dtype], ys.data_ptr(), pitch(ys), slots.data_ptr(),
-             None if weights is None else weights.data_ptr(), y.data_ptr(), H, T, k, R, H)
+    if elsewhere(dev, stream):
+        with on(dev, stream):
+            return combine(ys, slots, weights)
+    y = ys.new_empty((T, H))
+    call("kebab_expert_combine", dev, CODES[ys.dtype], ys.data_ptr(), pitch(ys), slots.data_ptr(),
+         None if weights is None else weights.data_ptr(), y.data_ptr(), H, T, k, R, H)
     return y
 
 
@@ -118,13 +128,14 @@ def combine_backward(dy, ys, slots, weights, stream=None):
     R = ys.shape[0]
     if ys.shape[1] != H:
         raise bad("combine_backward: dy has rows of %d, ys of %d" % (H, ys.shape[1]))
-    k = _slots(what, slots, T, dev)
+    k = _check_slots(what, slots, T, dev)
     dense(what, "weights", weights, (T, k), _F32, dev)
-    with on(dev, stream):
-        dys = torch.empty((R, H), dtype=dy.dtype, device=dy.device)
-        dweights = torch.empty((T, k), dtype=torch.float32, device=dy.device)
-        call("kebab_expert_combine_backward", CODES[dy.dtype], dy.data_ptr(), pitch(dy), ys.data_ptr(), pitch(ys),
-             slots.data_ptr(), weights.data_ptr(), dys.data_ptr(), H, dweights.data_ptr(), T, k, R, H)
+    if elsewhere(dev, stream):
+        with on(dev, stream):
+            return combine_backward(dy, ys, slots, weights)
+    dys, dweights = dy.new_empty((R, H)), dy.new_empty((T, k), dtype=torch.float32)
+    call("kebab_expert_combine_backward", dev, CODES[dy.dtype], dy.data_ptr(), pitch(dy), ys.data_ptr(), pitch(ys),
+         slots.data_ptr(), weights.data_ptr(), dys.data_ptr(), H, dweights.data_ptr(), T, k, R, H)
     return dys, dweights
 
 
@@ -146,20 +157,21 @@ def gemm_grouped(X, W, offsets, Y=None, opmode="RC", stream=None):
     dev = tensor(what, "X", X, 2, _FLOATS)
     R, K = X.shape
     tensor(what, "W", W, 3, (X.dtype,), dev)
-    E = W.shape[0]
-    N, Kw = (W.shape[1], W.shape[2]) if m == "RC" else (W.shape[2], W.shape[1])
+    E, N, Kw = W.shape if m == "RC" else (W.shape[0], W.shape[2], W.shape[1])
     if Kw != K:
         raise bad("gemm_grouped: inner dimensions differ: X has %d, W %d" % (K, Kw))
     dense(what, "offsets", offsets, (E + 1,), _I32, dev)
-    with on(dev, stream):
-        if Y is None:
-            Y = torch.empty((R, N), dtype=X.dtype, device=X.device)
-        else:
-            tensor(what, "Y", Y, 2, (X.dtype,), dev)
-            if tuple(Y.shape) != (R, N):
-                raise bad("gemm_grouped: Y must be [%d, %d], got %s" % (R, N, tuple(Y.shape)))
-        call("kebab_gemm_grouped", CODES[X.dtype], X.data_ptr(), pitch(X), W.data_ptr(), *stacked(W), Y.data_ptr(),
-             pitch(Y), offsets.data_ptr(), E, R, N, K, m.encode())
+    if Y is not None:
+        tensor(what, "Y", Y, 2, (X.dtype,), dev)
+        if Y.shape != (R, N):
+            raise bad("gemm_grouped: Y must be [%d, %d], got %s" % (R, N, tuple(Y.shape)))
+    if elsewhere(dev, stream):
+        with on(dev, stream):
+            return gemm_grouped(X, W, offsets, Y, m)
+    Y = X.new_empty((R, N)) if Y is None else Y
+    ldw, w_stride = stacked(W)
+    call("kebab_gemm_grouped", dev, CODES[X.dtype], X.data_ptr(), pitch(X), W.data_ptr(), ldw, w_stride, Y.data_ptr(),
+         pitch(Y), offsets.data_ptr(), E, R, N, K, m.encode())
     return Y
 
 
@@ -179,11 +191,12 @@ def gemm_grouped_dw(X, dY, offsets, dW=None, opmode="RC", stream=None):
     E = offsets.shape[0] - 1
     dense(what, "offsets", offsets, (E + 1,), _I32, dev)
     shape = (E, N, K) if m == "RC" else (E, K, N)
-    with on(dev, stream):
-        if dW is None:
-            dW = torch.empty(shape, dtype=X.dtype, device=X.device)
-        else:
-            dense(what, "dW", dW, shape, (X.dtype,), dev)
-        call("kebab_gemm_grouped_dw", CODES[X.dtype], X.data_ptr(), pitch(X), dY.data_ptr(), pitch(dY), dW.data_ptr(),
-             offsets.data_ptr(), E, R, N, K, m.encode())
+    if dW is not None:
+        dense(what, "dW", dW, shape, (X.dtype,), dev)
+    if elsewhere(dev, stream):
+        with on(dev, stream):
+            return gemm_grouped_dw(X, dY, offsets, dW, m)
+    dW = X.new_empty(shape) if dW is None else dW
+    call("kebab_gemm_grouped_dw", dev, CODES[X.dtype], X.data_ptr(), pitch(X), dY.data_ptr(), pitch(dY), dW.data_ptr(),
+         offsets.data_ptr(), E, R, N, K, m.encode())
     return dW
