@@ -25,6 +25,7 @@ struct GroupedProblem {
   const float* scale = nullptr;    // IN_I8: per row of X
   const float* w_scale = nullptr;  // IN_I8: per (e, n)
   const void* bias = nullptr;      // IN_I8, output type, per n
+  bool early = false;  // the kernel before on the stream makes only X and scale (and waited for its own predecessors)
   cudaStream_t stream;
 };
 
@@ -43,6 +44,8 @@ __device__ __forceinline__ void group_range(const int32_t* offsets, int e, int R
 
 int launch_grouped_simt(const GroupedProblem& p);
 int launch_grouped_umma(const GroupedProblem& p);
+int launch_grouped_gemv(const GroupedProblem& p);
+bool grouped_gemv_ok(const GroupedProblem& p);  // at most 8 rows, whole 16-byte runs
 // Whether TMA can address X and W (and dY): the others take the CUDA cores.
 bool grouped_tma_ok(const GroupedProblem& p);
 

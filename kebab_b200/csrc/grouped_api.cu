@@ -47,15 +47,17 @@ int parse_mode(const char* what, const char* opmode, bool* kn) {
 }
 
 int run(const GroupedProblem& p) {
+  if (p.R > 0 && grouped_gemv_ok(p)) return launch_grouped_gemv(p);
   // dw without rows has no operand for a tensor map; it only writes zeros.
   if (p.R > 0 && grouped_tma_ok(p)) return launch_grouped_umma(p);
   return launch_grouped_simt(p);
 }
 
-int run_i8(const char* what, int out, const int8_t* q, int64_t ldq, const float* scale, const int8_t* Wq, int64_t ldw,
+int run_i8(int out, const int8_t* q, int64_t ldq, const float* scale, const int8_t* Wq, int64_t ldw,
            int64_t w_stride, const float* w_scale, const void* bias, void* Y, int64_t ldy, const int32_t* offsets,
-           int64_t E, int64_t R, int64_t N, int64_t K, kebab_stream_t stream) {
+           int64_t E, int64_t R, int64_t N, int64_t K, bool early, kebab_stream_t stream) {
   GroupedProblem p = {};
+  p.early = early;
   p.in = IN_I8, p.out = out;
   p.X = q, p.ldx = ldq, p.W = Wq, p.ldw = ldw, p.w_stride = w_stride, p.Y = Y, p.ldy = ldy;
   p.offsets = offsets, p.E = E, p.R = R, p.N = N, p.K = K;
@@ -137,7 +139,7 @@ int kebab_gemm_i8(kebab_dtype out, const int8_t* q, int64_t ldq, const float* sc
     int rc = check_i8(what, out, q, ldq, Wq, ldw, 0, w_scale, Y, ldy, 1, M, N, K);
     if (rc || M == 0) return rc;
     if (!scale) return fail(KEBAB_EINVAL, "gemm_i8: null pointer");
-    return run_i8(what, out, q, ldq, scale, Wq, ldw, 0, w_scale, bias, Y, ldy, nullptr, 1, M, N, K, stream);
+    return run_i8(out, q, ldq, scale, Wq, ldw, 0, w_scale, bias, Y, ldy, nullptr, 1, M, N, K, false, stream);
   });
 }
 
@@ -149,7 +151,7 @@ int kebab_gemm_grouped_i8(kebab_dtype out, const int8_t* q, int64_t ldq, const f
     int rc = check_i8(what, out, q, ldq, Wq, ldw, w_stride, w_scale, Y, ldy, E, R, N, K);
     if (rc || R == 0) return rc;
     if (!scale || !offsets) return fail(KEBAB_EINVAL, "gemm_grouped_i8: null pointer");
-    return run_i8(what, out, q, ldq, scale, Wq, ldw, w_stride, w_scale, nullptr, Y, ldy, offsets, E, R, N, K, stream);
+    return run_i8(out, q, ldq, scale, Wq, ldw, w_stride, w_scale, nullptr, Y, ldy, offsets, E, R, N, K, false, stream);
   });
 }
 
@@ -177,7 +179,7 @@ int kebab_linear_i8(kebab_dtype dtype, const void* X, int64_t ldx, const int8_t*
     int8_t* q = static_cast<int8_t*>(workspace);
     float* scale = reinterpret_cast<float*>(q + M * ldq);
     if ((rc = kebab_quantize_i8(dtype, X, ldx, q, ldq, scale, M, K, stream))) return rc;
-    return run_i8(what, dtype, q, ldq, scale, Wq, ldw, w_stride, w_scale, bias, Y, ldy, offsets, E, M, N, K, stream);
+    return run_i8(dtype, q, ldq, scale, Wq, ldw, w_stride, w_scale, bias, Y, ldy, offsets, E, M, N, K, true, stream);
   });
 }
 
