@@ -311,6 +311,7 @@ int launch(const GroupedProblem& p) {
   const int64_t steps = (p.K * (int64_t)sizeof(T) + 511) / 512;
   g.splits = 1;
   while (g.splits < WARPS && units * g.splits < 16 * dev->sm_count && steps >= 4 * g.splits) g.splits *= 2;
+  if (getenv("KB_SPLITS")) g.splits = atoi(getenv("KB_SPLITS"));
   const int per_block = WARPS / g.splits * NR;
   PdlLaunch l(dim3((unsigned)((p.N + per_block - 1) / per_block), groups), dim3(WARPS * 32), 0, p.stream);
   e = cudaLaunchKernelEx(&l.cfg, gemv_rc_kernel<T, TO>, (const GemvArgs)g);
@@ -320,7 +321,7 @@ int launch(const GroupedProblem& p) {
 
 bool grouped_gemv_ok(const GroupedProblem& p) {
   const int64_t v = p.in == IN_I8 ? 16 : 8;
-  return !p.dw && p.R <= MAX_ROWS && (p.kn ? p.N : p.K) % v == 0 && grouped_tma_ok(p);
+  return !p.dw && p.R <= (getenv("KB_GEMV") ? atoi(getenv("KB_GEMV")) : MAX_ROWS) && (p.kn ? p.N : p.K) % v == 0 && grouped_tma_ok(p);
 }
 
 int launch_grouped_gemv(const GroupedProblem& p) {

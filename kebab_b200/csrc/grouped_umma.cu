@@ -1,17 +1,26 @@
 // Grouped and 8-bit integer products on the tensor cores: persistent CTA pairs
 // (cta_group::2) over the tiles of every group, whatever their sizes.
 //
-// The MMA's 256 rows are the output's contiguous dimension and its columns the
+// The MMA's rows are the output's contiguous dimension and its columns the
 // other one, so that a lane of TMEM is a column of the row-major result:
 //   forward (RC, RR)  rows: n (a W_e panel), columns: up to 256 rows of the
 //                     group, contraction: k
 //   dw                rows: the contiguous dimension of dW_e, columns: the
 //                     other, contraction: the group's rows
+// A tile is a panel of 512 rows (two MMAs of 256 that share the staged columns)
+// or, where that would leave the pairs few tiles each, of 256. Its halves take
+// turns on two accumulators of up to 256 columns. With 512-row panels both are
+// in use, so the next tile's MMAs wait for the epilogue: its 8 warps read the
+// halves into registers (as pairs of outputs), hand each back at once, and only
+// then store.
+//
 // Ragged sizes cost what they are: a forward tile is as wide as its rows need
 // (a multiple of 32; N is a field of the instruction descriptor), a group of
-// 257 rows gives two tiles of 160 and 97 and not 256 and 1, and no group is
-// padded in memory. Which tile belongs to which group is worked out on the
-// device, from the offsets, by a prefix sum that every CTA does for itself.
+// 514 rows gives tiles of 192, 192 and 160 columns and not 256, 256 and 32, and
+// no group is padded in memory. Which tile belongs to which group is worked out
+// on the device: every CTA sorts the groups' tiles by cost (widest, or in dw
+// longest, first) and sums them up for itself, and the pairs take them in turn,
+// back and forth, which leaves their loads within one small tile of each other.
 //
 // Edges: a forward tile may read past its group's end (the columns are not
 // stored; a column does not reach its neighbours). In dw the contraction runs
@@ -19,10 +28,13 @@
 // (a NaN there would spread): the last 16-row step is cleared in shared memory
 // after it has landed, and steps beyond it are not issued.
 //
-// Ring: 3 stages of two 128-byte K-blocks (64 16-bit or 128 8-bit elements) of
-// 128 rows of each operand a CTA; two accumulators of 256 columns, so that the
-// epilogue of a tile runs under the next one's MMAs. Warps: TMA producer, MMA
-// issuer, 4 epilogue warps, as in gemm_umma.cuh.
+// Ring: 4 stages of 48 KB a CTA, each one 128-byte K-block (64 16-bit or 128
+// 8-bit elements) of a 512-row panel and its columns, or two K-blocks of a
+// 256-row panel where no tile is wider than 128 columns (few rows: bound by the
+// weights' bytes, and 256 contiguous bytes a weight row and stage are fetched
+// faster than 128); else 6 stages of 32 KB. Warps: TMA producer, MMA issuer,
+// 8 epilogue warps, and one that works out the tiles ahead of them (finding a
+// tile's place takes about 2000 cycles, as long as 16 MMAs).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -50,82 +62,263 @@ struct TileArgs {
   const float* w_scale;
   const void* bias;
   int pdl;
+  int sort;
   WaitCtx ctx;
 };
 
+constexpr int THREADS = 352;
+// Tiles are sorted by cost where that can pay: from 2048 rows (a product of
+// fewer takes about as long as its weights' bytes in any order), and up to 512
+// entries (the ranks take entries^2 / 352 comparisons a thread).
+constexpr int SORT_ROWS = 2048, SORT_LIMIT = 512;
+
 struct GSmem {
-  static constexpr int STAGES = 3, KPS = 2;
   static constexpr int SUB = 128 * 128;  // 128 rows of 128 bytes: one K-block of one operand
-  static constexpr int OFF_A = 0;
-  static constexpr int OFF_B = OFF_A + STAGES * KPS * SUB;
-  static constexpr int OFF_C = OFF_B + STAGES * KPS * SUB;
+  static constexpr int RING = 12 * SUB;
+  static constexpr int MAX_STAGES = 6;
+  static constexpr int OFF_C = RING;
   static constexpr int C_SUB = 32 * 32 * 2;
-  static constexpr int OFF_BAR = OFF_C + 4 * 2 * C_SUB;
+  static constexpr int OFF_BAR = OFF_C + 8 * C_SUB;
   // full, empty, tail_full, tail_done a stage; tmem_full and tmem_empty twice; drain
-  static constexpr int NUM_BARS = 4 * STAGES + 5;
-  static constexpr int OFF_GROUPS = OFF_BAR + NUM_BARS * 8 + 16;
-  static constexpr int bytes(int E) { return OFF_GROUPS + (3 * E + 1) * 4; }
-  static constexpr int ALLOC = OFF_GROUPS + (3 * kMaxExperts + 1) * 4 + 1024;
+  static constexpr int TILES = 4;  // descriptions of tiles in flight: full and empty each
+  static constexpr int NUM_BARS = 4 * MAX_STAGES + 5 + 2 * TILES;
+  static constexpr int OFF_TILES = (OFF_BAR + NUM_BARS * 8 + 4 + 15) / 16 * 16;
+  static constexpr int OFF_TABLE = OFF_TILES + TILES * 32;
+  // first[entries + 1] (int), entry[entries] (uint16, sorted only), entries <= 2 E
+  static constexpr int bytes(int E) { return OFF_TABLE + (2 * E + 1) * 4 + 2 * E * 2; }
+  static constexpr int ALLOC = OFF_TABLE + (2 * kMaxExperts + 1) * 4 + 2 * kMaxExperts * 2 + 1024;
   static_assert(ALLOC <= 232448, "shared memory budget exceeded");
 };
 
-// Where each group's tiles start (first[e] .. first[e + 1]), in shared memory.
-struct Groups {
-  const int* first;  // [E + 1]
-  const int* begin;  // [E]
-  const int* rows;   // [E]
+// a / b for 0 <= a, 0 < b. Below 2^22 by a float quotient, put right by one
+// step: every role divides a few times a tile, on its critical path.
+__device__ __forceinline__ int divide(int a, int b) {
+  if (a >= 1 << 22) return a / b;
+  int q = (int)__fdividef((float)a, (float)b);
+  const int r = a - q * b;
+  if (r < 0) --q;
+  else if (r >= b) ++q;
+  return q;
+}
+
+// The tiles in the order in which they are dealt out. Entry i has the column
+// blocks first[i] .. first[i + 1] - 1, each of `panels` tiles. Unsorted, an
+// entry is a group. Sorted, it is a group (dw), or a group's full-width or its
+// last column block (forward).
+struct Table {
+  const int* first;
+  const uint16_t* entry;  // sorted: group (dw), or group * 2 + (1: the last block)
+  bool sorted;
+  int entries, panels;    // panels: tiles along the MMA-row side
+  int nsub;               // 256-row halves of a panel
+  int kps;                // K-blocks a stage
 };
 
-struct Tile {
-  int e, a0, b0, width;  // group, first row and column of the tile, its columns (a multiple of 32)
+struct alignas(16) Tile {
+  int e, a0, b0, width;  // group (-1: no more tiles), first row and column of the tile, its columns (a multiple of 32)
+  int nsub;              // halves of the panel that exist here
   int begin, rows;       // the group's rows
   int blocks;            // 128-byte K-blocks of the contraction
 };
 
-template <int MODE>
-__device__ __forceinline__ int tiles_b(const TileArgs& g, int rows) {
-  return ((MODE == MODE_DW ? g.DB : rows) + 255) / 256;
+// Columns of a group's tiles: equal shares of at most 256, and what is left for the last.
+struct Widths {
+  int count, full, last;
+  __device__ __forceinline__ Widths(int rows) {
+    count = (rows + 255) / 256;
+    full = last = (rows + 31) / 32 * 32;
+    if (count > 1) {
+      full = (divide(rows + count - 1, count) + 31) / 32 * 32;
+      last = (rows - (count - 1) * full + 31) / 32 * 32;
+    }
+  }
+};
+
+// Tile `local` of panels x blocks: eight panels share the passes over the
+// columns, so that the 74 pairs hold about 8 x 9 tiles at a time.
+__device__ __forceinline__ void raster(int local, int panels, int blocks, int& pa, int& cb) {
+  if (blocks == 1) {
+    pa = local;
+    cb = 0;
+  } else {
+    const int group = divide(local, 8 * blocks), in_group = local - group * 8 * blocks;
+    const int height = min(8, panels - group * 8);
+    cb = divide(in_group, height);
+    pa = group * 8 + in_group - cb * height;
+  }
 }
 
 template <int MODE, int EPB>
-__device__ __forceinline__ Tile tile_of(int t, const TileArgs& g, const Groups& gr) {
+__device__ __forceinline__ Tile tile_of(int t, const TileArgs& g, const Table& tab) {
   Tile x;
-  int lo = 0, hi = g.E - 1;  // the last group that starts at or before t
+  int lo = 0, hi = tab.entries - 1;  // the last entry that starts at or before t
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (gr.first[mid] <= t) lo = mid;
+    if (tab.first[mid] * tab.panels <= t) lo = mid;
     else hi = mid - 1;
   }
-  x.e = lo;
-  x.begin = gr.begin[lo];
-  x.rows = gr.rows[lo];
-  const int ta = (g.DA + 255) / 256, tb = tiles_b<MODE>(g, x.rows);
-  int ma, mb;
-  // Eight panels of the row side share the passes over the column side: the
-  // 74 pairs then hold about 8 x 9 tiles at a time, near square.
-  tile_coords(t - gr.first[lo], ta, tb, 8, ma, mb);
-  x.a0 = ma * 256;
+  const int id = tab.sorted ? tab.entry[lo] : lo, local = t - tab.first[lo] * tab.panels;
+  x.e = MODE == MODE_DW || !tab.sorted ? id : id >> 1;
+  group_range(g.offsets, x.e, g.R, x.begin, x.rows);
+  int pa, cb;
   if (MODE == MODE_DW) {
+    raster(local, tab.panels, (g.DB + 255) / 256, pa, cb);
     x.width = 256;
+    x.b0 = cb * 256;
     x.blocks = (x.rows + EPB - 1) / EPB;
   } else {
-    x.width = ((x.rows + tb - 1) / tb + 31) / 32 * 32;  // equal shares
+    const Widths w(x.rows);
+    if (!tab.sorted) {
+      raster(local, tab.panels, w.count, pa, cb);
+    } else if (id & 1) {
+      pa = local;
+      cb = w.count - 1;
+    } else {
+      raster(local, tab.panels, w.count - 1, pa, cb);
+    }
+    x.width = cb == w.count - 1 ? w.last : w.full;
+    x.b0 = cb * w.full;
     x.blocks = (g.K + EPB - 1) / EPB;
   }
-  x.b0 = mb * x.width;
+  x.a0 = pa * 256 * tab.nsub;
+  x.nsub = min(tab.nsub, (g.DA - x.a0 + 255) / 256);
   return x;
 }
 
+// The same from lane 0, for code of a whole warp.
+__device__ __forceinline__ Tile uniform(const Tile& x) {
+  auto u = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+  return {u(x.e), u(x.a0), u(x.b0), u(x.width), u(x.nsub), u(x.begin), u(x.rows), u(x.blocks)};
+}
+
+// Block-wide sum of one value a thread before this thread's; `total` of all.
+__device__ __forceinline__ int scan_before(int v, int* sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int at = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, at, d);
+    if (lane >= d) at += up;
+  }
+  if (lane == 31) sums[warp] = at;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    const int s = sums[w];
+    if (w < warp) before += s;
+    total += s;
+  }
+  __syncthreads();
+  return before + at - v;
+}
+
+// Makes the table, by all threads of the CTA. `scratch`: 3 ints an entry and 16.
+template <int MODE, bool I8>
+__device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* first, uint16_t* entry, int* scratch) {
+  constexpr bool DW = MODE == MODE_DW;
+  // 512-row panels from this many 256-row tiles a pair (0: never). Measured
+  // under the power cap, us: forward 16381 x 4096 x 2048 over 14 uneven groups
+  // (15 tiles a pair) 245 against 252; dw with 7 tiles a pair (4 groups of 8192
+  // rows) 430 against 477: a 256-row dw tile needs four copies a K-block, whose
+  // issue is as long as its MMAs. 8-bit: 4093 x 28672 x 8192 735 against 682
+  // (the epilogue, which scales every sum, stands between two tiles' MMAs).
+  constexpr int WIDE_FROM = I8 ? 0 : DW ? 4 : 8;
+  int* sums = scratch;  // [16]
+  int* cost = scratch + 16;
+  const int tb = (g.DB + 255) / 256;
+  const bool sorted = g.sort;
+  const int n = DW || !sorted ? g.E : 2 * g.E;
+  int wide = 0;  // some tile of more than 128 columns
+  int total = 0;
+  if (!sorted) {
+    for (int i0 = 0; i0 < n; i0 += THREADS) {
+      const int i = i0 + threadIdx.x;
+      int b = 0;
+      if (i < n) {
+        int begin, rows;
+        group_range(g.offsets, i, g.R, begin, rows);
+        b = DW ? tb : (rows + 255) / 256;
+        wide |= DW || rows > 128;
+      }
+      int all;
+      const int at = total + scan_before(b, sums, all);
+      if (i < n) first[i] = at;
+      total += all;
+    }
+    wide = __syncthreads_or(wide);
+  } else {
+    int* blocks = cost + (n + 3) / 4 * 4;  // column blocks of the entry
+    int* by_rank = blocks + n;
+    for (int i = threadIdx.x; i < (n + 3) / 4 * 4; i += THREADS) {
+      int c = -1, b = 0;
+      if (i < n) {
+        int begin, rows;
+        group_range(g.offsets, DW ? i : i >> 1, g.R, begin, rows);
+        if (DW) {
+          c = rows;
+          b = tb;
+        } else {
+          const Widths w(rows);
+          c = (i & 1) ? w.last : w.count > 1 ? w.full : 0;
+          b = w.count == 0 ? 0 : (i & 1) ? 1 : w.count - 1;
+        }
+        wide |= DW || c > 128;
+        blocks[i] = b;
+      }
+      cost[i] = c;
+    }
+    wide = __syncthreads_or(wide);
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+      const int c = cost[i];
+      int rank = 0;
+      for (int j = 0; j < n; j += 4) {
+        const int4 o = *reinterpret_cast<const int4*>(cost + j);
+        rank += (o.x > c || (o.x == c && j < i)) + (o.y > c || (o.y == c && j + 1 < i)) +
+                (o.z > c || (o.z == c && j + 2 < i)) + (o.w > c || (o.w == c && j + 3 < i));
+      }
+      entry[rank] = (uint16_t)i;
+      by_rank[rank] = blocks[i];
+    }
+    __syncthreads();
+    for (int i0 = 0; i0 < n; i0 += THREADS) {
+      const int i = i0 + threadIdx.x;
+      int all;
+      const int at = total + scan_before(i < n ? by_rank[i] : 0, sums, all);
+      if (i < n) first[i] = at;
+      total += all;
+    }
+  }
+  if (threadIdx.x == 0) first[n] = total;
+  Table tab;
+  tab.first = first;
+  tab.entry = entry;
+  tab.sorted = sorted;
+  tab.entries = n;
+  const int p256 = (g.DA + 255) / 256;
+  tab.nsub = WIDE_FROM > 0 && (int64_t)total * p256 >= (int64_t)WIDE_FROM * pairs ? 2 : 1;
+  tab.panels = tab.nsub == 2 ? (g.DA + 511) / 512 : p256;
+  tab.kps = tab.nsub == 1 && !wide ? 2 : 1;
+  return tab;
+}
+
+// Forward: the rows of X in boxes of 64, 32 and 16, for shares of a tile's
+// columns under 128.
+struct ColumnMaps {
+  CUtensorMap box[3];
+};
+
 template <typename TO, bool I8, int MODE>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(THREADS, 1)
     grouped_umma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                        const __grid_constant__ CUtensorMap tmB16, const __grid_constant__ CUtensorMap tmC,
+                        const __grid_constant__ ColumnMaps tmBs, const __grid_constant__ CUtensorMap tmC,
                         const TileArgs g) {
   using L = GSmem;
   constexpr bool DW = MODE == MODE_DW;
   constexpr bool A_MN = MODE != MODE_RC, B_MN = DW;
   constexpr int EPB = I8 ? 128 : 64;  // elements of the contraction in a K-block
-  constexpr int STAGES = L::STAGES, KPS = L::KPS;
+  constexpr int STAGES = L::MAX_STAGES;
   constexpr uint32_t IDESC = (I8 ? umma_idesc_i8(256, 0) : umma_idesc_f16(256, 0, ElemTraits<TO>::kBf16)) |
                              (A_MN ? (1u << 15) : 0u) | (B_MN ? (1u << 16) : 0u);
 
@@ -138,12 +331,19 @@ __global__ void __launch_bounds__(192, 1)
   uint64_t* tmem_full = tail_done + STAGES;
   uint64_t* tmem_empty = tmem_full + 2;
   uint64_t* drain = tmem_empty + 2;
+  uint64_t* tile_full = drain + 1;
+  uint64_t* tile_empty = tile_full + L::TILES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + L::NUM_BARS);
-  int* s_first = reinterpret_cast<int*>(smem + L::OFF_GROUPS);
-  int* s_begin = s_first + g.E + 1;
-  int* s_rows = s_begin + g.E;
+  Tile* s_tiles = reinterpret_cast<Tile*>(smem + L::OFF_TILES);
+  int* s_first = reinterpret_cast<int*>(smem + L::OFF_TABLE);
+  uint16_t* s_entry = reinterpret_cast<uint16_t*>(s_first + 2 * g.E + 1);
 
-  const int warp = threadIdx.x >> 5;
+  // The shuffle tells the compiler that a warp takes one path. The producer and
+  // the issuer run with all lanes, one of which is elected at each copy or MMA,
+  // so that addresses and descriptors stay in uniform registers: a branch on
+  // the lane around the whole loop cost about 100 cycles an MMA to issue, of
+  // the 128 that a 256 x 256 x 16 takes.
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
@@ -161,290 +361,373 @@ __global__ void __launch_bounds__(192, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tmem_full[a], 1);
-      mbar_init(&tmem_empty[a], 4 * 2);
+      mbar_init(&tmem_empty[a], 8 * 2);
+    }
+    for (int a = 0; a < L::TILES; ++a) {
+      mbar_init(&tile_full[a], 1);
+      mbar_init(&tile_empty[a], 9 + (DW || leader ? 1 : 0));  // the warps that read descriptions
     }
     mbar_init(drain, 1);
     fence_barrier_init();
   }
+  __syncwarp();
   if (warp == 1) {
     tmem_alloc<2>(tmem_slot, 512);
     tmem_relinquish<2>();
   }
+  __syncwarp();
+  cluster_arrive_release();  // the pair's barriers; the other half is below
   if (g.pdl) {
     pdl_wait();
     pdl_launch_dependents();
   }
-  if (warp == 2) {
-    // Prefix sum of the groups' tiles: a lane takes a run of groups.
-    const int per = (g.E + 31) / 32, e0 = lane * per, ta = (g.DA + 255) / 256;
-    int sum = 0;
-    for (int i = 0; i < per && e0 + i < g.E; ++i) {
-      int begin, rows;
-      group_range(g.offsets, e0 + i, g.R, begin, rows);
-      s_begin[e0 + i] = begin;
-      s_rows[e0 + i] = rows;
-      sum += ta * tiles_b<MODE>(g, rows);
-    }
-    int at = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, at, d);
-      if (lane >= d) at += up;
-    }
-    if (lane == 31) s_first[g.E] = at;
-    at -= sum;
-    for (int i = 0; i < per && e0 + i < g.E; ++i) {
-      s_first[e0 + i] = at;
-      at += ta * tiles_b<MODE>(g, s_rows[e0 + i]);
-    }
-  }
-  __syncwarp();
+  const int pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+  const Table tab = make_table<MODE, I8>(g, pairs, s_first, s_entry, reinterpret_cast<int*>(smem));
+  // The table's scratch is in the ring: order it before the copies into it.
+  fence_proxy_async_smem();
   tc_fence_before();
-  cluster_sync();
+  __syncthreads();
+  cluster_wait_acquire();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const Groups gr{s_first, s_begin, s_rows};
-  const int num_tiles = s_first[g.E];
-  const int step = gridDim.x / 2;
+  const int kps = tab.kps;
+  // A stage: the panel's K-blocks (or halves), then the columns'.
+  const int stages = tab.nsub + kps == 3 ? 4 : 6;
+  const int a_bytes = tab.nsub * kps * L::SUB, stage_bytes = a_bytes + L::SUB;
+  // The i-th tile of this pair, for a whole warp; e < 0 after the last.
+  auto next_tile = [&](int i) {
+    const int at = i % L::TILES;
+    Tile x;
+    if (__all_sync(0xffffffffu, mbar_wait(&tile_full[at], i / L::TILES & 1, ctx, SITE_TILE))) x = uniform(s_tiles[at]);
+    else x.e = -1;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&tile_empty[at]);
+    return x;
+  };
+  auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      uint32_t issued = 0, parity = 0;  // a bit a stage
-      const uint32_t full_leader0 = mapa_shared(smem_u32(&full[0]), 0);
-      for (int t = blockIdx.x / 2; ok && t < num_tiles; t += step) {
-        const Tile x = tile_of<MODE, EPB>(t, g, gr);
-        const int half = x.width / 2;
-        const int a0 = x.a0 + (int)rank * 128, b0 = x.b0 + (int)rank * half;
-        const uint32_t block_bytes = L::SUB + half * 128;
-        for (int kb = 0; kb < x.blocks; kb += KPS) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u, ctx, SITE_EMPTY)) {
-            ok = false;
-            break;
-          }
-          const int nq = min(KPS, x.blocks - kb);
-          // A group's last stage that does not end on a 16-row step: each CTA
-          // waits for its own bytes and clears the rows past the end.
-          const bool tail = DW && kb + KPS >= x.blocks && (x.rows & 15) != 0;
-          uint32_t bar = full_leader0 + stage * 8u;
-          if (tail && !leader) {
-            mbar_arrive_expect_tx(&tail_full[stage], nq * block_bytes);
-            bar = mapa_shared(smem_u32(&tail_full[stage]), rank);
-          } else if (leader) {
-            mbar_arrive_expect_tx(&full[stage], (tail ? 1 : 2) * nq * block_bytes);
-          }
-          for (int q = 0; q < nq; ++q) {
-            uint8_t* sA = smem + L::OFF_A + (stage * KPS + q) * L::SUB;
-            uint8_t* sB = smem + L::OFF_B + (stage * KPS + q) * L::SUB;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    uint32_t issued = 0, parity = 0;  // a bit a stage
+    const uint32_t full_leader0 = mapa_shared(smem_u32(&full[0]), 0);
+    const uint32_t tail_mine0 = mapa_shared(smem_u32(&tail_full[0]), rank);
+    for (int i = 0; ok; ++i) {
+      const Tile x = next_tile(i);
+      if (x.e < 0) break;
+      const int half = x.width / 2;
+      const int a0 = x.a0 + (int)rank * 128, b0 = x.b0 + (int)rank * half;
+      const uint32_t block_bytes = x.nsub * L::SUB + half * 128;
+      for (int kb = 0; kb < x.blocks; kb += kps) {
+        ok = all_ok(mbar_wait(&empty[stage], phase ^ 1u, ctx, SITE_EMPTY));
+        if (!ok) break;
+        // A group's last stage that does not end on a 16-row step: each CTA
+        // waits for its own bytes and clears the rows past the end.
+        const bool tail = DW && kb + 1 == x.blocks && (x.rows & 15) != 0;
+        const int nq = min(kps, x.blocks - kb);
+        const uint32_t bar = (tail && !leader ? tail_mine0 : full_leader0) + stage * 8u;
+        uint8_t* sA = smem + stage * stage_bytes;
+        uint8_t* sB = sA + a_bytes;
+        if (elect_one()) {
+          if (leader) mbar_arrive_expect_tx(&full[stage], (tail ? 1 : 2) * nq * block_bytes);
+          else if (tail) mbar_arrive_expect_tx(&tail_full[stage], block_bytes);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            if (q >= nq) break;
             const int k0 = (kb + q) * EPB;
-            if constexpr (MODE == MODE_RC) {
-              tma_load_3d_pair(sA, &tmA, bar, k0, a0, x.e);
-            } else if constexpr (MODE == MODE_RR) {
-              tma_load_3d_pair(sA, &tmA, bar, a0, k0, x.e);
-              tma_load_3d_pair(sA + 8192, &tmA, bar, a0 + 64, k0, x.e);
-            } else {
-              tma_load_2d_pair(sA, &tmA, bar, a0, x.begin + k0);
-              tma_load_2d_pair(sA + 8192, &tmA, bar, a0 + 64, x.begin + k0);
-              tma_load_2d_pair(sB, &tmB, bar, b0, x.begin + k0);
-              tma_load_2d_pair(sB + 8192, &tmB, bar, b0 + 64, x.begin + k0);
-            }
-            if constexpr (!DW) {
-              if (half == 128) {
-                tma_load_2d_pair(sB, &tmB, bar, k0, x.begin + b0);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              if (s >= x.nsub) break;
+              uint8_t* dst = sA + (q + s) * L::SUB;
+              const int as = a0 + s * 256;
+              if constexpr (MODE == MODE_RC) {
+                tma_load_3d_pair(dst, &tmA, bar, k0, as, x.e);
+              } else if constexpr (MODE == MODE_RR) {
+                tma_load_3d_pair(dst, &tmA, bar, as, k0, x.e);
+                tma_load_3d_pair(dst + 8192, &tmA, bar, as + 64, k0, x.e);
               } else {
-                for (int r = 0; r < half; r += 16) tma_load_2d_pair(sB + r * 128, &tmB16, bar, k0, x.begin + b0 + r);
+                tma_load_2d_pair(dst, &tmA, bar, as, x.begin + k0);
+                tma_load_2d_pair(dst + 8192, &tmA, bar, as + 64, x.begin + k0);
               }
             }
           }
-          issued |= 1u << stage;
-          parity = (parity & ~(1u << stage)) | (phase << stage);
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            if (q >= nq) break;
+            const int k0 = (kb + q) * EPB;
+            uint8_t* dst = sB + q * half * 128;
+            if constexpr (DW) {
+              tma_load_2d_pair(dst, &tmB, bar, b0, x.begin + k0);
+              tma_load_2d_pair(dst + 8192, &tmB, bar, b0 + 64, x.begin + k0);
+            } else if (half == 128) {
+              tma_load_2d_pair(dst, &tmB, bar, k0, x.begin + b0);
+            } else {
+              int r = 0;
+#pragma unroll
+              for (int m = 0; m < 3; ++m) {
+                if (half & (64 >> m)) {
+                  tma_load_2d_pair(dst + r * 128, &tmBs.box[m], bar, k0, x.begin + b0 + r);
+                  r += 64 >> m;
+                }
+              }
+            }
           }
         }
+        __syncwarp();
+        issued |= 1u << stage;
+        parity = (parity & ~(1u << stage)) | (phase << stage);
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
       }
-      if (!ok && leader) {
-        // Abort: let the copies still in flight land before the CTA exits.
-        WaitCtx drain_ctx{ctx.status, 50000000ull};
-        for (int s = 0; s < STAGES; ++s)
-          if (issued >> s & 1u) mbar_wait(&full[s], parity >> s & 1u, drain_ctx, SITE_DRAIN);
-      }
+    }
+    if (!ok && leader) {
+      // Abort: let the copies still in flight land before the CTA exits.
+      WaitCtx drain_ctx{ctx.status, 50000000ull};
+      for (int s = 0; s < stages; ++s)
+        if (issued >> s & 1u) mbar_wait(&full[s], parity >> s & 1u, drain_ctx, SITE_DRAIN);
     }
   } else if (warp == 1) {
     // ------------------------------------------ MMA issuer (leader); in dw the
-    // whole warp of both CTAs clears the rows past a group's end.
-    if (DW || (leader && lane == 0)) {
+    // warp of both CTAs clears the rows past a group's end.
+    if (DW || leader) {
       int stage = 0;
       uint32_t phase = 0, tail_parity = 0;
-      int acc = 0;
-      uint32_t acc_phase = 0;
+      uint32_t halves = 0;  // accumulators used so far: slot = bit 0, phase = bit 1
       bool ok = true, any_issued = false;
       const uint32_t tail_done_leader0 = mapa_shared(smem_u32(&tail_done[0]), 0);
-      for (int t = blockIdx.x / 2; ok && t < num_tiles; t += step) {
-        const Tile x = tile_of<MODE, EPB>(t, g, gr);
-        if (x.blocks == 0) continue;  // dw of a group without rows
-        if (leader) {
-          ok = mbar_wait(&tmem_empty[acc], acc_phase ^ 1u, ctx, SITE_TMEM_EMPTY);
-          if constexpr (DW) ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-        }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * 256);
+      const uint32_t ring = smem_u32(smem);
+      const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
+      for (int i = 0; ok; ++i) {
+        const Tile x = next_tile(i);
+        if (x.e < 0) break;
         const uint32_t idesc = IDESC | (uint32_t)(x.width >> 3) << 17;
-        for (int kb = 0; kb < x.blocks; kb += KPS) {
+        const uint32_t b_block = x.width / 2 * 128;  // bytes of a K-block of the columns
+        for (int kb = 0; kb < x.blocks; kb += kps) {
           const int left = DW ? x.rows - kb * EPB : 0;  // dw: rows of the group in this stage and later
-          const bool tail = DW && kb + KPS >= x.blocks && (x.rows & 15) != 0;
-          if (leader) {
-            ok = mbar_wait(&full[stage], phase, ctx, SITE_FULL);
-          } else if (DW && tail) {
-            ok = mbar_wait(&tail_full[stage], tail_parity >> stage & 1u, ctx, SITE_FULL);
-          }
+          const bool tail = DW && kb + 1 == x.blocks && (x.rows & 15) != 0;
+          if (leader) ok = mbar_wait(&full[stage], phase, ctx, SITE_FULL);
+          else if (tail) ok = mbar_wait(&tail_full[stage], tail_parity >> stage & 1u, ctx, SITE_FULL);
+          ok = all_ok(ok);
           if constexpr (DW) {
-            ok = __all_sync(0xffffffffu, ok);
             if (ok && tail) {
-              // Rows left .. the end of its 16-row step, in the two boxes of
-              // 64 columns of each operand (128-byte rows; the swizzle stays
-              // within a row).
-              const int q = left / EPB, r = left % EPB, n = (16 - (r & 15)) * 8;
-              uint8_t* sA = smem + L::OFF_A + (stage * KPS + q) * L::SUB + r * 128;
-              uint8_t* sB = smem + L::OFF_B + (stage * KPS + q) * L::SUB + r * 128;
-              for (int i = lane; i < n; i += 32) {
+              // Rows left .. the end of its 16-row step, in every box of 64
+              // columns (128-byte rows; the swizzle stays within a row).
+              uint8_t* sA = smem + stage * stage_bytes;
+              uint8_t* sB = sA + a_bytes;
+              const int n = (16 - (left & 15)) * 8;
+              for (int c = lane; c < n; c += 32) {
+                const int at = left * 128 + c * 16;
                 const uint4 zero = make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(sA + i * 16) = zero;
-                *reinterpret_cast<uint4*>(sA + 8192 + i * 16) = zero;
-                *reinterpret_cast<uint4*>(sB + i * 16) = zero;
-                *reinterpret_cast<uint4*>(sB + 8192 + i * 16) = zero;
+                for (int box = 0; box < 2 * x.nsub; ++box) *reinterpret_cast<uint4*>(sA + box * 8192 + at) = zero;
+                for (int box = 0; box < 2; ++box) *reinterpret_cast<uint4*>(sB + box * 8192 + at) = zero;
               }
               fence_proxy_async_smem();
               __syncwarp();
               if (!leader) {
                 if (lane == 0) mbar_arrive_cluster(tail_done_leader0 + stage * 8u);
+                __syncwarp();
               } else {
-                ok = mbar_wait_cluster(&tail_done[stage], tail_parity >> stage & 1u, ctx, SITE_FULL);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = all_ok(mbar_wait_cluster(&tail_done[stage], tail_parity >> stage & 1u, ctx, SITE_FULL));
               }
               tail_parity ^= 1u << stage;
             }
           }
           if (!ok) break;
-          if (leader && (!DW || lane == 0)) {
+          if (leader) {
             tc_fence_after();
-            const uint32_t a_addr = smem_u32(smem + L::OFF_A + stage * KPS * L::SUB);
-            const uint32_t b_addr = smem_u32(smem + L::OFF_B + stage * KPS * L::SUB);
-            const int nq = min(KPS, x.blocks - kb);
+            const uint32_t a_addr = ring + stage * stage_bytes, b_addr = a_addr + a_bytes;
+            const bool first = kb == 0, last = kb + kps >= x.blocks;
+            const int nq = min(kps, x.blocks - kb);
+            const int steps = DW ? min(4, (left + 15) / 16) : 4;  // of 32 bytes (dw: 16 rows) a K-block
 #pragma unroll
-            for (int q = 0; q < KPS; ++q) {
-              if (q >= nq) break;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if (DW && (q * 4 + k) * 16 >= left) break;
-                const uint64_t ad = operand_desc<A_MN>(a_addr + q * L::SUB, k);
-                const uint64_t bd = operand_desc<B_MN>(b_addr + q * L::SUB, k);
-                const uint32_t accumulate = (kb | q | k) != 0 ? 1u : 0u;
-                if constexpr (I8) umma_i8<2>(d_tmem, ad, bd, idesc, accumulate);
-                else umma_f16_cg2(d_tmem, ad, bd, idesc, accumulate);
+            for (int s = 0; s < 2; ++s) {
+              if (s >= x.nsub) break;
+              const uint32_t slot = (halves + s) & 1u;
+              if (first) {
+                ok = all_ok(mbar_wait(&tmem_empty[slot], ((halves + s) >> 1 & 1u) ^ 1u, ctx, SITE_TMEM_EMPTY));
+                if (!ok) break;
+                tc_fence_after();
               }
+              const uint32_t d_tmem = tmem_u + slot * 256;
+              const uint64_t a0 = operand_desc<A_MN>(a_addr + s * L::SUB, 0), b0 = operand_desc<B_MN>(b_addr, 0);
+              const uint64_t a1 = operand_desc<A_MN>(a_addr + L::SUB, 0), b1 = operand_desc<B_MN>(b_addr + b_block, 0);
+              if (elect_one()) {
+                // Addresses in 16 bytes: 32 bytes a step along rows, 16 rows of 128 bytes across them.
+                if (!DW || steps == 4) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const uint64_t ad = a0 + k * (A_MN ? 128 : 2), bd = b0 + k * (B_MN ? 128 : 2);
+                    const uint32_t accumulate = k == 0 && first ? 0u : 1u;
+                    if constexpr (I8) umma_i8<2>(d_tmem, ad, bd, idesc, accumulate);
+                    else umma_f16_cg2(d_tmem, ad, bd, idesc, accumulate);
+                  }
+                } else if constexpr (DW) {
+                  for (int k = 0; k < steps; ++k)
+                    umma_f16_cg2(d_tmem, a0 + k * 128, b0 + k * 128, idesc, k == 0 && first ? 0u : 1u);
+                }
+                if (!DW && nq == 2) {
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const uint64_t ad = a1 + k * (A_MN ? 128 : 2), bd = b1 + k * (B_MN ? 128 : 2);
+                    if constexpr (I8) umma_i8<2>(d_tmem, ad, bd, idesc, 1u);
+                    else umma_f16_cg2(d_tmem, ad, bd, idesc, 1u);
+                  }
+                }
+                if (last) umma_commit_cg2_mc(&tmem_full[slot], 0x3);
+              }
+              __syncwarp();
+              any_issued = true;
             }
-            any_issued = true;
-            umma_commit_cg2_mc(&empty[stage], 0x3);
+            if (!ok) break;
+            if (elect_one()) umma_commit_cg2_mc(&empty[stage], 0x3);
           }
-          if constexpr (DW) __syncwarp();
-          if (++stage == STAGES) {
+          __syncwarp();
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (!ok) break;
-        if (leader && (!DW || lane == 0)) umma_commit_cg2_mc(&tmem_full[acc], 0x3);
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1u;
+        if (x.blocks) halves += x.nsub;
       }
-      if (!ok && any_issued) {
+      if (!ok && any_issued && elect_one()) {
         // Abort: wait for the MMAs already issued before TMEM is freed.
         umma_commit_cg2_mc(drain, 0x1);
         WaitCtx drain_ctx{ctx.status, 50000000ull};
         mbar_wait(drain, 0, drain_ctx, SITE_DRAIN);
       }
     }
+  } else if (warp == 10) {
+    // ------------------------------------------------------- tiles, in order
+    const int num_tiles = s_first[tab.entries] * tab.panels;
+    for (int i = 0;; ++i) {
+      // Back and forth over the pairs.
+      const int t = i * pairs + ((i & 1) ? pairs - 1 - pair : pair);
+      Tile x;
+      x.e = -1;
+      if (t < num_tiles) x = tile_of<MODE, EPB>(t, g, tab);
+      const int at = i % L::TILES;
+      if (!all_ok(mbar_wait(&tile_empty[at], (i / L::TILES & 1) ^ 1u, ctx, SITE_TILE))) break;
+      if (lane == 0) {
+        s_tiles[at] = x;
+        mbar_arrive(&tile_full[at]);
+      }
+      __syncwarp();
+      if (x.e < 0) break;
+    }
   } else {
     // -------------------------------------------------------------- epilogue
-    const int q = warp & 3;  // TMEM lane quarter this warp may access
-    TO* stage_c = reinterpret_cast<TO*>(smem + L::OFF_C + (warp - 2) * 2 * L::C_SUB);
-    const uint32_t tmem_empty_leader0 = mapa_shared(smem_u32(&tmem_empty[0]), 0);
-    int acc = 0;
-    uint32_t acc_phase = 0;
+    const int q = warp & 3;             // TMEM lane quarter this warp may access
+    const int side = (warp - 2) / 4;    // which half of a tile's columns it takes
+    uint16_t* stage_c = reinterpret_cast<uint16_t*>(smem + L::OFF_C + (warp - 2) * L::C_SUB);
     int sub = 0;
-    for (int t = blockIdx.x / 2; t < num_tiles; t += step) {
-      const Tile x = tile_of<MODE, EPB>(t, g, gr);
-      const int a_warp = x.a0 + (int)rank * 128 + q * 32;  // this warp's first row of the tile
-      const int a = a_warp + lane;
+    const uint32_t tmem_empty_leader0 = mapa_shared(smem_u32(&tmem_empty[0]), 0);
+    const uint32_t t_quarter = tmem_base + ((uint32_t)(q * 32) << 16);
+    uint32_t halves = 0;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      const Tile x = next_tile(i);
+      if (x.e < 0) break;
       const int limit = DW ? g.DB : x.rows;  // columns end here
-      const int chunks = x.width / 32;
-      float sw = 0.f, bias = 0.f;
+      const int chunks = x.width / 32;       // of 16 columns, of this warp
+      const int d0 = side * chunks * 16;     // its first column in the tile
+      const int a_warp0 = x.a0 + (int)rank * 128 + q * 32;
+      const bool some = x.blocks != 0;  // dw of a group without rows: zeros
+      float sx[4];                      // 8-bit: sx[c] is the scale of column d0 + 32 c + lane
       if constexpr (I8) {
-        if (a < g.DA) {
-          sw = g.w_scale[(int64_t)x.e * g.DA + a];
-          if (g.bias) bias = (float)static_cast<const TO*>(g.bias)[a];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int b = x.b0 + d0 + c * 32 + lane;
+          sx[c] = 2 * c < chunks && b < limit ? g.scale[x.begin + b] : 0.f;
         }
       }
-      const bool some = x.blocks != 0;
-      if (some && !mbar_wait(&tmem_full[acc], acc_phase, ctx, SITE_TMEM_FULL)) break;
-      tc_fence_after();
-      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 256);
-#pragma unroll 1
-      for (int c = 0; c < chunks; ++c) {
-        uint32_t v[32];
-        if (some) {
-          tmem_ld_32x32b_x32(t_row + (uint32_t)(c * 32), v);
-          tmem_ld_wait();
-          if (c == chunks - 1) {
-            // Accumulator fully read: hand it back to the MMA issuer.
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(tmem_empty_leader0 + (uint32_t)acc * 8u);
-          }
-        } else {
+      // out[s][c][j]: columns 16 c + 2 j and the next of this thread's row of half s, as outputs.
+      uint32_t out[2][8][8];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0u;
-        }
-        const int b = x.b0 + c * 32;  // this chunk's first column
-        if (a_warp >= g.DA || b >= limit) continue;
+      for (int s = 0; s < 2; ++s) {
+        if (s >= x.nsub || !ok) break;
+        float sw = 0.f, bias = 0.f;
         if constexpr (I8) {
-          const float sx = b + lane < limit ? g.scale[x.begin + b + lane] : 0.f;
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            v[j] = __float_as_uint((float)(int)v[j] * (sw * __shfl_sync(0xffffffffu, sx, j)) + bias);
+          const int a = a_warp0 + s * 256 + lane;
+          if (a < g.DA) {
+            sw = g.w_scale[(int64_t)x.e * g.DA + a];
+            if (g.bias) bias = (float)static_cast<const TO*>(g.bias)[a];
+          }
         }
-        if (g.tma_out && (DW || b + 32 <= limit)) {
-          TO* buf = stage_c + (sub & 1) * (32 * 32);
+        const uint32_t slot = halves & 1u;
+        if (some) {
+          ok = all_ok(mbar_wait(&tmem_full[slot], halves >> 1 & 1u, ctx, SITE_TMEM_FULL));
+          if (!ok) break;
+          ++halves;
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          if (c >= chunks) break;
+          uint32_t v[16];
+          if (some) {
+            tmem_ld_32x32b_x16(t_quarter + slot * 256 + (uint32_t)(d0 + c * 16), v);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = 0u;
+          }
+          if constexpr (I8) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              v[j] = __float_as_uint((float)(int)v[j] * (sw * __shfl_sync(0xffffffffu, sx[c / 2], c % 2 * 16 + j)) + bias);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) out[s][c][j] = pack2(TO(), __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+        }
+        if (some) {
+          // This warp's share read: hand it back to the MMA issuer.
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(tmem_empty_leader0 + slot * 8u);
+        }
+      }
+      if (!ok) break;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int a_warp = a_warp0 + s * 256;
+        if (s >= x.nsub || a_warp >= g.DA) break;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const int b = x.b0 + d0 + c * 16;
+          if (c >= chunks || b >= limit) break;
+          uint16_t* buf = stage_c + (sub & 1) * (16 * 32);
+          ++sub;
           if (lane == 0) tma_store_wait_read<1>();  // the store that used `buf` has read it
           __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) buf[j * 32 + lane] = ElemTraits<TO>::cvt(__uint_as_float(v[j]));
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (DW) tma_store_3d(&tmC, buf, a_warp, b, x.e);
-            else tma_store_2d(&tmC, buf, a_warp, x.begin + b);
-            tma_store_commit();
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t two = out[s][c][j];
+            buf[(2 * j) * 32 + lane] = (uint16_t)(two & 0xFFFFu);
+            buf[(2 * j + 1) * 32 + lane] = (uint16_t)(two >> 16);
           }
-          ++sub;
-        } else if (a < g.DA) {
-          // The group ends inside the chunk (the next rows are another
-          // group's), or TMA cannot address Y: 64 bytes a warp and column.
-          TO* out = static_cast<TO*>(g.Y) + (DW ? (int64_t)x.e * g.DB + b : (int64_t)x.begin + b) * g.ldy + a;
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (b + j < limit) out[j * g.ldy] = ElemTraits<TO>::cvt(__uint_as_float(v[j]));
+          if (g.tma_out && (DW || b + 16 <= limit)) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (DW) tma_store_3d(&tmC, buf, a_warp, b, x.e);
+              else tma_store_2d(&tmC, buf, a_warp, x.begin + b);
+            }
+          } else if (a_warp + lane < g.DA) {
+            // The group ends inside the chunk (the next rows are another
+            // group's), or TMA cannot address Y: 64 bytes a warp and column.
+            // Every thread reads what it wrote.
+            uint16_t* y = static_cast<uint16_t*>(g.Y) +
+                          (DW ? (int64_t)x.e * g.DB + b : (int64_t)x.begin + b) * g.ldy + a_warp + lane;
+            const int n = min(16, limit - b);
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) y[j * g.ldy] = buf[j * 32 + lane];
+          }
+          if (lane == 0) tma_store_commit();
         }
-      }
-      if (some) {
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1u;
       }
     }
     // The CTA may exit once its last stores have read their staging buffers.
@@ -499,7 +782,10 @@ int launch(const GroupedProblem& p) {
   g.w_scale = p.w_scale;
   g.bias = p.bias;
   g.pdl = pdl_enabled() ? 1 : 0;
-  CUtensorMap tA, tB, tB16, tC;
+
+  g.sort = p.R >= SORT_ROWS && (DW ? p.E : 2 * p.E) <= SORT_LIMIT;
+  CUtensorMap tA, tB, tC;
+  ColumnMaps tBs;
   int64_t tiles;
   if constexpr (!DW) {
     g.DA = (int)p.N;
@@ -507,7 +793,9 @@ int launch(const GroupedProblem& p) {
     if (MODE == MODE_RC) rc = map3(&tA, p.W, type, ES, p.E, p.N, p.K, p.ldw, p.w_stride, 128, EPB, 128);
     else rc = map3(&tA, p.W, type, ES, p.E, p.K, p.N, p.ldw, p.w_stride, 64, 64, 128);
     if (rc || (rc = map2(&tB, p.X, type, ES, p.R, p.K, p.ldx, 128, EPB, 128)) ||
-        (rc = map2(&tB16, p.X, type, ES, p.R, p.K, p.ldx, 16, EPB, 128)))
+        (rc = map2(&tBs.box[0], p.X, type, ES, p.R, p.K, p.ldx, 64, EPB, 128)) ||
+        (rc = map2(&tBs.box[1], p.X, type, ES, p.R, p.K, p.ldx, 32, EPB, 128)) ||
+        (rc = map2(&tBs.box[2], p.X, type, ES, p.R, p.K, p.ldx, 16, EPB, 128)))
       return rc;
     tiles = (p.N + 255) / 256 * (p.R / 256 + std::min(p.E, p.R));  // at most
   } else {
@@ -521,14 +809,14 @@ int launch(const GroupedProblem& p) {
     if ((rc = map2(&tA, a, type, ES, p.R, g.DA, lda, 64, 64, 128)) ||
         (rc = map2(&tB, b, type, ES, p.R, g.DB, ldb, 64, 64, 128)))
       return rc;
-    tB16 = tB;
+    tBs = {{tB, tB, tB}};  // not used
     tiles = p.E * ((g.DA + 255) / 256) * ((g.DB + 255) / 256);
   }
   if (tiles > INT32_MAX / 2) return fail(KEBAB_EINVAL, "grouped product: too many tiles");
   g.tma_out = (reinterpret_cast<uintptr_t>(p.Y) & 15u) == 0 && g.ldy % 8 == 0;
   if (!g.tma_out) tC = tA;  // not used
-  else if (DW) rc = map3(&tC, p.Y, p.out, 2, p.E, g.DB, g.DA, g.ldy, g.ldy * g.DB, 32, 32, 0);
-  else rc = map2(&tC, p.Y, p.out, 2, p.R, p.N, p.ldy, 32, 32, 0);
+  else if (DW) rc = map3(&tC, p.Y, p.out, 2, p.E, g.DB, g.DA, g.ldy, g.ldy * g.DB, 16, 32, 0);
+  else rc = map2(&tC, p.Y, p.out, 2, p.R, p.N, p.ldy, 16, 32, 0);
   if (rc) return rc;
 
   auto kern = grouped_umma_kernel<TO, I8, MODE>;
@@ -542,7 +830,7 @@ int launch(const GroupedProblem& p) {
     err[di] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GSmem::ALLOC);
     max_pairs[di] = dev->sm_count / 2;
     if (err[di] != cudaSuccess) return;
-    PdlLaunch q(dim3(2 * max_pairs[di]), dim3(192), GSmem::ALLOC, nullptr, 2);
+    PdlLaunch q(dim3(2 * max_pairs[di]), dim3(THREADS), GSmem::ALLOC, nullptr, 2);
     q.cfg.numAttrs = 1;
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kern, &q.cfg) == cudaSuccess && n > 0) max_pairs[di] = std::min(n, max_pairs[di]);
@@ -550,8 +838,8 @@ int launch(const GroupedProblem& p) {
   });
   if (err[di] != cudaSuccess) return cuda_fail(err[di], "cudaFuncSetAttribute(max dynamic smem)");
   const int pairs = (int)std::min<int64_t>(tiles, max_pairs[di]);
-  PdlLaunch l(dim3(2 * pairs), dim3(192), smem, p.stream, 2);
-  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, tA, tB, tB16, tC, g);
+  PdlLaunch l(dim3(2 * pairs), dim3(THREADS), smem, p.stream, 2);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, tA, tB, tBs, tC, g);
   return e == cudaSuccess ? KEBAB_OK : cuda_fail(e, "grouped tcgen05 launch");
 }
 

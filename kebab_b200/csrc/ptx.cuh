@@ -31,6 +31,7 @@ enum WaitSite : uint32_t {
   SITE_DRAIN = 8,       // teardown drain after an abort
   SITE_PARTIAL = 9,     // stream-K owner waiting for a contributor's partial
   SITE_BCHUNK = 10,     // gated GEMM producer waiting for a chunk of B to arrive
+  SITE_TILE = 11,       // grouped product: a tile's description, or a free place for one
 };
 
 // Where a kernel reports a failed wait, and how long a wait may take.
