@@ -44,8 +44,8 @@ __device__ __forceinline__ void group_range(const int32_t* offsets, int e, int R
 
 int launch_grouped_simt(const GroupedProblem& p);
 int launch_grouped_umma(const GroupedProblem& p);
-int launch_grouped_gemv(const GroupedProblem& p);
-bool grouped_gemv_ok(const GroupedProblem& p);  // at most 8 rows, whole 16-byte runs
+int launch_grouped_skinny(const GroupedProblem& p);
+constexpr int64_t kSkinnyRows = 64;
 // Whether TMA can address X and W (and dY): the others take the CUDA cores.
 bool grouped_tma_ok(const GroupedProblem& p);
 
