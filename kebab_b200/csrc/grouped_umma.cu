@@ -10,9 +10,12 @@
 // A tile is a panel of 512 rows (two MMAs of 256 that share the staged columns)
 // or, where that would leave the pairs few tiles each, of 256. Its halves take
 // turns on two accumulators of up to 256 columns. With 512-row panels both are
-// in use, so the next tile's MMAs wait for the epilogue: its 8 warps read the
-// halves into registers (as pairs of outputs), hand each back at once, and only
-// then store.
+// in use at once, so the second half runs one K-block behind the first: each
+// accumulator then has two K-blocks' MMAs of the other half (1024 cycles)
+// between its last MMA and the next tile's first, in which the 8 epilogue warps
+// read it into registers (as pairs of outputs) and hand it back; they store
+// afterwards. Without the lag the issuer waited 4300 of 36800 cycles a tile
+// (2048 terms).
 //
 // Ragged sizes cost what they are: a forward tile is as wide as its rows need
 // (a multiple of 32; N is a field of the instruction descriptor), a group of
@@ -501,11 +504,54 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t tail_done_leader0 = mapa_shared(smem_u32(&tail_done[0]), 0);
       const uint32_t ring = smem_u32(smem);
       const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
+      // The MMAs of half `s` over the stage `at`, whose first K-block is kb;
+      // `left`: dw's rows of the group from there on.
+      auto issue = [&](const Tile& x, uint32_t idesc, int s, int at, int kb, bool last, int left) {
+        const uint32_t slot = (halves + s) & 1u;
+        if (kb == 0) {
+          if (!all_ok(mbar_wait(&tmem_empty[slot], ((halves + s) >> 1 & 1u) ^ 1u, ctx, SITE_TMEM_EMPTY))) return false;
+          tc_fence_after();
+        }
+        const uint32_t a_addr = ring + at * stage_bytes + s * L::SUB, b_addr = ring + at * stage_bytes + a_bytes;
+        const uint32_t d_tmem = tmem_u + slot * 256;
+        const uint64_t a0 = operand_desc<A_MN>(a_addr, 0), b0 = operand_desc<B_MN>(b_addr, 0);
+        const uint64_t a1 = operand_desc<A_MN>(a_addr + L::SUB, 0);
+        const uint64_t b1 = operand_desc<B_MN>(b_addr + x.width / 2 * 128, 0);
+        const int nq = min(kps, x.blocks - kb);
+        const int steps = DW ? min(4, (left + 15) / 16) : 4;  // of 32 bytes (dw: 16 rows) a K-block
+        if (elect_one()) {
+          // Addresses in 16 bytes: 32 bytes a step along rows, 16 rows of 128 bytes across them.
+          if (!DW || steps == 4) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint64_t ad = a0 + k * (A_MN ? 128 : 2), bd = b0 + k * (B_MN ? 128 : 2);
+              const uint32_t accumulate = k == 0 && kb == 0 ? 0u : 1u;
+              if constexpr (I8) umma_i8<2>(d_tmem, ad, bd, idesc, accumulate);
+              else umma_f16_cg2(d_tmem, ad, bd, idesc, accumulate);
+            }
+          } else if constexpr (DW) {
+            for (int k = 0; k < steps; ++k)
+              umma_f16_cg2(d_tmem, a0 + k * 128, b0 + k * 128, idesc, k == 0 && kb == 0 ? 0u : 1u);
+          }
+          if (!DW && nq == 2) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint64_t ad = a1 + k * (A_MN ? 128 : 2), bd = b1 + k * (B_MN ? 128 : 2);
+              if constexpr (I8) umma_i8<2>(d_tmem, ad, bd, idesc, 1u);
+              else umma_f16_cg2(d_tmem, ad, bd, idesc, 1u);
+            }
+          }
+          if (s + 1 == x.nsub) umma_commit_cg2_mc(&empty[at], 0x3);  // the stage's last reader
+          if (last) umma_commit_cg2_mc(&tmem_full[slot], 0x3);
+        }
+        __syncwarp();
+        any_issued = true;
+        return true;
+      };
       for (int i = 0; ok; ++i) {
         const Tile x = next_tile(i);
         if (x.e < 0) break;
         const uint32_t idesc = IDESC | (uint32_t)(x.width >> 3) << 17;
-        const uint32_t b_block = x.width / 2 * 128;  // bytes of a K-block of the columns
         for (int kb = 0; kb < x.blocks; kb += kps) {
           const int left = DW ? x.rows - kb * EPB : 0;  // dw: rows of the group in this stage and later
           const bool tail = DW && kb + 1 == x.blocks && (x.rows & 15) != 0;
@@ -539,51 +585,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (!ok) break;
           if (leader) {
             tc_fence_after();
-            const uint32_t a_addr = ring + stage * stage_bytes, b_addr = a_addr + a_bytes;
-            const bool first = kb == 0, last = kb + kps >= x.blocks;
-            const int nq = min(kps, x.blocks - kb);
-            const int steps = DW ? min(4, (left + 15) / 16) : 4;  // of 32 bytes (dw: 16 rows) a K-block
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              if (s >= x.nsub) break;
-              const uint32_t slot = (halves + s) & 1u;
-              if (first) {
-                ok = all_ok(mbar_wait(&tmem_empty[slot], ((halves + s) >> 1 & 1u) ^ 1u, ctx, SITE_TMEM_EMPTY));
-                if (!ok) break;
-                tc_fence_after();
-              }
-              const uint32_t d_tmem = tmem_u + slot * 256;
-              const uint64_t a0 = operand_desc<A_MN>(a_addr + s * L::SUB, 0), b0 = operand_desc<B_MN>(b_addr, 0);
-              const uint64_t a1 = operand_desc<A_MN>(a_addr + L::SUB, 0), b1 = operand_desc<B_MN>(b_addr + b_block, 0);
-              if (elect_one()) {
-                // Addresses in 16 bytes: 32 bytes a step along rows, 16 rows of 128 bytes across them.
-                if (!DW || steps == 4) {
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    const uint64_t ad = a0 + k * (A_MN ? 128 : 2), bd = b0 + k * (B_MN ? 128 : 2);
-                    const uint32_t accumulate = k == 0 && first ? 0u : 1u;
-                    if constexpr (I8) umma_i8<2>(d_tmem, ad, bd, idesc, accumulate);
-                    else umma_f16_cg2(d_tmem, ad, bd, idesc, accumulate);
-                  }
-                } else if constexpr (DW) {
-                  for (int k = 0; k < steps; ++k)
-                    umma_f16_cg2(d_tmem, a0 + k * 128, b0 + k * 128, idesc, k == 0 && first ? 0u : 1u);
-                }
-                if (!DW && nq == 2) {
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    const uint64_t ad = a1 + k * (A_MN ? 128 : 2), bd = b1 + k * (B_MN ? 128 : 2);
-                    if constexpr (I8) umma_i8<2>(d_tmem, ad, bd, idesc, 1u);
-                    else umma_f16_cg2(d_tmem, ad, bd, idesc, 1u);
-                  }
-                }
-                if (last) umma_commit_cg2_mc(&tmem_full[slot], 0x3);
-              }
-              __syncwarp();
-              any_issued = true;
-            }
+            const bool last = kb + kps >= x.blocks;
+            ok = issue(x, idesc, 0, stage, kb, last, left);
+            if (ok && x.nsub == 2 && kb > 0) ok = issue(x, idesc, 1, stage == 0 ? stages - 1 : stage - 1, kb - 1, false, EPB);
+            if (ok && x.nsub == 2 && last) ok = issue(x, idesc, 1, stage, kb, true, left);
             if (!ok) break;
-            if (elect_one()) umma_commit_cg2_mc(&empty[stage], 0x3);
           }
           __syncwarp();
           if (++stage == stages) {
@@ -664,24 +670,31 @@ __global__ void __launch_bounds__(THREADS, 1)
           ++halves;
           tc_fence_after();
         }
+        // The sum of column `col` of 32, of which lane j of `scales` has column j's scale.
+        auto value = [&](uint32_t v, float scales, int col) {
+          if constexpr (I8) return (float)(int)v * (sw * __shfl_sync(0xffffffffu, scales, col)) + bias;
+          else return __uint_as_float(v);
+        };
+        const uint32_t src = t_quarter + slot * 256 + (uint32_t)d0;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          if (c >= chunks) break;
-          uint32_t v[16];
+        for (int c = 0; c < 4; ++c) {
+          if (2 * c >= chunks) break;
+          // With an odd number of chunks the last 16 columns are not this warp's, and not used.
+          uint32_t v[2][16];
           if (some) {
-            tmem_ld_32x32b_x16(t_quarter + slot * 256 + (uint32_t)(d0 + c * 16), v);
+            tmem_ld_32x32b_x16(src + c * 32, v[0]);
+            tmem_ld_32x32b_x16(src + c * 32 + 16, v[1]);
             tmem_ld_wait();
           } else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = 0u;
-          }
-          if constexpr (I8) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              v[j] = __float_as_uint((float)(int)v[j] * (sw * __shfl_sync(0xffffffffu, sx[c / 2], c % 2 * 16 + j)) + bias);
+            for (int j = 0; j < 16; ++j) v[0][j] = v[1][j] = 0u;
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) out[s][c][j] = pack2(TO(), __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              out[s][2 * c + u][j] =
+                  pack2(TO(), value(v[u][2 * j], sx[c], u * 16 + 2 * j), value(v[u][2 * j + 1], sx[c], u * 16 + 2 * j + 1));
         }
         if (some) {
           // This warp's share read: hand it back to the MMA issuer.
