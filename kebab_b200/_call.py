@@ -47,7 +47,7 @@ def tensor(what, name, t, dim, dtypes, device=None):
         raise bad("%s: %s must have %d dimension(s), got %s" % (what, name, dim, tuple(t.shape)))
     if t.dtype not in dtypes:
         raise bad("%s: %s has type %s" % (what, name, t.dtype))
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel():
         raise bad("%s: rows of %s must be contiguous" % (what, name))
     at = t.get_device()
     if device is not None and at != device:
