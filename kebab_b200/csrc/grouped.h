@@ -45,7 +45,6 @@ __device__ __forceinline__ void group_range(const int32_t* offsets, int e, int R
 int launch_grouped_simt(const GroupedProblem& p);
 int launch_grouped_umma(const GroupedProblem& p);
 int launch_grouped_skinny(const GroupedProblem& p);
-constexpr int64_t kSkinnyRows = 64;
 // Whether TMA can address X and W (and dY): the others take the CUDA cores.
 bool grouped_tma_ok(const GroupedProblem& p);
 
@@ -55,6 +54,10 @@ int guarded(F&& f) noexcept {
   try {
     return f();
   } catch (...) {
+    try {
+      set_error("out of host memory");
+    } catch (...) {
+    }
     return KEBAB_ECUDA;
   }
 }

@@ -46,14 +46,21 @@ int parse_mode(const char* what, const char* opmode, bool* kn) {
   return fail(KEBAB_EINVAL, std::string(what) + ": opmode must be RC or RR, got " + m);
 }
 
-// Up to 64 rows the skinny kernel: 64 x 8192 x 8192 int8 20.5 us against 23.6 of
-// the persistent one, 8 rows of 8 experts 4096 x 2048 23.8 against 26.5, 64 rows
-// of 44 experts 2048 x 2048 60.3 against 59.6; at 128 x 8192 x 8192 they cross
-// (26.7 and 26.1).
+// The skinny kernel up to 128 rows, and where the persistent one would have
+// tiles for less than half of its CTA pairs. us, skinny against persistent:
+// int8 64 x 8192 x 8192 19.4 and 23.1, 128 rows 24.2 and 25.8, 256 rows (32
+// tiles) 28.3 and 34.0, 400 rows (64 tiles) 35.8 and 34.8; 1024 x 1024 x 8192 (16
+// tiles) 24.3 and 35.4; 16-bit 200 rows of 16 experts 2048 x 2048 25.1 and 27.2,
+// 100 rows of 64 experts 1024 x 1024 27.3 and 26.9.
 int run(const GroupedProblem& p) {
   // dw without rows has no operand for a tensor map; it only writes zeros.
   if (p.R == 0 || !grouped_tma_ok(p)) return launch_grouped_simt(p);
-  return !p.dw && p.R <= kSkinnyRows ? launch_grouped_skinny(p) : launch_grouped_umma(p);
+  if (p.dw) return launch_grouped_umma(p);
+  DeviceInfo* dev = nullptr;
+  const int rc = device_info(&dev);
+  if (rc) return rc;
+  const int64_t tiles = (p.N + 255) / 256 * (p.offsets ? p.R / 256 + std::min(p.E, p.R) : (p.R + 255) / 256);
+  return p.R <= 128 || tiles <= dev->sm_count / 4 ? launch_grouped_skinny(p) : launch_grouped_umma(p);
 }
 
 int run_i8(int out, const int8_t* q, int64_t ldq, const float* scale, const int8_t* Wq, int64_t ldw,

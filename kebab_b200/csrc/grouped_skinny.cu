@@ -1,16 +1,18 @@
-// Grouped and 8-bit integer products for few rows on the tensor cores: up to
-// 64 rows of X, bound by the weights' bytes.
+// Grouped and 8-bit integer products for few rows, or few tiles, on the tensor
+// cores: bound by the weights' bytes, or by how many SMs have work.
 //
 // A CTA multiplies 128 weight rows n (the MMA's row side, so that a lane of
-// TMEM is a column of Y) with all rows of one group, padded to a multiple of
-// 16. Where that gives too few CTAs to keep the memory busy, a cluster of S of
-// them splits k: each ends with a partial sum in TMEM, sends every other CTA
-// the 128 / S of its rows that that one finishes (st.async, counted on the
-// receiver's barrier), and adds up its own rows over the S partials in rank
-// order. No workspace, no atomics, and the same bits every time.
+// TMEM is a column of Y) with up to 128 rows of one group (equal shares of a
+// larger group, padded to a multiple of 16). Where that gives too few CTAs, a
+// cluster of S of them splits k: each ends with a partial sum in TMEM, sends
+// every other CTA the 128 / S of its rows that that one finishes (st.async,
+// counted on the receiver's barrier), and adds up its own rows over the S
+// partials in rank order. No workspace, no atomics, and the same bits every
+// time.
 //
-// Ring: a stage is two 128-byte K-blocks (256 contiguous bytes a weight row);
-// with one CTA an SM or two, up to 190 KB are in flight.
+// Ring: a stage is two 128-byte K-blocks (256 contiguous bytes a weight row) up
+// to 64 rows of X, else one; with one CTA an SM or two, up to 190 KB are in
+// flight.
 //
 // In linear_i8 the kernel before this one only makes the codes and scales of X
 // (`early`): the first weights are fetched while it still runs.
@@ -26,15 +28,18 @@
 
 namespace kb {
 namespace {
-constexpr int THREADS = 224;  // warps: copies of W, MMA issuer, 4 epilogue warps, copies of X
+// Warps: copies of W, MMA issuer, 8 epilogue warps, copies of X. The epilogue is
+// bound by latency, a warp or two a scheduler: of 256 x 1024 x 8192 int8 (8
+// splits) the exchange and the output took 6.1 us with 4 warps, 4.8 with 8.
+constexpr int EPI = 8, X_WARP = 2 + EPI, THREADS = 32 * (3 + EPI);
 constexpr int SUB = 128 * 128;
-constexpr int MAX_STAGES = 8, KPS = 2, MAX_ROWS = (int)kSkinnyRows;
+constexpr int MAX_STAGES = 8, MAX_WIDTH = 128;
 
 struct SkinnyArgs {
   const int32_t* offsets;
   int E, R, N, K;
   int splits;
-  int stages, x_rows;  // stages, rows of X that a stage has room for
+  int kps, stages, x_rows;  // K-blocks a stage, stages, rows of X that a stage has room for
   void* Y;
   int64_t ldy;
   const float* scale;
@@ -57,42 +62,59 @@ __device__ __forceinline__ void send16(uint32_t dst, uint32_t bar, uint32_t a, u
                : "memory");
 }
 
-// The group that is the `nth` of those with rows, by all threads of the block.
-__device__ bool nth_group(const SkinnyArgs& g, int nth, int& e, int& begin, int& rows) {
-  __shared__ int s_count[THREADS / 32], s_found[3];
+// Rows begin .. begin + rows - 1 of group e: the `nth` of the shares (of at most
+// MAX_WIDTH rows) of all groups, by all threads of the block; false if there
+// are fewer.
+__device__ bool nth_share(const SkinnyArgs& g, int nth, int& e, int& begin, int& rows) {
+  __shared__ int s_count[THREADS / 32], s_found[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int at = nth;  // the share within its group
   if (g.offsets == nullptr) {
     e = 0;
     begin = 0;
     rows = g.R;
-    return nth == 0;
-  }
-  if (threadIdx.x == 0) s_found[0] = -1;
-  int before = 0;
-  for (int e0 = 0; e0 < g.E; e0 += THREADS) {
-    int b = 0, n = 0;
-    if (e0 + (int)threadIdx.x < g.E) group_range(g.offsets, e0 + threadIdx.x, g.R, b, n);
-    const uint32_t some = __ballot_sync(0xffffffffu, n > 0);
-    if (lane == 0) s_count[warp] = __popc(some);
-    __syncthreads();
-    int at = before + __popc(some & ((1u << lane) - 1u));
+  } else {
+    if (threadIdx.x == 0) s_found[0] = -1;
+    int before = 0;
+    for (int e0 = 0; e0 < g.E; e0 += THREADS) {
+      int b = 0, n = 0;
+      if (e0 + (int)threadIdx.x < g.E) group_range(g.offsets, e0 + threadIdx.x, g.R, b, n);
+      const int shares = (n + MAX_WIDTH - 1) / MAX_WIDTH;
+      int sum = shares;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-      if (w < warp) at += s_count[w];
-      before += s_count[w];
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += up;
+      }
+      if (lane == 31) s_count[warp] = sum;
+      __syncthreads();
+      int first = before + sum - shares;
+#pragma unroll
+      for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) first += s_count[w];
+        before += s_count[w];
+      }
+      if (first <= nth && nth < first + shares) {
+        s_found[0] = e0 + threadIdx.x;
+        s_found[1] = b;
+        s_found[2] = n;
+        s_found[3] = nth - first;
+      }
+      __syncthreads();
+      if (before > nth) break;
     }
-    if (n > 0 && at == nth) {
-      s_found[0] = e0 + threadIdx.x;
-      s_found[1] = b;
-      s_found[2] = n;
-    }
-    __syncthreads();
-    if (before > nth) break;
+    e = s_found[0];
+    if (e < 0) return false;
+    begin = s_found[1];
+    rows = s_found[2];
+    at = s_found[3];
   }
-  e = s_found[0];
-  begin = s_found[1];
-  rows = min(s_found[2], MAX_ROWS);
-  return e >= 0;
+  const int shares = (rows + MAX_WIDTH - 1) / MAX_WIDTH;
+  if (at >= shares) return false;
+  const int share = (rows + shares - 1) / shares;
+  begin += at * share;
+  rows = min(share, rows - at * share);
+  return rows > 0;
 }
 
 template <typename TO, bool I8, bool RR>
@@ -110,7 +132,7 @@ __global__ void __launch_bounds__(THREADS)
     pdl_launch_dependents();
   }
   int e, begin, rows;
-  if (!nth_group(g, blockIdx.y, e, begin, rows)) {  // the whole cluster leaves
+  if (!nth_share(g, blockIdx.y, e, begin, rows)) {  // the whole cluster leaves
     if (early) pdl_wait();
     return;
   }
@@ -119,11 +141,11 @@ __global__ void __launch_bounds__(THREADS)
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full, recv_full;
   __shared__ uint32_t tmem_slot;
-  __shared__ float s_scale[MAX_ROWS];
+  __shared__ float s_scale[MAX_WIDTH];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int S = g.splits, stages = g.stages;
+  const int S = g.splits, kps = g.kps, stages = g.stages;
   const int width = (rows + 15) / 16 * 16;  // columns of the MMA
-  const int x_block = g.x_rows * 128, stage_bytes = KPS * (SUB + x_block);
+  const int w_bytes = kps * SUB, x_block = g.x_rows * 128, stage_bytes = w_bytes + kps * x_block;
   float* recv = reinterpret_cast<float*>(smem + stages * stage_bytes);  // [S][128 / S][stride]
   const int stride = width + 4, share = 128 / S;                        // floats of a row; rows this CTA finishes
   const int rank = S > 1 ? (int)cluster_ctarank() : 0;
@@ -142,7 +164,7 @@ __global__ void __launch_bounds__(THREADS)
   }
   __syncwarp();
   if (warp == 1) {
-    tmem_alloc<1>(&tmem_slot, 64);
+    tmem_alloc<1>(&tmem_slot, 128);
     tmem_relinquish<1>();
   }
   tc_fence_before();
@@ -152,15 +174,15 @@ __global__ void __launch_bounds__(THREADS)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  // This CTA's K-blocks, a multiple of KPS but at the end.
+  // This CTA's K-blocks, a multiple of kps but at the end.
   const int total = (g.K + EPB - 1) / EPB;
-  const int per = ((total + S - 1) / S + KPS - 1) / KPS * KPS;
+  const int per = ((total + S - 1) / S + kps - 1) / kps * kps;
   const int kb0 = min(total, rank * per), kb1 = min(total, kb0 + per);
   auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
 
-  if (warp == 0 || warp == 6) {
+  if (warp == 0 || warp == X_WARP) {
     // ---------------------------------------- producers: of W (warp 0), of X
-    // (warp 6). One warp for both took 1.2 us longer to fill the ring. A stage's
+    // (the last warp). One warp for both took 1.2 us longer to fill the ring. A stage's
     // bytes are all announced by the first; those of X may land before that.
     const bool of_w = warp == 0;
     const uint32_t block_bytes = SUB + width * 128;
@@ -168,13 +190,13 @@ __global__ void __launch_bounds__(THREADS)
     int stage = 0;
     uint32_t phase = 1, filled = 0, parity = 0;  // the last two: a bit a stage
     bool ok = true;
-    for (int kb = kb0; kb < kb1; kb += KPS) {
+    for (int kb = kb0; kb < kb1; kb += kps) {
       ok = all_ok(mbar_wait(&empty[stage], phase, ctx, SITE_EMPTY));
       if (!ok) break;
-      const int nq = min(KPS, kb1 - kb);
+      const int nq = min(kps, kb1 - kb);
       if (elect_one()) {
         if (of_w) mbar_arrive_expect_tx(&full[stage], nq * block_bytes);
-        uint8_t* dst = smem + stage * stage_bytes + (of_w ? 0 : KPS * SUB);
+        uint8_t* dst = smem + stage * stage_bytes + (of_w ? 0 : w_bytes);
         for (int q = 0; q < nq; ++q) {
           const int k0 = (kb + q) * EPB;
           if (of_w) {
@@ -187,9 +209,13 @@ __global__ void __launch_bounds__(THREADS)
             dst += SUB;
           } else {
             int r = 0;
+            if (width == 128) {
+              tma_load_2d(dst, &tmX.box[0], &full[stage], k0, begin);
+              r = 64;
+            }
 #pragma unroll
             for (int m = 0; m < 3; ++m) {
-              if (width & (64 >> m)) {
+              if ((width - r) & (64 >> m)) {
                 tma_load_2d(dst + r * 128, &tmX.box[m], &full[stage], k0, begin + r);
                 r += 64 >> m;
               }
@@ -220,12 +246,12 @@ __global__ void __launch_bounds__(THREADS)
     const uint32_t ring = smem_u32(smem), d_tmem = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t idesc = IDESC | (uint32_t)(__shfl_sync(0xffffffffu, width, 0) >> 3) << 17;
     bool ok = true;
-    for (int kb = kb0; kb < kb1; kb += KPS) {
+    for (int kb = kb0; kb < kb1; kb += kps) {
       ok = all_ok(mbar_wait(&full[stage], phase, ctx, SITE_FULL));
       if (!ok) break;
       tc_fence_after();
-      const uint32_t w_addr = ring + stage * stage_bytes, x_addr = w_addr + KPS * SUB;
-      const int nq = min(KPS, kb1 - kb);
+      const uint32_t w_addr = ring + stage * stage_bytes, x_addr = w_addr + w_bytes;
+      const int nq = min(kps, kb1 - kb);
       const uint64_t a0 = operand_desc<RR>(w_addr, 0), b0 = operand_desc<false>(x_addr, 0);
       const uint64_t a1 = operand_desc<RR>(w_addr + SUB, 0), b1 = operand_desc<false>(x_addr + x_block, 0);
       if (elect_one()) {
@@ -257,10 +283,12 @@ __global__ void __launch_bounds__(THREADS)
     __syncwarp();
   } else {
     // -------------------------------------------------------------- epilogue
-    const int q = warp & 3, row = q * 32 + lane;
+    const int q = warp & 3, row = q * 32 + lane;  // TMEM lane quarter of this warp
+    const int side = (warp - 2) / 4;              // two warps a quarter take every second run of columns
+    const int et = threadIdx.x - 64;
     if (early) pdl_wait();  // the scales
-    if (I8 && threadIdx.x - 64 < rows) s_scale[threadIdx.x - 64] = g.scale[begin + threadIdx.x - 64];
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (I8 && et < rows) s_scale[et] = g.scale[begin + et];
+    asm volatile("bar.sync 1, 256;" ::: "memory");
     if (S > 1) {
       // The barrier completes once every peer's rows have landed.
       if (threadIdx.x == 64) mbar_arrive_expect_tx(&recv_full, (uint32_t)((S - 1) * share * width * 4));
@@ -280,7 +308,7 @@ __global__ void __launch_bounds__(THREADS)
       }
       TO* y = static_cast<TO*>(g.Y) + (int64_t)begin * g.ldy + n;
 #pragma unroll 1
-      for (int c = 0; c < width; c += 16) {
+      for (int c = side * 16; c < width; c += EPI / 4 * 16) {
         uint32_t v[16];
         tmem_ld_32x32b_x16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
         tmem_ld_wait();
@@ -297,7 +325,7 @@ __global__ void __launch_bounds__(THREADS)
       const uint32_t bar = mapa_shared(smem_u32(&recv_full), owner);
       const uint32_t dst = mapa_shared(smem_u32(recv + place), owner);
 #pragma unroll 1
-      for (int c = 0; c < width; c += 16) {
+      for (int c = side * 16; c < width; c += EPI / 4 * 16) {
         uint32_t v[16];
         if (some && ok) {
           tmem_ld_32x32b_x16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
@@ -313,10 +341,10 @@ __global__ void __launch_bounds__(THREADS)
         }
       }
       ok = all_ok(mbar_wait(&recv_full, 0, ctx, SITE_PARTIAL)) && ok;
-      // The rows that this CTA keeps were written by one of its warps.
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      // The rows that this CTA keeps were written by some of its warps.
+      asm volatile("bar.sync 1, 256;" ::: "memory");
       // Neighbouring threads take neighbouring n of one column of Y's.
-      const int t = threadIdx.x - 64, r = t % share, n = n0 + rank * share + r;
+      const int r = et % share, n = n0 + rank * share + r;
       float sw = 0.f, bias = 0.f;
       if (I8 && n < g.N) {
         sw = g.w_scale[(int64_t)e * g.N + n];
@@ -328,7 +356,7 @@ __global__ void __launch_bounds__(THREADS)
         // column: 7.4 us of 24).
         TO* y = static_cast<TO*>(g.Y) + (int64_t)begin * g.ldy + n;
 #pragma unroll 2
-        for (int c = t / share * 4; c < rows; c += S * 4) {
+        for (int c = et / share * 4; c < rows; c += EPI / 4 * S * 4) {
           uint4 part[8];
 #pragma unroll
           for (int s = 0; s < 8; ++s)
@@ -352,7 +380,7 @@ __global__ void __launch_bounds__(THREADS)
       }
     }
   }
-  if ((warp < 2 || warp == 6) && S > 1) {
+  if ((warp < 2 || warp == X_WARP) && S > 1) {
     __syncwarp();
     cluster_wait_acquire();
   }
@@ -363,7 +391,7 @@ __global__ void __launch_bounds__(THREADS)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc<1>(tmem, 64);
+    tmem_dealloc<1>(tmem, 128);
   }
 }
 
@@ -393,31 +421,44 @@ int launch(const GroupedProblem& p) {
     const uint32_t xb[2] = {(uint32_t)EPB, 64u >> m};
     if ((rc = make_tmap(&tX.box[m], p.X, type, 2, xd, xs, xb, 128))) return rc;
   }
-  // As many splits as keep one CTA an SM (a power of two, at least four
-  // K-blocks each): tiles of the groups that can have rows.
-  const int64_t groups = p.offsets ? std::min(p.R, p.E) : 1;
-  const int64_t tiles = (p.N + 127) / 128 * groups, blocks = (p.K + EPB - 1) / EPB;
+  // Once per device and instantiation: the shared-memory opt-in, and how many
+  // clusters of 2, 4 and 8 such CTAs the device holds at once (fewer than its
+  // SMs would give: a cluster stays within a GPC).
+  auto kern = grouped_skinny_kernel<TO, I8, RR>;
+  constexpr int ONE_CTA = 221 * 1024;
+  static std::once_flag once[64];
+  static cudaError_t err[64];
+  static int clusters[64][9];
+  const int di = dev->device & 63;
+  std::call_once(once[di], [&] {
+    err[di] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024);
+    for (int s = 2; s <= 8 && err[di] == cudaSuccess; s *= 2) {
+      PdlLaunch q(dim3(dev->sm_count / s * s), dim3(THREADS), ONE_CTA, nullptr, s);
+      q.cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &q.cfg) == cudaSuccess) clusters[di][s] = n;
+      (void)cudaGetLastError();
+    }
+  });
+  if (err[di] != cudaSuccess) return cuda_fail(err[di], "cudaFuncSetAttribute(max dynamic smem)");
+  // As many splits as run in one wave (a power of two, at least four K-blocks
+  // each), for the shares that the groups can have.
+  const int64_t shares = p.offsets ? p.R / MAX_WIDTH + std::min(p.R, p.E) : (p.R + MAX_WIDTH - 1) / MAX_WIDTH;
+  const int64_t tiles = (p.N + 127) / 128 * shares, blocks = (p.K + EPB - 1) / EPB;
   g.splits = 1;
-  while (g.splits < 8 && tiles * g.splits * 2 <= dev->sm_count && blocks >= g.splits * 8) g.splits *= 2;
-  const int width = (int)((p.R + 15) / 16 * 16);  // of the widest group there can be
+  while (g.splits < 8 && tiles <= clusters[di][g.splits * 2] && blocks >= g.splits * 8) g.splits *= 2;
+  const int width = (int)std::min<int64_t>(MAX_WIDTH, (p.R + 15) / 16 * 16);  // of the widest share there can be
   g.x_rows = width;
-  const int stage = KPS * (SUB + width * 128);
+  g.kps = width <= 64 ? 2 : 1;
+  const int stage = g.kps * (SUB + width * 128);
   const int recv = g.splits > 1 ? 128 * (width + 4) * 4 : 0;
   // One CTA an SM takes most of the shared memory; with more CTAs than SMs two share it.
   const int budget = (tiles * g.splits > dev->sm_count ? 110 : 220) * 1024 - recv;
   g.stages = std::max(2, std::min(MAX_STAGES, budget / stage));
   const int smem = g.stages * stage + recv + 1024;
-  auto kern = grouped_skinny_kernel<TO, I8, RR>;
-  static std::once_flag once[64];
-  static cudaError_t err[64];
-  const int di = dev->device & 63;
-  std::call_once(once[di], [&] {
-    err[di] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024);
-  });
-  if (err[di] != cudaSuccess) return cuda_fail(err[di], "cudaFuncSetAttribute(max dynamic smem)");
   const int64_t x = (p.N + 127) / 128 * g.splits;
-  if (x > INT32_MAX) return fail(KEBAB_EINVAL, "grouped product: too many tiles");
-  PdlLaunch l(dim3((unsigned)x, (unsigned)groups), dim3(THREADS), smem, p.stream, g.splits);
+  if (x > INT32_MAX || shares > 65535) return fail(KEBAB_EINVAL, "grouped product: too many tiles");
+  PdlLaunch l(dim3((unsigned)x, (unsigned)shares), dim3(THREADS), smem, p.stream, g.splits);
   const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, tW, tX, (const SkinnyArgs)g);
   return e == cudaSuccess ? KEBAB_OK : cuda_fail(e, "few-rows tcgen05 launch");
 }

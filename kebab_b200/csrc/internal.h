@@ -46,7 +46,8 @@ int make_tmap_2d_sw(CUtensorMap* out, const void* base, int dtype, uint64_t rows
 // Tensor map of `rank` (2 or 3) dimensions, innermost first: type KEBAB_F16,
 // KEBAB_BF16 or TMAP_U8, extents and box in elements, strides of dimensions
 // 1.. in bytes (multiples of 16; the base 16-byte aligned), swizzle 0, 32, 64
-// or 128 bytes.
+// or 128 bytes. Not cached: encoding takes about as long as a look-up (six maps
+// 0.3 us more a call).
 constexpr int TMAP_U8 = 100;
 int make_tmap(CUtensorMap* out, const void* base, int type, int rank, const uint64_t* dims, const uint64_t* strides,
               const uint32_t* box, int swizzle_bytes);

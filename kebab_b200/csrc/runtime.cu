@@ -200,40 +200,8 @@ int make_tmap_2d_sw(CUtensorMap* out, const void* base, int dtype, uint64_t rows
   return KEBAB_OK;
 }
 
-namespace {
-// Cache of make_tmap(), kept as the one above is.
-struct TmapNdKey {
-  const void* base;
-  uint64_t v[9];
-  bool operator==(const TmapNdKey& o) const { return base == o.base && std::memcmp(v, o.v, sizeof(v)) == 0; }
-};
-struct TmapNdHash {
-  size_t operator()(const TmapNdKey& k) const {
-    uint64_t h = reinterpret_cast<uintptr_t>(k.base) * 0x9E3779B97F4A7C15ull;
-    for (uint64_t v : k.v) h = (h ^ v) * 0x100000001B3ull;
-    return (size_t)h;
-  }
-};
-std::unordered_map<TmapNdKey, CUtensorMap, TmapNdHash> g_tmaps_nd;  // guarded by g_tmap_mu
-}  // namespace
-
 int make_tmap(CUtensorMap* out, const void* base, int type, int rank, const uint64_t* dims, const uint64_t* strides,
               const uint32_t* box, int swizzle_bytes) {
-  int dev = 0;
-  (void)cudaGetDevice(&dev);
-  const bool three = rank == 3;
-  const TmapNdKey key{base,
-                      {(uint64_t)dev << 32 | (uint64_t)type << 16 | (uint64_t)rank << 12 | (uint64_t)swizzle_bytes, dims[0],
-                       dims[1], three ? dims[2] : 0, strides[0], three ? strides[1] : 0, box[0], box[1],
-                       three ? box[2] : 0}};
-  {
-    std::lock_guard<std::mutex> lk(g_tmap_mu);
-    auto it = g_tmaps_nd.find(key);
-    if (it != g_tmaps_nd.end()) {
-      *out = it->second;
-      return KEBAB_OK;
-    }
-  }
   int rc = get_encoder();
   if (rc) return rc;
   const cuuint32_t ones[3] = {1, 1, 1};
@@ -252,9 +220,6 @@ int make_tmap(CUtensorMap* out, const void* base, int type, int rank, const uint
                                                     : CU_TENSOR_MAP_SWIZZLE_NONE,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(KEBAB_EINVAL, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(r));
-  std::lock_guard<std::mutex> lk(g_tmap_mu);
-  if (g_tmaps_nd.size() >= kTmapCap) g_tmaps_nd.clear();
-  g_tmaps_nd.emplace(key, *out);
   return KEBAB_OK;
 }
 
@@ -399,7 +364,6 @@ void kebab_shutdown(void) {
   {
     std::lock_guard<std::mutex> lk(g_tmap_mu);
     g_tmaps.clear();
-    g_tmaps_nd.clear();
   }
   std::lock_guard<std::mutex> lk(g_mu);
   for (auto& kv : g_sk)
