@@ -41,25 +41,29 @@ def bad(msg):
 def tensor(what, name, t, dim, dtypes, device=None):
     """Checks that `t` is a CUDA tensor of that rank and type with contiguous
     rows, on `device` if given; returns its device index."""
+    if isinstance(t, torch.Tensor):
+        at = t.get_device()
+        if (at >= 0 and t.dim() == dim and t.dtype in dtypes and (device is None or at == device) and
+                (t.stride(-1) == 1 or t.shape[-1] <= 1 or not t.numel())):
+            return at
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise bad("%s: %s must be a CUDA tensor" % (what, name))
     if t.dim() != dim:
         raise bad("%s: %s must have %d dimension(s), got %s" % (what, name, dim, tuple(t.shape)))
     if t.dtype not in dtypes:
         raise bad("%s: %s has type %s" % (what, name, t.dtype))
-    if t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel():
-        raise bad("%s: rows of %s must be contiguous" % (what, name))
-    at = t.get_device()
     if device is not None and at != device:
         raise bad("%s: %s is on another device" % (what, name))
-    return at
+    raise bad("%s: rows of %s must be contiguous" % (what, name))
 
 
 def dense(what, name, t, shape, dtypes, device):
     """As tensor(), of that very shape and contiguous throughout."""
+    if (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype in dtypes and t.get_device() == device and
+            t.is_contiguous()):
+        return
     tensor(what, name, t, len(shape), dtypes, device)
-    if t.shape != shape or not t.is_contiguous():
-        raise bad("%s: %s must be a contiguous tensor of shape %s, got %s" % (what, name, tuple(shape), tuple(t.shape)))
+    raise bad("%s: %s must be a contiguous tensor of shape %s, got %s" % (what, name, tuple(shape), tuple(t.shape)))
 
 
 def pitch(t):

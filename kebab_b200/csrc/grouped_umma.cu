@@ -115,6 +115,7 @@ struct Table {
   int entries, panels;    // panels: tiles along the MMA-row side
   int nsub;               // 256-row halves of a panel
   int kps;                // K-blocks a stage
+  int cap;                // columns that a tile may have
 };
 
 struct alignas(16) Tile {
@@ -124,11 +125,11 @@ struct alignas(16) Tile {
   int blocks;            // 128-byte K-blocks of the contraction
 };
 
-// Columns of a group's tiles: equal shares of at most 256, and what is left for the last.
+// Columns of a group's tiles: equal shares of at most `cap`, and what is left for the last.
 struct Widths {
   int count, full, last;
-  __device__ __forceinline__ Widths(int rows) {
-    count = (rows + 255) / 256;
+  __device__ __forceinline__ Widths(int rows, int cap) {
+    count = (rows + cap - 1) / cap;
     full = last = (rows + 31) / 32 * 32;
     if (count > 1) {
       full = (divide(rows + count - 1, count) + 31) / 32 * 32;
@@ -170,7 +171,7 @@ __device__ __forceinline__ Tile tile_of(int t, const TileArgs& g, const Table& t
     x.b0 = cb * 256;
     x.blocks = (x.rows + EPB - 1) / EPB;
   } else {
-    const Widths w(x.rows);
+    const Widths w(x.rows, tab.cap);
     if (!tab.sorted) {
       raster(local, tab.panels, w.count, pa, cb);
     } else if (id & 1) {
@@ -235,15 +236,27 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
   const int n = DW || !sorted ? g.E : 2 * g.E;
   int wide = 0;  // some tile of more than 128 columns
   int total = 0;
+  int cap = 256;
   if (!sorted) {
+    // Few rows a group: tiles of at most 128 columns keep two K-blocks a stage
+    // for all, and the weights of the few larger groups come twice, from L2.
+    if constexpr (!DW) {
+      int busy = 0;
+      for (int i0 = 0; i0 < n; i0 += THREADS) {
+        int begin, rows = 0;
+        if (i0 + (int)threadIdx.x < n) group_range(g.offsets, i0 + threadIdx.x, g.R, begin, rows);
+        busy += __syncthreads_count(rows > 0);
+      }
+      if (g.R < 128 * busy) cap = 128;
+    }
     for (int i0 = 0; i0 < n; i0 += THREADS) {
       const int i = i0 + threadIdx.x;
       int b = 0;
       if (i < n) {
         int begin, rows;
         group_range(g.offsets, i, g.R, begin, rows);
-        b = DW ? tb : (rows + 255) / 256;
-        wide |= DW || rows > 128;
+        b = DW ? tb : (rows + cap - 1) / cap;
+        wide |= DW || (cap > 128 && rows > 128);
       }
       int all;
       const int at = total + scan_before(b, sums, all);
@@ -263,7 +276,7 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
           c = rows;
           b = tb;
         } else {
-          const Widths w(rows);
+          const Widths w(rows, 256);
           c = (i & 1) ? w.last : w.count > 1 ? w.full : 0;
           b = w.count == 0 ? 0 : (i & 1) ? 1 : w.count - 1;
         }
@@ -303,6 +316,7 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
   tab.nsub = WIDE_FROM > 0 && (int64_t)total * p256 >= (int64_t)WIDE_FROM * pairs ? 2 : 1;
   tab.panels = tab.nsub == 2 ? (g.DA + 511) / 512 : p256;
   tab.kps = tab.nsub == 1 && !wide ? 2 : 1;
+  tab.cap = cap;
   return tab;
 }
 
@@ -397,12 +411,13 @@ __global__ void __launch_bounds__(THREADS, 1)
   // A stage: the panel's K-blocks (or halves), then the columns'.
   const int stages = tab.nsub + kps == 3 ? 4 : 6;
   const int a_bytes = tab.nsub * kps * L::SUB, stage_bytes = a_bytes + L::SUB;
-  // The i-th tile of this pair, for a whole warp; e < 0 after the last.
+  // The i-th tile of this pair, for a whole warp; e is -1 after the last, and -2
+  // where the wait for it ran out.
   auto next_tile = [&](int i) {
     const int at = i % L::TILES;
     Tile x;
     if (__all_sync(0xffffffffu, mbar_wait(&tile_full[at], i / L::TILES & 1, ctx, SITE_TILE))) x = uniform(s_tiles[at]);
-    else x.e = -1;
+    else x.e = -2;
     __syncwarp();
     if (lane == 0) mbar_arrive(&tile_empty[at]);
     return x;
@@ -419,7 +434,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t tail_mine0 = mapa_shared(smem_u32(&tail_full[0]), rank);
     for (int i = 0; ok; ++i) {
       const Tile x = next_tile(i);
-      if (x.e < 0) break;
+      if (x.e < 0) {
+        ok = x.e == -1;
+        break;
+      }
       const int half = x.width / 2;
       const int a0 = x.a0 + (int)rank * 128, b0 = x.b0 + (int)rank * half;
       const uint32_t block_bytes = x.nsub * L::SUB + half * 128;
@@ -550,7 +568,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       for (int i = 0; ok; ++i) {
         const Tile x = next_tile(i);
-        if (x.e < 0) break;
+        if (x.e < 0) {
+          ok = x.e == -1;
+          break;
+        }
         const uint32_t idesc = IDESC | (uint32_t)(x.width >> 3) << 17;
         for (int kb = 0; kb < x.blocks; kb += kps) {
           const int left = DW ? x.rows - kb * EPB : 0;  // dw: rows of the group in this stage and later
@@ -795,7 +816,6 @@ int launch(const GroupedProblem& p) {
   g.w_scale = p.w_scale;
   g.bias = p.bias;
   g.pdl = pdl_enabled() ? 1 : 0;
-
   g.sort = p.R >= SORT_ROWS && (DW ? p.E : 2 * p.E) <= SORT_LIMIT;
   CUtensorMap tA, tB, tC;
   ColumnMaps tBs;
@@ -810,7 +830,7 @@ int launch(const GroupedProblem& p) {
         (rc = map2(&tBs.box[1], p.X, type, ES, p.R, p.K, p.ldx, 32, EPB, 128)) ||
         (rc = map2(&tBs.box[2], p.X, type, ES, p.R, p.K, p.ldx, 16, EPB, 128)))
       return rc;
-    tiles = (p.N + 255) / 256 * (p.R / 256 + std::min(p.E, p.R));  // at most
+    tiles = (p.N + 255) / 256 * (p.R / 128 + std::min(p.E, p.R));  // at most
   } else {
     // The contiguous dimension of dW is X's (RC) or dY's (RR) columns.
     const void* a = p.kn ? p.W : p.X;

@@ -73,11 +73,13 @@ def route_backward(logits, routing, dweights, renormalize=True, stream=None):
     return d
 
 
-def _check_slots(what, slots, T, dev):
+def _check_slots(what, slots, dev, T=None):
+    """(T, k) of slots, whose tokens are T if that is given."""
     tensor(what, "slots", slots, 2, _I32, dev)
-    k = slots.shape[1]
-    dense(what, "slots", slots, (T, k), _I32, dev)
-    return k
+    shape = tuple(slots.shape)
+    if not slots.is_contiguous() or (T is not None and shape[0] != T):
+        raise bad("%s: slots must be a contiguous tensor of [%s, k], got %s" % (what, "T" if T is None else T, shape))
+    return shape
 
 
 def dispatch(x, slots, rows=None, stream=None):
@@ -87,7 +89,7 @@ def dispatch(x, slots, rows=None, stream=None):
     what = "dispatch"
     dev = tensor(what, "x", x, 2, _FLOATS)
     T, H = x.shape
-    k = _check_slots(what, slots, T, dev)
+    k = _check_slots(what, slots, dev, T)[1]
     if elsewhere(dev, stream):
         with on(dev, stream):
             return dispatch(x, slots, rows)
@@ -104,9 +106,7 @@ def combine(ys, slots, weights=None, stream=None):
     what = "combine"
     dev = tensor(what, "ys", ys, 2, _FLOATS)
     R, H = ys.shape
-    tensor(what, "slots", slots, 2, _I32, dev)
-    T = slots.shape[0]
-    k = _check_slots(what, slots, T, dev)
+    T, k = _check_slots(what, slots, dev)
     if weights is not None:
         dense(what, "weights", weights, (T, k), _F32, dev)
     if elsewhere(dev, stream):
@@ -128,7 +128,7 @@ def combine_backward(dy, ys, slots, weights, stream=None):
     R = ys.shape[0]
     if ys.shape[1] != H:
         raise bad("combine_backward: dy has rows of %d, ys of %d" % (H, ys.shape[1]))
-    k = _check_slots(what, slots, T, dev)
+    k = _check_slots(what, slots, dev, T)[1]
     dense(what, "weights", weights, (T, k), _F32, dev)
     if elsewhere(dev, stream):
         with on(dev, stream):
@@ -189,7 +189,6 @@ def gemm_grouped_dw(X, dY, offsets, dW=None, opmode="RC", stream=None):
     N = dY.shape[1]
     tensor(what, "offsets", offsets, 1, _I32, dev)
     E = offsets.shape[0] - 1
-    dense(what, "offsets", offsets, (E + 1,), _I32, dev)
     shape = (E, N, K) if m == "RC" else (E, K, N)
     if dW is not None:
         dense(what, "dW", dW, shape, (X.dtype,), dev)

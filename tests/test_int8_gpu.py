@@ -103,6 +103,17 @@ def i8_bound(y, size, dtype):
     return UNIT[name] * (y.abs() + size * 2.0 ** -21) + size * 2.0 ** -21 + TINY[name]
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("M,K", [(1024, 8), (1025, 250), (1030, 256), (1100, 520), (2000, 1024), (1027, 2048), (1500, 2056)])
+def test_quantize_many_rows(cuda, M, K, dtype):
+    import kebab_b200 as kb
+    x = randn((M, K), dtype_of(dtype), M + K)
+    q, scale = kb.quantize_i8(x)
+    wq, ws = quantize_plain(x.float().cpu().numpy())
+    np.testing.assert_array_equal(q.cpu().numpy(), wq)
+    np.testing.assert_array_equal(scale.cpu().numpy(), ws)
+
+
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
 @pytest.mark.parametrize("M,N,K", [(1, 8, 16), (1, 513, 1024), (2, 256, 8192), (4, 1000, 2064), (7, 129, 160), (8, 512, 512),
                                    (9, 640, 4096), (16, 1, 32), (31, 257, 528), (64, 1024, 2048), (65, 384, 272),
