@@ -14,8 +14,12 @@
 // accumulator then has two K-blocks' MMAs of the other half (1024 cycles)
 // between its last MMA and the next tile's first, in which the 8 epilogue warps
 // read it into registers (as pairs of outputs) and hand it back; they store
-// afterwards. Without the lag the issuer waited 4300 of 36800 cycles a tile
-// (2048 terms).
+// afterwards. One half at a time, in a loop: unrolled over both, the epilogue
+// was bound by fetching its instructions (dw of 352 rows over 108 experts, 2552
+// x 2648, all stores: 1000 us against 635). Tiles of 16 K-blocks or more store
+// by TMA, whose pace leaves the operands' copies alone: 32768 x 8192 x 4096 over
+// 8 groups 1757 us against 1810 with stores from registers, which shorter tiles
+// use (the 635 us would be 1000).
 //
 // Ragged sizes cost what they are: a forward tile is as wide as its rows need
 // (a multiple of 32; N is a field of the instruction descriptor), a group of
@@ -58,7 +62,7 @@ struct TileArgs {
   int DA;      // extent of the MMA-row side: N (forward) or dW's contiguous dimension
   int DB;      // dw: the other dimension of dW
   int K;       // forward: contraction length
-  int tma_out;
+  int vec_out;  // rows of Y on 16-byte boundaries
   void* Y;
   int64_t ldy;
   const float* scale;
@@ -74,13 +78,15 @@ constexpr int THREADS = 352;
 // fewer takes about as long as its weights' bytes in any order), and up to 512
 // entries (the ranks take entries^2 / 352 comparisons a thread).
 constexpr int SORT_ROWS = 2048, SORT_LIMIT = 512;
+// K-blocks of a tile from which its stores go by TMA.
+constexpr int PACED_FROM = 16;
 
 struct GSmem {
   static constexpr int SUB = 128 * 128;  // 128 rows of 128 bytes: one K-block of one operand
   static constexpr int RING = 12 * SUB;
   static constexpr int MAX_STAGES = 6;
   static constexpr int OFF_C = RING;
-  static constexpr int C_SUB = 32 * 32 * 2;
+  static constexpr int C_SUB = 32 * 32 * 2 + 128 * 4;  // an epilogue warp's: 32 columns of 32 values, 128 scales
   static constexpr int OFF_BAR = OFF_C + 8 * C_SUB;
   // full, empty, tail_full, tail_done a stage; tmem_full and tmem_empty twice; drain
   static constexpr int TILES = 4;  // descriptions of tiles in flight: full and empty each
@@ -238,16 +244,26 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
   int total = 0;
   int cap = 256;
   if (!sorted) {
-    // Few rows a group: tiles of at most 128 columns keep two K-blocks a stage
-    // for all, and the weights of the few larger groups come twice, from L2.
+    // The widest tile of 256, 192 or 128 columns, by the waves over the pairs and
+    // the rows that a tile's K-block copies (256 of the panel and its columns,
+    // which take as long as its MMAs or longer). 128 also keeps two K-blocks a
+    // stage. 1267 rows over 3 groups, 3320 x 5224: 76 us
+    // with 256 (78 tiles on 74 pairs), 68 so.
     if constexpr (!DW) {
-      int busy = 0;
+      int c256 = 0, c192 = 0, c128 = 0;
       for (int i0 = 0; i0 < n; i0 += THREADS) {
-        int begin, rows = 0;
+        int begin, rows = 0, two, one;
         if (i0 + (int)threadIdx.x < n) group_range(g.offsets, i0 + threadIdx.x, g.R, begin, rows);
-        busy += __syncthreads_count(rows > 0);
+        scan_before((rows + 255) / 256 << 16 | (rows + 191) / 192, sums, two);
+        scan_before((rows + 127) / 128, sums, one);
+        c256 += two >> 16;
+        c192 += two & 0xffff;
+        c128 += one;
       }
-      if (g.R < 128 * busy) cap = 128;
+      const int panels = (g.DA + 255) / 256;
+      auto cost = [&](int blocks, int width) { return (int64_t)((blocks * panels + pairs - 1) / pairs) * (256 + width); };
+      if (cost(c192, 192) < cost(c256, 256)) cap = 192;
+      if (cost(c128, 128) <= min(cost(c192, 192), cost(c256, 256))) cap = 128;
     }
     for (int i0 = 0; i0 < n; i0 += THREADS) {
       const int i = i0 + threadIdx.x;
@@ -369,7 +385,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
-    tma_prefetch_desc(&tmC);
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -649,8 +664,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     // -------------------------------------------------------------- epilogue
     const int q = warp & 3;             // TMEM lane quarter this warp may access
     const int side = (warp - 2) / 4;    // which half of a tile's columns it takes
-    uint16_t* stage_c = reinterpret_cast<uint16_t*>(smem + L::OFF_C + (warp - 2) * L::C_SUB);
-    int sub = 0;
+    uint32_t* stage_c = reinterpret_cast<uint32_t*>(smem + L::OFF_C + (warp - 2) * L::C_SUB);  // [16 pairs][32 values]
+    float* s_scale = reinterpret_cast<float*>(stage_c + 16 * 32);
     const uint32_t tmem_empty_leader0 = mapa_shared(smem_u32(&tmem_empty[0]), 0);
     const uint32_t t_quarter = tmem_base + ((uint32_t)(q * 32) << 16);
     uint32_t halves = 0;
@@ -659,26 +674,23 @@ __global__ void __launch_bounds__(THREADS, 1)
       const Tile x = next_tile(i);
       if (x.e < 0) break;
       const int limit = DW ? g.DB : x.rows;  // columns end here
-      const int chunks = x.width / 32;       // of 16 columns, of this warp
-      const int d0 = side * chunks * 16;     // its first column in the tile
-      const int a_warp0 = x.a0 + (int)rank * 128 + q * 32;
-      const bool some = x.blocks != 0;  // dw of a group without rows: zeros
-      float sx[4];                      // 8-bit: sx[c] is the scale of column d0 + 32 c + lane
+      const int cols = x.width / 2;          // of this warp, a multiple of 16
+      const int d0 = side * cols;            // its first column in the tile
+      const bool some = x.blocks != 0;       // dw of a group without rows: zeros
       if constexpr (I8) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int b = x.b0 + d0 + c * 32 + lane;
-          sx[c] = 2 * c < chunks && b < limit ? g.scale[x.begin + b] : 0.f;
+        __syncwarp();
+        for (int c = lane; c < cols; c += 32) {
+          const int b = x.b0 + d0 + c;
+          s_scale[c] = b < limit ? g.scale[x.begin + b] : 0.f;
         }
+        __syncwarp();
       }
-      // out[s][c][j]: columns 16 c + 2 j and the next of this thread's row of half s, as outputs.
-      uint32_t out[2][8][8];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (s >= x.nsub || !ok) break;
+#pragma unroll 1
+      for (int s = 0; s < x.nsub; ++s) {
+        const int a_warp = x.a0 + s * 256 + (int)rank * 128 + q * 32;  // this warp's first row of the half
         float sw = 0.f, bias = 0.f;
         if constexpr (I8) {
-          const int a = a_warp0 + s * 256 + lane;
+          const int a = a_warp + lane;
           if (a < g.DA) {
             sw = g.w_scale[(int64_t)x.e * g.DA + a];
             if (g.bias) bias = (float)static_cast<const TO*>(g.bias)[a];
@@ -691,31 +703,26 @@ __global__ void __launch_bounds__(THREADS, 1)
           ++halves;
           tc_fence_after();
         }
-        // The sum of column `col` of 32, of which lane j of `scales` has column j's scale.
-        auto value = [&](uint32_t v, float scales, int col) {
-          if constexpr (I8) return (float)(int)v * (sw * __shfl_sync(0xffffffffu, scales, col)) + bias;
-          else return __uint_as_float(v);
-        };
-        const uint32_t src = t_quarter + slot * 256 + (uint32_t)d0;
+        // Columns 32 c + 2 j and the next of this thread's row, as outputs (an odd
+        // last run of 16 is read as 32; what is past it is not used).
+        uint32_t out[4][16];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (2 * c >= chunks) break;
-          // With an odd number of chunks the last 16 columns are not this warp's, and not used.
-          uint32_t v[2][16];
+          if (c * 32 >= cols) break;
+          uint32_t v[32];
           if (some) {
-            tmem_ld_32x32b_x16(src + c * 32, v[0]);
-            tmem_ld_32x32b_x16(src + c * 32 + 16, v[1]);
+            tmem_ld_32x32b_x32(t_quarter + slot * 256 + (uint32_t)(d0 + c * 32), v);
             tmem_ld_wait();
           } else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[0][j] = v[1][j] = 0u;
+            for (int j = 0; j < 32; ++j) v[j] = 0u;
+          }
+          if constexpr (I8) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint((float)(int)v[j] * (sw * s_scale[c * 32 + j]) + bias);
           }
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              out[s][2 * c + u][j] =
-                  pack2(TO(), value(v[u][2 * j], sx[c], u * 16 + 2 * j), value(v[u][2 * j + 1], sx[c], u * 16 + 2 * j + 1));
+          for (int j = 0; j < 16; ++j) out[c][j] = pack2(TO(), __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
         }
         if (some) {
           // This warp's share read: hand it back to the MMA issuer.
@@ -723,50 +730,75 @@ __global__ void __launch_bounds__(THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(tmem_empty_leader0 + slot * 8u);
         }
-      }
-      if (!ok) break;
+        if (a_warp >= g.DA) continue;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int a_warp = a_warp0 + s * 256;
-        if (s >= x.nsub || a_warp >= g.DA) break;
+        for (int c = 0; c < 4; ++c) {
+          const int b = x.b0 + d0 + c * 32;
+          const int n = min(min(32, cols - c * 32), limit - b);  // columns to store
+          if (n <= 0) break;
+          uint16_t* y = static_cast<uint16_t*>(g.Y) +
+                        (DW ? (int64_t)x.e * g.DB + b : (int64_t)x.begin + b) * g.ldy + a_warp;
+          if (g.vec_out && x.blocks >= PACED_FROM && n == 32) {
+            // 16 columns at a time by TMA, staged in two buffers in turn.
+            uint16_t* b16 = reinterpret_cast<uint16_t*>(stage_c);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const int b = x.b0 + d0 + c * 16;
-          if (c >= chunks || b >= limit) break;
-          uint16_t* buf = stage_c + (sub & 1) * (16 * 32);
-          ++sub;
-          if (lane == 0) tma_store_wait_read<1>();  // the store that used `buf` has read it
-          __syncwarp();
+            for (int u = 0; u < 2; ++u, b16 += 16 * 32) {
+              if (lane == 0) tma_store_wait_read<1>();  // the store that used this buffer has read it
+              __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t two = out[s][c][j];
-            buf[(2 * j) * 32 + lane] = (uint16_t)(two & 0xFFFFu);
-            buf[(2 * j + 1) * 32 + lane] = (uint16_t)(two >> 16);
-          }
-          if (g.tma_out && (DW || b + 16 <= limit)) {
-            fence_proxy_async_smem();
+              for (int j = 0; j < 8; ++j) {
+                const uint32_t two = out[c][u * 8 + j];
+                b16[(2 * j) * 32 + lane] = (uint16_t)(two & 0xFFFFu);
+                b16[(2 * j + 1) * 32 + lane] = (uint16_t)(two >> 16);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                if constexpr (DW) tma_store_3d(&tmC, b16, a_warp, b + u * 16, x.e);
+                else tma_store_2d(&tmC, b16, a_warp, x.begin + b + u * 16);
+                tma_store_commit();
+              }
+            }
+          } else if (g.vec_out) {
+            if (lane == 0) tma_store_wait_read<0>();
+            // Transposed through shared memory as pairs of columns: a lane reads 8
+            // rows of a pair and stores 16 bytes of each column.
+            __syncwarp();  // the run before has been read
+#pragma unroll
+            for (int j = 0; j < 16; ++j) stage_c[j * 32 + lane] = out[c][j];
             __syncwarp();
-            if (lane == 0) {
-              if constexpr (DW) tma_store_3d(&tmC, buf, a_warp, b, x.e);
-              else tma_store_2d(&tmC, buf, a_warp, x.begin + b);
+            const int a = lane % 4 * 8;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int pair = u * 8 + lane / 4;
+              const uint4 l = *reinterpret_cast<const uint4*>(stage_c + pair * 32 + a);
+              const uint4 h = *reinterpret_cast<const uint4*>(stage_c + pair * 32 + a + 4);
+              uint16_t* to = y + (2 * pair) * g.ldy + a;
+              if (a_warp + a < g.DA) {
+                if (2 * pair < n)
+                  *reinterpret_cast<uint4*>(to) =
+                      make_uint4(__byte_perm(l.x, l.y, 0x5410), __byte_perm(l.z, l.w, 0x5410),
+                                 __byte_perm(h.x, h.y, 0x5410), __byte_perm(h.z, h.w, 0x5410));
+                if (2 * pair + 1 < n)
+                  *reinterpret_cast<uint4*>(to + g.ldy) =
+                      make_uint4(__byte_perm(l.x, l.y, 0x7632), __byte_perm(l.z, l.w, 0x7632),
+                                 __byte_perm(h.x, h.y, 0x7632), __byte_perm(h.z, h.w, 0x7632));
+              }
             }
           } else if (a_warp + lane < g.DA) {
-            // The group ends inside the chunk (the next rows are another
-            // group's), or TMA cannot address Y: 64 bytes a warp and column.
-            // Every thread reads what it wrote.
-            uint16_t* y = static_cast<uint16_t*>(g.Y) +
-                          (DW ? (int64_t)x.e * g.DB + b : (int64_t)x.begin + b) * g.ldy + a_warp + lane;
-            const int n = min(16, limit - b);
-#pragma unroll 4
-            for (int j = 0; j < n; ++j) y[j * g.ldy] = buf[j * 32 + lane];
+            // Rows of Y on odd boundaries: 64 bytes a column and warp.
+            y += lane;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              if (2 * j < n) y[(2 * j) * g.ldy] = (uint16_t)(out[c][j] & 0xFFFFu);
+              if (2 * j + 1 < n) y[(2 * j + 1) * g.ldy] = (uint16_t)(out[c][j] >> 16);
+            }
           }
-          if (lane == 0) tma_store_commit();
         }
       }
     }
     // The CTA may exit once its last stores have read their staging buffers.
     if (lane == 0) tma_store_wait_read<0>();
-    __syncwarp();
   }
 
   // ------------------------------------------------------------- teardown
@@ -817,7 +849,7 @@ int launch(const GroupedProblem& p) {
   g.bias = p.bias;
   g.pdl = pdl_enabled() ? 1 : 0;
   g.sort = p.R >= SORT_ROWS && (DW ? p.E : 2 * p.E) <= SORT_LIMIT;
-  CUtensorMap tA, tB, tC;
+  CUtensorMap tA, tB;
   ColumnMaps tBs;
   int64_t tiles;
   if constexpr (!DW) {
@@ -846,11 +878,14 @@ int launch(const GroupedProblem& p) {
     tiles = p.E * ((g.DA + 255) / 256) * ((g.DB + 255) / 256);
   }
   if (tiles > INT32_MAX / 2) return fail(KEBAB_EINVAL, "grouped product: too many tiles");
-  g.tma_out = (reinterpret_cast<uintptr_t>(p.Y) & 15u) == 0 && g.ldy % 8 == 0;
-  if (!g.tma_out) tC = tA;  // not used
-  else if (DW) rc = map3(&tC, p.Y, p.out, 2, p.E, g.DB, g.DA, g.ldy, g.ldy * g.DB, 16, 32, 0);
-  else rc = map2(&tC, p.Y, p.out, 2, p.R, p.N, p.ldy, 16, 32, 0);
-  if (rc) return rc;
+  // Whole runs of 8 (DA too: a run stays within its row).
+  CUtensorMap tC = tA;  // not used unless vec_out
+  g.vec_out = (reinterpret_cast<uintptr_t>(p.Y) & 15u) == 0 && g.ldy % 8 == 0 && g.DA % 8 == 0;
+  if (g.vec_out) {
+    if (DW) rc = map3(&tC, p.Y, p.out, 2, p.E, g.DB, g.DA, g.ldy, g.ldy * g.DB, 16, 32, 0);
+    else rc = map2(&tC, p.Y, p.out, 2, p.R, p.N, p.ldy, 16, 32, 0);
+    if (rc) return rc;
+  }
 
   auto kern = grouped_umma_kernel<TO, I8, MODE>;
   const int smem = GSmem::bytes(g.E) + 1024;

@@ -1,11 +1,11 @@
 // Quantisation of rows to 8-bit integers with one scale a row.
 //
-// One block a row, or (rows of up to 2048) one warp: the row is read once, 16 bytes a thread and step, and kept
-// in registers as it is stored while they find its largest magnitude (as
-// the largest bit pattern of |x|, so that a NaN stands above everything and is
-// not lost); the codes are then made from the registers. Rows longer than the
-// registers hold are read a second time, from L2. Bound by memory: 2 bytes read
-// and 1 written for each 16-bit value; 4093 x 8192 BF16 17.5 us, 5.7 TB/s (26.6
+// One block a row, or (rows of up to 2048) one warp: the row is read once, 16
+// bytes a thread and step, and kept in registers as it is stored while they find
+// its largest magnitude (as the largest bit pattern of |x|, so that a NaN stands
+// above everything and is not lost); the codes are then made from the registers.
+// Rows longer than the registers hold are read a second time, from L2. Bound by
+// memory: 2 bytes read and 1 written for each 16-bit value; 4093 x 8192 BF16 17.5 us, 5.7 TB/s (26.6
 // with conversion instructions and 8 warps a row), 30000 x 520 13 us (31 with
 // a block a row).
 //
