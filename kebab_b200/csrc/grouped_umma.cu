@@ -12,14 +12,14 @@
 // turns on two accumulators of up to 256 columns. With 512-row panels both are
 // in use at once, so the second half runs one K-block behind the first: each
 // accumulator then has two K-blocks' MMAs of the other half (1024 cycles)
-// between its last MMA and the next tile's first, in which the 8 epilogue warps
-// read it into registers (as pairs of outputs) and hand it back; they store
+// between its last MMA and the next tile's first, in which 8 epilogue warps read
+// it into registers (as pairs of outputs) and hand it back; they store
 // afterwards. One half at a time, in a loop: unrolled over both, the epilogue
 // was bound by fetching its instructions (dw of 352 rows over 108 experts, 2552
-// x 2648, all stores: 1000 us against 635). Tiles of 16 K-blocks or more store
-// by TMA, whose pace leaves the operands' copies alone: 32768 x 8192 x 4096 over
-// 8 groups 1757 us against 1810 with stores from registers, which shorter tiles
-// use (the 635 us would be 1000).
+// x 2648: 1000 us against 656). Tiles of 16 K-blocks or more store by TMA, whose
+// pace leaves the operands' copies alone: 32768 x 8192 x 4096 over 8 groups 1757
+// us against 1810 with stores from registers. Shorter ones store from registers
+// (the dw above, now 578 us, takes 618 by TMA).
 //
 // Ragged sizes cost what they are: a forward tile is as wide as its rows need
 // (a multiple of 32; N is a field of the instruction descriptor), a group of
@@ -39,8 +39,8 @@
 // 8-bit elements) of a 512-row panel and its columns, or two K-blocks of a
 // 256-row panel where no tile is wider than 128 columns (few rows: bound by the
 // weights' bytes, and 256 contiguous bytes a weight row and stage are fetched
-// faster than 128); else 6 stages of 32 KB. Warps: TMA producer, MMA issuer,
-// 8 epilogue warps, and one that works out the tiles ahead of them (finding a
+// faster than 128); else 6 stages of 32 KB. Warps: TMA producer, MMA issuer, 8
+// or (dw) 16 epilogue warps, and one that works out the tiles ahead of them (finding a
 // tile's place takes about 2000 cycles, as long as 16 MMAs).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -70,32 +70,50 @@ struct TileArgs {
   const void* bias;
   int pdl;
   int sort;
+  int entries;  // of the table of tiles
   WaitCtx ctx;
 };
 
-constexpr int THREADS = 352;
+// Epilogue warps: a set of 8 that takes every half in turn, or (dw) one for each
+// accumulator. dw's contraction is short and its outputs many, so that what the
+// epilogue takes to store a half would delay its reading of the next: 16384 x
+// 4096 x 2048, burst, 1024 rows a group 207 us against 222 with one set, 256 rows
+// 378 against 405. The forward tiles are longer, and the registers that a thread
+// then has too few: 32768 x 8192 x 4096 over 8 groups 1808 us with one, 1853 with
+// two.
+template <int MODE>
+struct Warps {
+  static constexpr int SETS = MODE == MODE_DW ? 2 : 1;
+  static constexpr int EPILOGUE = 8 * SETS;
+  static constexpr int THREADS = 32 * (EPILOGUE + 3);  // and producer, issuer, tiles
+};
 // Tiles are sorted by cost where that can pay: from 2048 rows (a product of
 // fewer takes about as long as its weights' bytes in any order), and up to 512
-// entries (the ranks take entries^2 / 352 comparisons a thread).
+// entries (the ranks take entries^2 / 352 (dw 608) comparisons a thread).
 constexpr int SORT_ROWS = 2048, SORT_LIMIT = 512;
 // K-blocks of a tile from which its stores go by TMA.
 constexpr int PACED_FROM = 16;
 
+template <int SETS>
 struct GSmem {
   static constexpr int SUB = 128 * 128;  // 128 rows of 128 bytes: one K-block of one operand
   static constexpr int RING = 12 * SUB;
   static constexpr int MAX_STAGES = 6;
   static constexpr int OFF_C = RING;
-  static constexpr int C_SUB = 32 * 32 * 2 + 128 * 4;  // an epilogue warp's: 32 columns of 32 values, 128 scales
-  static constexpr int OFF_BAR = OFF_C + 8 * C_SUB;
+  static constexpr int RUN = 32 / SETS;  // columns that an epilogue warp stores at a time
+  static constexpr int C_SUB = RUN * 32 * 2 + 128 * 4;  // its: a run of columns of 32 values, 128 scales
+  static constexpr int OFF_BAR = OFF_C + 8 * SETS * C_SUB;
   // full, empty, tail_full, tail_done a stage; tmem_full and tmem_empty twice; drain
   static constexpr int TILES = 4;  // descriptions of tiles in flight: full and empty each
   static constexpr int NUM_BARS = 4 * MAX_STAGES + 5 + 2 * TILES;
   static constexpr int OFF_TILES = (OFF_BAR + NUM_BARS * 8 + 4 + 15) / 16 * 16;
   static constexpr int OFF_TABLE = OFF_TILES + TILES * 32;
-  // first[entries + 1] (int), entry[entries] (uint16, sorted only), entries <= 2 E
-  static constexpr int bytes(int E) { return OFF_TABLE + (2 * E + 1) * 4 + 2 * E * 2; }
-  static constexpr int ALLOC = OFF_TABLE + (2 * kMaxExperts + 1) * 4 + 2 * kMaxExperts * 2 + 1024;
+  // first[entries + 1] (int), entry[entries] (uint16, sorted only)
+  static constexpr int bytes(int entries, bool sorted) {
+    return OFF_TABLE + (entries + 1) * 4 + (sorted ? entries * 2 : 0) + 1024;
+  }
+  static constexpr int ALLOC =
+      OFF_TABLE + std::max((kMaxExperts + 1) * 4, (SORT_LIMIT + 1) * 4 + SORT_LIMIT * 2) + 1024;
   static_assert(ALLOC <= 232448, "shared memory budget exceeded");
 };
 
@@ -202,6 +220,7 @@ __device__ __forceinline__ Tile uniform(const Tile& x) {
 }
 
 // Block-wide sum of one value a thread before this thread's; `total` of all.
+template <int THREADS>
 __device__ __forceinline__ int scan_before(int v, int* sums, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int at = v;
@@ -224,10 +243,11 @@ __device__ __forceinline__ int scan_before(int v, int* sums, int& total) {
   return before + at - v;
 }
 
-// Makes the table, by all threads of the CTA. `scratch`: 3 ints an entry and 16.
+// Makes the table, by all threads of the CTA. `scratch`: 3 ints an entry and 32.
 template <int MODE, bool I8>
 __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* first, uint16_t* entry, int* scratch) {
   constexpr bool DW = MODE == MODE_DW;
+  constexpr int THREADS = Warps<MODE>::THREADS;
   // 512-row panels from this many 256-row tiles a pair (0: never). Measured
   // under the power cap, us: forward 16381 x 4096 x 2048 over 14 uneven groups
   // (15 tiles a pair) 245 against 252; dw with 7 tiles a pair (4 groups of 8192
@@ -235,11 +255,11 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
   // issue is as long as its MMAs. 8-bit: 4093 x 28672 x 8192 735 against 682
   // (the epilogue, which scales every sum, stands between two tiles' MMAs).
   constexpr int WIDE_FROM = I8 ? 0 : DW ? 4 : 8;
-  int* sums = scratch;  // [16]
-  int* cost = scratch + 16;
+  int* sums = scratch;  // [32]
+  int* cost = scratch + 32;
   const int tb = (g.DB + 255) / 256;
   const bool sorted = g.sort;
-  const int n = DW || !sorted ? g.E : 2 * g.E;
+  const int n = g.entries;
   int wide = 0;  // some tile of more than 128 columns
   int total = 0;
   int cap = 256;
@@ -247,15 +267,15 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
     // The widest tile of 256, 192 or 128 columns, by the waves over the pairs and
     // the rows that a tile's K-block copies (256 of the panel and its columns,
     // which take as long as its MMAs or longer). 128 also keeps two K-blocks a
-    // stage. 1267 rows over 3 groups, 3320 x 5224: 76 us
-    // with 256 (78 tiles on 74 pairs), 68 so.
+    // stage. 1267 rows over 3 groups, 3320 x 5224: 76 us with 256
+    // (78 tiles on 74 pairs), 68 so.
     if constexpr (!DW) {
       int c256 = 0, c192 = 0, c128 = 0;
       for (int i0 = 0; i0 < n; i0 += THREADS) {
         int begin, rows = 0, two, one;
         if (i0 + (int)threadIdx.x < n) group_range(g.offsets, i0 + threadIdx.x, g.R, begin, rows);
-        scan_before((rows + 255) / 256 << 16 | (rows + 191) / 192, sums, two);
-        scan_before((rows + 127) / 128, sums, one);
+        scan_before<THREADS>((rows + 255) / 256 << 16 | (rows + 191) / 192, sums, two);
+        scan_before<THREADS>((rows + 127) / 128, sums, one);
         c256 += two >> 16;
         c192 += two & 0xffff;
         c128 += one;
@@ -275,7 +295,7 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
         wide |= DW || (cap > 128 && rows > 128);
       }
       int all;
-      const int at = total + scan_before(b, sums, all);
+      const int at = total + scan_before<THREADS>(b, sums, all);
       if (i < n) first[i] = at;
       total += all;
     }
@@ -317,7 +337,7 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
     for (int i0 = 0; i0 < n; i0 += THREADS) {
       const int i = i0 + threadIdx.x;
       int all;
-      const int at = total + scan_before(i < n ? by_rank[i] : 0, sums, all);
+      const int at = total + scan_before<THREADS>(i < n ? by_rank[i] : 0, sums, all);
       if (i < n) first[i] = at;
       total += all;
     }
@@ -343,11 +363,12 @@ struct ColumnMaps {
 };
 
 template <typename TO, bool I8, int MODE>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     grouped_umma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ ColumnMaps tmBs, const __grid_constant__ CUtensorMap tmC,
                         const TileArgs g) {
-  using L = GSmem;
+  using W = Warps<MODE>;
+  using L = GSmem<W::SETS>;
   constexpr bool DW = MODE == MODE_DW;
   constexpr bool A_MN = MODE != MODE_RC, B_MN = DW;
   constexpr int EPB = I8 ? 128 : 64;  // elements of the contraction in a K-block
@@ -369,7 +390,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + L::NUM_BARS);
   Tile* s_tiles = reinterpret_cast<Tile*>(smem + L::OFF_TILES);
   int* s_first = reinterpret_cast<int*>(smem + L::OFF_TABLE);
-  uint16_t* s_entry = reinterpret_cast<uint16_t*>(s_first + 2 * g.E + 1);
+  uint16_t* s_entry = reinterpret_cast<uint16_t*>(s_first + g.entries + 1);
 
   // The shuffle tells the compiler that a warp takes one path. The producer and
   // the issuer run with all lanes, one of which is elected at each copy or MMA,
@@ -397,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int a = 0; a < L::TILES; ++a) {
       mbar_init(&tile_full[a], 1);
-      mbar_init(&tile_empty[a], 9 + (DW || leader ? 1 : 0));  // the warps that read descriptions
+      mbar_init(&tile_empty[a], W::EPILOGUE + 1 + (DW || leader ? 1 : 0));  // the warps that read descriptions
     }
     mbar_init(drain, 1);
     fence_barrier_init();
@@ -642,7 +663,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         mbar_wait(drain, 0, drain_ctx, SITE_DRAIN);
       }
     }
-  } else if (warp == 10) {
+  } else if (warp == W::EPILOGUE + 2) {
     // ------------------------------------------------------- tiles, in order
     const int num_tiles = s_first[tab.entries] * tab.panels;
     for (int i = 0;; ++i) {
@@ -663,9 +684,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else {
     // -------------------------------------------------------------- epilogue
     const int q = warp & 3;             // TMEM lane quarter this warp may access
-    const int side = (warp - 2) / 4;    // which half of a tile's columns it takes
-    uint32_t* stage_c = reinterpret_cast<uint32_t*>(smem + L::OFF_C + (warp - 2) * L::C_SUB);  // [16 pairs][32 values]
-    float* s_scale = reinterpret_cast<float*>(stage_c + 16 * 32);
+    const int side = (warp - 2) / 4 % 2;  // which half of a tile's columns it takes
+    const uint32_t set = (warp - 2) / 8;  // of two sets, the accumulator it reads
+    constexpr int RUN = L::RUN;
+    uint32_t* stage_c = reinterpret_cast<uint32_t*>(smem + L::OFF_C + (warp - 2) * L::C_SUB);  // [RUN / 2 pairs][32 values]
+    float* s_scale = reinterpret_cast<float*>(stage_c + RUN / 2 * 32);
     const uint32_t tmem_empty_leader0 = mapa_shared(smem_u32(&tmem_empty[0]), 0);
     const uint32_t t_quarter = tmem_base + ((uint32_t)(q * 32) << 16);
     uint32_t halves = 0;
@@ -687,6 +710,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
 #pragma unroll 1
       for (int s = 0; s < x.nsub; ++s) {
+        const uint32_t slot = (some ? halves : s) & 1u, use = halves >> 1;
+        if (some) ++halves;
+        if (W::SETS == 2 && slot != set) continue;
         const int a_warp = x.a0 + s * 256 + (int)rank * 128 + q * 32;  // this warp's first row of the half
         float sw = 0.f, bias = 0.f;
         if constexpr (I8) {
@@ -696,33 +722,33 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (g.bias) bias = (float)static_cast<const TO*>(g.bias)[a];
           }
         }
-        const uint32_t slot = halves & 1u;
         if (some) {
-          ok = all_ok(mbar_wait(&tmem_full[slot], halves >> 1 & 1u, ctx, SITE_TMEM_FULL));
+          ok = all_ok(mbar_wait(&tmem_full[slot], use & 1u, ctx, SITE_TMEM_FULL));
           if (!ok) break;
-          ++halves;
           tc_fence_after();
         }
-        // Columns 32 c + 2 j and the next of this thread's row, as outputs (an odd
+        // Columns RUN c + 2 j and the next of this thread's row, as outputs (an odd
         // last run of 16 is read as 32; what is past it is not used).
-        uint32_t out[4][16];
+        uint32_t out[128 / RUN][RUN / 2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c * 32 >= cols) break;
-          uint32_t v[32];
+        for (int c = 0; c < 128 / RUN; ++c) {
+          if (c * RUN >= cols) break;
+          uint32_t v[RUN];
           if (some) {
-            tmem_ld_32x32b_x32(t_quarter + slot * 256 + (uint32_t)(d0 + c * 32), v);
+            const uint32_t at = t_quarter + slot * 256 + (uint32_t)(d0 + c * RUN);
+            if constexpr (RUN == 32) tmem_ld_32x32b_x32(at, v);
+            else tmem_ld_32x32b_x16(at, v);
             tmem_ld_wait();
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0u;
+            for (int j = 0; j < RUN; ++j) v[j] = 0u;
           }
           if constexpr (I8) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint((float)(int)v[j] * (sw * s_scale[c * 32 + j]) + bias);
+            for (int j = 0; j < RUN; ++j) v[j] = __float_as_uint((float)(int)v[j] * (sw * s_scale[c * RUN + j]) + bias);
           }
 #pragma unroll
-          for (int j = 0; j < 16; ++j) out[c][j] = pack2(TO(), __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+          for (int j = 0; j < RUN / 2; ++j) out[c][j] = pack2(TO(), __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
         }
         if (some) {
           // This warp's share read: hand it back to the MMA issuer.
@@ -732,30 +758,30 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (a_warp >= g.DA) continue;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int b = x.b0 + d0 + c * 32;
-          const int n = min(min(32, cols - c * 32), limit - b);  // columns to store
+        for (int c = 0; c < 128 / RUN; ++c) {
+          const int b = x.b0 + d0 + c * RUN;
+          const int n = min(min(RUN, cols - c * RUN), limit - b);  // columns to store
           if (n <= 0) break;
           uint16_t* y = static_cast<uint16_t*>(g.Y) +
                         (DW ? (int64_t)x.e * g.DB + b : (int64_t)x.begin + b) * g.ldy + a_warp;
-          if (g.vec_out && x.blocks >= PACED_FROM && n == 32) {
-            // 16 columns at a time by TMA, staged in two buffers in turn.
+          if (g.vec_out && x.blocks >= PACED_FROM && n == RUN) {
+            // Half a run at a time by TMA, staged in two buffers in turn.
             uint16_t* b16 = reinterpret_cast<uint16_t*>(stage_c);
 #pragma unroll
-            for (int u = 0; u < 2; ++u, b16 += 16 * 32) {
+            for (int u = 0; u < 2; ++u, b16 += RUN / 2 * 32) {
               if (lane == 0) tma_store_wait_read<1>();  // the store that used this buffer has read it
               __syncwarp();
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const uint32_t two = out[c][u * 8 + j];
+              for (int j = 0; j < RUN / 4; ++j) {
+                const uint32_t two = out[c][u * (RUN / 4) + j];
                 b16[(2 * j) * 32 + lane] = (uint16_t)(two & 0xFFFFu);
                 b16[(2 * j + 1) * 32 + lane] = (uint16_t)(two >> 16);
               }
               fence_proxy_async_smem();
               __syncwarp();
               if (lane == 0) {
-                if constexpr (DW) tma_store_3d(&tmC, b16, a_warp, b + u * 16, x.e);
-                else tma_store_2d(&tmC, b16, a_warp, x.begin + b + u * 16);
+                if constexpr (DW) tma_store_3d(&tmC, b16, a_warp, b + u * (RUN / 2), x.e);
+                else tma_store_2d(&tmC, b16, a_warp, x.begin + b + u * (RUN / 2));
                 tma_store_commit();
               }
             }
@@ -765,11 +791,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             // rows of a pair and stores 16 bytes of each column.
             __syncwarp();  // the run before has been read
 #pragma unroll
-            for (int j = 0; j < 16; ++j) stage_c[j * 32 + lane] = out[c][j];
+            for (int j = 0; j < RUN / 2; ++j) stage_c[j * 32 + lane] = out[c][j];
             __syncwarp();
             const int a = lane % 4 * 8;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < RUN / 16; ++u) {
               const int pair = u * 8 + lane / 4;
               const uint4 l = *reinterpret_cast<const uint4*>(stage_c + pair * 32 + a);
               const uint4 h = *reinterpret_cast<const uint4*>(stage_c + pair * 32 + a + 4);
@@ -789,7 +815,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             // Rows of Y on odd boundaries: 64 bytes a column and warp.
             y += lane;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
+            for (int j = 0; j < RUN / 2; ++j) {
               if (2 * j < n) y[(2 * j) * g.ldy] = (uint16_t)(out[c][j] & 0xFFFFu);
               if (2 * j + 1 < n) y[(2 * j + 1) * g.ldy] = (uint16_t)(out[c][j] >> 16);
             }
@@ -833,6 +859,8 @@ template <typename TO, bool I8, int MODE>
 int launch(const GroupedProblem& p) {
   constexpr bool DW = MODE == MODE_DW;
   constexpr int EPB = I8 ? 128 : 64, ES = I8 ? 1 : 2;
+  using W = Warps<MODE>;
+  using L = GSmem<W::SETS>;
   const int type = I8 ? TMAP_U8 : p.in;
   int rc;
   DeviceInfo* dev = nullptr;
@@ -882,23 +910,24 @@ int launch(const GroupedProblem& p) {
   CUtensorMap tC = tA;  // not used unless vec_out
   g.vec_out = (reinterpret_cast<uintptr_t>(p.Y) & 15u) == 0 && g.ldy % 8 == 0 && g.DA % 8 == 0;
   if (g.vec_out) {
-    if (DW) rc = map3(&tC, p.Y, p.out, 2, p.E, g.DB, g.DA, g.ldy, g.ldy * g.DB, 16, 32, 0);
-    else rc = map2(&tC, p.Y, p.out, 2, p.R, p.N, p.ldy, 16, 32, 0);
+    if (DW) rc = map3(&tC, p.Y, p.out, 2, p.E, g.DB, g.DA, g.ldy, g.ldy * g.DB, L::RUN / 2, 32, 0);
+    else rc = map2(&tC, p.Y, p.out, 2, p.R, p.N, p.ldy, L::RUN / 2, 32, 0);
     if (rc) return rc;
   }
 
   auto kern = grouped_umma_kernel<TO, I8, MODE>;
-  const int smem = GSmem::bytes(g.E) + 1024;
+  g.entries = DW || !g.sort ? g.E : 2 * g.E;
+  const int smem = L::bytes(g.entries, g.sort);
   // Once per device and instantiation: the shared-memory opt-in and how many pairs fit.
   static std::once_flag once[64];
   static cudaError_t err[64];
   static int max_pairs[64];
   const int di = dev->device & 63;
   std::call_once(once[di], [&] {
-    err[di] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GSmem::ALLOC);
+    err[di] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC);
     max_pairs[di] = dev->sm_count / 2;
     if (err[di] != cudaSuccess) return;
-    PdlLaunch q(dim3(2 * max_pairs[di]), dim3(THREADS), GSmem::ALLOC, nullptr, 2);
+    PdlLaunch q(dim3(2 * max_pairs[di]), dim3(W::THREADS), L::ALLOC, nullptr, 2);
     q.cfg.numAttrs = 1;
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kern, &q.cfg) == cudaSuccess && n > 0) max_pairs[di] = std::min(n, max_pairs[di]);
@@ -906,8 +935,8 @@ int launch(const GroupedProblem& p) {
   });
   if (err[di] != cudaSuccess) return cuda_fail(err[di], "cudaFuncSetAttribute(max dynamic smem)");
   const int pairs = (int)std::min<int64_t>(tiles, max_pairs[di]);
-  PdlLaunch l(dim3(2 * pairs), dim3(THREADS), smem, p.stream, 2);
-  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, tA, tB, tBs, tC, g);
+  PdlLaunch ln(dim3(2 * pairs), dim3(W::THREADS), smem, p.stream, 2);
+  const cudaError_t e = cudaLaunchKernelEx(&ln.cfg, kern, tA, tB, tBs, tC, g);
   return e == cudaSuccess ? KEBAB_OK : cuda_fail(e, "grouped tcgen05 launch");
 }
 

@@ -5,9 +5,9 @@
 // its largest magnitude (as the largest bit pattern of |x|, so that a NaN stands
 // above everything and is not lost); the codes are then made from the registers.
 // Rows longer than the registers hold are read a second time, from L2. Bound by
-// memory: 2 bytes read and 1 written for each 16-bit value; 4093 x 8192 BF16 17.5 us, 5.7 TB/s (26.6
-// with conversion instructions and 8 warps a row), 30000 x 520 13 us (31 with
-// a block a row).
+// memory: 2 bytes read and 1 written for each 16-bit value; 4093 x 8192 BF16
+// 17.5 us, 5.7 TB/s (26.6 with conversion instructions and 8 warps a row), 30000
+// x 520 13 us (31 with a block a row).
 //
 // The code is x * (127 / amax), one multiplication by a once-rounded quotient:
 // a division of every value would cost about ten instructions each, and the
