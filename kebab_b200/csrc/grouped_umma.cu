@@ -85,11 +85,12 @@ template <int MODE>
 struct Warps {
   static constexpr int SETS = MODE == MODE_DW ? 2 : 1;
   static constexpr int EPILOGUE = 8 * SETS;
-  static constexpr int THREADS = 32 * (EPILOGUE + 3);  // and producer, issuer, tiles
+  static constexpr int TAIL = MODE == MODE_DW ? 1 : 0;         // the one that clears rows past a group's end
+  static constexpr int THREADS = 32 * (EPILOGUE + TAIL + 3);  // and producer, issuer, tiles
 };
 // Tiles are sorted by cost where that can pay: from 2048 rows (a product of
 // fewer takes about as long as its weights' bytes in any order), and up to 512
-// entries (the ranks take entries^2 / 352 (dw 608) comparisons a thread).
+// entries (the ranks take entries^2 / 352 (dw 640) comparisons a thread).
 constexpr int SORT_ROWS = 2048, SORT_LIMIT = 512;
 // K-blocks of a tile from which its stores go by TMA.
 constexpr int PACED_FROM = 16;
@@ -380,8 +381,8 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* empty = full + STAGES;
-  uint64_t* tail_full = empty + STAGES;  // dw, in the peer: its own bytes of a group's last stage
-  uint64_t* tail_done = tail_full + STAGES;  // dw, in the leader: the peer has cleared its share of it
+  uint64_t* tail_full = empty + STAGES;  // dw: this CTA's bytes of a group's last stage, where it is to be cleared
+  uint64_t* tail_done = tail_full + STAGES;  // dw, in the leader: both CTAs have cleared their shares of it
   uint64_t* tmem_full = tail_done + STAGES;
   uint64_t* tmem_empty = tmem_full + 2;
   uint64_t* drain = tmem_empty + 2;
@@ -410,7 +411,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
       mbar_init(&tail_full[s], 1);
-      mbar_init(&tail_done[s], 1);
+      mbar_init(&tail_done[s], 2);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tmem_full[a], 1);
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     }
     for (int a = 0; a < L::TILES; ++a) {
       mbar_init(&tile_full[a], 1);
-      mbar_init(&tile_empty[a], W::EPILOGUE + 1 + (DW || leader ? 1 : 0));  // the warps that read descriptions
+      mbar_init(&tile_empty[a], W::EPILOGUE + W::TAIL + 1 + (leader ? 1 : 0));  // the warps that read descriptions
     }
     mbar_init(drain, 1);
     fence_barrier_init();
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    uint32_t issued = 0, parity = 0;  // a bit a stage
+    uint32_t issued = 0, parity = 0, tails = 0, tail_parity = 0;  // a bit a stage; tail_parity: of its next tail
     const uint32_t full_leader0 = mapa_shared(smem_u32(&full[0]), 0);
     const uint32_t tail_mine0 = mapa_shared(smem_u32(&tail_full[0]), rank);
     for (int i = 0; ok; ++i) {
@@ -481,15 +482,17 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         ok = all_ok(mbar_wait(&empty[stage], phase ^ 1u, ctx, SITE_EMPTY));
         if (!ok) break;
         // A group's last stage that does not end on a 16-row step: each CTA
-        // waits for its own bytes and clears the rows past the end.
+        // waits for its own bytes and clears the rows past the end (`full` only
+        // moves on).
         const bool tail = DW && kb + 1 == x.blocks && (x.rows & 15) != 0;
         const int nq = min(kps, x.blocks - kb);
-        const uint32_t bar = (tail && !leader ? tail_mine0 : full_leader0) + stage * 8u;
+        const uint32_t bar = (tail ? tail_mine0 : full_leader0) + stage * 8u;
         uint8_t* sA = smem + stage * stage_bytes;
         uint8_t* sB = sA + a_bytes;
         if (elect_one()) {
-          if (leader) mbar_arrive_expect_tx(&full[stage], (tail ? 1 : 2) * nq * block_bytes);
-          else if (tail) mbar_arrive_expect_tx(&tail_full[stage], block_bytes);
+          if (tail) mbar_arrive_expect_tx(&tail_full[stage], block_bytes);
+          if (leader && tail) mbar_arrive(&full[stage]);
+          else if (leader) mbar_arrive_expect_tx(&full[stage], 2 * nq * block_bytes);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             if (q >= nq) break;
@@ -534,28 +537,34 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         }
         __syncwarp();
         issued |= 1u << stage;
-        parity = (parity & ~(1u << stage)) | (phase << stage);
+        if (tail) {
+          tails |= 1u << stage;
+          tail_parity ^= 1u << stage;
+        } else {
+          tails &= ~(1u << stage);
+          parity = (parity & ~(1u << stage)) | (phase << stage);
+        }
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
       }
     }
-    if (!ok && leader) {
+    if (!ok) {
       // Abort: let the copies still in flight land before the CTA exits.
       WaitCtx drain_ctx{ctx.status, 50000000ull};
-      for (int s = 0; s < stages; ++s)
-        if (issued >> s & 1u) mbar_wait(&full[s], parity >> s & 1u, drain_ctx, SITE_DRAIN);
+      for (int s = 0; s < stages; ++s) {
+        if (tails >> s & 1u) mbar_wait(&tail_full[s], (tail_parity >> s & 1u) ^ 1u, drain_ctx, SITE_DRAIN);
+        else if (leader && (issued >> s & 1u)) mbar_wait(&full[s], parity >> s & 1u, drain_ctx, SITE_DRAIN);
+      }
     }
   } else if (warp == 1) {
-    // ------------------------------------------ MMA issuer (leader); in dw the
-    // warp of both CTAs clears the rows past a group's end.
-    if (DW || leader) {
+    // ------------------------------------------------------ MMA issuer (leader)
+    if (leader) {
       int stage = 0;
       uint32_t phase = 0, tail_parity = 0;
       uint32_t halves = 0;  // accumulators used so far: slot = bit 0, phase = bit 1
       bool ok = true, any_issued = false;
-      const uint32_t tail_done_leader0 = mapa_shared(smem_u32(&tail_done[0]), 0);
       const uint32_t ring = smem_u32(smem);
       const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
       // The MMAs of half `s` over the stage `at`, whose first K-block is kb;
@@ -612,42 +621,20 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         for (int kb = 0; kb < x.blocks; kb += kps) {
           const int left = DW ? x.rows - kb * EPB : 0;  // dw: rows of the group in this stage and later
           const bool tail = DW && kb + 1 == x.blocks && (x.rows & 15) != 0;
-          if (leader) ok = mbar_wait(&full[stage], phase, ctx, SITE_FULL);
-          else if (tail) ok = mbar_wait(&tail_full[stage], tail_parity >> stage & 1u, ctx, SITE_FULL);
+          if (tail) {
+            ok = mbar_wait_cluster(&tail_done[stage], tail_parity >> stage & 1u, ctx, SITE_FULL);
+            tail_parity ^= 1u << stage;
+          } else {
+            ok = mbar_wait(&full[stage], phase, ctx, SITE_FULL);
+          }
           ok = all_ok(ok);
-          if constexpr (DW) {
-            if (ok && tail) {
-              // Rows left .. the end of its 16-row step, in every box of 64
-              // columns (128-byte rows; the swizzle stays within a row).
-              uint8_t* sA = smem + stage * stage_bytes;
-              uint8_t* sB = sA + a_bytes;
-              const int n = (16 - (left & 15)) * 8;
-              for (int c = lane; c < n; c += 32) {
-                const int at = left * 128 + c * 16;
-                const uint4 zero = make_uint4(0, 0, 0, 0);
-                for (int box = 0; box < 2 * x.nsub; ++box) *reinterpret_cast<uint4*>(sA + box * 8192 + at) = zero;
-                for (int box = 0; box < 2; ++box) *reinterpret_cast<uint4*>(sB + box * 8192 + at) = zero;
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (!leader) {
-                if (lane == 0) mbar_arrive_cluster(tail_done_leader0 + stage * 8u);
-                __syncwarp();
-              } else {
-                ok = all_ok(mbar_wait_cluster(&tail_done[stage], tail_parity >> stage & 1u, ctx, SITE_FULL));
-              }
-              tail_parity ^= 1u << stage;
-            }
-          }
           if (!ok) break;
-          if (leader) {
-            tc_fence_after();
-            const bool last = kb + kps >= x.blocks;
-            ok = issue(x, idesc, 0, stage, kb, last, left);
-            if (ok && x.nsub == 2 && kb > 0) ok = issue(x, idesc, 1, stage == 0 ? stages - 1 : stage - 1, kb - 1, false, EPB);
-            if (ok && x.nsub == 2 && last) ok = issue(x, idesc, 1, stage, kb, true, left);
-            if (!ok) break;
-          }
+          tc_fence_after();
+          const bool last = kb + kps >= x.blocks;
+          ok = issue(x, idesc, 0, stage, kb, last, left);
+          if (ok && x.nsub == 2 && kb > 0) ok = issue(x, idesc, 1, stage == 0 ? stages - 1 : stage - 1, kb - 1, false, EPB);
+          if (ok && x.nsub == 2 && last) ok = issue(x, idesc, 1, stage, kb, true, left);
+          if (!ok) break;
           __syncwarp();
           if (++stage == stages) {
             stage = 0;
@@ -680,6 +667,38 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
       }
       __syncwarp();
       if (x.e < 0) break;
+    }
+  } else if (DW && warp == W::EPILOGUE + 3) {
+    // --------------------------------------- zeros past the ends of dw's groups
+    // (by the issuer itself, between two tiles' MMAs, it took 1.3 us a tile)
+    int stage = 0;
+    uint32_t tail_parity = 0;
+    const uint32_t tail_done_leader0 = mapa_shared(smem_u32(&tail_done[0]), 0);
+    for (int i = 0;; ++i) {
+      const Tile x = next_tile(i);
+      if (x.e < 0) break;
+      if (x.blocks != 0 && (x.rows & 15) != 0) {
+        const int at = (stage + x.blocks - 1) % stages;
+        if (!all_ok(mbar_wait(&tail_full[at], tail_parity >> at & 1u, ctx, SITE_FULL))) break;
+        // Rows left .. the end of its 16-row step, in every box of 64 columns
+        // (128-byte rows; the swizzle stays within a row).
+        uint8_t* sA = smem + at * stage_bytes;
+        uint8_t* sB = sA + a_bytes;
+        const int left = x.rows - (x.blocks - 1) * EPB;
+        const int n = (16 - (left & 15)) * 8;
+        for (int c = lane; c < n; c += 32) {
+          const int to = left * 128 + c * 16;
+          const uint4 zero = make_uint4(0, 0, 0, 0);
+          for (int box = 0; box < 2 * x.nsub; ++box) *reinterpret_cast<uint4*>(sA + box * 8192 + to) = zero;
+          for (int box = 0; box < 2; ++box) *reinterpret_cast<uint4*>(sB + box * 8192 + to) = zero;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(tail_done_leader0 + at * 8u);
+        __syncwarp();
+        tail_parity ^= 1u << at;
+      }
+      stage = (stage + x.blocks) % stages;
     }
   } else {
     // -------------------------------------------------------------- epilogue

@@ -159,9 +159,17 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const 
 // As mbar_wait, for a barrier that threads of another CTA of the cluster
 // arrive at after writing: acquires at cluster scope.
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, const WaitCtx& ctx, uint32_t site) {
-  const bool ok = mbar_wait(bar, parity, ctx, site);
-  asm volatile("fence.acq_rel.cluster;" ::: "memory");
-  return ok;
+  if (!mbar_wait(bar, parity, ctx, site)) return false;
+  // Complete by now: the same test, acquiring for the cluster.
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 // As mbar_wait, but sleeps `backoff_ns` between polls once the first few have
