@@ -478,13 +478,17 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
       const int half = x.width / 2;
       const int a0 = x.a0 + (int)rank * 128, b0 = x.b0 + (int)rank * half;
       const uint32_t block_bytes = x.nsub * L::SUB + half * 128;
-      for (int kb = 0; kb < x.blocks; kb += kps) {
+      const bool has_tail = DW && (x.rows & 15) != 0, early = has_tail && x.blocks > 1;
+      for (int j = 0; j < x.blocks; j += kps) {
+        // The tail's K-block comes before the one that precedes it, which gives
+        // the time to clear it.
+        const int kb = early && j >= x.blocks - 2 ? 2 * x.blocks - 3 - j : j;
         ok = all_ok(mbar_wait(&empty[stage], phase ^ 1u, ctx, SITE_EMPTY));
         if (!ok) break;
         // A group's last stage that does not end on a 16-row step: each CTA
         // waits for its own bytes and clears the rows past the end (`full` only
         // moves on).
-        const bool tail = DW && kb + 1 == x.blocks && (x.rows & 15) != 0;
+        const bool tail = has_tail && kb + 1 == x.blocks;
         const int nq = min(kps, x.blocks - kb);
         const uint32_t bar = (tail ? tail_mine0 : full_leader0) + stage * 8u;
         uint8_t* sA = smem + stage * stage_bytes;
@@ -618,23 +622,33 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
           break;
         }
         const uint32_t idesc = IDESC | (uint32_t)(x.width >> 3) << 17;
+        const bool has_tail = DW && (x.rows & 15) != 0, early = has_tail && x.blocks > 1;
+        int before = 0;  // the stage of the K-block before
         for (int kb = 0; kb < x.blocks; kb += kps) {
           const int left = DW ? x.rows - kb * EPB : 0;  // dw: rows of the group in this stage and later
-          const bool tail = DW && kb + 1 == x.blocks && (x.rows & 15) != 0;
-          if (tail) {
-            ok = mbar_wait_cluster(&tail_done[stage], tail_parity >> stage & 1u, ctx, SITE_FULL);
-            tail_parity ^= 1u << stage;
+          // Of a group with a tail, the last two K-blocks' stages are the other way round.
+          int at = stage;
+          uint32_t ph = phase;
+          if (early && kb == x.blocks - 2 && ++at == stages) {
+            at = 0;
+            ph ^= 1u;
+          }
+          if (early && kb == x.blocks - 1) at = stage == 0 ? stages - 1 : stage - 1;
+          if (has_tail && kb + 1 == x.blocks) {
+            ok = mbar_wait_cluster(&tail_done[at], tail_parity >> at & 1u, ctx, SITE_FULL);
+            tail_parity ^= 1u << at;
           } else {
-            ok = mbar_wait(&full[stage], phase, ctx, SITE_FULL);
+            ok = mbar_wait(&full[at], ph, ctx, SITE_FULL);
           }
           ok = all_ok(ok);
           if (!ok) break;
           tc_fence_after();
           const bool last = kb + kps >= x.blocks;
-          ok = issue(x, idesc, 0, stage, kb, last, left);
-          if (ok && x.nsub == 2 && kb > 0) ok = issue(x, idesc, 1, stage == 0 ? stages - 1 : stage - 1, kb - 1, false, EPB);
-          if (ok && x.nsub == 2 && last) ok = issue(x, idesc, 1, stage, kb, true, left);
+          ok = issue(x, idesc, 0, at, kb, last, left);
+          if (ok && x.nsub == 2 && kb > 0) ok = issue(x, idesc, 1, before, kb - 1, false, EPB);
+          if (ok && x.nsub == 2 && last) ok = issue(x, idesc, 1, at, kb, true, left);
           if (!ok) break;
+          before = at;
           __syncwarp();
           if (++stage == stages) {
             stage = 0;
@@ -678,7 +692,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
       const Tile x = next_tile(i);
       if (x.e < 0) break;
       if (x.blocks != 0 && (x.rows & 15) != 0) {
-        const int at = (stage + x.blocks - 1) % stages;
+        const int at = (stage + max(x.blocks - 2, 0)) % stages;
         if (!all_ok(mbar_wait(&tail_full[at], tail_parity >> at & 1u, ctx, SITE_FULL))) break;
         // Rows left .. the end of its 16-row step, in every box of 64 columns
         // (128-byte rows; the swizzle stays within a row).
