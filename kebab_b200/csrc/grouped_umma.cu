@@ -25,9 +25,12 @@
 // (a multiple of 32; N is a field of the instruction descriptor), a group of
 // 514 rows gives tiles of 192, 192 and 160 columns and not 256, 256 and 32, and
 // no group is padded in memory. Which tile belongs to which group is worked out
-// on the device: every CTA sorts the groups' tiles by cost (widest, or in dw
-// longest, first) and sums them up for itself, and the pairs take them in turn,
-// back and forth, which leaves their loads within one small tile of each other.
+// on the device: every CTA sorts the groups by their tiles' cost (widest, or in
+// dw longest, first) and sums them up for itself, and the pairs take the tiles
+// in turn, back and forth, which leaves their loads within a tile of each other.
+// A group's tiles stay together, so that its weights are read once: with the
+// last, narrower tiles of all groups at the end, 16381 x 4096 x 2048 over 14
+// groups took 252 us and 464 MB from memory, and takes 243 and 322.
 //
 // Edges: a forward tile may read past its group's end (the columns are not
 // stored; a column does not reach its neighbours). In dw the contraction runs
@@ -70,7 +73,6 @@ struct TileArgs {
   const void* bias;
   int pdl;
   int sort;
-  int entries;  // of the table of tiles
   WaitCtx ctx;
 };
 
@@ -90,7 +92,7 @@ struct Warps {
 };
 // Tiles are sorted by cost where that can pay: from 2048 rows (a product of
 // fewer takes about as long as its weights' bytes in any order), and up to 512
-// entries (the ranks take entries^2 / 352 (dw 640) comparisons a thread).
+// groups (the ranks take groups^2 / 352 (dw 640) comparisons a thread).
 constexpr int SORT_ROWS = 2048, SORT_LIMIT = 512;
 // K-blocks of a tile from which its stores go by TMA.
 constexpr int PACED_FROM = 16;
@@ -109,9 +111,9 @@ struct GSmem {
   static constexpr int NUM_BARS = 4 * MAX_STAGES + 5 + 2 * TILES;
   static constexpr int OFF_TILES = (OFF_BAR + NUM_BARS * 8 + 4 + 15) / 16 * 16;
   static constexpr int OFF_TABLE = OFF_TILES + TILES * 32;
-  // first[entries + 1] (int), entry[entries] (uint16, sorted only)
-  static constexpr int bytes(int entries, bool sorted) {
-    return OFF_TABLE + (entries + 1) * 4 + (sorted ? entries * 2 : 0) + 1024;
+  // first[E + 1] (int), entry[E] (uint16, sorted only)
+  static constexpr int bytes(int E, bool sorted) {
+    return OFF_TABLE + (E + 1) * 4 + (sorted ? E * 2 : 0) + 1024;
   }
   static constexpr int ALLOC =
       OFF_TABLE + std::max((kMaxExperts + 1) * 4, (SORT_LIMIT + 1) * 4 + SORT_LIMIT * 2) + 1024;
@@ -129,15 +131,14 @@ __device__ __forceinline__ int divide(int a, int b) {
   return q;
 }
 
-// The tiles in the order in which they are dealt out. Entry i has the column
-// blocks first[i] .. first[i + 1] - 1, each of `panels` tiles. Unsorted, an
-// entry is a group. Sorted, it is a group (dw), or a group's full-width or its
-// last column block (forward).
+// The tiles in the order in which they are dealt out. Group entry[i] (unsorted:
+// group i) has the column blocks first[i] .. first[i + 1] - 1, each of `panels`
+// tiles.
 struct Table {
   const int* first;
-  const uint16_t* entry;  // sorted: group (dw), or group * 2 + (1: the last block)
+  const uint16_t* entry;
   bool sorted;
-  int entries, panels;    // panels: tiles along the MMA-row side
+  int panels;             // tiles along the MMA-row side
   int nsub;               // 256-row halves of a panel
   int kps;                // K-blocks a stage
   int cap;                // columns that a tile may have
@@ -150,17 +151,17 @@ struct alignas(16) Tile {
   int blocks;            // 128-byte K-blocks of the contraction
 };
 
-// Columns of a group's tiles: equal shares of at most `cap`, and what is left for the last.
+// Columns of a group's tiles: equal shares of at most `cap`, in runs of 32, the wider ones first.
 struct Widths {
-  int count, full, last;
+  int count, narrow, wider;  // `wider` of the tiles have 32 columns more
   __device__ __forceinline__ Widths(int rows, int cap) {
+    const int runs = (rows + 31) / 32;
     count = (rows + cap - 1) / cap;
-    full = last = (rows + 31) / 32 * 32;
-    if (count > 1) {
-      full = (divide(rows + count - 1, count) + 31) / 32 * 32;
-      last = (rows - (count - 1) * full + 31) / 32 * 32;
-    }
+    const int per = count > 1 ? divide(runs, count) : runs;
+    wider = runs - per * count;
+    narrow = per * 32;
   }
+  __device__ __forceinline__ int widest() const { return narrow + (wider > 0 ? 32 : 0); }
 };
 
 // Tile `local` of panels x blocks: eight panels share the passes over the
@@ -180,14 +181,14 @@ __device__ __forceinline__ void raster(int local, int panels, int blocks, int& p
 template <int MODE, int EPB>
 __device__ __forceinline__ Tile tile_of(int t, const TileArgs& g, const Table& tab) {
   Tile x;
-  int lo = 0, hi = tab.entries - 1;  // the last entry that starts at or before t
+  int lo = 0, hi = g.E - 1;  // the last group that starts at or before t
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (tab.first[mid] * tab.panels <= t) lo = mid;
     else hi = mid - 1;
   }
-  const int id = tab.sorted ? tab.entry[lo] : lo, local = t - tab.first[lo] * tab.panels;
-  x.e = MODE == MODE_DW || !tab.sorted ? id : id >> 1;
+  const int local = t - tab.first[lo] * tab.panels;
+  x.e = tab.sorted ? tab.entry[lo] : lo;
   group_range(g.offsets, x.e, g.R, x.begin, x.rows);
   int pa, cb;
   if (MODE == MODE_DW) {
@@ -197,16 +198,9 @@ __device__ __forceinline__ Tile tile_of(int t, const TileArgs& g, const Table& t
     x.blocks = (x.rows + EPB - 1) / EPB;
   } else {
     const Widths w(x.rows, tab.cap);
-    if (!tab.sorted) {
-      raster(local, tab.panels, w.count, pa, cb);
-    } else if (id & 1) {
-      pa = local;
-      cb = w.count - 1;
-    } else {
-      raster(local, tab.panels, w.count - 1, pa, cb);
-    }
-    x.width = cb == w.count - 1 ? w.last : w.full;
-    x.b0 = cb * w.full;
+    raster(local, tab.panels, w.count, pa, cb);
+    x.width = w.narrow + (cb < w.wider ? 32 : 0);
+    x.b0 = cb * w.narrow + min(cb, w.wider) * 32;
     x.blocks = (g.K + EPB - 1) / EPB;
   }
   x.a0 = pa * 256 * tab.nsub;
@@ -244,7 +238,7 @@ __device__ __forceinline__ int scan_before(int v, int* sums, int& total) {
   return before + at - v;
 }
 
-// Makes the table, by all threads of the CTA. `scratch`: 3 ints an entry and 32.
+// Makes the table, by all threads of the CTA. `scratch`: 3 ints a group and 40.
 template <int MODE, bool I8>
 __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* first, uint16_t* entry, int* scratch) {
   constexpr bool DW = MODE == MODE_DW;
@@ -260,7 +254,7 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
   int* cost = scratch + 32;
   const int tb = (g.DB + 255) / 256;
   const bool sorted = g.sort;
-  const int n = g.entries;
+  const int n = g.E;
   int wide = 0;  // some tile of more than 128 columns
   int total = 0;
   int cap = 256;
@@ -302,20 +296,20 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
     }
     wide = __syncthreads_or(wide);
   } else {
-    int* blocks = cost + (n + 3) / 4 * 4;  // column blocks of the entry
+    int* blocks = cost + (n + 3) / 4 * 4;  // column blocks of the group
     int* by_rank = blocks + n;
     for (int i = threadIdx.x; i < (n + 3) / 4 * 4; i += THREADS) {
       int c = -1, b = 0;
       if (i < n) {
         int begin, rows;
-        group_range(g.offsets, DW ? i : i >> 1, g.R, begin, rows);
+        group_range(g.offsets, i, g.R, begin, rows);
         if (DW) {
           c = rows;
           b = tb;
         } else {
           const Widths w(rows, 256);
-          c = (i & 1) ? w.last : w.count > 1 ? w.full : 0;
-          b = w.count == 0 ? 0 : (i & 1) ? 1 : w.count - 1;
+          c = w.widest();
+          b = w.count;
         }
         wide |= DW || c > 128;
         blocks[i] = b;
@@ -348,7 +342,6 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
   tab.first = first;
   tab.entry = entry;
   tab.sorted = sorted;
-  tab.entries = n;
   const int p256 = (g.DA + 255) / 256;
   tab.nsub = WIDE_FROM > 0 && (int64_t)total * p256 >= (int64_t)WIDE_FROM * pairs ? 2 : 1;
   tab.panels = tab.nsub == 2 ? (g.DA + 511) / 512 : p256;
@@ -391,7 +384,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + L::NUM_BARS);
   Tile* s_tiles = reinterpret_cast<Tile*>(smem + L::OFF_TILES);
   int* s_first = reinterpret_cast<int*>(smem + L::OFF_TABLE);
-  uint16_t* s_entry = reinterpret_cast<uint16_t*>(s_first + g.entries + 1);
+  uint16_t* s_entry = reinterpret_cast<uint16_t*>(s_first + g.E + 1);
 
   // The shuffle tells the compiler that a warp takes one path. The producer and
   // the issuer run with all lanes, one of which is elected at each copy or MMA,
@@ -666,7 +659,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     }
   } else if (warp == W::EPILOGUE + 2) {
     // ------------------------------------------------------- tiles, in order
-    const int num_tiles = s_first[tab.entries] * tab.panels;
+    const int num_tiles = s_first[g.E] * tab.panels;
     for (int i = 0;; ++i) {
       // Back and forth over the pairs.
       const int t = i * pairs + ((i & 1) ? pairs - 1 - pair : pair);
@@ -909,7 +902,7 @@ int launch(const GroupedProblem& p) {
   g.w_scale = p.w_scale;
   g.bias = p.bias;
   g.pdl = pdl_enabled() ? 1 : 0;
-  g.sort = p.R >= SORT_ROWS && (DW ? p.E : 2 * p.E) <= SORT_LIMIT;
+  g.sort = p.R >= SORT_ROWS && p.E <= SORT_LIMIT;
   CUtensorMap tA, tB;
   ColumnMaps tBs;
   int64_t tiles;
@@ -949,8 +942,7 @@ int launch(const GroupedProblem& p) {
   }
 
   auto kern = grouped_umma_kernel<TO, I8, MODE>;
-  g.entries = DW || !g.sort ? g.E : 2 * g.E;
-  const int smem = L::bytes(g.entries, g.sort);
+  const int smem = L::bytes(g.E, g.sort);
   // Once per device and instantiation: the shared-memory opt-in and how many pairs fit.
   static std::once_flag once[64];
   static cudaError_t err[64];
