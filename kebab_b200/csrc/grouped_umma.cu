@@ -16,10 +16,11 @@
 // it into registers (as pairs of outputs) and hand it back; they store
 // afterwards. One half at a time, in a loop: unrolled over both, the epilogue
 // was bound by fetching its instructions (dw of 352 rows over 108 experts, 2552
-// x 2648: 1000 us against 656). Tiles of 16 K-blocks or more store by TMA, whose
-// pace leaves the operands' copies alone: 32768 x 8192 x 4096 over 8 groups 1757
-// us against 1810 with stores from registers. Shorter ones store from registers
-// (the dw above, now 578 us, takes 618 by TMA).
+// x 2648: 1000 us against 656). Tiles of 16 K-blocks or more (dw: 4) store by
+// TMA, whose pace leaves the operands' copies alone: 32768 x 8192 x 4096 over 8
+// groups 1757 us against 1810 with stores from registers, dw of 32 groups of 512
+// rows, 4096 x 2048, 240 against 246. Shorter ones store from registers (dw of 43
+// groups of 95 rows, 4040 x 1272, 165 us against 181 by TMA).
 //
 // Ragged sizes cost what they are: a forward tile is as wide as its rows need
 // (a multiple of 32; N is a field of the instruction descriptor), a group of
@@ -79,7 +80,7 @@ struct TileArgs {
 // Epilogue warps: a set of 8 that takes every half in turn, or (dw) one for each
 // accumulator. dw's contraction is short and its outputs many, so that what the
 // epilogue takes to store a half would delay its reading of the next: 16384 x
-// 4096 x 2048, burst, 1024 rows a group 207 us against 222 with one set, 256 rows
+// 4096 x 2048, burst, 1024 rows a group 204 us against 222 with one set, 256 rows
 // 378 against 405. The forward tiles are longer, and the registers that a thread
 // then has too few: 32768 x 8192 x 4096 over 8 groups 1808 us with one, 1853 with
 // two.
@@ -87,15 +88,13 @@ template <int MODE>
 struct Warps {
   static constexpr int SETS = MODE == MODE_DW ? 2 : 1;
   static constexpr int EPILOGUE = 8 * SETS;
-  static constexpr int TAIL = MODE == MODE_DW ? 1 : 0;         // the one that clears rows past a group's end
+  static constexpr int TAIL = MODE == MODE_DW ? 1 : 0;        // the one that writes zeros
   static constexpr int THREADS = 32 * (EPILOGUE + TAIL + 3);  // and producer, issuer, tiles
 };
 // Tiles are sorted by cost where that can pay: from 2048 rows (a product of
 // fewer takes about as long as its weights' bytes in any order), and up to 512
 // groups (the ranks take groups^2 / 352 (dw 640) comparisons a thread).
 constexpr int SORT_ROWS = 2048, SORT_LIMIT = 512;
-// K-blocks of a tile from which its stores go by TMA.
-constexpr int PACED_FROM = 16;
 
 template <int SETS>
 struct GSmem {
@@ -365,6 +364,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
   using L = GSmem<W::SETS>;
   constexpr bool DW = MODE == MODE_DW;
   constexpr bool A_MN = MODE != MODE_RC, B_MN = DW;
+  constexpr int PACED_FROM = DW ? 4 : 16;  // K-blocks of a tile from which its stores go by TMA
   constexpr int EPB = I8 ? 128 : 64;  // elements of the contraction in a K-block
   constexpr int STAGES = L::MAX_STAGES;
   constexpr uint32_t IDESC = (I8 ? umma_idesc_i8(256, 0) : umma_idesc_f16(256, 0, ElemTraits<TO>::kBf16)) |
@@ -684,7 +684,27 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     for (int i = 0;; ++i) {
       const Tile x = next_tile(i);
       if (x.e < 0) break;
-      if (x.blocks != 0 && (x.rows & 15) != 0) {
+      if (x.blocks == 0) {
+        // A group without rows: the whole tile, each CTA every other column, 512
+        // contiguous bytes a step (108 experts of 2552 x 2648, all but one empty:
+        // 340 us, 680 from the epilogue, whose warps write 64 bytes at a time).
+        const int b0 = x.b0 + (int)rank, columns = (min(x.b0 + x.width, g.DB) - b0 + 1) / 2;
+        const int end = min(x.a0 + x.nsub * 256, g.DA);
+        uint16_t* y = static_cast<uint16_t*>(g.Y) + ((int64_t)x.e * g.DB + b0) * g.ldy;
+        if (g.vec_out) {
+          const int a = x.a0 + lane * 8;
+          const bool one = a < end, two = a + 256 < end;
+          y += a;
+#pragma unroll 8
+          for (int c = 0; c < columns; ++c, y += 2 * g.ldy) {
+            if (one) *reinterpret_cast<uint4*>(y) = make_uint4(0, 0, 0, 0);
+            if (two) *reinterpret_cast<uint4*>(y + 256) = make_uint4(0, 0, 0, 0);
+          }
+        } else {
+          for (int c = 0; c < columns; ++c, y += 2 * g.ldy)
+            for (int a = x.a0 + lane; a < end; a += 32) y[a] = 0;
+        }
+      } else if ((x.rows & 15) != 0) {
         const int at = (stage + max(x.blocks - 2, 0)) % stages;
         if (!all_ok(mbar_wait(&tail_full[at], tail_parity >> at & 1u, ctx, SITE_FULL))) break;
         // Rows left .. the end of its 16-row step, in every box of 64 columns
@@ -725,7 +745,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
       const int limit = DW ? g.DB : x.rows;  // columns end here
       const int cols = x.width / 2;          // of this warp, a multiple of 16
       const int d0 = side * cols;            // its first column in the tile
-      const bool some = x.blocks != 0;       // dw of a group without rows: zeros
+      if (DW && x.blocks == 0) continue;  // zeros, by another warp
       if constexpr (I8) {
         __syncwarp();
         for (int c = lane; c < cols; c += 32) {
@@ -736,8 +756,8 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
       }
 #pragma unroll 1
       for (int s = 0; s < x.nsub; ++s) {
-        const uint32_t slot = (some ? halves : s) & 1u, use = halves >> 1;
-        if (some) ++halves;
+        const uint32_t slot = halves & 1u, use = halves >> 1;
+        ++halves;
         if (W::SETS == 2 && slot != set) continue;
         const int a_warp = x.a0 + s * 256 + (int)rank * 128 + q * 32;  // this warp's first row of the half
         float sw = 0.f, bias = 0.f;
@@ -748,11 +768,9 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
             if (g.bias) bias = (float)static_cast<const TO*>(g.bias)[a];
           }
         }
-        if (some) {
-          ok = all_ok(mbar_wait(&tmem_full[slot], use & 1u, ctx, SITE_TMEM_FULL));
-          if (!ok) break;
-          tc_fence_after();
-        }
+        ok = all_ok(mbar_wait(&tmem_full[slot], use & 1u, ctx, SITE_TMEM_FULL));
+        if (!ok) break;
+        tc_fence_after();
         // Columns RUN c + 2 j and the next of this thread's row, as outputs (an odd
         // last run of 16 is read as 32; what is past it is not used).
         uint32_t out[128 / RUN][RUN / 2];
@@ -760,15 +778,10 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         for (int c = 0; c < 128 / RUN; ++c) {
           if (c * RUN >= cols) break;
           uint32_t v[RUN];
-          if (some) {
-            const uint32_t at = t_quarter + slot * 256 + (uint32_t)(d0 + c * RUN);
-            if constexpr (RUN == 32) tmem_ld_32x32b_x32(at, v);
-            else tmem_ld_32x32b_x16(at, v);
-            tmem_ld_wait();
-          } else {
-#pragma unroll
-            for (int j = 0; j < RUN; ++j) v[j] = 0u;
-          }
+          const uint32_t at = t_quarter + slot * 256 + (uint32_t)(d0 + c * RUN);
+          if constexpr (RUN == 32) tmem_ld_32x32b_x32(at, v);
+          else tmem_ld_32x32b_x16(at, v);
+          tmem_ld_wait();
           if constexpr (I8) {
 #pragma unroll
             for (int j = 0; j < RUN; ++j) v[j] = __float_as_uint((float)(int)v[j] * (sw * s_scale[c * RUN + j]) + bias);
@@ -776,12 +789,10 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
 #pragma unroll
           for (int j = 0; j < RUN / 2; ++j) out[c][j] = pack2(TO(), __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
         }
-        if (some) {
-          // This warp's share read: hand it back to the MMA issuer.
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(tmem_empty_leader0 + slot * 8u);
-        }
+        // This warp's share read: hand it back to the MMA issuer.
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(tmem_empty_leader0 + slot * 8u);
         if (a_warp >= g.DA) continue;
 #pragma unroll
         for (int c = 0; c < 128 / RUN; ++c) {
