@@ -342,6 +342,41 @@ def test_grouped_rows_of_no_group(cuda, rows):
     assert (dW[1] == 0).all()
 
 
+@pytest.mark.parametrize("opmode", ["RC", "RR"])
+@pytest.mark.parametrize("N,K,extra", [(1032, 1048, 0), (1031, 1047, 9)])
+@pytest.mark.parametrize("counts", [
+    [0, 1, 15, 16, 17, 63, 0, 64, 65, 79, 127, 128, 129, 130, 0, 0, 200, 255, 320, 3],
+    [0] * 9 + [1000, 1023, 1, 0, 2] + [0] * 3])
+def test_grouped_gradient_ends(cuda, counts, N, K, extra, opmode):
+    """dW of groups that end anywhere in a 64-row block and of groups without
+    rows, enough tiles for the widest panels, outputs on even and odd pitches,
+    and neighbours whose rows are not finite."""
+    import torch
+    import kebab_b200 as kb
+    dt = torch.bfloat16
+    R = sum(counts)
+    X, dY = randn((R, K), dt, 1), randn((R, N), dt, 2)
+    shape = (len(counts), N, K) if opmode == "RC" else (len(counts), K, N)
+
+    def run(x, dy):
+        dW = torch.full(shape, float("nan"), dtype=dt, device="cuda")
+        return kb.gemm_grouped_dw(pitched(x, extra, 0), pitched(dy, extra, 0), offsets_of(counts), dW=dW, opmode=opmode)
+    got = run(X, dY)
+    want, size = dw_plain(X, dY, counts, opmode)
+    assert_within(got, want, product_bound(want, size, max(counts), dt), "dW")
+    odd = [e for e in range(len(counts)) if counts[e] and e % 2]
+    at = 0
+    for e, c in enumerate(counts):
+        if e in odd:
+            X[at:at + c], dY[at:at + c] = float("inf"), float("nan")
+        at += c
+    again = run(X, dY)
+    for e in range(len(counts)):
+        assert torch.isnan(again[e]).all() if e in odd else torch.equal(again[e], got[e])
+    rc, code = kb.device_status()
+    assert rc == kb.OK, hex(code)
+
+
 def test_grouped_infinities_stay_in_their_group(cuda):
     """A group's NaN and infinite rows do not reach its neighbours, in the
     products or in dW, although tiles read past a group's end."""
