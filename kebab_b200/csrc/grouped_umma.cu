@@ -261,9 +261,9 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
     // The widest tile of 256, 192 or 128 columns, by the waves over the pairs and
     // the rows that a tile's K-block copies (256 of the panel and its columns,
     // which take as long as its MMAs or longer). 128 also keeps two K-blocks a
-    // stage. 1267 rows over 3 groups, 3320 x 5224: 76 us with 256
-    // (78 tiles on 74 pairs), 68 so.
-    if constexpr (!DW) {
+    // stage. 1267 rows over 3 groups, 3320 x 5224: 76 us with 256 (78 tiles on 74
+    // pairs), 68 so. Of 65536 rows or more (more groups than are sorted) it is 256.
+    if (!DW && g.R < 65536) {
       int c256 = 0, c192 = 0, c128 = 0;
       for (int i0 = 0; i0 < n; i0 += THREADS) {
         int begin, rows = 0, two, one;
@@ -275,7 +275,9 @@ __device__ __forceinline__ Table make_table(const TileArgs& g, int pairs, int* f
         c128 += one;
       }
       const int panels = (g.DA + 255) / 256;
-      auto cost = [&](int blocks, int width) { return (int64_t)((blocks * panels + pairs - 1) / pairs) * (256 + width); };
+      auto cost = [&](int blocks, int width) {
+        return ((int64_t)blocks * panels + pairs - 1) / pairs * (256 + width);
+      };
       if (cost(c192, 192) < cost(c256, 256)) cap = 192;
       if (cost(c128, 128) <= min(cost(c192, 192), cost(c256, 256))) cap = 128;
     }
@@ -733,7 +735,8 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     const int side = (warp - 2) / 4 % 2;  // which half of a tile's columns it takes
     const uint32_t set = (warp - 2) / 8;  // of two sets, the accumulator it reads
     constexpr int RUN = L::RUN;
-    uint32_t* stage_c = reinterpret_cast<uint32_t*>(smem + L::OFF_C + (warp - 2) * L::C_SUB);  // [RUN / 2 pairs][32 values]
+    // [RUN / 2 pairs][32 values]
+    uint32_t* stage_c = reinterpret_cast<uint32_t*>(smem + L::OFF_C + (warp - 2) * L::C_SUB);
     float* s_scale = reinterpret_cast<float*>(stage_c + RUN / 2 * 32);
     const uint32_t tmem_empty_leader0 = mapa_shared(smem_u32(&tmem_empty[0]), 0);
     const uint32_t t_quarter = tmem_base + ((uint32_t)(q * 32) << 16);
@@ -787,7 +790,8 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
             for (int j = 0; j < RUN; ++j) v[j] = __float_as_uint((float)(int)v[j] * (sw * s_scale[c * RUN + j]) + bias);
           }
 #pragma unroll
-          for (int j = 0; j < RUN / 2; ++j) out[c][j] = pack2(TO(), __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+          for (int j = 0; j < RUN / 2; ++j)
+            out[c][j] = pack2(TO(), __uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
         }
         // This warp's share read: hand it back to the MMA issuer.
         tc_fence_before();
@@ -966,7 +970,8 @@ int launch(const GroupedProblem& p) {
     PdlLaunch q(dim3(2 * max_pairs[di]), dim3(W::THREADS), L::ALLOC, nullptr, 2);
     q.cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kern, &q.cfg) == cudaSuccess && n > 0) max_pairs[di] = std::min(n, max_pairs[di]);
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &q.cfg) == cudaSuccess && n > 0)
+      max_pairs[di] = std::min(n, max_pairs[di]);
     (void)cudaGetLastError();
   });
   if (err[di] != cudaSuccess) return cuda_fail(err[di], "cudaFuncSetAttribute(max dynamic smem)");
