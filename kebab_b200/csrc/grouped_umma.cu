@@ -16,11 +16,12 @@
 // it into registers (as pairs of outputs) and hand it back; they store
 // afterwards. One half at a time, in a loop: unrolled over both, the epilogue
 // was bound by fetching its instructions (dw of 352 rows over 108 experts, 2552
-// x 2648: 1000 us against 656). Tiles of 16 K-blocks or more (dw: 4) store by
-// TMA, whose pace leaves the operands' copies alone: 32768 x 8192 x 4096 over 8
-// groups 1757 us against 1810 with stores from registers, dw of 32 groups of 512
-// rows, 4096 x 2048, 240 against 246. Shorter ones store from registers (dw of 43
-// groups of 95 rows, 4040 x 1272, 165 us against 181 by TMA).
+// x 2648: 1000 us against 656). Tiles of 8 K-blocks or more store by TMA, whose
+// pace leaves the operands' copies alone: 32768 x 8192 x 4096 over 8 groups 1757
+// us against 1810 with stores from registers, 24831 x 7112 x 776 277 against 284,
+// dw of 32 groups of 512 rows, 4096 x 2048, 240 against 246. Shorter ones store
+// from registers (dw of 43 groups of 95 rows, 4040 x 1272, 165 us against 181 by
+// TMA).
 //
 // Ragged sizes cost what they are: a forward tile is as wide as its rows need
 // (a multiple of 32; N is a field of the instruction descriptor), a group of
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
   using L = GSmem<W::SETS>;
   constexpr bool DW = MODE == MODE_DW;
   constexpr bool A_MN = MODE != MODE_RC, B_MN = DW;
-  constexpr int PACED_FROM = DW ? 4 : 16;  // K-blocks of a tile from which its stores go by TMA
+  constexpr int PACED_FROM = 8;  // K-blocks of a tile from which its stores go by TMA
   constexpr int EPB = I8 ? 128 : 64;  // elements of the contraction in a K-block
   constexpr int STAGES = L::MAX_STAGES;
   constexpr uint32_t IDESC = (I8 ? umma_idesc_i8(256, 0) : umma_idesc_f16(256, 0, ElemTraits<TO>::kBf16)) |
