@@ -24,7 +24,10 @@ def quantize_i8(X, stream=None):
     if isinstance(X, torch.Tensor) and X.dim() != 2:
         if X.dim() == 0:
             raise bad("quantize_i8: X must have at least one dimension")
-        q, scale = quantize_i8(X.reshape(-1, X.shape[-1]), stream)
+        if X.is_cuda and elsewhere(X.get_device(), stream):
+            with on(X.get_device(), stream):  # reshape copies what cannot be viewed as rows: on the call's stream
+                return quantize_i8(X)
+        q, scale = quantize_i8(X.reshape(-1, X.shape[-1]))
         return q.view(X.shape), scale.view(X.shape[:-1])
     dev = tensor("quantize_i8", "X", X, 2, _ANY)
     if elsewhere(dev, stream):
