@@ -27,6 +27,8 @@ def quantize_i8(X, stream=None):
         if X.is_cuda and elsewhere(X.get_device(), stream):
             with on(X.get_device(), stream):  # reshape copies what cannot be viewed as rows: on the call's stream
                 return quantize_i8(X)
+        if X.shape[-1] == 0:
+            raise bad("quantize_i8: rows of X must not be empty")
         q, scale = quantize_i8(X.reshape(-1, X.shape[-1]))
         return q.view(X.shape), scale.view(X.shape[:-1])
     dev = tensor("quantize_i8", "X", X, 2, _ANY)

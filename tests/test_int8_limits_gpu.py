@@ -24,3 +24,14 @@ def test_quantize_strided_stack_on_a_stream(cuda):
         same = torch.equal(q, want[0]) and torch.equal(scale, want[1])
     torch.cuda.synchronize()
     assert q.shape == X.shape and scale.shape == X.shape[:-1] and same
+
+
+def test_quantize_refuses_empty_rows(cuda):
+    import torch
+    import kebab_b200 as kb
+    for shape in ((0,), (2, 0), (2, 3, 0), (0, 4, 0)):
+        with pytest.raises(kb.KebabError) as e:
+            kb.quantize_i8(torch.zeros(shape, device="cuda"))
+        assert e.value.code == kb.EINVAL, shape
+    q, scale = kb.quantize_i8(torch.zeros((0, 3, 8), device="cuda"))
+    assert q.shape == (0, 3, 8) and scale.shape == (0, 3)
