@@ -8,8 +8,9 @@ training and in serving.
 
 The layer is y[t] = sum_j w[t, j] W2_e (silu(Wg_e x[t]) * Wu_e x[t]) over the k
 experts e = e[t, j] that its router picks. `route`, `dispatch`, `combine` and
-`grouped_linear` below are the operators as differentiable functions. Nothing
-is copied to the host in a step: the ragged sizes stay on the device.
+`grouped_linear` below are the operators as functions with a first gradient; a
+second one raises (their backwards are calls that autograd does not see).
+Nothing is copied to the host in a step: the ragged sizes stay on the device.
 
 `python -m kebab_b200.moe` trains a small layer on a synthetic task and then
 serves single tokens with its experts quantised.
@@ -18,6 +19,7 @@ import argparse
 import sys
 
 import torch
+from torch.autograd.function import once_differentiable
 
 import kebab_b200 as kb
 
@@ -33,6 +35,7 @@ class _Route(torch.autograd.Function):
         return tuple(r)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dweights, *_):
         logits, *r = ctx.saved_tensors
         return kb.route_backward(logits, kb.Routing(*r), dweights.contiguous(), ctx.renormalize), None, None
@@ -45,6 +48,7 @@ class _Dispatch(torch.autograd.Function):
         return kb.dispatch(_rows(x), slots)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dxs):
         (slots,) = ctx.saved_tensors
         return kb.combine(_rows(dxs), slots), None
@@ -58,6 +62,7 @@ class _Combine(torch.autograd.Function):
         return kb.combine(ys, slots, weights)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         dys, dweights = kb.combine_backward(_rows(dy), *ctx.saved_tensors)
         return dys, None, dweights
@@ -71,6 +76,7 @@ class _GroupedLinear(torch.autograd.Function):
         return kb.gemm_grouped(x, w, offsets)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
         dy = _rows(dy)
