@@ -6,7 +6,9 @@
  *   Y[m, n] = scale[m] * w_scale[n] * sum_k q[m, k] * Wq[n, k]  (+ bias[n]),
  *
  * with amax_m the largest magnitude of row m, ties of rint to even, the sum
- * in 32-bit integers (exact; K <= 131072) and one rounding to the output type.
+ * in 32-bit integers and one rounding to the output type. The sum is exact:
+ * given codes are any int8 (-128 too), with K <= 131071; the codes made here
+ * are -127 .. 127, and kebab_linear_i8 takes K <= 131072.
  *
  * Plain C, device pointers, asynchronous on `stream`, status codes and
  * kebab_last_error() as in kebab.h. Rows are contiguous; `ld*` are row pitches

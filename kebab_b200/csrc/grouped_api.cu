@@ -76,12 +76,20 @@ int run_i8(int out, const int8_t* q, int64_t ldq, const float* scale, const int8
   return run(p);
 }
 
+// The longest K whose 32-bit sums are exact. Any codes: a product is at most
+// 2^14 (-128 twice), and 2^17 of them are 2^31. The codes that linear_i8 makes
+// are at least -127, products with any weights at most 127 * 2^7.
+constexpr int64_t kMaxKAny = (int64_t(1) << 17) - 1, kMaxKQuantized = int64_t(1) << 17;
+static_assert(kMaxKAny << 14 <= INT32_MAX && kMaxKQuantized * 127 * 128 <= INT32_MAX, "sums fit 32 bits");
+
 int check_i8(const char* what, int out, const void* X, int64_t ldx, const int8_t* Wq, int64_t ldw, int64_t w_stride,
-             const float* w_scale, const void* Y, int64_t ldy, int64_t E, int64_t R, int64_t N, int64_t K) {
+             const float* w_scale, const void* Y, int64_t ldy, int64_t E, int64_t R, int64_t N, int64_t K,
+             int64_t max_k) {
   int rc;
   if ((rc = check_type(what, out)) || (rc = check_sizes(what, E, R, N, K))) return rc;
-  if (K > 131072)  // 2^17 products of at most 2^14 stay below 2^31
-    return fail(KEBAB_EINVAL, std::string(what) + ": K above 131072 could overflow the 32-bit sums");
+  if (K > max_k)
+    return fail(KEBAB_EINVAL, std::string(what) + ": K above " + std::to_string(max_k) +
+                                  " could overflow the 32-bit sums");
   if ((rc = check_pitch(what, "X", ldx, K)) || (rc = check_pitch(what, "W", ldw, K)) ||
       (rc = check_pitch(what, "Y", ldy, N)))
     return rc;
@@ -146,7 +154,7 @@ int kebab_gemm_i8(kebab_dtype out, const int8_t* q, int64_t ldq, const float* sc
                   kebab_stream_t stream) {
   return guarded([&] {
     const char* what = "gemm_i8";
-    int rc = check_i8(what, out, q, ldq, Wq, ldw, 0, w_scale, Y, ldy, 1, M, N, K);
+    int rc = check_i8(what, out, q, ldq, Wq, ldw, 0, w_scale, Y, ldy, 1, M, N, K, kMaxKAny);
     if (rc || M == 0) return rc;
     if (!scale) return fail(KEBAB_EINVAL, "gemm_i8: null pointer");
     return run_i8(out, q, ldq, scale, Wq, ldw, 0, w_scale, bias, Y, ldy, nullptr, 1, M, N, K, false, stream);
@@ -158,7 +166,7 @@ int kebab_gemm_grouped_i8(kebab_dtype out, const int8_t* q, int64_t ldq, const f
                           const int32_t* offsets, int64_t E, int64_t R, int64_t N, int64_t K, kebab_stream_t stream) {
   return guarded([&] {
     const char* what = "gemm_grouped_i8";
-    int rc = check_i8(what, out, q, ldq, Wq, ldw, w_stride, w_scale, Y, ldy, E, R, N, K);
+    int rc = check_i8(what, out, q, ldq, Wq, ldw, w_stride, w_scale, Y, ldy, E, R, N, K, kMaxKAny);
     if (rc || R == 0) return rc;
     if (!scale || !offsets) return fail(KEBAB_EINVAL, "gemm_grouped_i8: null pointer");
     return run_i8(out, q, ldq, scale, Wq, ldw, w_stride, w_scale, nullptr, Y, ldy, offsets, E, R, N, K, false, stream);
@@ -176,7 +184,7 @@ int kebab_linear_i8(kebab_dtype dtype, const void* X, int64_t ldx, const int8_t*
                     int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, kebab_stream_t stream) {
   return guarded([&] {
     const char* what = "linear_i8";
-    int rc = check_i8(what, dtype, X, ldx, Wq, ldw, w_stride, w_scale, Y, ldy, E, M, N, K);
+    int rc = check_i8(what, dtype, X, ldx, Wq, ldw, w_stride, w_scale, Y, ldy, E, M, N, K, kMaxKQuantized);
     if (rc) return rc;
     if (offsets ? bias != nullptr : E != 1)
       return fail(KEBAB_EINVAL, offsets ? "linear_i8: a grouped product takes no bias"

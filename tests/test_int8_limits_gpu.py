@@ -1,7 +1,9 @@
-"""8-bit integer operators: the stream that a copy inside a call runs on."""
+"""8-bit integer operators: the stream that a copy inside a call runs on, and
+the longest sums."""
 import pytest
 
-from operator_util import randn
+from operator_util import assert_within, randn
+from test_int8_gpu import i8_bound
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +37,41 @@ def test_quantize_refuses_empty_rows(cuda):
         assert e.value.code == kb.EINVAL, shape
     q, scale = kb.quantize_i8(torch.zeros((0, 3, 8), device="cuda"))
     assert q.shape == (0, 3, 8) and scale.shape == (0, 3)
+
+
+@pytest.mark.parametrize("M,N", [(3, 300), (200, 300), (1000, 2561)])
+def test_longest_sums(cuda, M, N):
+    """Codes of -128 on both sides over the longest K that is admitted: sums
+    just below 2^31, in each kernel."""
+    import torch
+    import kebab_b200 as kb
+    K = 131071
+    q = torch.full((M, K + 1), -128, dtype=torch.int8, device="cuda")
+    wq = torch.full((N, K + 1), -128, dtype=torch.int8, device="cuda")
+    s, ws = torch.full((M,), 2.0 ** -20, device="cuda"), torch.full((N,), 2.0 ** -6, device="cuda")
+    want = torch.full((M, N), float(K << 14) * 2.0 ** -26, dtype=torch.float64, device="cuda")
+    bound = i8_bound(want, want.abs(), torch.bfloat16)
+    assert_within(kb.gemm_i8(q[:, :K], s, wq[:, :K], ws), want, bound, "Y")
+    offsets = torch.tensor([0, M], dtype=torch.int32, device="cuda")
+    assert_within(kb.gemm_grouped_i8(q[:, :K], s, wq[None, :, :K], ws[None], offsets), want, bound, "grouped")
+    if M == 3:  # rows that TMA cannot address
+        a, b = q.view(-1)[:M * K].view(M, K), wq.view(-1)[:N * K].view(N, K)
+        assert_within(kb.gemm_i8(a, s, b, ws), want, bound, "Y")
+
+
+def test_longest_sums_refused(cuda):
+    import torch
+    import kebab_b200 as kb
+    K = 131072
+    q = torch.full((8, K), -128, dtype=torch.int8, device="cuda")
+    s = torch.ones(8, device="cuda")
+    for call in (lambda: kb.gemm_i8(q, s, q, s),
+                 lambda: kb.gemm_grouped_i8(q, s, q[None], s[None], torch.tensor([0, 8], dtype=torch.int32, device="cuda"))):
+        with pytest.raises(kb.KebabError) as e:
+            call()
+        assert e.value.code == kb.EINVAL and "overflow" in str(e.value)
+    # Codes of linear_i8's activations end at -127: K = 131072 stays below 2^31.
+    x = torch.ones((8, K), dtype=torch.bfloat16, device="cuda")
+    y = kb.linear_i8(x, q, s * 2.0 ** -20)
+    want = torch.full((8, 8), -127.0 * 128 * K * 2.0 ** -20 / 127, dtype=torch.float64, device="cuda")
+    assert_within(y, want, i8_bound(want, want.abs(), torch.bfloat16) + want.abs() * 2.0 ** -23, "Y")
