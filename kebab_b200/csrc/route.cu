@@ -25,6 +25,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <mutex>
 
 #include "grouped.h"
 #include "kebab/experts.h"
@@ -397,14 +398,38 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteBackArgs
       static_cast<T*>(g.dlogits)[(t0 + m) * g.ldd + expert[m]] = from_float<T>(w[m] * (dw[m] - dot[m]));
 }
 
+// Shared memory of a block for E experts and k choices.
+constexpr size_t route_smem(int E, int k, bool one) {
+  return (size_t)(E * (1 + MASK_WORDS) + (one ? E + 1 : 0)) * sizeof(int) + (size_t)STEP * k * 6;
+}
+
+template <typename T, int LANES, int V, bool ONE>
+int route_smem_limit() {
+  // Once per device, for the most that this kernel is launched with: the limit
+  // belongs to the kernel, and other threads may be launching it.
+  constexpr size_t most = route_smem(LANES * V, MAX_CHOICES, ONE);
+  static std::once_flag once[64];
+  static cudaError_t err[64];
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  const int di = dev & 63;
+  std::call_once(once[di], [&] {
+    err[di] = cudaFuncSetAttribute(route_kernel<T, LANES, V, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+  });
+  return err[di] == cudaSuccess ? KEBAB_OK : cuda_fail(err[di], "cudaFuncSetAttribute(max dynamic smem)");
+}
+
 template <typename T, int LANES, int V>
 int launch_route(RouteArgs& g, cudaStream_t stream) {
   const bool one = g.T <= ONE_BLOCK;
-  const size_t smem = (size_t)(g.E * (1 + MASK_WORDS) + (one ? g.E + 1 : 0)) * sizeof(int) + (size_t)STEP * g.k * 6;
+  const size_t smem = route_smem(g.E, g.k, one);
   auto kern = one ? route_kernel<T, LANES, V, true> : route_kernel<T, LANES, V, false>;
+  if (smem > 48 * 1024) {
+    const int rc = one ? route_smem_limit<T, LANES, V, true>() : route_smem_limit<T, LANES, V, false>();
+    if (rc) return rc;
+  }
   cudaError_t e = cudaSuccess;
-  if (smem > 48 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
   const int blocks = one ? 1 : std::min(BLOCKS, (g.T + 63) / 64);
   g.chunk = one ? ONE_BLOCK : (g.T + blocks - 1) / blocks;
   const int grid = one ? 1 : (g.T + g.chunk - 1) / g.chunk;
