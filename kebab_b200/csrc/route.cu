@@ -344,9 +344,11 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteBackArgs
     w[m] = dw[m] = 0.f;
     expert[m] = -1;
     if (lane < g.k) {
+      expert[m] = g.experts[t * g.k + lane];
       w[m] = g.weights[t * g.k + lane];
       dw[m] = g.dweights[t * g.k + lane];
-      expert[m] = g.experts[t * g.k + lane];
+      // A dropped choice: no part of <w, dw> either.
+      if ((unsigned)expert[m] >= (unsigned)g.E) w[m] = dw[m] = 0.f;
     }
     dot[m] = w[m] * dw[m];
     if (!g.renormalize) {

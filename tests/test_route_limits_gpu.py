@@ -1,9 +1,11 @@
-"""Routing from several host threads."""
+"""Routing from several host threads, and its gradient where a choice names no
+expert."""
 import threading
 
+import numpy as np
 import pytest
 
-from operator_util import randn
+from operator_util import UNIT, assert_within, dtype_of, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +39,36 @@ def test_route_from_two_threads(cuda):
         t.join()
     assert codes == [{kb.OK}] * 4, kb.last_error()
     assert differ == [[]] * 4
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("T,E,k,dtype", [(5, 8, 3, "float32"), (77, 64, 6, "bfloat16"), (50, 130, 7, "float16"), (33, 1024, 32, "float32")])
+def test_route_backward_dropped_choices(cuda, T, E, k, dtype, renormalize):
+    """A choice whose expert is outside [0, E) contributes nothing: not to its
+    own logit and not, through <w, dw>, to the others of its token."""
+    import torch
+    import kebab_b200 as kb
+    logits, dw = randn((T, E), dtype_of(dtype), T), randn((T, k), torch.float32, 2)
+    r = kb.route(logits, k, renormalize=renormalize)
+    gone = torch.rand((T, k), generator=torch.Generator().manual_seed(3)) < 0.4
+    gone[0], gone[1] = True, False
+    far = torch.where(torch.arange(k) % 2 == 0, -1, E).expand(T, k)
+    experts = torch.where(gone, far, r.experts.cpu()).int().cuda()
+    got = kb.route_backward(logits, r._replace(experts=experts), dw, renormalize=renormalize)
+    x, w, d = logits.double().cpu().numpy(), r.weights.double().cpu().numpy(), dw.double().cpu().numpy()
+    live = ~gone.numpy()
+    chosen = r.experts.cpu().numpy().astype(np.int64)
+    g, p = np.zeros_like(x), np.zeros_like(x)
+    np.put_along_axis(g, chosen, np.where(live, d, 0.0), 1)
+    if renormalize:
+        np.put_along_axis(p, chosen, np.where(live, w, 0.0), 1)
+    else:
+        p = np.exp(x - x.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+    dot = (w * d * live).sum(1, keepdims=True)
+    want = p * (g - dot)
+    size = p * (np.abs(g) + (w * np.abs(d) * live).sum(1, keepdims=True))
+    # As for the gradient of whole rows: the exponent's rounding, sums over E and k terms.
+    spread = (x.max(1) - x.min(1))[:, None]
+    bound = 2.0 ** -22 * (2 * spread + E + 40) * size + UNIT[dtype] * np.abs(want) + 2.0 ** -25
+    assert_within(got.cpu(), torch.from_numpy(want), torch.from_numpy(bound), "dlogits")
