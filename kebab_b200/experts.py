@@ -94,6 +94,8 @@ def dispatch(x, slots, rows=None, stream=None):
         with on(dev, stream):
             return dispatch(x, slots, rows)
     rows = T * k if rows is None else rows
+    if rows < 0:
+        raise bad("dispatch: rows = %s is negative" % rows)
     xs = x.new_empty((rows, H))
     call("kebab_expert_dispatch", dev, CODES[x.dtype], x.data_ptr(), pitch(x), slots.data_ptr(), xs.data_ptr(), H, T, k,
          rows, H)
@@ -189,6 +191,8 @@ def gemm_grouped_dw(X, dY, offsets, dW=None, opmode="RC", stream=None):
     N = dY.shape[1]
     tensor(what, "offsets", offsets, 1, _I32, dev)
     E = offsets.shape[0] - 1
+    if E < 1:
+        raise bad("gemm_grouped_dw: offsets must have E + 1 values for E >= 1 experts")
     shape = (E, N, K) if m == "RC" else (E, K, N)
     if dW is not None:
         dense(what, "dW", dW, shape, (X.dtype,), dev)
