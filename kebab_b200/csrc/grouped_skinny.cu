@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(THREADS)
           else send16(dst + (c + j) * 4, bar, v[j], v[j + 1], v[j + 2], v[j + 3]);
         }
       }
-      ok = all_ok(mbar_wait(&recv_full, 0, ctx, SITE_PARTIAL)) && ok;
+      ok = all_ok(mbar_wait_cluster(&recv_full, 0, ctx, SITE_PARTIAL)) && ok;
       // The rows that this CTA keeps were written by some of its warps.
       asm volatile("bar.sync 1, 256;" ::: "memory");
       // Neighbouring threads take neighbouring n of one column of Y's.
