@@ -179,6 +179,7 @@ __global__ void __launch_bounds__(THREADS)
   const int per = ((total + S - 1) / S + kps - 1) / kps * kps;
   const int kb0 = min(total, rank * per), kb1 = min(total, kb0 + per);
   auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
+  bool ok = true;  // of every wait of this warp
 
   if (warp == 0 || warp == X_WARP) {
     // ---------------------------------------- producers: of W (warp 0), of X
@@ -188,8 +189,7 @@ __global__ void __launch_bounds__(THREADS)
     const uint32_t block_bytes = SUB + width * 128;
     if (early && !of_w) pdl_wait();
     int stage = 0;
-    uint32_t phase = 1, filled = 0, parity = 0;  // the last two: a bit a stage
-    bool ok = true;
+    uint32_t phase = 1;
     for (int kb = kb0; kb < kb1; kb += kps) {
       ok = all_ok(mbar_wait(&empty[stage], phase, ctx, SITE_EMPTY));
       if (!ok) break;
@@ -225,27 +225,18 @@ __global__ void __launch_bounds__(THREADS)
         }
       }
       __syncwarp();
-      filled |= 1u << stage;
-      parity = (parity & ~(1u << stage)) | ((phase ^ 1u) << stage);
       if (++stage == stages) {
         stage = 0;
         phase ^= 1u;
       }
     }
     if (early && of_w) pdl_wait();  // every path of a grid waits before it ends
-    if (!ok && of_w) {
-      // Abort: let the copies still in flight land before the CTA exits.
-      WaitCtx drain_ctx{ctx.status, 50000000ull};
-      for (int s = 0; s < stages; ++s)
-        if (filled >> s & 1u) mbar_wait(&full[s], parity >> s & 1u, drain_ctx, SITE_DRAIN);
-    }
   } else if (warp == 1) {
     // ----------------------------------------------------------- MMA issuer
     int stage = 0;
     uint32_t phase = 0;
     const uint32_t ring = smem_u32(smem), d_tmem = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t idesc = IDESC | (uint32_t)(__shfl_sync(0xffffffffu, width, 0) >> 3) << 17;
-    bool ok = true;
     for (int kb = kb0; kb < kb1; kb += kps) {
       ok = all_ok(mbar_wait(&full[stage], phase, ctx, SITE_FULL));
       if (!ok) break;
@@ -296,8 +287,7 @@ __global__ void __launch_bounds__(THREADS)
       cluster_wait_acquire();  // second half: the peers' barriers are set up
     }
     const bool some = kb1 > kb0;
-    bool ok = !some || mbar_wait(&acc_full, 0, ctx, SITE_TMEM_FULL);
-    ok = all_ok(ok);
+    ok = all_ok(!some || mbar_wait(&acc_full, 0, ctx, SITE_TMEM_FULL));
     tc_fence_after();
     if (S == 1) {
       const int n = n0 + row;
@@ -388,7 +378,12 @@ __global__ void __launch_bounds__(THREADS)
   // every epilogue thread has waited for, so the CTA may end after this.
   __syncwarp();
   tc_fence_before();
-  __syncthreads();
+  if (__syncthreads_or(!ok)) {
+    // Some wait ran out. Every CTA sends its rows whatever its waits gave, so
+    // recv_full completes soon after the last of the peers has given up too.
+    if (S > 1) mbar_drain(&recv_full, 0, ctx.timeout_ns + 1000000000ull);
+    settle();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<1>(tmem, 128);

@@ -172,6 +172,19 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
   return ok != 0;
 }
 
+// After a wait that ran out, before the CTA gives up the memory that is still
+// in use: a wait for the phase that does not stop for a recorded error, bounded
+// by `limit_ns`; and time for copies and MMAs in flight, which take microseconds.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait(smem_u32(bar), parity) && globaltimer() - t0 < limit_ns) {
+  }
+}
+__device__ __forceinline__ void settle() {
+  const uint64_t t0 = globaltimer();
+  while (globaltimer() - t0 < 1000000ull) __nanosleep(1000);
+}
+
 // As mbar_wait, but sleeps `backoff_ns` between polls once the first few have
 // failed: for waits that are expected to be long (an epilogue waiting out a
 // whole main loop), where tight polling only burns issue slots and power.

@@ -1,0 +1,37 @@
+"""Products whose waits run out: the call ends, the status says so, and the
+next call is right."""
+import pytest
+
+from operator_util import counts_of, offsets_of, randn
+
+pytestmark = pytest.mark.gpu
+
+
+def check_aborts(call):
+    """Repeats with a budget of 1 us a wait, which most first copies exceed."""
+    import torch
+    import kebab_b200 as kb
+    want = call()
+    assert kb.device_status()[0] == kb.OK
+    kb.set_wait_timeout_us(1)
+    try:
+        for _ in range(20):
+            got = call()
+            rc, code = kb.device_status()
+            assert rc == kb.ETIMEOUT or (rc == kb.OK and torch.equal(got, want)), hex(code)
+    finally:
+        kb.set_wait_timeout_us(2000000)
+    for _ in range(3):
+        assert torch.equal(call(), want)
+    assert kb.device_status()[0] == kb.OK
+
+
+@pytest.mark.parametrize("R,E,N,K", [(8, 1, 1024, 8192), (100, 3, 520, 4096), (60, 40, 1024, 512)])
+def test_few_rows(cuda, R, E, N, K):
+    """Split over k by clusters (the first two) and by single CTAs."""
+    import torch
+    import kebab_b200 as kb
+    X, W, offsets = randn((R, K), torch.bfloat16, 1), randn((E, N, K), torch.bfloat16, 2), offsets_of(counts_of("even", R, E))
+    check_aborts(lambda: kb.gemm_grouped(X, W, offsets))
+    wq, ws = kb.quantize_i8(W[0])
+    check_aborts(lambda: kb.linear_i8(X, wq, ws))
