@@ -106,10 +106,10 @@ struct GSmem {
   static constexpr int RUN = 32 / SETS;  // columns that an epilogue warp stores at a time
   static constexpr int C_SUB = RUN * 32 * 2 + 128 * 4;  // its: a run of columns of 32 values, 128 scales
   static constexpr int OFF_BAR = OFF_C + 8 * SETS * C_SUB;
-  // full, empty, tail_full, tail_done a stage; tmem_full and tmem_empty twice; drain
+  // full, empty, tail_full, tail_done a stage; tmem_full and tmem_empty twice
   static constexpr int TILES = 4;  // descriptions of tiles in flight: full and empty each
-  static constexpr int NUM_BARS = 4 * MAX_STAGES + 5 + 2 * TILES;
-  static constexpr int OFF_TILES = (OFF_BAR + NUM_BARS * 8 + 4 + 15) / 16 * 16;
+  static constexpr int NUM_BARS = 4 * MAX_STAGES + 4 + 2 * TILES;
+  static constexpr int OFF_TILES = (OFF_BAR + NUM_BARS * 8 + 8 + 15) / 16 * 16;  // after the TMEM address, abort
   static constexpr int OFF_TABLE = OFF_TILES + TILES * 32;
   // first[E + 1] (int), entry[E] (uint16, sorted only)
   static constexpr int bytes(int E, bool sorted) {
@@ -381,10 +381,10 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
   uint64_t* tail_done = tail_full + STAGES;  // dw, in the leader: both CTAs have cleared their shares of it
   uint64_t* tmem_full = tail_done + STAGES;
   uint64_t* tmem_empty = tmem_full + 2;
-  uint64_t* drain = tmem_empty + 2;
-  uint64_t* tile_full = drain + 1;
+  uint64_t* tile_full = tmem_empty + 2;
   uint64_t* tile_empty = tile_full + L::TILES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + L::NUM_BARS);
+  uint32_t* s_abort = tmem_slot + 1;  // some wait of the pair ran out
   Tile* s_tiles = reinterpret_cast<Tile*>(smem + L::OFF_TILES);
   int* s_first = reinterpret_cast<int*>(smem + L::OFF_TABLE);
   uint16_t* s_entry = reinterpret_cast<uint16_t*>(s_first + g.E + 1);
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
       mbar_init(&tile_full[a], 1);
       mbar_init(&tile_empty[a], W::EPILOGUE + W::TAIL + 1 + (leader ? 1 : 0));  // the warps that read descriptions
     }
-    mbar_init(drain, 1);
+    *s_abort = 0;
     fence_barrier_init();
   }
   __syncwarp();
@@ -456,13 +456,12 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     return x;
   };
   auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
+  bool ok = true;  // of every wait of this warp
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     int stage = 0;
     uint32_t phase = 0;
-    bool ok = true;
-    uint32_t issued = 0, parity = 0, tails = 0, tail_parity = 0;  // a bit a stage; tail_parity: of its next tail
     const uint32_t full_leader0 = mapa_shared(smem_u32(&full[0]), 0);
     const uint32_t tail_mine0 = mapa_shared(smem_u32(&tail_full[0]), rank);
     for (int i = 0; ok; ++i) {
@@ -536,26 +535,10 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
           }
         }
         __syncwarp();
-        issued |= 1u << stage;
-        if (tail) {
-          tails |= 1u << stage;
-          tail_parity ^= 1u << stage;
-        } else {
-          tails &= ~(1u << stage);
-          parity = (parity & ~(1u << stage)) | (phase << stage);
-        }
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
-      }
-    }
-    if (!ok) {
-      // Abort: let the copies still in flight land before the CTA exits.
-      WaitCtx drain_ctx{ctx.status, 50000000ull};
-      for (int s = 0; s < stages; ++s) {
-        if (tails >> s & 1u) mbar_wait(&tail_full[s], (tail_parity >> s & 1u) ^ 1u, drain_ctx, SITE_DRAIN);
-        else if (leader && (issued >> s & 1u)) mbar_wait(&full[s], parity >> s & 1u, drain_ctx, SITE_DRAIN);
       }
     }
   } else if (warp == 1) {
@@ -564,7 +547,6 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
       int stage = 0;
       uint32_t phase = 0, tail_parity = 0;
       uint32_t halves = 0;  // accumulators used so far: slot = bit 0, phase = bit 1
-      bool ok = true, any_issued = false;
       const uint32_t ring = smem_u32(smem);
       const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
       // The MMAs of half `s` over the stage `at`, whose first K-block is kb;
@@ -608,7 +590,6 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
           if (last) umma_commit_cg2_mc(&tmem_full[slot], 0x3);
         }
         __syncwarp();
-        any_issued = true;
         return true;
       };
       for (int i = 0; ok; ++i) {
@@ -653,12 +634,6 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         }
         if (x.blocks) halves += x.nsub;
       }
-      if (!ok && any_issued && elect_one()) {
-        // Abort: wait for the MMAs already issued before TMEM is freed.
-        umma_commit_cg2_mc(drain, 0x1);
-        WaitCtx drain_ctx{ctx.status, 50000000ull};
-        mbar_wait(drain, 0, drain_ctx, SITE_DRAIN);
-      }
     }
   } else if (warp == W::EPILOGUE + 2) {
     // ------------------------------------------------------- tiles, in order
@@ -670,7 +645,8 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
       x.e = -1;
       if (t < num_tiles) x = tile_of<MODE, EPB>(t, g, tab);
       const int at = i % L::TILES;
-      if (!all_ok(mbar_wait(&tile_empty[at], (i / L::TILES & 1) ^ 1u, ctx, SITE_TILE))) break;
+      ok = all_ok(mbar_wait(&tile_empty[at], (i / L::TILES & 1) ^ 1u, ctx, SITE_TILE));
+      if (!ok) break;
       if (lane == 0) {
         s_tiles[at] = x;
         mbar_arrive(&tile_full[at]);
@@ -686,7 +662,10 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     const uint32_t tail_done_leader0 = mapa_shared(smem_u32(&tail_done[0]), 0);
     for (int i = 0;; ++i) {
       const Tile x = next_tile(i);
-      if (x.e < 0) break;
+      if (x.e < 0) {
+        ok = x.e == -1;
+        break;
+      }
       if (x.blocks == 0) {
         // A group without rows: the whole tile, each CTA every other column, 512
         // contiguous bytes a step (108 experts of 2552 x 2648, all but one empty:
@@ -709,7 +688,8 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
         }
       } else if ((x.rows & 15) != 0) {
         const int at = (stage + max(x.blocks - 2, 0)) % stages;
-        if (!all_ok(mbar_wait(&tail_full[at], tail_parity >> at & 1u, ctx, SITE_FULL))) break;
+        ok = all_ok(mbar_wait(&tail_full[at], tail_parity >> at & 1u, ctx, SITE_FULL));
+        if (!ok) break;
         // Rows left .. the end of its 16-row step, in every box of 64 columns
         // (128-byte rows; the swizzle stays within a row).
         uint8_t* sA = smem + at * stage_bytes;
@@ -742,10 +722,12 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     const uint32_t tmem_empty_leader0 = mapa_shared(smem_u32(&tmem_empty[0]), 0);
     const uint32_t t_quarter = tmem_base + ((uint32_t)(q * 32) << 16);
     uint32_t halves = 0;
-    bool ok = true;
     for (int i = 0; ok; ++i) {
       const Tile x = next_tile(i);
-      if (x.e < 0) break;
+      if (x.e < 0) {
+        ok = x.e == -1;
+        break;
+      }
       const int limit = DW ? g.DB : x.rows;  // columns end here
       const int cols = x.width / 2;          // of this warp, a multiple of 16
       const int d0 = side * cols;            // its first column in the tile
@@ -870,9 +852,13 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
   }
 
   // ------------------------------------------------------------- teardown
+  // A wait of either CTA ran out: both stay until what is in flight between them
+  // (copies, the pair's MMAs and their arrivals) has ended.
+  if (!ok && lane < 2) store_cluster(mapa_shared(smem_u32(s_abort), lane), 1);
   __syncwarp();
   tc_fence_before();
   cluster_sync();
+  if (*s_abort) settle();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<2>(tmem_base, 512);

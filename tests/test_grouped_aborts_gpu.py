@@ -35,3 +35,18 @@ def test_few_rows(cuda, R, E, N, K):
     check_aborts(lambda: kb.gemm_grouped(X, W, offsets))
     wq, ws = kb.quantize_i8(W[0])
     check_aborts(lambda: kb.linear_i8(X, wq, ws))
+
+
+@pytest.mark.parametrize("N", [2056, 8200])
+def test_persistent(cuda, N):
+    """Panels of 256 and of 512 rows, groups with odd ends and without rows."""
+    import torch
+    import kebab_b200 as kb
+    counts, K = [900, 0, 257, 1, 1500, 255, 1024, 33, 512, 130], 520
+    R, E, offsets = sum(counts), len(counts), offsets_of(counts)
+    X, W, dY = randn((R, K), torch.float16, 1), randn((E, N, K), torch.float16, 2), randn((R, N), torch.float16, 3)
+    check_aborts(lambda: kb.gemm_grouped(X, W, offsets))
+    check_aborts(lambda: kb.gemm_grouped(dY, W, offsets, opmode="RR"))
+    check_aborts(lambda: kb.gemm_grouped_dw(X, dY, offsets))
+    wq, ws = kb.quantize_i8(W)
+    check_aborts(lambda: kb.linear_grouped_i8(X, wq, ws, offsets))
