@@ -7,18 +7,20 @@ from operator_util import counts_of, offsets_of, randn
 pytestmark = pytest.mark.gpu
 
 
-def check_aborts(call):
-    """Repeats with a budget of 1 us a wait, which most first copies exceed."""
+def check_aborts(call, expires=False):
+    """Repeats with a budget of 1 us a wait. Whether a short wait reaches it is
+    chance (it is looked at every 64 polls); an epilogue's wait for a main loop
+    of a millisecond does."""
     import torch
     import kebab_b200 as kb
     want = call()
     assert kb.device_status()[0] == kb.OK
     kb.set_wait_timeout_us(1)
     try:
-        for _ in range(20):
+        for _ in range(4 if expires else 20):
             got = call()
             rc, code = kb.device_status()
-            assert rc == kb.ETIMEOUT or (rc == kb.OK and torch.equal(got, want)), hex(code)
+            assert rc == kb.ETIMEOUT or (rc == kb.OK and not expires and torch.equal(got, want)), hex(code)
     finally:
         kb.set_wait_timeout_us(2000000)
     for _ in range(3):
@@ -50,3 +52,24 @@ def test_persistent(cuda, N):
     check_aborts(lambda: kb.gemm_grouped_dw(X, dY, offsets))
     wq, ws = kb.quantize_i8(W)
     check_aborts(lambda: kb.linear_grouped_i8(X, wq, ws, offsets))
+
+
+def ramp(*shape):
+    """Small whole numbers, their sums exact."""
+    import torch
+    return (torch.arange(shape[-1], device="cuda") % 7).to(torch.bfloat16).expand(*shape).contiguous()
+
+
+@pytest.mark.parametrize("R,N,K", [(8, 128, 1 << 22), (8, 20480, 1 << 17), (512, 5120, 1 << 19)])
+def test_epilogue_gives_up(cuda, R, N, K):
+    """Clusters that split k, single CTAs, and pairs with several tiles each."""
+    import kebab_b200 as kb
+    X, W, offsets = ramp(R, K), ramp(1, N, K), offsets_of([R])
+    check_aborts(lambda: kb.gemm_grouped(X, W, offsets), expires=True)
+
+
+def test_epilogue_gives_up_in_dw(cuda):
+    import kebab_b200 as kb
+    R = (1 << 20) + 5
+    X, dY, offsets = ramp(R, 2560), ramp(R, 2560), offsets_of([R, 0])
+    check_aborts(lambda: kb.gemm_grouped_dw(X, dY, offsets), expires=True)
