@@ -639,11 +639,12 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     // ------------------------------------------------------- tiles, in order
     const int num_tiles = s_first[g.E] * tab.panels;
     for (int i = 0;; ++i) {
-      // Back and forth over the pairs.
-      const int t = i * pairs + ((i & 1) ? pairs - 1 - pair : pair);
+      // Back and forth over the pairs. (64 bits: groups that overlap, as offsets
+      // that fall make them, can have up to 2^31 tiles.)
+      const int64_t t = (int64_t)i * pairs + ((i & 1) ? pairs - 1 - pair : pair);
       Tile x;
       x.e = -1;
-      if (t < num_tiles) x = tile_of<MODE, EPB>(t, g, tab);
+      if (t < num_tiles) x = tile_of<MODE, EPB>((int)t, g, tab);
       const int at = i % L::TILES;
       ok = all_ok(mbar_wait(&tile_empty[at], (i / L::TILES & 1) ^ 1u, ctx, SITE_TILE));
       if (!ok) break;
