@@ -1,5 +1,5 @@
-"""8-bit integer operators: the stream that a copy inside a call runs on, and
-the longest sums."""
+"""8-bit integer operators: the stream that a copy inside a call runs on, the
+longest sums, and weights that are written right before they are read."""
 import pytest
 
 from operator_util import assert_within, randn
@@ -75,3 +75,31 @@ def test_longest_sums_refused(cuda):
     y = kb.linear_i8(x, q, s * 2.0 ** -20)
     want = torch.full((8, 8), -127.0 * 128 * K * 2.0 ** -20 / 127, dtype=torch.float64, device="cuda")
     assert_within(y, want, i8_bound(want, want.abs(), torch.bfloat16) + want.abs() * 2.0 ** -23, "Y")
+
+
+@pytest.mark.parametrize("M", [1, 64, 300])
+def test_weights_written_right_before(cuda, M):
+    """linear_i8 fetches weights while it still quantises; what the stream
+    wrote into them just before has to be there."""
+    import torch
+    import kebab_b200 as kb
+    N, K = 2048, 4096
+    x = randn((M, K), torch.bfloat16, 1)
+    stacks = [randn((N, K), torch.bfloat16, 2 + i) for i in range(3)]
+    want = []
+    for w in stacks:
+        q = kb.quantize_i8(w)
+        torch.cuda.synchronize()
+        want.append(kb.linear_i8(x, *q))
+        torch.cuda.synchronize()
+    wq, ws = torch.zeros((N, K), dtype=torch.int8, device="cuda"), torch.zeros(N, device="cuda")
+    got = []
+    for i in range(30):
+        q, s = kb.quantize_i8(stacks[i % 3])
+        if i % 2:  # written by a plain copy, or by the framework's own kernel
+            wq.copy_(q), ws.copy_(s)
+            q, s = wq, ws
+        got.append(kb.linear_i8(x, q, s))
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % 3]), i
