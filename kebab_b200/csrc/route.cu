@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouteBackArgs
       static_cast<T*>(g.dlogits)[(t0 + m) * g.ldd + expert[m]] = from_float<T>(w[m] * (dw[m] - dot[m]));
 }
 
-// Shared memory of a block for E experts and k choices.
+// Dynamic shared memory of a block for E experts and k choices.
 constexpr size_t route_smem(int E, int k, bool one) {
   return (size_t)(E * (1 + MASK_WORDS) + (one ? E + 1 : 0)) * sizeof(int) + (size_t)STEP * k * 6;
 }
@@ -427,7 +427,8 @@ int launch_route(RouteArgs& g, cudaStream_t stream) {
   const bool one = g.T <= ONE_BLOCK;
   const size_t smem = route_smem(g.E, g.k, one);
   auto kern = one ? route_kernel<T, LANES, V, true> : route_kernel<T, LANES, V, false>;
-  if (smem > 48 * 1024) {
+  // Up to 48 KB, s_sum included, need no opt-in.
+  if (smem + STEP * sizeof(float) > 48 * 1024) {
     const int rc = one ? route_smem_limit<T, LANES, V, true>() : route_smem_limit<T, LANES, V, false>();
     if (rc) return rc;
   }

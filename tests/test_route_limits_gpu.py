@@ -1,11 +1,12 @@
-"""Routing from several host threads, and its gradient where a choice names no
-expert."""
+"""Routing from several host threads, at the sizes where a block passes 48 KB of
+shared memory, and its gradient where a choice names no expert."""
 import threading
 
 import numpy as np
 import pytest
 
 from operator_util import UNIT, assert_within, dtype_of, randn
+from test_experts_gpu import check_route
 
 pytestmark = pytest.mark.gpu
 
@@ -39,6 +40,12 @@ def test_route_from_two_threads(cuda):
         t.join()
     assert codes == [{kb.OK}] * 4, kb.last_error()
     assert differ == [[]] * 4
+
+
+@pytest.mark.parametrize("T,E,k", [(414, 831, 12), (414, 810, 12), (200, 840, 12), (100, 831, 10), (128, 1001, 5), (129, 1024, 8),
+                                   (300, 512, 19), (300, 512, 20), (77, 600, 16), (300, 520, 20)])
+def test_route_around_48_kb(cuda, T, E, k):
+    check_route(randn((T, E), dtype_of("float32"), T), k, True)
 
 
 @pytest.mark.parametrize("renormalize", [True, False])
