@@ -400,6 +400,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
   const bool leader = rank == 0;
   const WaitCtx& ctx = g.ctx;
 
+  cluster_arrive_release();  // this CTA has started
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
@@ -421,15 +422,15 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
     fence_barrier_init();
   }
   __syncwarp();
-  cluster_arrive_release();  // the pair's barriers; the other half is below
+  // The pair allocates together: not before the other CTA has started. With
+  // kernels of several streams on the SMs a pair that did hung in it.
+  cluster_wait_acquire();
   if (warp == 1) {
-    // The pair allocates together: not before the other CTA has started. With
-    // kernels of several streams on the SMs a pair that did hung in it.
-    cluster_wait_acquire();
     tmem_alloc<2>(tmem_slot, 512);
     tmem_relinquish<2>();
   }
   __syncwarp();
+  cluster_arrive_release();  // the pair's barriers; the other half is below
   if (g.pdl) {
     pdl_wait();
     pdl_launch_dependents();
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
   fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
-  if (warp != 1) cluster_wait_acquire();
+  cluster_wait_acquire();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int kps = tab.kps;
