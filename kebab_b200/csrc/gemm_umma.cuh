@@ -328,6 +328,7 @@ __global__ void __launch_bounds__(UmmaEpi<BN>::THREADS, 1)
   ClockProbe probe;
   probe.begin(args.clk);
 
+  if constexpr (CG == 2) cluster_arrive_release();  // this CTA has started
   if (threadIdx.x == 0) {
 #ifdef KEBAB_SK_TRACE
     g_sk_trace[((size_t)blockIdx.x * 8 + 7) * 8 + 5] = globaltimer();
@@ -345,6 +346,12 @@ __global__ void __launch_bounds__(UmmaEpi<BN>::THREADS, 1)
     }
     mbar_init(drain, 1);
     fence_barrier_init();
+  }
+  // A pair allocates together: not before the other CTA has started (with
+  // kernels of several streams on the SMs a pair that does can hang in it).
+  if constexpr (CG == 2) {
+    __syncwarp();
+    cluster_wait_acquire();
   }
   if (warp == 1) {
     tmem_alloc<CG>(tmem_slot, TMEM_COLS);

@@ -79,6 +79,10 @@ __global__ void __launch_bounds__(128, 1) umma_probe_kernel(int iters, int n, in
     for (int i = threadIdx.x; i < 2048; i += blockDim.x) e[i] = 0x44;
     fence_proxy_async_smem();
   }
+  if constexpr (CG == 2) {  // a pair allocates together, once both of its CTAs have started
+    __syncwarp();
+    cluster_sync();
+  }
   if (warp == 0) {
     tmem_alloc<CG>(m.slot, COLS);
     tmem_relinquish<CG>();

@@ -63,3 +63,21 @@ def test_several_streams(cuda):
     run_together(operators(), 4, 3.0)
     rc, code = kb.device_status()
     assert rc == kb.OK, hex(code)
+
+
+def test_pair_kernels_on_several_streams(cuda):
+    """The GEMM rungs of CTA pairs and the 2:4 product beside the grouped ones
+    (not stream-K, whose CTAs wait for one another)."""
+    import torch
+    import kebab_b200 as kb
+    ops = []
+    for version, (M, N, K) in ((105, (512, 1024, 512)), (105, (2048, 2048, 256)), (107, (512, 1024, 512)), (107, (2048, 4096, 512)),
+                               (112, (512, 768, 512)), (112, (2048, 1536, 512)), (104, (1024, 1024, 512))):
+        A, B = randn((M, K), torch.bfloat16, 1), randn((N, K), torch.bfloat16, 2)
+        ops.append(lambda A=A, B=B, v=version: kb.gemm(A, B, version=v))
+    A, B = randn((512, 1024), torch.float16, 3), randn((512, 1024), torch.float16, 4)
+    packed, E = kb.sparse24_compress(kb.sparse24_prune(A))
+    ops.append(lambda: kb.gemm_sparse24(packed, E, B))
+    run_together(ops + operators(), 4, 3.0)
+    rc, code = kb.device_status()
+    assert rc == kb.OK, hex(code)
