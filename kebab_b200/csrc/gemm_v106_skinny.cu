@@ -152,7 +152,8 @@ __global__ void __launch_bounds__(192, 1)
     int stage = 0;
     uint32_t phase = 0;
     for (int i = 0; i < nkb; ++i) {
-      if (!mbar_wait(&empty[stage], phase ^ 1u, ctx, SITE_EMPTY)) break;
+      ok = mbar_wait(&empty[stage], phase ^ 1u, ctx, SITE_EMPTY);
+      if (!ok) break;
       uint8_t* sBt = smem + stage * L::STAGE;
       uint8_t* sA = sBt + KSUB * L::BT_SUB;
       mbar_arrive_expect_tx(&full[stage], L::STAGE);
@@ -170,7 +171,8 @@ __global__ void __launch_bounds__(192, 1)
     int stage = 0;
     uint32_t phase = 0;
     for (int i = 0; i < nkb; ++i) {
-      if (!mbar_wait(&full[stage], phase, ctx, SITE_FULL)) break;
+      ok = mbar_wait(&full[stage], phase, ctx, SITE_FULL);
+      if (!ok) break;
       if (i == 0) SKY_TRACE(2);
       tc_fence_after();
       const uint32_t bt = smem_u32(smem + stage * L::STAGE);
@@ -204,6 +206,7 @@ __global__ void __launch_bounds__(192, 1)
       } else {
         ok = false;
       }
+      ok = __all_sync(0xffffffffu, ok) != 0;  // the warp loads from TMEM, or not, together
     }
   }
   if constexpr (!L::SEPARATE) {
@@ -255,7 +258,8 @@ __global__ void __launch_bounds__(192, 1)
     // Reduce this rank's slice of this thread's row over the S partials, in
     // rank order (deterministic). The local block was written by this thread;
     // the peers' blocks are complete once recv_full flips.
-    const bool got = SPLITS == 1 || mbar_wait(recv_full, 0, ctx, SITE_PARTIAL);
+    const bool got = SPLITS == 1 || mbar_wait_cluster(recv_full, 0, ctx, SITE_PARTIAL);
+    ok = ok && got;
     if (threadIdx.x == 64) SKY_TRACE(12);
     const int c0 = m0 + ks * CS;
     const int n = n0 + row;
@@ -300,7 +304,12 @@ __global__ void __launch_bounds__(192, 1)
   // epilogue thread waited for, so the CTA may exit after this barrier.
   __syncwarp();
   tc_fence_before();
-  __syncthreads();
+  if (__syncthreads_or(!ok)) {
+    // Some wait ran out. Every CTA pushes its slices whatever its waits gave, so
+    // recv_full completes soon after the last of the peers has given up too.
+    if (SPLITS > 1) mbar_drain(recv_full, 0, ctx.timeout_ns + 1000000000ull);
+    settle();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<1>(tmem, TMEM_COLS);

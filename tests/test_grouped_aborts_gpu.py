@@ -73,3 +73,10 @@ def test_epilogue_gives_up_in_dw(cuda):
     R = (1 << 20) + 5
     X, dY, offsets = ramp(R, 2560), ramp(R, 2560), offsets_of([R, 0])
     check_aborts(lambda: kb.gemm_grouped_dw(X, dY, offsets), expires=True)
+
+
+def test_epilogue_gives_up_in_split_gemm(cuda):
+    """The dense swap-AB rung, which splits k over a cluster in the same way."""
+    import kebab_b200 as kb
+    A, B = ramp(8, 1 << 22), ramp(128, 1 << 22)
+    check_aborts(lambda: kb.gemm(A, B, version=106), expires=True)
