@@ -8,7 +8,9 @@
 //   dw       i = n, j = k, p = row of the group   ("RR": i = k, j = n)
 // A block computes a 64 x 64 tile with 16 x 16 threads of 4 x 4 outputs each,
 // 16 terms of p at a time from shared memory. It is bound by its loads and
-// shared-memory reads (two 16-byte reads feed 16 multiply-adds).
+// shared-memory reads (two 16-byte reads feed 16 multiply-adds): 4096 rows over 8
+// groups, 4096 x 4100, 16 bits, 5970 us where 4096 x 4096 take 133 on the tensor
+// cores; 8 bits and one row of 4096 x 4100 474 against 7.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -126,7 +126,9 @@ __global__ void __launch_bounds__(THREADS)
                              (RR ? (1u << 15) : 0u);
   const bool early = g.early && g.pdl;
   // A kernel that touches memory before its predecessor is done must not let
-  // its successor start.
+  // its successor start. The successor of others may start before this CTA has
+  // allocated TMEM: beside its 83 KB or more of shared memory only another CTA
+  // of this kernel fits, and their 128 columns each.
   if (!early && g.pdl) {
     pdl_wait();
     pdl_launch_dependents();

@@ -674,7 +674,7 @@ __global__ void __launch_bounds__(Warps<MODE>::THREADS, 1)
       if (x.blocks == 0) {
         // A group without rows: the whole tile, each CTA every other column, 512
         // contiguous bytes a step (108 experts of 2552 x 2648, all but one empty:
-        // 340 us, 680 from the epilogue, whose warps write 64 bytes at a time).
+        // 306 us, 680 from the epilogue, whose warps write 64 bytes at a time).
         const int b0 = x.b0 + (int)rank, columns = (min(x.b0 + x.width, g.DB) - b0 + 1) / 2;
         const int end = min(x.a0 + x.nsub * 256, g.DA);
         uint16_t* y = static_cast<uint16_t*>(g.Y) + ((int64_t)x.e * g.DB + b0) * g.ldy;

@@ -11,7 +11,8 @@
 //
 // The code is x * (127 / amax), one multiplication by a once-rounded quotient:
 // a division of every value would cost about ten instructions each, and the
-// two roundings differ only where x / scale lies within 2^-22 of a tie.
+// two roundings differ only where x / scale lies within 2^-22 of its own size of
+// a tie (2^-15 for codes near 127).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

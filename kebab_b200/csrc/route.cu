@@ -16,7 +16,9 @@
 // each block writes its counts by expert, and a second launch, with the same
 // split, adds the counts of all earlier blocks and all lower experts.
 //
-// Bound by latency for few tokens and by the choices' instructions for many; the
+// Bound by latency for few tokens and by the choices' instructions for many (32768
+// tokens of 64 experts, 6 choices: 917 for a warp's 4 tokens, issued in 65 % of
+// the active cycles); the second launch waits for memory (it issues in 11 %). The
 // logits' bytes are few. A whole warp a token reduces with the warp-wide
 // instructions, fewer lanes with shuffles: 1 token of 128 experts, 8 choices,
 // 3.7 us with 32 lanes and 5.9 with 16; 32768 tokens of 64 experts, 6 choices,
@@ -321,6 +323,8 @@ struct RouteBackArgs {
 // Otherwise, with p the softmax over all: dl = p (dw - <w, dw>), dw 0 where not
 // chosen. The lanes write the row as if nothing were chosen, and then the k
 // chosen places (w is p there).
+// 32768 tokens of 64 experts, 6 choices: 8.6 us, bound by its instructions (issued
+// in 71 % of the cycles).
 // Tokens that a warp has in flight, by the logits a lane holds of each.
 template <int VPL>
 struct BackShape {
