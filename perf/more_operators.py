@@ -380,7 +380,8 @@ def _exact_f4(x):
     x = x.double()
     b = _blocks(x)
     top = b.abs().amax(-1, keepdim=True)
-    e = torch.where(top > 0, torch.ceil(torch.log2(torch.where(top > 0, top, 1.0) / 6)), -127.0).clamp(min=-127)
+    e = torch.where(top > 0, torch.round(torch.log2(torch.where(top > 0, top, 1.0) / 6)), -127.0)
+    e = (e + (top > 6 * torch.exp2(e)).double()).clamp(min=-127)  # the logarithm itself may be off by a little
     v = b.abs() / torch.exp2(e)
     middle = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, 1e300], dtype=torch.float64, device=x.device)
     code = torch.bucketize(v, middle)  # how many of them are below v; on one: the lower code, unless that is odd
