@@ -339,12 +339,15 @@ def gemm_sparse24(A_packed, E, B, C=None, stream=None):
 
 
 # ----------------------------------------------------------------------------- language-model operators
-# Mixture-of-experts and 8-bit integer operators; their modules import torch,
-# so they are loaded on first use.
+# Mixture-of-experts operators, 8-bit integer and 4-bit products, norms; their
+# modules import torch, so they are loaded on first use.
 _OPERATORS = {"quantize_i8": "int8", "gemm_i8": "int8", "gemm_grouped_i8": "int8", "linear_i8": "int8",
               "linear_grouped_i8": "int8", "Routing": "experts", "route": "experts", "route_backward": "experts",
               "dispatch": "experts", "combine": "experts", "combine_backward": "experts", "gemm_grouped": "experts",
-              "gemm_grouped_dw": "experts"}
+              "gemm_grouped_dw": "experts", "rms_norm": "norm", "rms_norm_i8": "norm", "rms_norm_backward": "norm",
+              "Normed8": "norm", "F4": "f4", "F4Tokens": "f4", "quantize_f4": "f4", "quantize_f4_tokens": "f4",
+              "dequantize_f4": "f4", "gemm_f4": "f4", "gemm_grouped_f4": "f4", "linear_f4": "f4",
+              "linear_grouped_f4": "f4", "FEW_TOKENS": "layer", "expert_layer": "layer", "expert_layer_i8": "layer"}
 
 
 def __getattr__(name):

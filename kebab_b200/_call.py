@@ -7,7 +7,7 @@ import torch
 from . import BF16, EINVAL, F16, F32, KebabError, lib
 from . import check as _check
 
-P, I, L = c.c_void_p, c.c_int, c.c_int64
+P, I, L, F = c.c_void_p, c.c_int, c.c_int64, c.c_float
 _SIGNATURES = {
     "kebab_quantize_i8": [I, P, L, P, L, P, L, L, P],
     "kebab_gemm_i8": [I, P, L, P, P, L, P, P, P, L, L, L, L, P],
@@ -20,6 +20,17 @@ _SIGNATURES = {
     "kebab_expert_combine_backward": [I, P, L, P, L, P, P, P, L, P, L, I, L, L, P],
     "kebab_gemm_grouped": [I, P, L, P, L, L, P, L, P, L, L, L, L, c.c_char_p, P],
     "kebab_gemm_grouped_dw": [I, P, L, P, L, P, P, L, L, L, L, c.c_char_p, P],
+    "kebab_rms_norm": [I, I, P, L, P, L, P, F, P, L, P, L, L, L, P],
+    "kebab_rms_norm_i8": [I, I, P, L, P, L, P, F, P, L, P, L, P, L, P, L, L, P],
+    "kebab_rms_norm_backward": [I, I, P, L, P, L, P, F, P, L, P, L, P, P, L, L, L, P],
+    "kebab_quantize_f4": [I, P, L, L, P, P, L, L, L, P],
+    "kebab_quantize_f4_tokens": [I, P, L, P, P, L, L, P],
+    "kebab_dequantize_f4": [I, P, P, P, L, L, L, P],
+    "kebab_gemm_f4": [I, P, P, P, P, P, P, L, L, L, L, P],
+    "kebab_gemm_grouped_f4": [I, P, P, P, P, P, L, P, L, L, L, L, P],
+    "kebab_linear_f4": [I, P, L, P, P, P, P, L, P, L, L, L, L, P, L, P],
+    "kebab_expert_layer": [I, P, L, P, P, P, P, L, L, L, I, I, L, L, P, L, P],
+    "kebab_expert_layer_i8": [I, P, L, P, P, P, P, P, P, L, L, L, I, I, L, L, P, L, P],
 }
 CODES = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
 _functions = {}

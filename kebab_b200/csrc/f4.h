@@ -1,0 +1,30 @@
+// Internal declarations of the 4-bit floating-point products.
+#pragma once
+#include "grouped.h"
+
+namespace kb {
+
+// Y[r, n] = sum_k X[r, k] W_e(n, k) for the rows r of group e, of quantised
+// operands stored as include/kebab/f4.h says.
+struct F4Problem {
+  int out;  // KEBAB_F16 or KEBAB_BF16
+  const uint8_t* x_codes;
+  const uint8_t* x_scales;
+  const uint8_t* w_codes;
+  const uint8_t* w_scales;
+  const void* bias;  // output type, per n, or null
+  void* Y;
+  int64_t ldy;
+  const int32_t* offsets;  // E + 1 device integers; null: one group of all R rows
+  int64_t E, R, N, K;
+  bool early;  // the kernel before on the stream makes only the codes and scales of X
+  cudaStream_t stream;
+};
+
+constexpr int F4_SLACK = 160;  // entries of token scales past the last row
+
+__host__ __device__ inline int64_t f4_pitch(int64_t K) { return (K + 31) / 32 * 16; }  // bytes of a row's codes
+
+int launch_f4_simt(const F4Problem& p);
+
+}  // namespace kb

@@ -1,0 +1,91 @@
+// C entry points of the 4-bit floating-point products (include/kebab/f4.h):
+// argument checks and the choice of kernel.
+#include <string>
+
+#include "f4.h"
+#include "kebab/f4.h"
+
+namespace kb {
+namespace {
+constexpr int64_t kMaxDim = int64_t(1) << 30;  // leaves room for tile arithmetic in 32 bits
+
+int run(const char* what, const F4Problem& p) {
+  if (p.out != KEBAB_F16 && p.out != KEBAB_BF16)
+    return fail(KEBAB_ENOTSUP, std::string(what) + ": only F16 and BF16 are implemented");
+  if (p.E < 1 || p.E > kMaxExperts)
+    return fail(KEBAB_EINVAL, std::string(what) + ": number of experts " + std::to_string(p.E) + " is not in 1.." +
+                                  std::to_string(kMaxExperts));
+  if (p.R < 0 || p.N <= 0 || p.K <= 0 || p.R > kMaxDim || p.N > kMaxDim || p.K > kMaxDim)
+    return fail(KEBAB_EINVAL, std::string(what) + ": invalid dimensions rows=" + std::to_string(p.R) +
+                                  " N=" + std::to_string(p.N) + " K=" + std::to_string(p.K));
+  if (p.ldy < p.N)
+    return fail(KEBAB_EINVAL, std::string(what) + ": row pitch of Y (" + std::to_string(p.ldy) +
+                                  ") is below its row length (" + std::to_string(p.N) + ")");
+  if (!p.w_codes || !p.w_scales || (p.R > 0 && (!p.x_codes || !p.x_scales || !p.Y)))
+    return fail(KEBAB_EINVAL, std::string(what) + ": null pointer");
+  auto off16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) != 0; };
+  if (off16(p.w_codes) || off16(p.w_scales) || off16(p.x_codes) || off16(p.x_scales))
+    return fail(KEBAB_EINVAL, std::string(what) + ": codes and scales must be 16-byte aligned");
+  if (p.R == 0) return KEBAB_OK;
+  return launch_f4_simt(p);
+}
+}  // namespace
+}  // namespace kb
+
+using namespace kb;
+
+extern "C" {
+
+int kebab_gemm_f4(kebab_dtype out, const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes,
+                  const uint8_t* w_scales, const void* bias, void* Y, int64_t ldy, int64_t M, int64_t N, int64_t K,
+                  kebab_stream_t stream) {
+  return guarded([&] {
+    return run("gemm_f4", {out, x_codes, x_scales, w_codes, w_scales, bias, Y, ldy, nullptr, 1, M, N, K, false,
+                           reinterpret_cast<cudaStream_t>(stream)});
+  });
+}
+
+int kebab_gemm_grouped_f4(kebab_dtype out, const uint8_t* x_codes, const uint8_t* x_scales, const uint8_t* w_codes,
+                          const uint8_t* w_scales, void* Y, int64_t ldy, const int32_t* offsets, int64_t E, int64_t R,
+                          int64_t N, int64_t K, kebab_stream_t stream) {
+  return guarded([&] {
+    if (R > 0 && !offsets) return fail(KEBAB_EINVAL, "gemm_grouped_f4: null pointer");
+    return run("gemm_grouped_f4", {out, x_codes, x_scales, w_codes, w_scales, nullptr, Y, ldy, offsets, E, R, N, K,
+                                   false, reinterpret_cast<cudaStream_t>(stream)});
+  });
+}
+
+// Codes (a multiple of 16 bytes), then the scales.
+int64_t kebab_linear_f4_workspace(int64_t M, int64_t K) {
+  const int64_t codes = kebab_f4_code_bytes(M, K);
+  return codes < 0 ? codes : codes + kebab_f4_token_scale_bytes(M, K);
+}
+
+int kebab_linear_f4(kebab_dtype dtype, const void* X, int64_t ldx, const uint8_t* w_codes, const uint8_t* w_scales,
+                    const void* bias, void* Y, int64_t ldy, const int32_t* offsets, int64_t E, int64_t M, int64_t N,
+                    int64_t K, void* workspace, int64_t workspace_bytes, kebab_stream_t stream) {
+  return guarded([&] {
+    const char* what = "linear_f4";
+    if (offsets ? bias != nullptr : E != 1)
+      return fail(KEBAB_EINVAL, offsets ? "linear_f4: a grouped product takes no bias"
+                                        : "linear_f4: without offsets there is one weight matrix (E = 1)");
+    F4Problem p = {dtype, nullptr, nullptr, w_codes, w_scales, bias, Y, ldy, offsets, E, 0, N, K, false,
+                   reinterpret_cast<cudaStream_t>(stream)};
+    int rc = run(what, p);  // the checks
+    if (rc) return rc;
+    if (M < 0 || M > kMaxDim) return fail(KEBAB_EINVAL, "linear_f4: invalid dimensions rows=" + std::to_string(M));
+    if (ldx < K) return fail(KEBAB_EINVAL, "linear_f4: row pitch of X is below its row length");
+    if (M == 0) return KEBAB_OK;
+    if (!X || !Y) return fail(KEBAB_EINVAL, "linear_f4: null pointer");
+    if (!workspace || workspace_bytes < kebab_linear_f4_workspace(M, K) ||
+        (reinterpret_cast<uintptr_t>(workspace) & 15u))
+      return fail(KEBAB_EINVAL, "linear_f4: the workspace is null, too small or not 16-byte aligned");
+    uint8_t* codes = static_cast<uint8_t*>(workspace);
+    uint8_t* scales = codes + kebab_f4_code_bytes(M, K);
+    if ((rc = kebab_quantize_f4_tokens(dtype, X, ldx, codes, scales, M, K, stream))) return rc;
+    p.x_codes = codes, p.x_scales = scales, p.R = M, p.early = true;
+    return run(what, p);
+  });
+}
+
+}  // extern "C"

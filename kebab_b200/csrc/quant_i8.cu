@@ -24,39 +24,6 @@ namespace kb {
 namespace {
 constexpr int THREADS = 128;
 
-// W values as they are stored (F32: two registers of 16 bytes).
-template <typename T, int W>
-struct Run {
-  static constexpr int N = W == 8 ? (int)sizeof(T) / 2 : 1;
-  uint4 raw[N];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (W == 8) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
-    } else {
-      raw[0].x = __float_as_uint(to_float(*p));
-    }
-  }
-  __device__ __forceinline__ void values(float (&v)[W]) const {
-    if constexpr (W == 8 && sizeof(T) == 2) {
-      unpack((const T*)nullptr, raw[0], v);
-    } else if constexpr (W == 8) {
-      const uint32_t b[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[N - 1].x, raw[N - 1].y, raw[N - 1].z, raw[N - 1].w};
-#pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = __uint_as_float(b[u]);
-    } else {
-      v[0] = __uint_as_float(raw[0].x);
-    }
-  }
-};
-
-template <int W>
-__device__ __forceinline__ uint32_t largest(const float (&v)[W], uint32_t top) {
-#pragma unroll
-  for (int u = 0; u < W; ++u) top = max(top, abs_bits(v[u]));
-  return top;
-}
-
 // VEC: 8 values a step in 16-byte (F32: 2 x 16-byte) loads and 8-byte stores;
 // otherwise one value a step. ROW threads take a row (a warp or the block) and
 // keep HELD steps in registers.

@@ -9,6 +9,13 @@ namespace kb {
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+template <int W>
+__device__ __forceinline__ uint32_t largest(const float (&v)[W], uint32_t top) {
+#pragma unroll
+  for (int u = 0; u < W; ++u) top = max(top, abs_bits(v[u]));
+  return top;
+}
+
 struct RowScale {
   float scale, inv;  // inv 0: the row's codes are 0
 };

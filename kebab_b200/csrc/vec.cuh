@@ -66,11 +66,58 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[W]) {
     alignas(16) T h[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) h[u] = from_float<T>(v[u]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(h)[i];
   } else {
 #pragma unroll
     for (int u = 0; u < W; ++u) p[u] = from_float<T>(v[u]);
   }
 }
+
+// W values of a row as they are stored (W = 8 of F32: two registers of 16 bytes).
+template <typename T, int W>
+struct Run {
+  static constexpr int N = W == 8 ? (int)sizeof(T) / 2 : 1;
+  uint4 raw[N];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (W == 8) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+      raw[0].x = __float_as_uint(to_float(*p));
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (W == 8) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+    } else {
+      *p = from_float<T>(__uint_as_float(raw[0].x));
+    }
+  }
+  __device__ __forceinline__ void values(float (&v)[W]) const {
+    if constexpr (W == 8 && sizeof(T) == 2) {
+      unpack((const T*)nullptr, raw[0], v);
+    } else if constexpr (W == 8) {
+      const uint32_t b[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[N - 1].x, raw[N - 1].y, raw[N - 1].z, raw[N - 1].w};
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = __uint_as_float(b[u]);
+    } else {
+      v[0] = __uint_as_float(raw[0].x);
+    }
+  }
+  // The values, rounded to T.
+  __device__ __forceinline__ void set(const float (&v)[W]) {
+    if constexpr (W == 8) {
+      alignas(16) T h[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) h[u] = from_float<T>(v[u]);
+#pragma unroll
+      for (int i = 0; i < N; ++i) raw[i] = reinterpret_cast<const uint4*>(h)[i];
+    } else {
+      raw[0].x = __float_as_uint(to_float(from_float<T>(v[0])));
+    }
+  }
+};
 
 }  // namespace kb
