@@ -21,10 +21,23 @@ struct F4Problem {
   cudaStream_t stream;
 };
 
+constexpr int64_t F4_MAX_ROWS = int64_t(1) << 27;  // of tokens
 constexpr int F4_SLACK = 160;  // entries of token scales past the last row
 
 __host__ __device__ inline int64_t f4_pitch(int64_t K) { return (K + 31) / 32 * 16; }  // bytes of a row's codes
 
+// Tensor maps of the operands. Codes: bytes, boxes of 128 bytes of 128 weight
+// rows, or of `rows` tokens. Scales: as pairs of bytes, boxes of two runs of 128
+// values, each 512 bytes.
+struct F4Maps {
+  CUtensorMap w;         // {byte, n, e}
+  CUtensorMap w_scales;  // {0, tile}
+  CUtensorMap x_scales;  // {8 * token, run}
+};
+int f4_maps(const F4Problem& p, F4Maps* m);
+int f4_token_map(const F4Problem& p, int rows, CUtensorMap* m);
+
 int launch_f4_simt(const F4Problem& p);
+int launch_f4_skinny(const F4Problem& p);
 
 }  // namespace kb

@@ -6,6 +6,28 @@
 #include "kebab/f4.h"
 
 namespace kb {
+
+int f4_maps(const F4Problem& p, F4Maps* m) {
+  const uint64_t pitch = f4_pitch(p.K), k_tiles = (p.K + 127) / 128, n_tiles = (p.N + 127) / 128;
+  const uint64_t w_dims[3] = {pitch, (uint64_t)p.N, (uint64_t)p.E}, w_strides[2] = {pitch, pitch * p.N};
+  const uint64_t ws_dims[2] = {256, p.E * n_tiles * k_tiles}, ws_strides[1] = {512};
+  const uint64_t xs_dims[2] = {(uint64_t)(p.R + F4_SLACK) * 8, k_tiles};
+  const uint64_t xs_strides[1] = {(uint64_t)(p.R + F4_SLACK) * 16};
+  const uint32_t w_box[3] = {128, 128, 1}, s_box[2] = {256, 2};
+  int rc;
+  if ((rc = make_tmap(&m->w, p.w_codes, TMAP_U8, 3, w_dims, w_strides, w_box, 128)) ||
+      (rc = make_tmap(&m->w_scales, p.w_scales, KEBAB_F16, 2, ws_dims, ws_strides, s_box, 0)))
+    return rc;
+  return make_tmap(&m->x_scales, p.x_scales, KEBAB_F16, 2, xs_dims, xs_strides, s_box, 0);
+}
+
+int f4_token_map(const F4Problem& p, int rows, CUtensorMap* m) {
+  const uint64_t pitch = f4_pitch(p.K);
+  const uint64_t dims[2] = {pitch, (uint64_t)p.R}, strides[1] = {pitch};
+  const uint32_t box[2] = {128, (uint32_t)rows};
+  return make_tmap(m, p.x_codes, TMAP_U8, 2, dims, strides, box, 128);
+}
+
 namespace {
 constexpr int64_t kMaxDim = int64_t(1) << 30;  // leaves room for tile arithmetic in 32 bits
 
@@ -18,6 +40,9 @@ int run(const char* what, const F4Problem& p) {
   if (p.R < 0 || p.N <= 0 || p.K <= 0 || p.R > kMaxDim || p.N > kMaxDim || p.K > kMaxDim)
     return fail(KEBAB_EINVAL, std::string(what) + ": invalid dimensions rows=" + std::to_string(p.R) +
                                   " N=" + std::to_string(p.N) + " K=" + std::to_string(p.K));
+  // Coordinates of the scales' tensor maps are 32 bits.
+  if (p.R > F4_MAX_ROWS || p.E * ((p.N + 127) / 128) * ((p.K + 127) / 128) > INT32_MAX)
+    return fail(KEBAB_EINVAL, std::string(what) + ": more than 2^27 rows, or than 2^31 runs of 128 x 128 weights");
   if (p.ldy < p.N)
     return fail(KEBAB_EINVAL, std::string(what) + ": row pitch of Y (" + std::to_string(p.ldy) +
                                   ") is below its row length (" + std::to_string(p.N) + ")");
@@ -27,7 +52,7 @@ int run(const char* what, const F4Problem& p) {
   if (off16(p.w_codes) || off16(p.w_scales) || off16(p.x_codes) || off16(p.x_scales))
     return fail(KEBAB_EINVAL, std::string(what) + ": codes and scales must be 16-byte aligned");
   if (p.R == 0) return KEBAB_OK;
-  return launch_f4_simt(p);
+  return p.R <= 128 ? launch_f4_skinny(p) : launch_f4_simt(p);
 }
 }  // namespace
 }  // namespace kb
@@ -73,7 +98,7 @@ int kebab_linear_f4(kebab_dtype dtype, const void* X, int64_t ldx, const uint8_t
                    reinterpret_cast<cudaStream_t>(stream)};
     int rc = run(what, p);  // the checks
     if (rc) return rc;
-    if (M < 0 || M > kMaxDim) return fail(KEBAB_EINVAL, "linear_f4: invalid dimensions rows=" + std::to_string(M));
+    if (M < 0 || M > F4_MAX_ROWS) return fail(KEBAB_EINVAL, "linear_f4: invalid dimensions rows=" + std::to_string(M));
     if (ldx < K) return fail(KEBAB_EINVAL, "linear_f4: row pitch of X is below its row length");
     if (M == 0) return KEBAB_OK;
     if (!X || !Y) return fail(KEBAB_EINVAL, "linear_f4: null pointer");

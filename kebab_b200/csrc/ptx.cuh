@@ -477,6 +477,38 @@ __device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64
         : "memory");
 }
 
+// 4-bit floating point (e2m1) with a power-of-two scale for every 32 values, both
+// operands K-major: K = 64 per instruction, FP32 accumulation. `sf`: which two
+// bytes of a scale word in TMEM belong to the instruction, 0 (the lower) or 2.
+__host__ __device__ constexpr uint32_t umma_idesc_mxf4(int M, int N, int sf) {
+  return (static_cast<uint32_t>(sf) << 4)          // B's scales
+         | (1u << 7) | (1u << 10)                  // A, B format: e2m1
+         | (static_cast<uint32_t>(N >> 3) << 17)   // N / 8
+         | (1u << 23)                              // scale format: ue8m0
+         | (static_cast<uint32_t>(M >> 7) << 27)   // M / 128
+         | (static_cast<uint32_t>(sf) << 29);      // A's scales
+}
+template <int CG>
+__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+        : "memory");
+}
+
 // 2:4 sparse A: logical K = 32 per instruction; metadata at TMEM `e_tmem`.
 template <int CG>
 __device__ __forceinline__ void umma_f16_sp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t e_tmem,
@@ -505,6 +537,16 @@ __device__ __forceinline__ void tmem_cp_128x128b(uint32_t taddr, uint64_t sdesc)
     asm volatile("tcgen05.cp.cta_group::1.128x128b [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
   else
     asm volatile("tcgen05.cp.cta_group::2.128x128b [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+
+// Shared memory -> TMEM copy of 32 rows x 128 bits (4 columns), the same into
+// each of the four lane quarters: 128 scale words, word 32 c + lane in column c.
+template <int CG>
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t sdesc) {
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
 }
 
 // Signal `bar` (this CTA) once all tcgen05 ops issued so far by this thread complete.

@@ -212,7 +212,7 @@ int64_t kebab_f4_weight_scale_bytes(int64_t N, int64_t K) {
 }
 
 int64_t kebab_f4_token_scale_bytes(int64_t R, int64_t K) {
-  if (R < 0 || K <= 0 || R > kMaxDim || K > kMaxDim) return -KEBAB_EINVAL;
+  if (R < 0 || K <= 0 || R > F4_MAX_ROWS || K > kMaxDim) return -KEBAB_EINVAL;
   return (K + 127) / 128 * (R + F4_SLACK) * 16;
 }
 
@@ -235,6 +235,7 @@ int kebab_quantize_f4_tokens(kebab_dtype dtype, const void* X, int64_t ldx, uint
   return guarded([&] {
     const int rc = check_any("quantize_f4_tokens", dtype, 1, R, K, true);
     if (rc) return rc;
+    if (R > F4_MAX_ROWS) return fail(KEBAB_EINVAL, "quantize_f4_tokens: more than 2^27 rows");
     if (ldx < K) return fail(KEBAB_EINVAL, "quantize_f4_tokens: the row pitch is below the row length");
     if (R == 0) return KEBAB_OK;
     if (!X || !codes || !scales) return fail(KEBAB_EINVAL, "quantize_f4_tokens: null pointer");
