@@ -37,7 +37,7 @@ struct F4Maps {
 int f4_maps(const F4Problem& p, F4Maps* m);
 int f4_token_map(const F4Problem& p, int rows, CUtensorMap* m);
 
-int launch_f4_simt(const F4Problem& p);
+int launch_f4_umma(const F4Problem& p);
 int launch_f4_skinny(const F4Problem& p);
 
 }  // namespace kb

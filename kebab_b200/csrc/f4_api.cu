@@ -1,5 +1,6 @@
 // C entry points of the 4-bit floating-point products (include/kebab/f4.h):
 // argument checks and the choice of kernel.
+#include <algorithm>
 #include <string>
 
 #include "f4.h"
@@ -41,8 +42,8 @@ int run(const char* what, const F4Problem& p) {
     return fail(KEBAB_EINVAL, std::string(what) + ": invalid dimensions rows=" + std::to_string(p.R) +
                                   " N=" + std::to_string(p.N) + " K=" + std::to_string(p.K));
   // Coordinates of the scales' tensor maps are 32 bits.
-  if (p.R > F4_MAX_ROWS || p.E * ((p.N + 127) / 128) * ((p.K + 127) / 128) > INT32_MAX)
-    return fail(KEBAB_EINVAL, std::string(what) + ": more than 2^27 rows, or than 2^31 runs of 128 x 128 weights");
+  if (p.R > F4_MAX_ROWS || p.E * ((p.N + 127) / 128) * ((p.K + 127) / 128) > (1 << 30))
+    return fail(KEBAB_EINVAL, std::string(what) + ": more than 2^27 rows, or than 2^30 runs of 128 x 128 weights");
   if (p.ldy < p.N)
     return fail(KEBAB_EINVAL, std::string(what) + ": row pitch of Y (" + std::to_string(p.ldy) +
                                   ") is below its row length (" + std::to_string(p.N) + ")");
@@ -52,7 +53,13 @@ int run(const char* what, const F4Problem& p) {
   if (off16(p.w_codes) || off16(p.w_scales) || off16(p.x_codes) || off16(p.x_scales))
     return fail(KEBAB_EINVAL, std::string(what) + ": codes and scales must be 16-byte aligned");
   if (p.R == 0) return KEBAB_OK;
-  return p.R <= 128 ? launch_f4_skinny(p) : launch_f4_simt(p);
+  DeviceInfo* dev = nullptr;
+  const int rc = device_info(&dev);
+  if (rc) return rc;
+  // The few-rows kernel up to 128 rows, and where the persistent one would have
+  // tiles for less than half of its CTA pairs.
+  const int64_t tiles = (p.N + 255) / 256 * (p.offsets ? p.R / 240 + std::min(p.E, p.R) : (p.R + 239) / 240);
+  return p.R <= 128 || tiles <= dev->sm_count / 4 ? launch_f4_skinny(p) : launch_f4_umma(p);
 }
 }  // namespace
 }  // namespace kb
