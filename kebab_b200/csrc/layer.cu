@@ -1,95 +1,765 @@
-// A mixture-of-experts layer for a few tokens: a warp an output.
+// A mixture-of-experts feed-forward layer for up to 16 tokens, in two launches.
+//
+// The first computes the router's logits (a block an expert; for 8-bit experts
+// also the codes of the tokens) and clears what the second counts in. The second
+// is one CTA an SM, all resident (a cooperative launch): every CTA finds the
+// top-k choices by itself, takes an equal share of the hidden values of all
+// chosen experts (a gate row and an up row each), meets the others at a grid
+// barrier, and takes an equal share of the layer's outputs, over all chosen
+// experts. So the sum over a token's experts needs no further exchange, and the
+// results do not depend on who comes first.
+//
+// Bound by the chosen experts' bytes, and by latency for few of them. One warp
+// copies the CTA's weights, which are contiguous rows, through a ring of 32 KB
+// stages; it does not wait at the grid barrier, so that the second product's
+// weights arrive meanwhile. Eight warps multiply on the tensor cores (mma.sync,
+// 16 weight rows by 8 tokens: the tokens are so few that this takes a tenth of
+// the time that the bytes take, and unlike a tile of 128 rows it lets the CTAs
+// share the rows evenly). They split the row's length in steps of 64 bytes:
+// lane (g, c) of a warp reads the 16 bytes c of the step from rows g and g + 8,
+// which are the operand registers of two MMAs if the tokens' values are read in
+// the same order, since a sum over k may take its terms in any.
+//
+// All tokens are multiplied with every chosen expert, and a token takes the
+// results of its own experts only: nothing is multiplied by zero, so what other
+// experts hold (infinities, NaN) does not reach it.
+//
+// The hidden values stay in FP32. For 16-bit weights they enter the second
+// product as the sum of two 16-bit numbers (at least 16 bits of them), scaled by
+// the power of two that brings the largest of a choice's values to [2^13, 2^14);
+// for 8-bit weights as codes of that largest value / 127. The largest is found
+// with atomic maxima, which do not depend on their order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+#include <mutex>
 #include <string>
+#include <type_traits>
 
 #include "grouped.h"
-#include "kebab/experts.h"
-#include "kebab/int8.h"
 #include "kebab/layer.h"
 #include "quant_i8.cuh"
 
 namespace kb {
 namespace {
 
-__device__ __forceinline__ float warp_sum(float v) {
+constexpr int MAX_TOKENS = KEBAB_FEW_TOKENS, MAX_K = 32;
+constexpr int WARPS = 8, THREADS = 32 * (WARPS + 1);  // and the copying one
+constexpr int CHUNK = 2048;                           // bytes of a row in a stage, at most
+constexpr int STAGE = 16 * CHUNK, STAGES = 5;
+constexpr int STEPS = CHUNK / 64 / WARPS;             // steps of a chunk that a warp takes, at most
+constexpr int MT = 4;                                 // 16-row tiles of a pass
+constexpr int RED = 68;                               // floats from one token's partial sums (64 rows) to the next's
+
+struct LayerArgs {
+  const void* x;
+  int64_t ldx;
+  const void* w_in;
+  const void* w_out;
+  const float* in_scale;
+  const float* out_scale;
+  void* y;
+  int64_t ldy;
+  int T, E, k, H, D;
+  int renormalize;
+  int fast;   // weight rows on 16-byte boundaries: copied by the bulk engine
+  int vec_x;  // rows of x (or of its codes) on 16-byte boundaries
+  const float* router;
+  // The workspace.
+  float* logits;      // [T][E]
+  float* hidden;      // [T k][D]
+  uint32_t* top;      // [T k]: bits of the largest |hidden|
+  float* x_scale;     // [T], 8-bit
+  int8_t* x_codes;    // [T][x_pitch], 8-bit
+  int x_pitch;
+  uint32_t* arrived;  // CTAs at the grid barrier
+  int pdl;
+  WaitCtx ctx;
+};
+
+// ------------------------------------------------------------------- logits
+
+template <typename T>
+__global__ void __launch_bounds__(256) layer_logits_kernel(const LayerArgs g) {
+  __shared__ float part[8][MAX_TOKENS];
+  __shared__ uint32_t tops[8];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const T* x = static_cast<const T*>(g.x);
+  if (blockIdx.x >= g.E) {
+    // Codes of a token, nearest to 127 x / amax, ties to even. Of 16-bit values
+    // the product is exact and the quotient distinguishes ties from others.
+    const int t = blockIdx.x - g.E;
+    x += t * g.ldx;
+    uint32_t top = 0;
+    for (int h = threadIdx.x; h < g.H; h += 256) top = max(top, abs_bits(to_float(x[h])));
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
 #pragma unroll
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  return v;
-}
-__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
-
-template <typename T>
-__global__ void logits_kernel(const T* x, int64_t ldx, const float* router, float* logits, int E, int H) {
-  const int e = blockIdx.x, t = blockIdx.y;
-  float v = 0.f;
-  for (int h = threadIdx.x; h < H; h += 32) v += to_float(x[t * ldx + h]) * router[(int64_t)e * H + h];
-  v = warp_sum(v);
-  if (threadIdx.x == 0) logits[t * E + e] = v;
-}
-
-// Codes of the rows of x, nearest with ties to even.
-template <typename T>
-__global__ void codes_kernel(const T* x, int64_t ldx, int8_t* q, float* scale, int H) {
-  const int t = blockIdx.x;
-  uint32_t top = 0;
-  for (int h = threadIdx.x; h < H; h += 32) top = max(top, abs_bits(to_float(x[t * ldx + h])));
-  top = __reduce_max_sync(0xffffffffu, top);
-  const RowScale s = row_scale(top);
-  for (int h = threadIdx.x; h < H; h += 32)
-    q[(int64_t)t * H + h] = s.inv == 0.f ? 0 : (int8_t)rintf(to_float(x[t * ldx + h]) * 127.f / __uint_as_float(top));
-  if (threadIdx.x == 0) scale[t] = s.scale;
-}
-
-// Row `t` of x against `row` of a weight matrix.
-template <typename A, typename W>
-__device__ __forceinline__ float dot(const A* a, const W* w, int n) {
-  if constexpr (sizeof(W) == 1) {
-    int v = 0;
-    for (int i = threadIdx.x; i < n; i += 32) v += (int)a[i] * (int)w[i];
-    return (float)warp_sum(v);
-  } else {
+    for (int w = 0; w < 8; ++w) top = max(top, tops[w]);
+    const RowScale s = row_scale(top);
+    const float amax = __uint_as_float(top);
+    int8_t* q = g.x_codes + (int64_t)t * g.x_pitch;
+    for (int h = threadIdx.x; h < g.x_pitch; h += 256)
+      q[h] = h < g.H && s.inv != 0.f ? (int8_t)__float2int_rn(to_float(x[h]) * 127.f / amax) : 0;
+    if (threadIdx.x == 0) g.x_scale[t] = s.scale;
+    return;
+  }
+  const int e = blockIdx.x;
+  if (e == 0) {
+    for (int i = threadIdx.x; i < g.T * g.k; i += 256) g.top[i] = 0;
+    if (threadIdx.x == 0) *g.arrived = 0;
+  }
+  const float* r = g.router + (int64_t)e * g.H;
+  float sum[MAX_TOKENS];
+#pragma unroll
+  for (int t = 0; t < MAX_TOKENS; ++t) sum[t] = 0.f;
+  // Eight values a step on any boundary, so that the order of the sum is the same.
+  const bool vec_r = (reinterpret_cast<uintptr_t>(r) & 15u) == 0;
+  for (int h = threadIdx.x * 8; h < g.H; h += 256 * 8) {
+    const bool whole = h + 8 <= g.H;
+    float w[8], v[8];
+    if (whole && vec_r) {
+      load_row<8>(r + h, w);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = h + i < g.H ? r[h + i] : 0.f;
+    }
+#pragma unroll
+    for (int t = 0; t < MAX_TOKENS; ++t) {
+      if (t >= g.T) break;
+      const T* row = x + t * g.ldx;
+      if (whole && g.vec_x) {
+        load_row<8>(row + h, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = h + i < g.H ? to_float(row[h + i]) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[t] += v[i] * w[i];
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MAX_TOKENS; ++t) {
+    if (t >= g.T) break;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], d);
+    if (lane == 0) part[warp][t] = sum[t];
+  }
+  __syncthreads();
+  if (threadIdx.x < g.T) {
     float v = 0.f;
-    for (int i = threadIdx.x; i < n; i += 32) v += to_float(a[i]) * to_float(w[i]);
-    return warp_sum(v);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v += part[w][threadIdx.x];
+    g.logits[threadIdx.x * g.E + e] = v;
   }
 }
 
-template <typename A, typename W>
-__global__ void up_kernel(const A* x, int64_t ldx, const W* w_in, const float* in_scale, const float* x_scale,
-                          const int32_t* experts, float* a, int k, int H, int D) {
-  const int i = blockIdx.x, j = blockIdx.y, t = j / k;
-  const int64_t e = experts[j];
-  float g = dot(x + t * ldx, w_in + (e * 2 * D + i) * H, H), u = dot(x + t * ldx, w_in + (e * 2 * D + D + i) * H, H);
-  if (in_scale) {
-    g *= x_scale[t] * in_scale[e * 2 * D + i];
-    u *= x_scale[t] * in_scale[e * 2 * D + D + i];
+// -------------------------------------------------------------------- layer
+
+template <typename T, bool I8>
+struct Mma;
+template <>
+struct Mma<__half, false> {
+  using Acc = float;
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
-  if (threadIdx.x == 0) a[(int64_t)j * D + i] = g / (1.f + expf(-g)) * u;
+};
+template <>
+struct Mma<__nv_bfloat16, false> {
+  using Acc = float;
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+template <typename T>
+struct Mma<T, true> {
+  using Acc = int;
+  static __device__ __forceinline__ void mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ uint32_t two(__half, float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t two(__nv_bfloat16, float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <typename T, typename A, typename W>
-__global__ void down_kernel(const A* a, const W* w_out, const float* out_scale, const float* a_scale,
-                            const int32_t* experts, const float* weights, T* y, int64_t ldy, int k, int H, int D) {
-  const int n = blockIdx.x, t = blockIdx.y;
-  float sum = 0.f;
-  for (int j = t * k; j < (t + 1) * k; ++j) {
-    const int64_t e = experts[j];
-    float v = dot(a + (int64_t)j * D, w_out + (e * H + n) * D, D);
-    if (out_scale) v *= a_scale[j] * out_scale[e * H + n];
-    sum += weights[j] * v;
+// How rows of `bytes` lie in the ring: chunks of equal size (a multiple of 64
+// bytes), tiles of 16 rows at a pitch, `units` tiles to a stage.
+struct Shape {
+  int64_t bytes;
+  int chunks, chunk, pitch, unit, units;
+  __device__ __forceinline__ Shape(int64_t row, bool fast) {
+    bytes = row;
+    chunks = (int)((row + CHUNK - 1) / CHUNK);
+    chunk = (int)((row + 64 * (int64_t)chunks - 1) / (64 * (int64_t)chunks)) * 64;
+    // Rows in one piece are copied together, as they lie.
+    pitch = fast && chunks == 1 ? (int)row : chunk;
+    unit = 16 * chunk;
+    units = STAGE / unit;
   }
-  if (threadIdx.x == 0) y[t * ldy + n] = from_float<T>(sum);
+  __device__ __forceinline__ int length(int c) const { return (int)min((int64_t)chunk, bytes - (int64_t)c * chunk); }
+};
+
+struct LayerSmem {
+  static constexpr int OFF_RED = STAGES * STAGE;
+  static __host__ __device__ constexpr int off_bar(int nt) { return OFF_RED + WARPS * nt * 8 * RED * 4; }
+  static __host__ __device__ constexpr int off_tables(int nt) { return off_bar(nt) + 2 * STAGES * 8 + 16; }
+  // weights, factors [T k] (float), experts [T k], active [T k], place of an
+  // active expert among a token's choices [T k][T] (bytes), flags [E] (bytes)
+  static __host__ __device__ int bytes(int nt, int T, int k, int E) {
+    const int n = T * k;
+    return off_tables(nt) + n * 16 + n * T + E + 16;
+  }
+};
+
+// The top-k choices of token t by one warp: as kebab_route.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  x += 0.f;  // -0 becomes +0: they are equal
+  if (x != x) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(x);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? (key ^ 0x80000000u) : ~key);  // NaN's key gives a NaN
+}
+__device__ void choose(const LayerArgs& g, int t, float* weights, int* experts) {
+  constexpr int V = kMaxExperts / 32;
+  const int lane = threadIdx.x & 31;
+  uint32_t key[V];
+#pragma unroll
+  for (int u = 0; u < V; ++u) {
+    if (u * 32 >= g.E) break;
+    const int e = u * 32 + lane;
+    key[u] = e < g.E ? order_key(__ldcg(g.logits + t * g.E + e)) : 0u;
+  }
+  float highest = 0.f, sum = 0.f, mine = 0.f;
+  for (int j = 0; j < g.k; ++j) {
+    uint32_t top = 0;
+    int e = 0;
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      if (u * 32 >= g.E) break;
+      if (key[u] > top) top = key[u], e = u * 32 + lane;
+    }
+    const uint32_t all = __reduce_max_sync(0xffffffffu, top);
+    e = (int)__reduce_min_sync(0xffffffffu, top == all ? (unsigned)e : 0xffffffffu);
+    const float v = key_value(all);
+    if (j == 0) {
+      highest = v;
+      if (!g.renormalize) {
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+          if (u * 32 >= g.E) break;
+          if (u * 32 + lane < g.E) sum += expf(key_value(key[u]) - highest);
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      }
+    }
+    const float p = highest == -INFINITY ? 0.f : expf(v - highest);  // all logits -inf: nothing to weigh
+    if (g.renormalize) sum += p;
+    if (lane == j) mine = p;
+    if (lane == 0) experts[j] = e;
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      if (u * 32 >= g.E) break;
+      if (e == u * 32 + lane) key[u] = 0;
+    }
+  }
+  if (lane < g.k) weights[lane] = mine / (highest == -INFINITY ? 1.f : sum);
+}
+
+// 2^n by which a choice's values are multiplied, for the bits of the largest
+// (0 or not finite: 1), and its inverse.
+__device__ __forceinline__ float power_for(uint32_t top, float& inverse) {
+  const int e = (int)(top >> 23) - 127;
+  const int n = top == 0 || e == 128 ? 0 : max(min(13 - e, 126), -126);
+  inverse = __uint_as_float((uint32_t)(127 - n) << 23);
+  return __uint_as_float((uint32_t)(127 + n) << 23);
+}
+
+template <typename TX, bool I8, int NT>
+__global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
+  using M = Mma<TX, I8>;
+  using Acc = typename M::Acc;
+  constexpr int ES = I8 ? 1 : 2;       // bytes of a weight
+  constexpr int PIECE = 16 / ES;       // values of 16 bytes
+  constexpr int PARTS = I8 ? 1 : 2;    // operands that a hidden value makes
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
+  uint32_t* red = reinterpret_cast<uint32_t*>(smem + LayerSmem::OFF_RED);  // [WARPS][NT][8][RED]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + LayerSmem::off_bar(NT));
+  uint64_t* empty = full + STAGES;
+  int* s_count = reinterpret_cast<int*>(empty + STAGES);  // active experts; whether the grid barrier failed
+  const int choices = g.T * g.k;
+  float* s_weight = reinterpret_cast<float*>(smem + LayerSmem::off_tables(NT));  // [T][k]
+  float* s_factor = s_weight + choices;                                          // [T][k]
+  int* s_expert = reinterpret_cast<int*>(s_factor + choices);                    // [T][k]
+  int* s_active = s_expert + choices;                                            // [active]
+  uint8_t* s_place = reinterpret_cast<uint8_t*>(s_active + choices);             // [active][T]: j, or 255
+  uint8_t* s_flag = s_place + choices * g.T;                                     // [E]
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const WaitCtx& ctx = g.ctx;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], WARPS);
+    }
+    fence_barrier_init();
+    s_count[1] = 0;
+  }
+  for (int i = threadIdx.x; i < choices * g.T; i += THREADS) s_place[i] = 255;
+  for (int i = threadIdx.x; i < g.E; i += THREADS) s_flag[i] = 0;
+  if (g.pdl) pdl_wait();
+  __syncthreads();
+  if (warp < WARPS) {
+    for (int t = warp; t < g.T; t += WARPS) {
+      choose(g, t, s_weight + t * g.k, s_expert + t * g.k);
+      __syncwarp();
+      if (lane < g.k) s_flag[s_expert[t * g.k + lane]] = 1;
+    }
+  }
+  __syncthreads();
+  // The chosen experts in ascending order, by one warp.
+  if (warp == 0) {
+    int n = 0;
+    for (int e0 = 0; e0 < g.E; e0 += 32) {
+      const bool is = e0 + lane < g.E && s_flag[e0 + lane];
+      const uint32_t mask = __ballot_sync(0xffffffffu, is);
+      if (is) s_active[n + __popc(mask & ((1u << lane) - 1u))] = e0 + lane;
+      n += __popc(mask);
+    }
+    if (lane == 0) s_count[0] = n;
+  }
+  __syncthreads();
+  const int active = s_count[0];
+  for (int i = threadIdx.x; i < choices; i += THREADS) {
+    const int e = s_expert[i];
+    int lo = 0, hi = active - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (s_active[mid] < e) lo = mid + 1;
+      else hi = mid;
+    }
+    s_place[lo * g.T + i / g.k] = (uint8_t)(i % g.k);
+  }
+  __syncthreads();
+
+  const int cta = blockIdx.x, ctas = gridDim.x;
+  // This CTA's share of the hidden values (counted over the chosen experts) and of the outputs.
+  const int64_t total = (int64_t)active * g.D, p0 = total * cta / ctas, p1 = total * (cta + 1) / ctas;
+  const int n0 = (int)((int64_t)g.H * cta / ctas), n1 = (int)((int64_t)g.H * (cta + 1) / ctas);
+  const Shape up((int64_t)g.H * ES, g.fast), down((int64_t)g.D * ES, g.fast);
+  constexpr int PAIRS = 8 * MT, ROWS = 16 * MT;  // hidden values, outputs of a pass
+  auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
+  bool ok = true;
+  int stage = 0;
+  uint32_t phase = 0;
+  auto advance = [&] {
+    if (++stage == STAGES) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  };
+
+  if (warp == WARPS) {
+    // ------------------------------------------------------------- copies
+    int left = 0;  // tiles that the stage has room for
+    // Chunk c of the rows src .. of a tile: `rows` of them, or (second) 8 places
+    // further on as many from `second`.
+    auto tile = [&](const Shape& s, const uint8_t* src, const uint8_t* second, int rows, int c) {
+      if (left == 0) {
+        ok = all_ok(mbar_wait(&empty[stage], phase ^ 1u, ctx, SITE_EMPTY));
+        if (!ok) return;
+        left = s.units;
+      }
+      uint8_t* dst = smem + stage * STAGE + (s.units - left) * s.unit;
+      const int len = s.length(c), copies = second ? 2 * rows : rows;
+      const int64_t at = (int64_t)c * s.chunk;
+      if (g.fast) {
+        if (lane == 0) mbar_expect_tx(&full[stage], copies * len);
+        __syncwarp();
+        if (s.chunks == 1) {
+          if (lane == 0) bulk_load(dst, src, rows * len, &full[stage]);
+          if (lane == 1 && second) bulk_load(dst + 8 * s.pitch, second, rows * len, &full[stage]);
+        } else if (second ? (lane & 7) < rows && lane < 16 : lane < rows) {
+          const uint8_t* from = second && lane >= 8 ? second + (lane - 8) * s.bytes : src + lane * s.bytes;
+          bulk_load(dst + lane * s.pitch, from + at, len, &full[stage]);
+        }
+      } else {
+        // Rows on any boundary, value by value, filled up with zeros to 16 bytes.
+        const int n = len / ES, padded = (n + PIECE - 1) / PIECE * PIECE;
+        for (int r = 0; r < copies; ++r) {
+          const bool is_second = r >= rows;
+          const uint8_t* from = (is_second ? second + (r - rows) * s.bytes : src + r * s.bytes) + at;
+          uint8_t* to = dst + (is_second ? 8 + r - rows : r) * s.pitch;
+          for (int i = lane; i < padded; i += 32) {
+            if constexpr (I8) to[i] = i < n ? from[i] : 0;
+            else reinterpret_cast<uint16_t*>(to)[i] = i < n ? reinterpret_cast<const uint16_t*>(from)[i] : 0;
+          }
+        }
+      }
+      __syncwarp();
+      if (--left == 0) {
+        if (lane == 0) mbar_arrive(&full[stage]);
+        __syncwarp();
+        advance();
+      }
+    };
+    auto finish = [&] {
+      if (left > 0) {
+        if (lane == 0) mbar_arrive(&full[stage]);
+        __syncwarp();
+        advance();
+        left = 0;
+      }
+    };
+    const uint8_t* w_in = static_cast<const uint8_t*>(g.w_in);
+    const uint8_t* w_out = static_cast<const uint8_t*>(g.w_out);
+    for (int64_t p = p0; p < p1 && ok;) {
+      const int a = (int)(p / g.D), i0 = (int)(p - (int64_t)a * g.D);
+      const int n = (int)min((int64_t)min(PAIRS, g.D - i0), p1 - p);
+      const uint8_t* gate = w_in + ((int64_t)s_active[a] * 2 * g.D + i0) * up.bytes;
+      for (int c = 0; c < up.chunks && ok; ++c)
+        for (int m = 0; m < n && ok; m += 8)
+          tile(up, gate + m * up.bytes, gate + ((int64_t)g.D + m) * up.bytes, min(8, n - m), c);
+      p += n;
+    }
+    if (ok) finish();
+    for (int r0 = n0; r0 < n1 && ok; r0 += ROWS) {
+      const int n = min(ROWS, n1 - r0);
+      for (int a = 0; a < active && ok; ++a) {
+        const uint8_t* w = w_out + ((int64_t)s_active[a] * g.H + r0) * down.bytes;
+        for (int c = 0; c < down.chunks && ok; ++c)
+          for (int m = 0; m < n && ok; m += 16) tile(down, w + m * down.bytes, nullptr, min(16, n - m), c);
+      }
+    }
+    if (ok) finish();
+  } else {
+    // ----------------------------------------------------------- products
+    const int gq = lane >> 2, cq = lane & 3;
+    using One = std::integral_constant<int, 1>;
+    using All = std::integral_constant<int, PARTS>;
+    int left = 0;
+    const uint8_t* at = nullptr;
+    Acc acc[MT][NT][4];
+    uint32_t b[STEPS][NT][PARTS][4];
+    auto clear = [&] {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[m][n][i] = 0;
+    };
+    auto release = [&] {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
+      advance();
+      left = 0;
+    };
+    // The next tile, with the first `parts` operands of every value.
+    auto multiply = [&](const Shape& s, int len, auto parts, Acc (&d)[NT][4]) {
+      if (left == 0) {
+        if (ok) ok = all_ok(mbar_wait(&full[stage], phase, ctx, SITE_FULL));
+        left = s.units;
+        at = smem + stage * STAGE;
+      } else {
+        at += s.unit;
+      }
+      const uint8_t* row = at + gq * s.pitch + cq * 16;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int off = (warp + i * WARPS) * 64;
+        if (off >= len) break;
+        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+        if (off + cq * 16 < len) {  // past the end of the row there may be anything
+          lo = *reinterpret_cast<const uint4*>(row + off);
+          hi = *reinterpret_cast<const uint4*>(row + 8 * s.pitch + off);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int p = 0; p < decltype(parts)::value; ++p) {
+            M::mma(d[n], lo.x, hi.x, lo.y, hi.y, b[i][n][p][0], b[i][n][p][1]);
+            M::mma(d[n], lo.z, hi.z, lo.w, hi.w, b[i][n][p][2], b[i][n][p][3]);
+          }
+      }
+      if (--left == 0) release();
+    };
+    // Partial sums of this warp, to be added up over the warps: token, then row.
+    auto put = [&](int m, int n, const uint32_t (&v)[4]) {
+      uint32_t* to = red + ((warp * NT + n) * 8 + 2 * cq) * RED + m * 16 + gq;
+      to[0] = v[0];
+      to[RED] = v[1];
+      to[8] = v[2];
+      to[RED + 8] = v[3];
+    };
+    auto meet = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    // The sum over the warps of row r of token t.
+    auto total_of = [&](int t, int r) {
+      const uint32_t* from = red + (t / 8 * 8 + t % 8) * RED + r;
+      Acc sum = 0;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const uint32_t v = from[w * NT * 8 * RED];
+        if constexpr (I8) sum += (int)v;
+        else sum += __uint_as_float(v);
+      }
+      return sum;
+    };
+
+    // Hidden values: a = silu(gate) * up.
+    for (int64_t p = p0; p < p1;) {
+      const int a = (int)(p / g.D), i0 = (int)(p - (int64_t)a * g.D);
+      const int n = (int)min((int64_t)min(PAIRS, g.D - i0), p1 - p);
+      clear();
+      for (int c = 0; c < up.chunks; ++c) {
+        const int len = up.length(c);
+        // The tokens' values of this warp's steps.
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int t = nt * 8 + gq, off = (warp + i * WARPS) * 64 + cq * 16;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (t < g.T && off < len) {
+              const int64_t k0 = ((int64_t)c * up.chunk + off) / ES;
+              if constexpr (I8) {
+                v = *reinterpret_cast<const uint4*>(g.x_codes + (int64_t)t * g.x_pitch + k0);
+              } else {
+                const uint16_t* x = static_cast<const uint16_t*>(g.x) + t * g.ldx + k0;
+                if (g.vec_x && k0 + 8 <= g.H) {
+                  v = *reinterpret_cast<const uint4*>(x);
+                } else {
+                  uint32_t h[8];
+#pragma unroll
+                  for (int u = 0; u < 8; ++u) h[u] = k0 + u < g.H ? x[u] : 0;
+                  v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+                }
+              }
+            }
+            b[i][nt][0][0] = v.x, b[i][nt][0][1] = v.y, b[i][nt][0][2] = v.z, b[i][nt][0][3] = v.w;
+          }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          if (m * 8 < n) multiply(up, len, One(), acc[m]);
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          uint32_t v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (I8) v[i] = (uint32_t)acc[m][nt][i];
+            else v[i] = __float_as_uint(acc[m][nt][i]);
+          }
+          put(m, nt, v);
+        }
+      meet();
+      // A warp a token, a lane a value.
+      for (int t = warp; t < g.T; t += WARPS) {
+        const int j = s_place[a * g.T + t];
+        if (j == 255) continue;
+        const int row = lane / 8 * 16 + lane % 8, i = i0 + lane;
+        float gate = (float)total_of(t, row), value = (float)total_of(t, row + 8);
+        if constexpr (I8) {
+          const float s = g.x_scale[t];
+          const float* scale = g.in_scale + (int64_t)s_active[a] * 2 * g.D + i;
+          gate *= s * (lane < n ? scale[0] : 0.f);
+          value *= s * (lane < n ? scale[g.D] : 0.f);
+        }
+        const float h = gate / (1.f + expf(-gate)) * value;
+        if (lane < n && ok) g.hidden[(int64_t)(t * g.k + j) * g.D + i] = h;
+        const uint32_t top = __reduce_max_sync(0xffffffffu, lane < n ? abs_bits(h) : 0u);
+        if (lane == 0) atomicMax(g.top + t * g.k + j, top);
+      }
+      meet();
+      p += n;
+    }
+    if (left > 0) release();
+
+    // The grid barrier.
+    __threadfence();
+    meet();
+    if (threadIdx.x == 0) {
+      asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(g.arrived) : "memory");
+      const uint64_t t0 = globaltimer();
+      for (uint32_t it = 1;; ++it) {
+        uint32_t n;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(g.arrived) : "memory");
+        if (n >= (uint32_t)ctas) break;
+        if ((it & 63u) == 0u) {
+          if (!aborted(ctx.status) && globaltimer() - t0 <= ctx.timeout_ns) continue;
+          record_error(ctx.status, DEV_TIMEOUT, SITE_GRID);
+          s_count[1] = 1;
+          break;
+        }
+      }
+      __threadfence();
+    }
+    meet();
+    if (s_count[1]) ok = false;
+    // What a choice's products are multiplied by: its weight and the inverse of its values' scale.
+    for (int i = threadIdx.x; i < choices; i += 32 * WARPS) {
+      const uint32_t top = __ldcg(g.top + i);
+      float inverse;
+      if constexpr (I8) inverse = row_scale(top).scale;
+      else power_for(top, inverse);
+      s_factor[i] = s_weight[i] * inverse;
+    }
+    meet();
+
+    // Outputs.
+    for (int r0 = n0; r0 < n1; r0 += ROWS) {
+      const int n = min(ROWS, n1 - r0);
+      float out[MT][NT][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) out[m][nt][i] = 0.f;
+      for (int a = 0; a < active; ++a) {
+        clear();
+        for (int c = 0; c < down.chunks; ++c) {
+          const int len = down.length(c);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int t = nt * 8 + gq;
+            const int j = t < g.T ? s_place[a * g.T + t] : 255;
+            const float* h = g.hidden + (int64_t)(j == 255 ? 0 : t * g.k + j) * g.D;
+            const uint32_t top = j == 255 ? 0u : __ldcg(g.top + t * g.k + j);
+            float scale, unused;
+            if constexpr (I8) scale = row_scale(top).inv;
+            else scale = power_for(top, unused);
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+              const int off = (warp + i * WARPS) * 64 + cq * 16;
+              float v[PIECE];
+#pragma unroll
+              for (int u = 0; u < PIECE; ++u) v[u] = 0.f;
+              if (j != 255 && off < len) {
+                const int64_t k0 = ((int64_t)c * down.chunk + off) / ES;
+                if (g.fast) {
+#pragma unroll
+                  for (int u = 0; u < PIECE; u += 4) {
+                    const float4 f = __ldcg(reinterpret_cast<const float4*>(h + k0 + u));
+                    v[u] = f.x, v[u + 1] = f.y, v[u + 2] = f.z, v[u + 3] = f.w;
+                  }
+                } else {
+#pragma unroll
+                  for (int u = 0; u < PIECE; ++u) v[u] = k0 + u < g.D ? __ldcg(h + k0 + u) : 0.f;
+                }
+              }
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                if constexpr (I8) {
+                  uint32_t code[4];
+#pragma unroll
+                  for (int u = 0; u < 4; ++u) code[u] = scale == 0.f ? 0u : code_bits(v[4 * q + u], scale);
+                  b[i][nt][0][q] = pack4(code[0], code[1], code[2], code[3]);
+                } else {
+                  const float x0 = v[2 * q] * scale, x1 = v[2 * q + 1] * scale;
+                  const uint32_t hi = two(TX(), x0, x1);
+                  const TX* parts = reinterpret_cast<const TX*>(&hi);
+                  // What the rounding left; of an infinity nothing.
+                  const float l0 = x0 - to_float(parts[0]), l1 = x1 - to_float(parts[1]);
+                  b[i][nt][0][q] = hi;
+                  b[i][nt][PARTS - 1][q] = two(TX(), isinf(x0) ? 0.f : l0, isinf(x1) ? 0.f : l1);
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            if (m * 16 < n) multiply(down, len, All(), acc[m]);
+        }
+        // Each token takes its own experts' products only.
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int t = nt * 8 + 2 * cq + u;
+            const int j = t < g.T ? s_place[a * g.T + t] : 255;
+            if (j == 255) continue;
+            const float factor = s_factor[t * g.k + j];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              if (m * 16 >= n) break;
+#pragma unroll
+              for (int v = 0; v < 2; ++v) {
+                float f = factor;
+                if constexpr (I8) {
+                  const int r = r0 + m * 16 + v * 8 + gq;
+                  f *= r < n1 ? g.out_scale[(int64_t)s_active[a] * g.H + r] : 0.f;
+                }
+                out[m][nt][2 * v + u] += f * (float)acc[m][nt][2 * v + u];
+              }
+            }
+          }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint32_t v[4] = {__float_as_uint(out[m][nt][0]), __float_as_uint(out[m][nt][1]),
+                                 __float_as_uint(out[m][nt][2]), __float_as_uint(out[m][nt][3])};
+          put(m, nt, v);
+        }
+      meet();
+      for (int t = warp; t < g.T; t += WARPS) {
+        for (int r = lane; r < n; r += 32) {
+          const uint32_t* from = red + t * RED + r;
+          float sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < WARPS; ++w) sum += __uint_as_float(from[w * NT * 8 * RED]);
+          if (ok) static_cast<TX*>(g.y)[t * g.ldy + r0 + r] = from_float<TX>(sum);
+        }
+      }
+      meet();
+    }
+    if (left > 0) release();
+  }
+  // A wait ran out: what is in flight has to land before the CTA leaves.
+  if (__syncthreads_or(!ok)) settle();
+}
+
+// ---------------------------------------------------------------- host side
 
 struct Sizes {
   int64_t T, E, k, H, D;
 };
 
-// logits, weights, a, its scales, those of x (F32); experts, slots, offsets (I32); codes of a and x.
-int64_t words(const Sizes& s) { return s.T * s.E + 4 * s.T * s.k + s.T * s.k * s.D + s.T + s.E + 1; }
-int64_t bytes(const Sizes& s) { return words(s) * 4 + s.T * s.k * s.D + s.T * s.H; }
+int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
+
+// logits, hidden values, their largest, the tokens' scales, the barrier's count; the tokens' codes.
+int64_t words(const Sizes& s) { return up16(s.T * s.E * 4) + up16(s.T * s.k * s.D * 4) + up16(s.T * s.k * 4) + 64 + 16; }
+int64_t bytes(const Sizes& s) { return words(s) + s.T * up16(s.H); }
 
 int check(const char* what, int dtype, const void* x, int64_t ldx, const void* router, const void* w_in,
           const void* w_out, const void* y, int64_t ldy, const Sizes& s, void* ws, int64_t ws_bytes) {
@@ -97,8 +767,10 @@ int check(const char* what, int dtype, const void* x, int64_t ldx, const void* r
   if (dtype != KEBAB_F16 && dtype != KEBAB_BF16) return fail(KEBAB_ENOTSUP, w + ": only F16 and BF16 are implemented");
   if (s.T < 0 || s.T > KEBAB_FEW_TOKENS)
     return fail(KEBAB_EINVAL, w + ": " + std::to_string(s.T) + " tokens are not in 0.." + std::to_string(KEBAB_FEW_TOKENS));
-  if (s.E < 1 || s.E > kMaxExperts) return fail(KEBAB_EINVAL, w + ": number of experts " + std::to_string(s.E) + " is not in 1..1024");
-  if (s.k < 1 || s.k > 32 || s.k > s.E) return fail(KEBAB_EINVAL, w + ": k = " + std::to_string(s.k) + " is not in 1..min(E, 32)");
+  if (s.E < 1 || s.E > kMaxExperts)
+    return fail(KEBAB_EINVAL, w + ": number of experts " + std::to_string(s.E) + " is not in 1.." + std::to_string(kMaxExperts));
+  if (s.k < 1 || s.k > MAX_K || s.k > s.E)
+    return fail(KEBAB_EINVAL, w + ": k = " + std::to_string(s.k) + " is not in 1..min(E, 32)");
   if (s.H <= 0 || s.D <= 0 || s.H > (1 << 24) || s.D > (1 << 24))
     return fail(KEBAB_EINVAL, w + ": invalid dimensions H=" + std::to_string(s.H) + " D=" + std::to_string(s.D));
   if (ldx < s.H || ldy < s.H) return fail(KEBAB_EINVAL, w + ": a row pitch is below the row length");
@@ -109,36 +781,59 @@ int check(const char* what, int dtype, const void* x, int64_t ldx, const void* r
   return KEBAB_OK;
 }
 
-template <typename T, typename W>
-int run(const T* x, int64_t ldx, const float* router, const W* w_in, const float* in_scale, const W* w_out,
-        const float* out_scale, T* y, int64_t ldy, const Sizes& s, int renormalize, void* ws, kebab_stream_t stream) {
-  constexpr bool I8 = sizeof(W) == 1;
-  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int Tk = (int)(s.T * s.k), H = (int)s.H, D = (int)s.D, k = (int)s.k;
-  float* logits = static_cast<float*>(ws);
-  float* weights = logits + s.T * s.E;
-  float* a = weights + Tk;
-  float* a_scale = a + (int64_t)Tk * D;
-  float* x_scale = a_scale + Tk;
-  int32_t* experts = reinterpret_cast<int32_t*>(x_scale + s.T);
-  int32_t* slots = experts + Tk;
-  int32_t* offsets = slots + Tk;
-  int8_t* qa = reinterpret_cast<int8_t*>(offsets + s.E + 1);
-  int8_t* qx = qa + (int64_t)Tk * D;
-  logits_kernel<<<dim3((unsigned)s.E, (unsigned)s.T), 32, 0, st>>>(x, ldx, router, logits, (int)s.E, H);
-  int rc = kebab_route(KEBAB_F32, logits, s.E, s.T, s.E, k, renormalize, weights, experts, offsets, slots, nullptr, 0, stream);
-  if (rc) return rc;
-  if constexpr (I8) {
-    codes_kernel<<<(unsigned)s.T, 32, 0, st>>>(x, ldx, qx, x_scale, H);
-    up_kernel<<<dim3(D, Tk), 32, 0, st>>>(qx, H, w_in, in_scale, x_scale, experts, a, k, H, D);
-    if ((rc = kebab_quantize_i8(KEBAB_F32, a, D, qa, D, a_scale, Tk, D, stream))) return rc;
-    down_kernel<<<dim3(H, (unsigned)s.T), 32, 0, st>>>(qa, w_out, out_scale, a_scale, experts, weights, y, ldy, k, H, D);
-  } else {
-    up_kernel<<<dim3(D, Tk), 32, 0, st>>>(x, ldx, w_in, in_scale, x_scale, experts, a, k, H, D);
-    down_kernel<<<dim3(H, (unsigned)s.T), 32, 0, st>>>(a, w_out, out_scale, a_scale, experts, weights, y, ldy, k, H, D);
-  }
-  const cudaError_t e = cudaGetLastError();
+template <typename TX, bool I8, int NT>
+int launch(LayerArgs& g, cudaStream_t stream) {
+  int rc;
+  DeviceInfo* dev = nullptr;
+  if ((rc = device_info(&dev)) || (rc = wait_ctx(&g.ctx))) return rc;
+  g.pdl = pdl_enabled();
+  auto kern = layer_kernel<TX, I8, NT>;
+  static std::once_flag once[64];
+  static cudaError_t err[64];
+  const int di = dev->device & 63;
+  std::call_once(once[di], [&] {
+    err[di] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   std::min(LayerSmem::bytes(NT, MAX_TOKENS, MAX_K, kMaxExperts) + 128, 232448));
+  });
+  if (err[di] != cudaSuccess) return cuda_fail(err[di], "cudaFuncSetAttribute(max dynamic smem)");
+  PdlLaunch first(dim3((unsigned)(g.E + (I8 ? g.T : 0))), dim3(256), 0, stream);
+  cudaError_t e = cudaLaunchKernelEx(&first.cfg, layer_logits_kernel<TX>, (const LayerArgs)g);
+  if (e != cudaSuccess) return cuda_fail(e, "expert_layer: logits launch");
+  const int smem = LayerSmem::bytes(NT, g.T, g.k, g.E) + 128;
+  PdlLaunch l(dim3((unsigned)dev->sm_count), dim3(THREADS), smem, stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeCooperative;
+  attr[0].val.cooperative = 1;
+  if (l.cfg.numAttrs) attr[1] = l.attr[0];
+  l.cfg.attrs = attr;
+  ++l.cfg.numAttrs;
+  e = cudaLaunchKernelEx(&l.cfg, kern, (const LayerArgs)g);
   return e == cudaSuccess ? KEBAB_OK : cuda_fail(e, "expert_layer launch");
+}
+
+template <bool I8>
+int run(int dtype, LayerArgs g, const Sizes& s, void* ws, kebab_stream_t stream) {
+  constexpr int ES = I8 ? 1 : 2;
+  g.T = (int)s.T, g.E = (int)s.E, g.k = (int)s.k, g.H = (int)s.H, g.D = (int)s.D;
+  uint8_t* at = static_cast<uint8_t*>(ws);
+  auto take = [&](int64_t n) {
+    uint8_t* p = at;
+    at += up16(n);
+    return p;
+  };
+  g.logits = reinterpret_cast<float*>(take(s.T * s.E * 4));
+  g.hidden = reinterpret_cast<float*>(take(s.T * s.k * s.D * 4));
+  g.top = reinterpret_cast<uint32_t*>(take(s.T * s.k * 4));
+  g.x_scale = reinterpret_cast<float*>(take(64));
+  g.arrived = reinterpret_cast<uint32_t*>(take(16));
+  g.x_codes = reinterpret_cast<int8_t*>(at);
+  g.x_pitch = (int)up16(s.H);
+  auto on16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  g.fast = on16(g.w_in) && on16(g.w_out) && s.H * ES % 16 == 0 && s.D * ES % 16 == 0;
+  g.vec_x = on16(g.x) && g.ldx % 8 == 0;
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == KEBAB_F16) return s.T <= 8 ? launch<__half, I8, 1>(g, st) : launch<__half, I8, 2>(g, st);
+  return s.T <= 8 ? launch<__nv_bfloat16, I8, 1>(g, st) : launch<__nv_bfloat16, I8, 2>(g, st);
 }
 }  // namespace
 }  // namespace kb
@@ -148,7 +843,7 @@ using namespace kb;
 extern "C" {
 
 int64_t kebab_expert_layer_workspace(int64_t T, int64_t E, int k, int64_t H, int64_t D) {
-  if (T < 0 || T > KEBAB_FEW_TOKENS || E < 1 || E > kMaxExperts || k < 1 || k > 32 || H <= 0 || D <= 0 ||
+  if (T < 0 || T > KEBAB_FEW_TOKENS || E < 1 || E > kMaxExperts || k < 1 || k > MAX_K || H <= 0 || D <= 0 ||
       H > (1 << 24) || D > (1 << 24))
     return -KEBAB_EINVAL;
   return bytes({T, E, k, H, D});
@@ -161,12 +856,10 @@ int kebab_expert_layer(kebab_dtype dtype, const void* x, int64_t ldx, const floa
     const Sizes s = {T, E, k, H, D};
     const int rc = check("expert_layer", dtype, x, ldx, router, w_in, w_out, y, ldy, s, workspace, workspace_bytes);
     if (rc || T == 0) return rc;
-    auto go = [&](auto t) {
-      using V = decltype(t);
-      return run(static_cast<const V*>(x), ldx, router, static_cast<const V*>(w_in), nullptr, static_cast<const V*>(w_out),
-                 nullptr, static_cast<V*>(y), ldy, s, renormalize, workspace, stream);
-    };
-    return dtype == KEBAB_F16 ? go(__half()) : go(__nv_bfloat16());
+    LayerArgs g = {};
+    g.x = x, g.ldx = ldx, g.router = router, g.w_in = w_in, g.w_out = w_out, g.y = y, g.ldy = ldy;
+    g.renormalize = renormalize;
+    return run<false>(dtype, g, s, workspace, stream);
   });
 }
 
@@ -178,14 +871,13 @@ int kebab_expert_layer_i8(kebab_dtype dtype, const void* x, int64_t ldx, const f
     const Sizes s = {T, E, k, H, D};
     const int rc = check("expert_layer_i8", dtype, x, ldx, router, w_in, w_out, y, ldy, s, workspace, workspace_bytes);
     if (rc || T == 0) return rc;
-    if (H > 131072 || D > 131072) return fail(KEBAB_EINVAL, "expert_layer_i8: H or D above 131072 could overflow the 32-bit sums");
+    if (H > 131072 || D > 131072)
+      return fail(KEBAB_EINVAL, "expert_layer_i8: H or D above 131072 could overflow the 32-bit sums");
     if (!in_scale || !out_scale) return fail(KEBAB_EINVAL, "expert_layer_i8: null pointer");
-    auto go = [&](auto t) {
-      using V = decltype(t);
-      return run(static_cast<const V*>(x), ldx, router, w_in, in_scale, w_out, out_scale, static_cast<V*>(y), ldy, s,
-                 renormalize, workspace, stream);
-    };
-    return dtype == KEBAB_F16 ? go(__half()) : go(__nv_bfloat16());
+    LayerArgs g = {};
+    g.x = x, g.ldx = ldx, g.router = router, g.w_in = w_in, g.in_scale = in_scale, g.w_out = w_out;
+    g.out_scale = out_scale, g.y = y, g.ldy = ldy, g.renormalize = renormalize;
+    return run<true>(dtype, g, s, workspace, stream);
   });
 }
 
