@@ -20,15 +20,14 @@
 // which are the operand registers of two MMAs if the tokens' values are read in
 // the same order, since a sum over k may take its terms in any.
 //
-// All tokens are multiplied with every chosen expert, and a token takes the
-// results of its own experts only: nothing is multiplied by zero, so what other
-// experts hold (infinities, NaN) does not reach it.
+// An expert's rows are multiplied with the tokens that chose it and added onto
+// those only: what other experts hold (infinities, NaN) does not reach a token.
 //
-// The hidden values stay in FP32. For 16-bit weights they enter the second
-// product as the sum of two 16-bit numbers (at least 16 bits of them), scaled by
-// the power of two that brings the largest of a choice's values to [2^13, 2^14);
-// for 8-bit weights as codes of that largest value / 127. The largest is found
-// with atomic maxima, which do not depend on their order.
+// For 16-bit weights the hidden values enter the second product as the sum of
+// two 16-bit numbers (at least 16 bits of them); F16 ones scaled by the power of
+// two that brings the largest of a choice's values to [2^13, 2^14). For 8-bit
+// weights they are codes of that largest value / 127. The largest is found with
+// atomic maxima, which do not depend on their order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -47,7 +46,7 @@ namespace {
 constexpr int MAX_TOKENS = KEBAB_FEW_TOKENS, MAX_K = 32;
 constexpr int WARPS = 8, THREADS = 32 * (WARPS + 1);  // and the copying one
 constexpr int CHUNK = 2048;                           // bytes of a row in a stage, at most
-constexpr int STAGE = 16 * CHUNK, STAGES = 5;
+constexpr int STAGE = 16 * (CHUNK + 64);
 constexpr int STEPS = CHUNK / 64 / WARPS;             // steps of a chunk that a warp takes, at most
 constexpr int MT = 4;                                 // 16-row tiles of a pass
 constexpr int RED = 68;                               // floats from one token's partial sums (64 rows) to the next's
@@ -68,7 +67,8 @@ struct LayerArgs {
   const float* router;
   // The workspace.
   float* logits;      // [T][E]
-  float* hidden;      // [T k][D]
+  void* hidden;       // [T k][d_pitch] floats, or twice as many of the weights' type: the rounded values, the rest
+  int d_pitch;
   uint32_t* top;      // [T k]: bits of the largest |hidden|
   float* x_scale;     // [T], 8-bit
   int8_t* x_codes;    // [T][x_pitch], 8-bit
@@ -81,7 +81,7 @@ struct LayerArgs {
 // ------------------------------------------------------------------- logits
 
 template <typename T>
-__global__ void __launch_bounds__(256) layer_logits_kernel(const LayerArgs g) {
+__global__ void __launch_bounds__(256) layer_logits_kernel(const LayerArgs g, int split) {
   __shared__ float part[8][MAX_TOKENS];
   __shared__ uint32_t tops[8];
   pdl_wait();
@@ -110,7 +110,17 @@ __global__ void __launch_bounds__(256) layer_logits_kernel(const LayerArgs g) {
   }
   const int e = blockIdx.x;
   if (e == 0) {
-    for (int i = threadIdx.x; i < g.T * g.k; i += 256) g.top[i] = 0;
+    for (int i = threadIdx.x; i < g.T * g.k; i += 256) {
+      g.top[i] = 0;
+      // The hidden values' rows are filled up with zeros (as floats or as pairs).
+      float* row = static_cast<float*>(g.hidden) + (int64_t)i * g.d_pitch;
+      if (split) {
+        T* hi = reinterpret_cast<T*>(row);
+        for (int d = g.D; d < g.d_pitch; ++d) hi[d] = hi[g.d_pitch + d] = from_float<T>(0.f);
+      } else {
+        for (int d = g.D; d < g.d_pitch; ++d) row[d] = 0.f;
+      }
+    }
     if (threadIdx.x == 0) *g.arrived = 0;
   }
   const float* r = g.router + (int64_t)e * g.H;
@@ -196,13 +206,11 @@ struct Mma<T, true> {
   }
 };
 
-__device__ __forceinline__ uint32_t two(__half, float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t two(__nv_bfloat16, float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
+// Whether hidden values are stored as two numbers of the weights' type: BF16 has
+// FP32's range, F16 needs a scale that is known only when all of them are.
+template <typename TX, bool I8>
+constexpr bool is_split() {
+  return !I8 && std::is_same<TX, __nv_bfloat16>::value;
 }
 
 // How rows of `bytes` lie in the ring: chunks of equal size (a multiple of 64
@@ -214,24 +222,32 @@ struct Shape {
     bytes = row;
     chunks = (int)((row + CHUNK - 1) / CHUNK);
     chunk = (int)((row + 64 * (int64_t)chunks - 1) / (64 * (int64_t)chunks)) * 64;
-    // Rows in one piece are copied together, as they lie.
-    pitch = fast && chunks == 1 ? (int)row : chunk;
-    unit = 16 * chunk;
+    // Short rows are copied together, as they lie. Others one by one, to an odd
+    // multiple of 64 bytes, so that the warps read two rows without a conflict.
+    pitch = fast && row < 512 ? (int)row : chunk + (chunk % 128 == 0 ? 64 : 0);
+    unit = 16 * pitch;
     units = STAGE / unit;
   }
+  __device__ __forceinline__ bool together() const { return pitch == bytes; }
   __device__ __forceinline__ int length(int c) const { return (int)min((int64_t)chunk, bytes - (int64_t)c * chunk); }
 };
 
+// Shared memory: the ring, the warps' partial sums, barriers, and tables of the
+// choices: weights, scales, factors (float [T k]), experts [T k], the chosen
+// experts in ascending order [T k], who chose them ([T k][T]: 32 t + j), how many
+// did (bytes [T k]), flags (bytes [E]).
+template <int NT>
 struct LayerSmem {
+  static constexpr int STAGES = NT == 1 ? 6 : 5;
   static constexpr int OFF_RED = STAGES * STAGE;
-  static __host__ __device__ constexpr int off_bar(int nt) { return OFF_RED + WARPS * nt * 8 * RED * 4; }
-  static __host__ __device__ constexpr int off_tables(int nt) { return off_bar(nt) + 2 * STAGES * 8 + 16; }
-  // weights, factors [T k] (float), experts [T k], active [T k], place of an
-  // active expert among a token's choices [T k][T] (bytes), flags [E] (bytes)
-  static __host__ __device__ int bytes(int nt, int T, int k, int E) {
+  static constexpr int OFF_BAR = OFF_RED + WARPS * NT * 8 * RED * 4;
+  static constexpr int OFF_TABLES = OFF_BAR + 2 * STAGES * 8 + 16;
+  static constexpr int bytes(int T, int k, int E) {
     const int n = T * k;
-    return off_tables(nt) + n * 16 + n * T + E + 16;
+    return OFF_TABLES + n * 20 + n * T * 2 + n + E + 128;  // and the alignment
   }
+  static constexpr int MOST = bytes(NT * 8, MAX_K, kMaxExperts);
+  static_assert(MOST <= 232448, "shared memory budget exceeded");
 };
 
 // The top-k choices of token t by one warp: as kebab_route.
@@ -304,22 +320,28 @@ template <typename TX, bool I8, int NT>
 __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
   using M = Mma<TX, I8>;
   using Acc = typename M::Acc;
+  using L = LayerSmem<NT>;
+  constexpr int STAGES = L::STAGES;
   constexpr int ES = I8 ? 1 : 2;       // bytes of a weight
   constexpr int PIECE = 16 / ES;       // values of 16 bytes
   constexpr int PARTS = I8 ? 1 : 2;    // operands that a hidden value makes
+  constexpr bool SPLIT = is_split<TX, I8>();
+  constexpr int RAW = I8 ? 4 : 2;      // registers of 16 bytes that hold a piece's hidden values as they are stored
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
-  uint32_t* red = reinterpret_cast<uint32_t*>(smem + LayerSmem::OFF_RED);  // [WARPS][NT][8][RED]
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + LayerSmem::off_bar(NT));
+  uint32_t* red = reinterpret_cast<uint32_t*>(smem + L::OFF_RED);  // [WARPS][NT * 8][RED]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* empty = full + STAGES;
-  int* s_count = reinterpret_cast<int*>(empty + STAGES);  // active experts; whether the grid barrier failed
+  int* s_count = reinterpret_cast<int*>(empty + STAGES);  // chosen experts; whether the grid barrier failed
   const int choices = g.T * g.k;
-  float* s_weight = reinterpret_cast<float*>(smem + LayerSmem::off_tables(NT));  // [T][k]
-  float* s_factor = s_weight + choices;                                          // [T][k]
-  int* s_expert = reinterpret_cast<int*>(s_factor + choices);                    // [T][k]
-  int* s_active = s_expert + choices;                                            // [active]
-  uint8_t* s_place = reinterpret_cast<uint8_t*>(s_active + choices);             // [active][T]: j, or 255
-  uint8_t* s_flag = s_place + choices * g.T;                                     // [E]
+  float* s_weight = reinterpret_cast<float*>(smem + L::OFF_TABLES);
+  float* s_scale = s_weight + choices;
+  float* s_factor = s_scale + choices;
+  int* s_expert = reinterpret_cast<int*>(s_factor + choices);
+  int* s_active = s_expert + choices;
+  uint16_t* s_who = reinterpret_cast<uint16_t*>(s_active + choices);
+  uint8_t* s_many = reinterpret_cast<uint8_t*>(s_who + choices * g.T);
+  uint8_t* s_flag = s_many + choices;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const WaitCtx& ctx = g.ctx;
 
@@ -331,7 +353,6 @@ __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
     fence_barrier_init();
     s_count[1] = 0;
   }
-  for (int i = threadIdx.x; i < choices * g.T; i += THREADS) s_place[i] = 255;
   for (int i = threadIdx.x; i < g.E; i += THREADS) s_flag[i] = 0;
   if (g.pdl) pdl_wait();
   __syncthreads();
@@ -343,7 +364,6 @@ __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
     }
   }
   __syncthreads();
-  // The chosen experts in ascending order, by one warp.
   if (warp == 0) {
     int n = 0;
     for (int e0 = 0; e0 < g.E; e0 += 32) {
@@ -356,15 +376,13 @@ __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
   }
   __syncthreads();
   const int active = s_count[0];
-  for (int i = threadIdx.x; i < choices; i += THREADS) {
-    const int e = s_expert[i];
-    int lo = 0, hi = active - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (s_active[mid] < e) lo = mid + 1;
-      else hi = mid;
-    }
-    s_place[lo * g.T + i / g.k] = (uint8_t)(i % g.k);
+  for (int a = threadIdx.x; a < active; a += THREADS) {
+    const int e = s_active[a];
+    int n = 0;
+    for (int t = 0; t < g.T; ++t)
+      for (int j = 0; j < g.k; ++j)
+        if (s_expert[t * g.k + j] == e) s_who[a * g.T + n++] = (uint16_t)(32 * t + j);
+    s_many[a] = (uint8_t)n;
   }
   __syncthreads();
 
@@ -402,7 +420,7 @@ __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
       if (g.fast) {
         if (lane == 0) mbar_expect_tx(&full[stage], copies * len);
         __syncwarp();
-        if (s.chunks == 1) {
+        if (s.together()) {
           if (lane == 0) bulk_load(dst, src, rows * len, &full[stage]);
           if (lane == 1 && second) bulk_load(dst + 8 * s.pitch, second, rows * len, &full[stage]);
         } else if (second ? (lane & 7) < rows && lane < 16 : lane < rows) {
@@ -460,6 +478,8 @@ __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
     if (ok) finish();
   } else {
     // ----------------------------------------------------------- products
+    // The columns of an MMA are the tokens that chose the expert. More than 8
+    // are rare; they take a second MMA, whose operands are not loaded ahead.
     const int gq = lane >> 2, cq = lane & 3;
     using One = std::integral_constant<int, 1>;
     using All = std::integral_constant<int, PARTS>;
@@ -481,8 +501,9 @@ __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
       advance();
       left = 0;
     };
-    // The next tile, with the first `parts` operands of every value.
-    auto multiply = [&](const Shape& s, int len, auto parts, Acc (&d)[NT][4]) {
+    // The next tile, with the first `parts` operands of every value, in two
+    // chains of MMAs.
+    auto multiply = [&](const Shape& s, int len, bool wide, auto parts, Acc (&d)[NT][4]) {
       if (left == 0) {
         if (ok) ok = all_ok(mbar_wait(&full[stage], phase, ctx, SITE_FULL));
         left = s.units;
@@ -490,7 +511,13 @@ __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
       } else {
         at += s.unit;
       }
+      constexpr bool TWO = decltype(parts)::value == 2;
       const uint8_t* row = at + gq * s.pitch + cq * 16;
+      Acc f[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[n][i] = 0;
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
         const int off = (warp + i * WARPS) * 64;
@@ -501,27 +528,24 @@ __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
           hi = *reinterpret_cast<const uint4*>(row + 8 * s.pitch + off);
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int p = 0; p < decltype(parts)::value; ++p) {
-            M::mma(d[n], lo.x, hi.x, lo.y, hi.y, b[i][n][p][0], b[i][n][p][1]);
-            M::mma(d[n], lo.z, hi.z, lo.w, hi.w, b[i][n][p][2], b[i][n][p][3]);
-          }
+        for (int n = 0; n < NT; ++n) {
+          if (n > 0 && !wide) break;
+          M::mma(d[n], lo.x, hi.x, lo.y, hi.y, b[i][n][0][0], b[i][n][0][1]);
+          if constexpr (TWO) M::mma(f[n], lo.x, hi.x, lo.y, hi.y, b[i][n][PARTS - 1][0], b[i][n][PARTS - 1][1]);
+          M::mma(TWO ? d[n] : f[n], lo.z, hi.z, lo.w, hi.w, b[i][n][0][2], b[i][n][0][3]);
+          if constexpr (TWO) M::mma(f[n], lo.z, hi.z, lo.w, hi.w, b[i][n][PARTS - 1][2], b[i][n][PARTS - 1][3]);
+        }
       }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[n][i] += f[n][i];
       if (--left == 0) release();
     };
-    // Partial sums of this warp, to be added up over the warps: token, then row.
-    auto put = [&](int m, int n, const uint32_t (&v)[4]) {
-      uint32_t* to = red + ((warp * NT + n) * 8 + 2 * cq) * RED + m * 16 + gq;
-      to[0] = v[0];
-      to[RED] = v[1];
-      to[8] = v[2];
-      to[RED + 8] = v[3];
-    };
     auto meet = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
-    // The sum over the warps of row r of token t.
+    // The sum over the warps of row r of column t.
     auto total_of = [&](int t, int r) {
-      const uint32_t* from = red + (t / 8 * 8 + t % 8) * RED + r;
+      const uint32_t* from = red + t * RED + r;
       Acc sum = 0;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
@@ -532,61 +556,81 @@ __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
       return sum;
     };
 
-    // Hidden values: a = silu(gate) * up.
+    // Hidden values: a = silu(gate) * up. The tokens' values of this warp's steps
+    // are loaded a chunk ahead.
+    uint4 next[STEPS];
+    auto fetch = [&](int a, int c, int n, uint4 (&to)[STEPS]) {
+      const int len = up.length(c), col = n * 8 + gq;
+      const bool is = col < s_many[a];
+      const int t = is ? s_who[a * g.T + col] >> 5 : 0;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int off = (warp + i * WARPS) * 64 + cq * 16;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (is && off < len) {
+          const int64_t k0 = ((int64_t)c * up.chunk + off) / ES;
+          if constexpr (I8) {
+            v = *reinterpret_cast<const uint4*>(g.x_codes + (int64_t)t * g.x_pitch + k0);
+          } else {
+            const uint16_t* x = static_cast<const uint16_t*>(g.x) + t * g.ldx + k0;
+            if (g.vec_x && k0 + 8 <= g.H) {
+              v = *reinterpret_cast<const uint4*>(x);
+            } else {
+              uint32_t h[8];
+#pragma unroll
+              for (int u = 0; u < 8; ++u) h[u] = k0 + u < g.H ? x[u] : 0;
+              v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+            }
+          }
+        }
+        to[i] = v;
+      }
+    };
+    auto operands = [&](int n, const uint4 (&from)[STEPS]) {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const uint4 v = from[i];
+        b[i][n][0][0] = v.x, b[i][n][0][1] = v.y, b[i][n][0][2] = v.z, b[i][n][0][3] = v.w;
+      }
+    };
+    if (p0 < p1) fetch((int)(p0 / g.D), 0, 0, next);
     for (int64_t p = p0; p < p1;) {
       const int a = (int)(p / g.D), i0 = (int)(p - (int64_t)a * g.D);
       const int n = (int)min((int64_t)min(PAIRS, g.D - i0), p1 - p);
+      const bool wide = NT > 1 && s_many[a] > 8;
       clear();
       for (int c = 0; c < up.chunks; ++c) {
+        operands(0, next);
+        if (wide) {
+          fetch(a, c, NT - 1, next);
+          operands(NT - 1, next);
+        }
+        if (c + 1 < up.chunks) fetch(a, c + 1, 0, next);
+        else if (p + n < p1) fetch(i0 + n < g.D ? a : a + 1, 0, 0, next);
         const int len = up.length(c);
-        // The tokens' values of this warp's steps.
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const int t = nt * 8 + gq, off = (warp + i * WARPS) * 64 + cq * 16;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (t < g.T && off < len) {
-              const int64_t k0 = ((int64_t)c * up.chunk + off) / ES;
-              if constexpr (I8) {
-                v = *reinterpret_cast<const uint4*>(g.x_codes + (int64_t)t * g.x_pitch + k0);
-              } else {
-                const uint16_t* x = static_cast<const uint16_t*>(g.x) + t * g.ldx + k0;
-                if (g.vec_x && k0 + 8 <= g.H) {
-                  v = *reinterpret_cast<const uint4*>(x);
-                } else {
-                  uint32_t h[8];
-#pragma unroll
-                  for (int u = 0; u < 8; ++u) h[u] = k0 + u < g.H ? x[u] : 0;
-                  v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-                }
-              }
-            }
-            b[i][nt][0][0] = v.x, b[i][nt][0][1] = v.y, b[i][nt][0][2] = v.z, b[i][nt][0][3] = v.w;
-          }
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-          if (m * 8 < n) multiply(up, len, One(), acc[m]);
+          if (m * 8 < n) multiply(up, len, wide, One(), acc[m]);
       }
+      // This warp's partial sums: column, then row.
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          uint32_t v[4];
+          if (nt > 0 && !wide) break;
+          uint32_t* to = red + ((warp * NT + nt) * 8 + 2 * cq) * RED + m * 16 + gq;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if constexpr (I8) v[i] = (uint32_t)acc[m][nt][i];
-            else v[i] = __float_as_uint(acc[m][nt][i]);
+            const Acc v = acc[m][nt][i];
+            to[(i & 1) * RED + (i >> 1) * 8] = *reinterpret_cast<const uint32_t*>(&v);
           }
-          put(m, nt, v);
         }
       meet();
-      // A warp a token, a lane a value.
-      for (int t = warp; t < g.T; t += WARPS) {
-        const int j = s_place[a * g.T + t];
-        if (j == 255) continue;
+      // A warp a column, a lane a value.
+      for (int col = warp; col < s_many[a]; col += WARPS) {
+        const int who = s_who[a * g.T + col], t = who >> 5, choice = t * g.k + (who & 31);
         const int row = lane / 8 * 16 + lane % 8, i = i0 + lane;
-        float gate = (float)total_of(t, row), value = (float)total_of(t, row + 8);
+        float gate = (float)total_of(col, row), value = (float)total_of(col, row + 8);
         if constexpr (I8) {
           const float s = g.x_scale[t];
           const float* scale = g.in_scale + (int64_t)s_active[a] * 2 * g.D + i;
@@ -594,9 +638,18 @@ __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
           value *= s * (lane < n ? scale[g.D] : 0.f);
         }
         const float h = gate / (1.f + expf(-gate)) * value;
-        if (lane < n && ok) g.hidden[(int64_t)(t * g.k + j) * g.D + i] = h;
-        const uint32_t top = __reduce_max_sync(0xffffffffu, lane < n ? abs_bits(h) : 0u);
-        if (lane == 0) atomicMax(g.top + t * g.k + j, top);
+        if constexpr (SPLIT) {
+          if (lane < n && ok) {
+            TX* to = static_cast<TX*>(g.hidden) + (int64_t)choice * 2 * g.d_pitch + i;
+            const TX hi = from_float<TX>(h);
+            to[0] = hi;
+            to[g.d_pitch] = from_float<TX>(isinf(to_float(hi)) ? 0.f : h - to_float(hi));  // what the rounding left
+          }
+        } else {
+          if (lane < n && ok) static_cast<float*>(g.hidden)[(int64_t)choice * g.d_pitch + i] = h;
+          const uint32_t top = __reduce_max_sync(0xffffffffu, lane < n ? abs_bits(h) : 0u);
+          if (lane == 0) atomicMax(g.top + choice, top);
+        }
       }
       meet();
       p += n;
@@ -624,90 +677,114 @@ __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
     }
     meet();
     if (s_count[1]) ok = false;
-    // What a choice's products are multiplied by: its weight and the inverse of its values' scale.
+    // What a choice's values are multiplied by before they are rounded, and its
+    // products after: the inverse, and the choice's weight.
     for (int i = threadIdx.x; i < choices; i += 32 * WARPS) {
-      const uint32_t top = __ldcg(g.top + i);
-      float inverse;
-      if constexpr (I8) inverse = row_scale(top).scale;
-      else power_for(top, inverse);
+      float inverse = 1.f;
+      if constexpr (I8) {
+        const RowScale code = row_scale(__ldcg(g.top + i));
+        s_scale[i] = code.inv;
+        inverse = code.scale;
+      } else if constexpr (!SPLIT) {
+        s_scale[i] = power_for(__ldcg(g.top + i), inverse);
+      }
       s_factor[i] = s_weight[i] * inverse;
     }
     meet();
 
-    // Outputs.
-    for (int r0 = n0; r0 < n1; r0 += ROWS) {
-      const int n = min(ROWS, n1 - r0);
-      float out[MT][NT][4];
+    // Outputs. The hidden values are loaded a chunk ahead, too.
+    uint4 raw[STEPS][RAW];
+    auto load = [&](int a, int c, int n) {
+      const int len = down.length(c), col = n * 8 + gq;
+      const bool is = col < s_many[a];
+      const int who = is ? s_who[a * g.T + col] : 0, choice = (who >> 5) * g.k + (who & 31);
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int i = 0; i < STEPS; ++i) {
+        const int off = (warp + i * WARPS) * 64 + cq * 16;
+        const int64_t k0 = ((int64_t)c * down.chunk + off) / ES;
+        const uint4* from;
+        if constexpr (SPLIT) from = reinterpret_cast<const uint4*>(static_cast<const TX*>(g.hidden) + (int64_t)choice * 2 * g.d_pitch + k0);
+        else from = reinterpret_cast<const uint4*>(static_cast<const float*>(g.hidden) + (int64_t)choice * g.d_pitch + k0);
+        const int64_t step = SPLIT ? g.d_pitch / 8 : 1;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int u = 0; u < RAW; ++u)
+          raw[i][u] = is && off < len ? __ldcg(from + u * step) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto convert = [&](int a, int n) {
+      if constexpr (SPLIT) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) out[m][nt][i] = 0.f;
-      for (int a = 0; a < active; ++a) {
-        clear();
-        for (int c = 0; c < down.chunks; ++c) {
-          const int len = down.length(c);
+        for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const int t = nt * 8 + gq;
-            const int j = t < g.T ? s_place[a * g.T + t] : 255;
-            const float* h = g.hidden + (int64_t)(j == 255 ? 0 : t * g.k + j) * g.D;
-            const uint32_t top = j == 255 ? 0u : __ldcg(g.top + t * g.k + j);
-            float scale, unused;
-            if constexpr (I8) scale = row_scale(top).inv;
-            else scale = power_for(top, unused);
+          for (int p = 0; p < 2; ++p) {
+            const uint4 v = raw[i][p];
+            uint32_t* to = b[i][n][p % PARTS];
+            to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+          }
+      } else {
+        const int col = n * 8 + gq;
+        const bool is = col < s_many[a];
+        const int who = is ? s_who[a * g.T + col] : 0;
+        const float scale = is ? s_scale[(who >> 5) * g.k + (who & 31)] : 0.f;
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-              const int off = (warp + i * WARPS) * 64 + cq * 16;
-              float v[PIECE];
+        for (int i = 0; i < STEPS; ++i) {
+          float v[RAW * 4];
 #pragma unroll
-              for (int u = 0; u < PIECE; ++u) v[u] = 0.f;
-              if (j != 255 && off < len) {
-                const int64_t k0 = ((int64_t)c * down.chunk + off) / ES;
-                if (g.fast) {
-#pragma unroll
-                  for (int u = 0; u < PIECE; u += 4) {
-                    const float4 f = __ldcg(reinterpret_cast<const float4*>(h + k0 + u));
-                    v[u] = f.x, v[u + 1] = f.y, v[u + 2] = f.z, v[u + 3] = f.w;
-                  }
-                } else {
-#pragma unroll
-                  for (int u = 0; u < PIECE; ++u) v[u] = k0 + u < g.D ? __ldcg(h + k0 + u) : 0.f;
-                }
-              }
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                if constexpr (I8) {
-                  uint32_t code[4];
-#pragma unroll
-                  for (int u = 0; u < 4; ++u) code[u] = scale == 0.f ? 0u : code_bits(v[4 * q + u], scale);
-                  b[i][nt][0][q] = pack4(code[0], code[1], code[2], code[3]);
-                } else {
-                  const float x0 = v[2 * q] * scale, x1 = v[2 * q + 1] * scale;
-                  const uint32_t hi = two(TX(), x0, x1);
-                  const TX* parts = reinterpret_cast<const TX*>(&hi);
-                  // What the rounding left; of an infinity nothing.
-                  const float l0 = x0 - to_float(parts[0]), l1 = x1 - to_float(parts[1]);
-                  b[i][nt][0][q] = hi;
-                  b[i][nt][PARTS - 1][q] = two(TX(), isinf(x0) ? 0.f : l0, isinf(x1) ? 0.f : l1);
-                }
-              }
-            }
+          for (int u = 0; u < RAW; ++u) {
+            v[4 * u] = __uint_as_float(raw[i][u].x), v[4 * u + 1] = __uint_as_float(raw[i][u].y);
+            v[4 * u + 2] = __uint_as_float(raw[i][u].z), v[4 * u + 3] = __uint_as_float(raw[i][u].w);
           }
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
-            if (m * 16 < n) multiply(down, len, All(), acc[m]);
+          for (int q = 0; q < 4; ++q) {
+            if constexpr (I8) {
+              uint32_t code[4];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) code[u] = code_bits(v[4 * q + u], scale);
+              b[i][n][0][q] = scale == 0.f ? 0u : pack4(code[0], code[1], code[2], code[3]);
+            } else {
+              const float x0 = v[2 * q] * scale, x1 = v[2 * q + 1] * scale;
+              const __half2 hi = __floats2half2_rn(x0, x1);
+              const float2 h = __half22float2(hi);
+              // What the rounding left; of an infinity nothing.
+              const __half2 lo = __floats2half2_rn(isinf(x0) ? 0.f : x0 - h.x, isinf(x1) ? 0.f : x1 - h.y);
+              b[i][n][0][q] = *reinterpret_cast<const uint32_t*>(&hi);
+              b[i][n][PARTS - 1][q] = *reinterpret_cast<const uint32_t*>(&lo);
+            }
+          }
         }
-        // Each token takes its own experts' products only.
+      }
+    };
+    if (n0 < n1) load(0, 0, 0);
+    float* sums = reinterpret_cast<float*>(red) + warp * NT * 8 * RED;  // this warp's: token, then row
+    for (int r0 = n0; r0 < n1; r0 += ROWS) {
+      const int n = min(ROWS, n1 - r0);
+      for (int i = lane; i < NT * 8 * RED; i += 32) sums[i] = 0.f;
+      __syncwarp();
+      for (int a = 0; a < active; ++a) {
+        const bool wide = NT > 1 && s_many[a] > 8;
+        clear();
+        for (int c = 0; c < down.chunks; ++c) {
+          convert(a, 0);
+          if (wide) {
+            load(a, c, NT - 1);
+            convert(a, NT - 1);
+          }
+          if (c + 1 < down.chunks) load(a, c + 1, 0);
+          else load(a + 1 < active ? a + 1 : 0, 0, 0);
+          const int len = down.length(c);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            if (m * 16 < n) multiply(down, len, wide, All(), acc[m]);
+        }
+        // Onto the tokens' sums.
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const int t = nt * 8 + 2 * cq + u;
-            const int j = t < g.T ? s_place[a * g.T + t] : 255;
-            if (j == 255) continue;
-            const float factor = s_factor[t * g.k + j];
+            const int col = nt * 8 + 2 * cq + u;
+            if (col >= s_many[a]) continue;
+            const int who = s_who[a * g.T + col], t = who >> 5;
+            const float factor = s_factor[t * g.k + (who & 31)];
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
               if (m * 16 >= n) break;
@@ -718,26 +795,19 @@ __global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
                   const int r = r0 + m * 16 + v * 8 + gq;
                   f *= r < n1 ? g.out_scale[(int64_t)s_active[a] * g.H + r] : 0.f;
                 }
-                out[m][nt][2 * v + u] += f * (float)acc[m][nt][2 * v + u];
+                sums[t * RED + m * 16 + v * 8 + gq] += f * (float)acc[m][nt][2 * v + u];
               }
             }
           }
+        __syncwarp();  // another lane may have the token's column of the next expert
       }
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const uint32_t v[4] = {__float_as_uint(out[m][nt][0]), __float_as_uint(out[m][nt][1]),
-                                 __float_as_uint(out[m][nt][2]), __float_as_uint(out[m][nt][3])};
-          put(m, nt, v);
-        }
       meet();
       for (int t = warp; t < g.T; t += WARPS) {
         for (int r = lane; r < n; r += 32) {
-          const uint32_t* from = red + t * RED + r;
+          const float* from = reinterpret_cast<const float*>(red) + t * RED + r;
           float sum = 0.f;
 #pragma unroll
-          for (int w = 0; w < WARPS; ++w) sum += __uint_as_float(from[w * NT * 8 * RED]);
+          for (int w = 0; w < WARPS; ++w) sum += from[w * NT * 8 * RED];
           if (ok) static_cast<TX*>(g.y)[t * g.ldy + r0 + r] = from_float<TX>(sum);
         }
       }
@@ -758,7 +828,7 @@ struct Sizes {
 int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
 
 // logits, hidden values, their largest, the tokens' scales, the barrier's count; the tokens' codes.
-int64_t words(const Sizes& s) { return up16(s.T * s.E * 4) + up16(s.T * s.k * s.D * 4) + up16(s.T * s.k * 4) + 64 + 16; }
+int64_t words(const Sizes& s) { return up16(s.T * s.E * 4) + s.T * s.k * up16(s.D) * 4 + up16(s.T * s.k * 4) + 64 + 16; }
 int64_t bytes(const Sizes& s) { return words(s) + s.T * up16(s.H); }
 
 int check(const char* what, int dtype, const void* x, int64_t ldx, const void* router, const void* w_in,
@@ -793,13 +863,13 @@ int launch(LayerArgs& g, cudaStream_t stream) {
   const int di = dev->device & 63;
   std::call_once(once[di], [&] {
     err[di] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   std::min(LayerSmem::bytes(NT, MAX_TOKENS, MAX_K, kMaxExperts) + 128, 232448));
+                                   LayerSmem<NT>::MOST);
   });
   if (err[di] != cudaSuccess) return cuda_fail(err[di], "cudaFuncSetAttribute(max dynamic smem)");
   PdlLaunch first(dim3((unsigned)(g.E + (I8 ? g.T : 0))), dim3(256), 0, stream);
-  cudaError_t e = cudaLaunchKernelEx(&first.cfg, layer_logits_kernel<TX>, (const LayerArgs)g);
+  cudaError_t e = cudaLaunchKernelEx(&first.cfg, layer_logits_kernel<TX>, (const LayerArgs)g, (int)is_split<TX, I8>());
   if (e != cudaSuccess) return cuda_fail(e, "expert_layer: logits launch");
-  const int smem = LayerSmem::bytes(NT, g.T, g.k, g.E) + 128;
+  const int smem = LayerSmem<NT>::bytes(g.T, g.k, g.E);
   PdlLaunch l(dim3((unsigned)dev->sm_count), dim3(THREADS), smem, stream);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeCooperative;
@@ -822,7 +892,8 @@ int run(int dtype, LayerArgs g, const Sizes& s, void* ws, kebab_stream_t stream)
     return p;
   };
   g.logits = reinterpret_cast<float*>(take(s.T * s.E * 4));
-  g.hidden = reinterpret_cast<float*>(take(s.T * s.k * s.D * 4));
+  g.d_pitch = (int)up16(s.D);
+  g.hidden = take(s.T * s.k * g.d_pitch * 4);
   g.top = reinterpret_cast<uint32_t*>(take(s.T * s.k * 4));
   g.x_scale = reinterpret_cast<float*>(take(64));
   g.arrived = reinterpret_cast<uint32_t*>(take(16));
