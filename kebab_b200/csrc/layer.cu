@@ -5,29 +5,29 @@
 // is one CTA an SM, all resident (a cooperative launch): every CTA finds the
 // top-k choices by itself, takes an equal share of the hidden values of all
 // chosen experts (a gate row and an up row each), meets the others at a grid
-// barrier, and takes an equal share of the layer's outputs, over all chosen
-// experts. So the sum over a token's experts needs no further exchange, and the
+// barrier, and takes an equal share of the rows of the chosen experts' second
+// matrices. A choice's outputs go to the workspace, weighted; whoever completes
+// a block of 32 outputs adds them up, in the order of the choices, so that the
 // results do not depend on who comes first.
 //
-// Bound by the chosen experts' bytes, and by latency for few of them. One warp
-// copies the CTA's weights, which are contiguous rows, through a ring of 32 KB
-// stages; it does not wait at the grid barrier, so that the second product's
-// weights arrive meanwhile. Eight warps multiply on the tensor cores (mma.sync,
-// 16 weight rows by 8 tokens: the tokens are so few that this takes a tenth of
-// the time that the bytes take, and unlike a tile of 128 rows it lets the CTAs
-// share the rows evenly). They split the row's length in steps of 64 bytes:
-// lane (g, c) of a warp reads the 16 bytes c of the step from rows g and g + 8,
-// which are the operand registers of two MMAs if the tokens' values are read in
-// the same order, since a sum over k may take its terms in any.
+// Bound by the chosen experts' bytes, and by latency for few of them. Weights
+// come by TMA in K-blocks of 128 bytes a row, through a ring of some 200 KB, as
+// the row side of tcgen05.mma (up to 128 rows; rows that the CTA does not own
+// are not loaded, and what the MMA reads in their place ends in rows that are
+// not used). The tokens, or the hidden values of the tokens that chose the
+// expert, are the 16 columns. A warp of its own copies the columns: at the grid
+// barrier only it waits, while the second matrices' rows arrive in the ring.
 //
-// An expert's rows are multiplied with the tokens that chose it and added onto
-// those only: what other experts hold (infinities, NaN) does not reach a token.
+// A token takes the products of its own experts only, from columns of its own:
+// what other experts or tokens hold (infinities, NaN) does not reach it.
 //
 // For 16-bit weights the hidden values enter the second product as the sum of
-// two 16-bit numbers (at least 16 bits of them); F16 ones scaled by the power of
-// two that brings the largest of a choice's values to [2^13, 2^14). For 8-bit
-// weights they are codes of that largest value / 127. The largest is found with
-// atomic maxima, which do not depend on their order.
+// two 16-bit numbers, 16 columns each (at least 16 bits of them); F16 ones scaled
+// by the power of two that brings the largest of a choice's values to [2^13,
+// 2^14). For 8-bit weights they are codes of that largest value / 127. The
+// largest is found with atomic maxima, which do not depend on their order; it is
+// known at the grid barrier, after which every CTA converts its share, and all
+// meet once more. BF16 has FP32's range: its values are split as they are made.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -36,6 +36,7 @@
 #include <string>
 #include <type_traits>
 
+#include "gemm_umma.cuh"
 #include "grouped.h"
 #include "kebab/layer.h"
 #include "quant_i8.cuh"
@@ -44,12 +45,17 @@ namespace kb {
 namespace {
 
 constexpr int MAX_TOKENS = KEBAB_FEW_TOKENS, MAX_K = 32;
-constexpr int WARPS = 8, THREADS = 32 * (WARPS + 1);  // and the copying one
-constexpr int CHUNK = 2048;                           // bytes of a row in a stage, at most
-constexpr int STAGE = 16 * (CHUNK + 64);
-constexpr int STEPS = CHUNK / 64 / WARPS;             // steps of a chunk that a warp takes, at most
-constexpr int MT = 4;                                 // 16-row tiles of a pass
-constexpr int RED = 68;                               // floats from one token's partial sums (64 rows) to the next's
+// Warps: copies of weights, MMA issuer, copies of columns, copies of weights,
+// four for the epilogue.
+constexpr int THREADS = 256, EPI_WARP = 4;
+constexpr int ROWS = 128;                 // weight rows of a pass
+constexpr int COLUMNS = 16 * 128;         // bytes of 16 columns of a K-block
+constexpr int MAX_SLOTS = 16, MAX_UNITS = 8;
+constexpr int TAIL = 128 * 128;           // what an MMA may read past the ring: the tables lie there
+constexpr int RING = 200 * 1024;
+constexpr int SLOT = 40 * 1024;           // bytes of a slot, about
+constexpr int BLOCK = 32;                 // outputs that are added up together
+constexpr int TMEM_COLS = 64;             // two sets of 32
 
 struct LayerArgs {
   const void* x;
@@ -62,26 +68,36 @@ struct LayerArgs {
   int64_t ldy;
   int T, E, k, H, D;
   int renormalize;
-  int fast;   // weight rows on 16-byte boundaries: copied by the bulk engine
-  int vec_x;  // rows of x (or of its codes) on 16-byte boundaries
+  int tma_w, tma_x;  // whether TMA can address the weights, x
+  int vec_x;         // rows of x on 16-byte boundaries
   const float* router;
   // The workspace.
   float* logits;      // [T][E]
-  void* hidden;       // [T k][d_pitch] floats, or twice as many of the weights' type: the rounded values, the rest
-  int d_pitch;
-  uint32_t* top;      // [T k]: bits of the largest |hidden|
+  float* hidden;      // [T k][D] by expert and token, not BF16
+  uint8_t* operand;   // [2][T k][d_bytes]: the rounded values, the rest; or [T k][d_bytes] codes
+  int d_bytes;
+  uint32_t* top;      // [T k]: bits of the largest |hidden|, not BF16
+  float* out;         // [T k][out_pitch]: weighted outputs of the choices
+  int out_pitch;
+  uint32_t* done;     // [ceil(H / BLOCK)]: rows of the block that are in `out`
   float* x_scale;     // [T], 8-bit
   int8_t* x_codes;    // [T][x_pitch], 8-bit
   int x_pitch;
-  uint32_t* arrived;  // CTAs at the grid barrier
+  uint32_t* arrived;  // [2]: CTAs at the grid barriers
   int pdl;
   WaitCtx ctx;
+};
+
+// Boxes of 8, 16, .. 64 weight rows: a copy costs about 100 cycles of a warp
+// whatever its height, and a pass has any height.
+struct RowBoxes {
+  CUtensorMap box[8];
 };
 
 // ------------------------------------------------------------------- logits
 
 template <typename T>
-__global__ void __launch_bounds__(256) layer_logits_kernel(const LayerArgs g, int split) {
+__global__ void __launch_bounds__(256) layer_logits_kernel(const LayerArgs g) {
   __shared__ float part[8][MAX_TOKENS];
   __shared__ uint32_t tops[8];
   pdl_wait();
@@ -110,18 +126,9 @@ __global__ void __launch_bounds__(256) layer_logits_kernel(const LayerArgs g, in
   }
   const int e = blockIdx.x;
   if (e == 0) {
-    for (int i = threadIdx.x; i < g.T * g.k; i += 256) {
-      g.top[i] = 0;
-      // The hidden values' rows are filled up with zeros (as floats or as pairs).
-      float* row = static_cast<float*>(g.hidden) + (int64_t)i * g.d_pitch;
-      if (split) {
-        T* hi = reinterpret_cast<T*>(row);
-        for (int d = g.D; d < g.d_pitch; ++d) hi[d] = hi[g.d_pitch + d] = from_float<T>(0.f);
-      } else {
-        for (int d = g.D; d < g.d_pitch; ++d) row[d] = 0.f;
-      }
-    }
-    if (threadIdx.x == 0) *g.arrived = 0;
+    for (int i = threadIdx.x; i < g.T * g.k; i += 256) g.top[i] = 0;
+    for (int i = threadIdx.x; i < (g.H + BLOCK - 1) / BLOCK; i += 256) g.done[i] = 0;
+    if (threadIdx.x < 2) g.arrived[threadIdx.x] = 0;
   }
   const float* r = g.router + (int64_t)e * g.H;
   float sum[MAX_TOKENS];
@@ -170,85 +177,12 @@ __global__ void __launch_bounds__(256) layer_logits_kernel(const LayerArgs g, in
 
 // -------------------------------------------------------------------- layer
 
-template <typename T, bool I8>
-struct Mma;
-template <>
-struct Mma<__half, false> {
-  using Acc = float;
-  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-};
-template <>
-struct Mma<__nv_bfloat16, false> {
-  using Acc = float;
-  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-};
-template <typename T>
-struct Mma<T, true> {
-  using Acc = int;
-  static __device__ __forceinline__ void mma(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-};
-
 // Whether hidden values are stored as two numbers of the weights' type: BF16 has
 // FP32's range, F16 needs a scale that is known only when all of them are.
 template <typename TX, bool I8>
 constexpr bool is_split() {
   return !I8 && std::is_same<TX, __nv_bfloat16>::value;
 }
-
-// How rows of `bytes` lie in the ring: chunks of equal size (a multiple of 64
-// bytes), tiles of 16 rows at a pitch, `units` tiles to a stage.
-struct Shape {
-  int64_t bytes;
-  int chunks, chunk, pitch, unit, units;
-  __device__ __forceinline__ Shape(int64_t row, bool fast) {
-    bytes = row;
-    chunks = (int)((row + CHUNK - 1) / CHUNK);
-    chunk = (int)((row + 64 * (int64_t)chunks - 1) / (64 * (int64_t)chunks)) * 64;
-    // Short rows are copied together, as they lie. Others one by one, to an odd
-    // multiple of 64 bytes, so that the warps read two rows without a conflict.
-    pitch = fast && row < 512 ? (int)row : chunk + (chunk % 128 == 0 ? 64 : 0);
-    unit = 16 * pitch;
-    units = STAGE / unit;
-  }
-  __device__ __forceinline__ bool together() const { return pitch == bytes; }
-  __device__ __forceinline__ int length(int c) const { return (int)min((int64_t)chunk, bytes - (int64_t)c * chunk); }
-};
-
-// Shared memory: the ring, the warps' partial sums, barriers, and tables of the
-// choices: weights, scales, factors (float [T k]), experts [T k], the chosen
-// experts in ascending order [T k], who chose them ([T k][T]: 32 t + j), how many
-// did (bytes [T k]), flags (bytes [E]).
-template <int NT>
-struct LayerSmem {
-  static constexpr int STAGES = NT == 1 ? 6 : 5;
-  static constexpr int OFF_RED = STAGES * STAGE;
-  static constexpr int OFF_BAR = OFF_RED + WARPS * NT * 8 * RED * 4;
-  static constexpr int OFF_TABLES = OFF_BAR + 2 * STAGES * 8 + 16;
-  static constexpr int bytes(int T, int k, int E) {
-    const int n = T * k;
-    return OFF_TABLES + n * 20 + n * T * 2 + n + E + 128;  // and the alignment
-  }
-  static constexpr int MOST = bytes(NT * 8, MAX_K, kMaxExperts);
-  static_assert(MOST <= 232448, "shared memory budget exceeded");
-};
 
 // The top-k choices of token t by one warp: as kebab_route.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -316,507 +250,573 @@ __device__ __forceinline__ float power_for(uint32_t top, float& inverse) {
   return __uint_as_float((uint32_t)(127 + n) << 23);
 }
 
-template <typename TX, bool I8, int NT>
-__global__ void __launch_bounds__(THREADS, 1) layer_kernel(const LayerArgs g) {
-  using M = Mma<TX, I8>;
-  using Acc = typename M::Acc;
-  using L = LayerSmem<NT>;
-  constexpr int STAGES = L::STAGES;
-  constexpr int ES = I8 ? 1 : 2;       // bytes of a weight
-  constexpr int PIECE = 16 / ES;       // values of 16 bytes
-  constexpr int PARTS = I8 ? 1 : 2;    // operands that a hidden value makes
-  constexpr bool SPLIT = is_split<TX, I8>();
-  constexpr int RAW = I8 ? 4 : 2;      // registers of 16 bytes that hold a piece's hidden values as they are stored
+// Shared memory past the ring: barriers, and tables of the choices.
+struct LayerSmem {
+  static constexpr int OFF_BAR = RING;
+  static constexpr int OFF_TABLES = OFF_BAR + (2 * MAX_SLOTS + 4) * 8 + 32;
+  // weights by place, weights, scales (float), places, chosen experts (int), [T k]; who chose an expert,
+  // places before it (uint16, [T k] and one); the same of all (int [E])
+  static __host__ __device__ constexpr int tables(int n, int E) { return OFF_TABLES + n * 20 + (n + 1) * 4 + E * 4; }
+  // The first product's rows, whose threads are the gate rows' or the up rows'.
+  static constexpr int EXCHANGE = ROWS * (MAX_TOKENS + 1) * 4;
+  static constexpr int bytes(int T, int k, int E) {
+    const int n = T * k;
+    const int end = tables(n, E) + EXCHANGE;
+    return (end > RING + TAIL ? end : RING + TAIL) + 1024;  // and the alignment
+  }
+};
+static_assert(LayerSmem::bytes(MAX_TOKENS, MAX_K, kMaxExperts) <= 232448, "shared memory budget exceeded");
+
+// The passes of a CTA: its share [at, end) of active x per rows, cut at the
+// experts' ends and then in equal parts of at most `most`. Where the CTAs divide
+// among the experts with at most an eighth of them left over, no share crosses
+// from one expert to the next, which costs a pass more (1 token, 8 experts: XXX).
+// Made by whole warps; the shuffles tell the compiler that a warp's lanes have
+// the same values.
+struct Passes {
+  int64_t at, end;
+  int per, most;
+  int a, first, rows;  // the expert (by its place among the chosen), the first row, rows
+  int left;            // rows of the segment after this pass
+  __device__ __forceinline__ Passes(int active, int per_expert, int most) : per(per_expert), most(most), rows(0), left(0) {
+    const int ctas = gridDim.x, cta = blockIdx.x, each = ctas / active;
+    if (each * active * 8 >= ctas * 7) {
+      const int64_t before = (int64_t)(cta / each) * per, i = cta % each;
+      at = cta < each * active ? before + per * i / each : 0;
+      end = cta < each * active ? before + per * (i + 1) / each : 0;
+    } else {
+      at = (int64_t)active * per * cta / ctas;
+      end = (int64_t)active * per * (cta + 1) / ctas;
+    }
+  }
+  __device__ __forceinline__ bool next() {
+    if (left > 0) {
+      first += rows;
+    } else {
+      if (at >= end) return false;
+      a = (int)(at / per);
+      first = (int)(at - (int64_t)a * per);
+      left = (int)min((int64_t)(per - first), end - at);
+      at += left;
+    }
+    const int passes = (left + most - 1) / most;
+    rows = (left + passes - 1) / passes;
+    rows = min(left, (rows + 7) / 8 * 8);  // whole boxes but for the last
+    left -= rows;
+    a = __shfl_sync(0xffffffffu, a, 0);
+    first = __shfl_sync(0xffffffffu, first, 0);
+    rows = __shfl_sync(0xffffffffu, rows, 0);
+    return true;
+  }
+};
+
+// One of the two products: rows of the first come in pairs, a gate row and an up
+// row; its columns are the tokens, those of the second the hidden values of the
+// expert's tokens, in `PARTS` operands.
+template <bool UP, int PARTS>
+struct Product {
+  static constexpr bool kUp = UP;
+  static constexpr int MATRICES = UP ? 2 : 1, MOST = ROWS / MATRICES;
+  static constexpr int OPERANDS = UP ? 1 : PARTS;
+  static constexpr int COLUMN_BYTES = OPERANDS * COLUMNS;
+};
+
+// How a pass lies in the ring: units of `bytes` (the matrices' rows, r8 each, then
+// the columns), `units` K-blocks to a slot.
+struct Layout {
+  int r8, bytes, units;
+  template <typename P>
+  __device__ __forceinline__ Layout(P, int rows, int slot) {
+    r8 = (rows + 7) / 8 * 8;
+    bytes = P::MATRICES * r8 * 128 + P::COLUMN_BYTES;
+    units = min(MAX_UNITS, slot / bytes);
+  }
+};
+
+template <typename TX, bool I8>
+__global__ void __launch_bounds__(THREADS, 1)
+    layer_kernel(const __grid_constant__ RowBoxes tmIn, const __grid_constant__ RowBoxes tmOut,
+                 const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmH, const LayerArgs g) {
+  constexpr int ES = I8 ? 1 : 2;              // bytes of a weight
+  constexpr int EPB = 128 / ES;               // values of a K-block
+  constexpr int PARTS = I8 ? 1 : 2;           // operands that a hidden value makes
+  constexpr bool SPLIT = is_split<TX, I8>();  // made in the first product's epilogue
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
-  uint32_t* red = reinterpret_cast<uint32_t*>(smem + L::OFF_RED);  // [WARPS][NT * 8][RED]
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
-  uint64_t* empty = full + STAGES;
-  int* s_count = reinterpret_cast<int*>(empty + STAGES);  // chosen experts; whether the grid barrier failed
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + LayerSmem::OFF_BAR);
+  uint64_t* empty = full + MAX_SLOTS;
+  uint64_t* acc_full = empty + MAX_SLOTS;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  int* s_count = reinterpret_cast<int*>(tmem_slot + 1);  // chosen experts
+  int* s_last = s_count + 1;                             // of the blocks of a pass, which it completed (bits)
   const int choices = g.T * g.k;
-  float* s_weight = reinterpret_cast<float*>(smem + L::OFF_TABLES);
-  float* s_scale = s_weight + choices;
-  float* s_factor = s_scale + choices;
-  int* s_expert = reinterpret_cast<int*>(s_factor + choices);
-  int* s_active = s_expert + choices;
-  uint16_t* s_who = reinterpret_cast<uint16_t*>(s_active + choices);
-  uint8_t* s_many = reinterpret_cast<uint8_t*>(s_who + choices * g.T);
-  uint8_t* s_flag = s_many + choices;
+  float* s_factor = reinterpret_cast<float*>(smem + LayerSmem::OFF_TABLES);  // by place: the choice's weight
+  float* s_weight = s_factor + choices;                                      // [T][k]
+  float* s_scale = s_weight + choices;                                       // by place
+  int* s_place = reinterpret_cast<int*>(s_scale + choices);                  // [T][k], at first the expert
+  int* s_active = s_place + choices;                                         // chosen experts, ascending
+  uint16_t* s_who = reinterpret_cast<uint16_t*>(s_active + choices);         // of each, the tokens that chose it (bits)
+  uint16_t* s_base = s_who + choices;                                        // of each, the place of its first choice
+  uint32_t* s_chose = reinterpret_cast<uint32_t*>(s_base + choices + 2);     // [E]: the tokens that chose it (bits)
+  uint32_t* s_rows = reinterpret_cast<uint32_t*>(smem + LayerSmem::tables(choices, g.E));  // [ROWS][MAX_TOKENS + 1]
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const WaitCtx& ctx = g.ctx;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], WARPS);
+    for (int s = 0; s < MAX_SLOTS; ++s) {
+      mbar_init(&full[s], 3);  // the copying warps
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&acc_full[s], 1);
+      mbar_init(&acc_empty[s], 4);
     }
     fence_barrier_init();
-    s_count[1] = 0;
   }
-  for (int i = threadIdx.x; i < g.E; i += THREADS) s_flag[i] = 0;
+  __syncwarp();
+  if (warp == 1) {
+    tmem_alloc<1>(tmem_slot, TMEM_COLS);
+    tmem_relinquish<1>();
+  }
+  // The tensor maps, whichever boxes the passes will need.
+  if (warp == 2 && lane < 18) {
+    const CUtensorMap* tm = lane < 8 ? &tmIn.box[lane] : lane < 16 ? &tmOut.box[lane - 8] : lane == 16 ? &tmX : &tmH;
+    if (lane == 17 || (lane == 16 ? g.tma_x : g.tma_w)) tma_prefetch_desc(tm);
+  }
+  for (int i = threadIdx.x; i < g.E; i += THREADS) s_chose[i] = 0;
   if (g.pdl) pdl_wait();
   __syncthreads();
-  if (warp < WARPS) {
-    for (int t = warp; t < g.T; t += WARPS) {
-      choose(g, t, s_weight + t * g.k, s_expert + t * g.k);
-      __syncwarp();
-      if (lane < g.k) s_flag[s_expert[t * g.k + lane]] = 1;
-    }
+  for (int t = warp; t < g.T; t += THREADS / 32) {
+    choose(g, t, s_weight + t * g.k, s_place + t * g.k);
+    __syncwarp();
+    if (lane < g.k) atomicOr(&s_chose[s_place[t * g.k + lane]], 1u << t);
   }
   __syncthreads();
   if (warp == 0) {
-    int n = 0;
+    int n = 0, before = 0;
     for (int e0 = 0; e0 < g.E; e0 += 32) {
-      const bool is = e0 + lane < g.E && s_flag[e0 + lane];
-      const uint32_t mask = __ballot_sync(0xffffffffu, is);
-      if (is) s_active[n + __popc(mask & ((1u << lane) - 1u))] = e0 + lane;
+      const uint32_t who = e0 + lane < g.E ? s_chose[e0 + lane] : 0u;
+      const uint32_t mask = __ballot_sync(0xffffffffu, who != 0);
+      if (mask == 0) continue;
+      int sum = __popc(who);
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += up;
+      }
+      if (who) {
+        const int a = n + __popc(mask & ((1u << lane) - 1u));
+        s_active[a] = e0 + lane;
+        s_who[a] = (uint16_t)who;
+        s_base[a] = (uint16_t)(before + sum - __popc(who));
+        s_chose[e0 + lane] = (who & 0xffffu) | (uint32_t)(before + sum - __popc(who)) << 16;
+      }
       n += __popc(mask);
+      before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (lane == 0) s_count[0] = n;
+    if (lane == 0) *s_count = n;
   }
   __syncthreads();
-  const int active = s_count[0];
-  for (int a = threadIdx.x; a < active; a += THREADS) {
-    const int e = s_active[a];
-    int n = 0;
-    for (int t = 0; t < g.T; ++t)
-      for (int j = 0; j < g.k; ++j)
-        if (s_expert[t * g.k + j] == e) s_who[a * g.T + n++] = (uint16_t)(32 * t + j);
-    s_many[a] = (uint8_t)n;
+  const int active = __shfl_sync(0xffffffffu, *s_count, 0);
+  for (int i = threadIdx.x; i < choices; i += THREADS) {
+    const uint32_t chose = s_chose[s_place[i]];  // and the place of the expert's first choice
+    const int place = (int)(chose >> 16) + __popc(chose & 0xffffu & ((1u << (i / g.k)) - 1u));
+    s_place[i] = place;
+    s_factor[place] = s_weight[i];
   }
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
 
-  const int cta = blockIdx.x, ctas = gridDim.x;
-  // This CTA's share of the hidden values (counted over the chosen experts) and of the outputs.
-  const int64_t total = (int64_t)active * g.D, p0 = total * cta / ctas, p1 = total * (cta + 1) / ctas;
-  const int n0 = (int)((int64_t)g.H * cta / ctas), n1 = (int)((int64_t)g.H * (cta + 1) / ctas);
-  const Shape up((int64_t)g.H * ES, g.fast), down((int64_t)g.D * ES, g.fast);
-  constexpr int PAIRS = 8 * MT, ROWS = 16 * MT;  // hidden values, outputs of a pass
+  // The ring's slots, by the longest pass that there can be.
+  using Up = Product<true, PARTS>;
+  using Down = Product<false, PARTS>;
+  auto longest = [&](auto product, int per) {
+    using P = decltype(product);
+    const int each = gridDim.x / active;  // CTAs of an expert (Passes)
+    const int64_t rows = each ? (per + each - 1) / each : ((int64_t)active * per + gridDim.x - 1) / gridDim.x;
+    const int share = (int)min((int64_t)P::MOST, rows);
+    return P::MATRICES * ((share + 7) / 8 * 8) * 128 + P::COLUMN_BYTES;
+  };
+  const int unit_bytes = max(longest(Up(), g.D), longest(Down(), g.H));
+  const int slot_bytes = unit_bytes * max(1, min(MAX_UNITS, SLOT / unit_bytes));
+  const int slots = min(MAX_SLOTS, RING / slot_bytes);
+  const int up_blocks = (g.H + EPB - 1) / EPB, down_blocks = (g.D + EPB - 1) / EPB;
+  const int box = g.T <= 8 ? 8 : 16;  // columns that are loaded
   auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
   bool ok = true;
-  int stage = 0;
+  int slot = 0;
   uint32_t phase = 0;
   auto advance = [&] {
-    if (++stage == STAGES) {
-      stage = 0;
+    if (++slot == slots) {
+      slot = 0;
       phase ^= 1u;
     }
   };
-
-  if (warp == WARPS) {
-    // ------------------------------------------------------------- copies
-    int left = 0;  // tiles that the stage has room for
-    // Chunk c of the rows src .. of a tile: `rows` of them, or (second) 8 places
-    // further on as many from `second`.
-    auto tile = [&](const Shape& s, const uint8_t* src, const uint8_t* second, int rows, int c) {
-      if (left == 0) {
-        ok = all_ok(mbar_wait(&empty[stage], phase ^ 1u, ctx, SITE_EMPTY));
-        if (!ok) return;
-        left = s.units;
-      }
-      uint8_t* dst = smem + stage * STAGE + (s.units - left) * s.unit;
-      const int len = s.length(c), copies = second ? 2 * rows : rows;
-      const int64_t at = (int64_t)c * s.chunk;
-      if (g.fast) {
-        if (lane == 0) mbar_expect_tx(&full[stage], copies * len);
-        __syncwarp();
-        if (s.together()) {
-          if (lane == 0) bulk_load(dst, src, rows * len, &full[stage]);
-          if (lane == 1 && second) bulk_load(dst + 8 * s.pitch, second, rows * len, &full[stage]);
-        } else if (second ? (lane & 7) < rows && lane < 16 : lane < rows) {
-          const uint8_t* from = second && lane >= 8 ? second + (lane - 8) * s.bytes : src + lane * s.bytes;
-          bulk_load(dst + lane * s.pitch, from + at, len, &full[stage]);
-        }
-      } else {
-        // Rows on any boundary, value by value, filled up with zeros to 16 bytes.
-        const int n = len / ES, padded = (n + PIECE - 1) / PIECE * PIECE;
-        for (int r = 0; r < copies; ++r) {
-          const bool is_second = r >= rows;
-          const uint8_t* from = (is_second ? second + (r - rows) * s.bytes : src + r * s.bytes) + at;
-          uint8_t* to = dst + (is_second ? 8 + r - rows : r) * s.pitch;
-          for (int i = lane; i < padded; i += 32) {
-            if constexpr (I8) to[i] = i < n ? from[i] : 0;
-            else reinterpret_cast<uint16_t*>(to)[i] = i < n ? reinterpret_cast<const uint16_t*>(from)[i] : 0;
-          }
-        }
-      }
-      __syncwarp();
-      if (--left == 0) {
-        if (lane == 0) mbar_arrive(&full[stage]);
-        __syncwarp();
-        advance();
-      }
-    };
-    auto finish = [&] {
-      if (left > 0) {
-        if (lane == 0) mbar_arrive(&full[stage]);
-        __syncwarp();
-        advance();
-        left = 0;
-      }
-    };
-    const uint8_t* w_in = static_cast<const uint8_t*>(g.w_in);
-    const uint8_t* w_out = static_cast<const uint8_t*>(g.w_out);
-    for (int64_t p = p0; p < p1 && ok;) {
-      const int a = (int)(p / g.D), i0 = (int)(p - (int64_t)a * g.D);
-      const int n = (int)min((int64_t)min(PAIRS, g.D - i0), p1 - p);
-      const uint8_t* gate = w_in + ((int64_t)s_active[a] * 2 * g.D + i0) * up.bytes;
-      for (int c = 0; c < up.chunks && ok; ++c)
-        for (int m = 0; m < n && ok; m += 8)
-          tile(up, gate + m * up.bytes, gate + ((int64_t)g.D + m) * up.bytes, min(8, n - m), c);
-      p += n;
-    }
-    if (ok) finish();
-    for (int r0 = n0; r0 < n1 && ok; r0 += ROWS) {
-      const int n = min(ROWS, n1 - r0);
-      for (int a = 0; a < active && ok; ++a) {
-        const uint8_t* w = w_out + ((int64_t)s_active[a] * g.H + r0) * down.bytes;
-        for (int c = 0; c < down.chunks && ok; ++c)
-          for (int m = 0; m < n && ok; m += 16) tile(down, w + m * down.bytes, nullptr, min(16, n - m), c);
-      }
-    }
-    if (ok) finish();
-  } else {
-    // ----------------------------------------------------------- products
-    // The columns of an MMA are the tokens that chose the expert. More than 8
-    // are rare; they take a second MMA, whose operands are not loaded ahead.
-    const int gq = lane >> 2, cq = lane & 3;
-    using One = std::integral_constant<int, 1>;
-    using All = std::integral_constant<int, PARTS>;
-    int left = 0;
-    const uint8_t* at = nullptr;
-    Acc acc[MT][NT][4];
-    uint32_t b[STEPS][NT][PARTS][4];
-    auto clear = [&] {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][n][i] = 0;
-    };
-    auto release = [&] {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[stage]);
-      advance();
-      left = 0;
-    };
-    // The next tile, with the first `parts` operands of every value, in two
-    // chains of MMAs.
-    auto multiply = [&](const Shape& s, int len, bool wide, auto parts, Acc (&d)[NT][4]) {
-      if (left == 0) {
-        if (ok) ok = all_ok(mbar_wait(&full[stage], phase, ctx, SITE_FULL));
-        left = s.units;
-        at = smem + stage * STAGE;
-      } else {
-        at += s.unit;
-      }
-      constexpr bool TWO = decltype(parts)::value == 2;
-      const uint8_t* row = at + gq * s.pitch + cq * 16;
-      Acc f[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[n][i] = 0;
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int off = (warp + i * WARPS) * 64;
-        if (off >= len) break;
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-        if (off + cq * 16 < len) {  // past the end of the row there may be anything
-          lo = *reinterpret_cast<const uint4*>(row + off);
-          hi = *reinterpret_cast<const uint4*>(row + 8 * s.pitch + off);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (n > 0 && !wide) break;
-          M::mma(d[n], lo.x, hi.x, lo.y, hi.y, b[i][n][0][0], b[i][n][0][1]);
-          if constexpr (TWO) M::mma(f[n], lo.x, hi.x, lo.y, hi.y, b[i][n][PARTS - 1][0], b[i][n][PARTS - 1][1]);
-          M::mma(TWO ? d[n] : f[n], lo.z, hi.z, lo.w, hi.w, b[i][n][0][2], b[i][n][0][3]);
-          if constexpr (TWO) M::mma(f[n], lo.z, hi.z, lo.w, hi.w, b[i][n][PARTS - 1][2], b[i][n][PARTS - 1][3]);
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[n][i] += f[n][i];
-      if (--left == 0) release();
-    };
-    auto meet = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
-    // The sum over the warps of row r of column t.
-    auto total_of = [&](int t, int r) {
-      const uint32_t* from = red + t * RED + r;
-      Acc sum = 0;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const uint32_t v = from[w * NT * 8 * RED];
-        if constexpr (I8) sum += (int)v;
-        else sum += __uint_as_float(v);
-      }
-      return sum;
-    };
-
-    // Hidden values: a = silu(gate) * up. The tokens' values of this warp's steps
-    // are loaded a chunk ahead.
-    uint4 next[STEPS];
-    auto fetch = [&](int a, int c, int n, uint4 (&to)[STEPS]) {
-      const int len = up.length(c), col = n * 8 + gq;
-      const bool is = col < s_many[a];
-      const int t = is ? s_who[a * g.T + col] >> 5 : 0;
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int off = (warp + i * WARPS) * 64 + cq * 16;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (is && off < len) {
-          const int64_t k0 = ((int64_t)c * up.chunk + off) / ES;
-          if constexpr (I8) {
-            v = *reinterpret_cast<const uint4*>(g.x_codes + (int64_t)t * g.x_pitch + k0);
-          } else {
-            const uint16_t* x = static_cast<const uint16_t*>(g.x) + t * g.ldx + k0;
-            if (g.vec_x && k0 + 8 <= g.H) {
-              v = *reinterpret_cast<const uint4*>(x);
-            } else {
-              uint32_t h[8];
-#pragma unroll
-              for (int u = 0; u < 8; ++u) h[u] = k0 + u < g.H ? x[u] : 0;
-              v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-            }
-          }
-        }
-        to[i] = v;
-      }
-    };
-    auto operands = [&](int n, const uint4 (&from)[STEPS]) {
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const uint4 v = from[i];
-        b[i][n][0][0] = v.x, b[i][n][0][1] = v.y, b[i][n][0][2] = v.z, b[i][n][0][3] = v.w;
-      }
-    };
-    if (p0 < p1) fetch((int)(p0 / g.D), 0, 0, next);
-    for (int64_t p = p0; p < p1;) {
-      const int a = (int)(p / g.D), i0 = (int)(p - (int64_t)a * g.D);
-      const int n = (int)min((int64_t)min(PAIRS, g.D - i0), p1 - p);
-      const bool wide = NT > 1 && s_many[a] > 8;
-      clear();
-      for (int c = 0; c < up.chunks; ++c) {
-        operands(0, next);
-        if (wide) {
-          fetch(a, c, NT - 1, next);
-          operands(NT - 1, next);
-        }
-        if (c + 1 < up.chunks) fetch(a, c + 1, 0, next);
-        else if (p + n < p1) fetch(i0 + n < g.D ? a : a + 1, 0, 0, next);
-        const int len = up.length(c);
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-          if (m * 8 < n) multiply(up, len, wide, One(), acc[m]);
-      }
-      // This warp's partial sums: column, then row.
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (nt > 0 && !wide) break;
-          uint32_t* to = red + ((warp * NT + nt) * 8 + 2 * cq) * RED + m * 16 + gq;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const Acc v = acc[m][nt][i];
-            to[(i & 1) * RED + (i >> 1) * 8] = *reinterpret_cast<const uint32_t*>(&v);
-          }
-        }
-      meet();
-      // A warp a column, a lane a value.
-      for (int col = warp; col < s_many[a]; col += WARPS) {
-        const int who = s_who[a * g.T + col], t = who >> 5, choice = t * g.k + (who & 31);
-        const int row = lane / 8 * 16 + lane % 8, i = i0 + lane;
-        float gate = (float)total_of(col, row), value = (float)total_of(col, row + 8);
-        if constexpr (I8) {
-          const float s = g.x_scale[t];
-          const float* scale = g.in_scale + (int64_t)s_active[a] * 2 * g.D + i;
-          gate *= s * (lane < n ? scale[0] : 0.f);
-          value *= s * (lane < n ? scale[g.D] : 0.f);
-        }
-        const float h = gate / (1.f + expf(-gate)) * value;
-        if constexpr (SPLIT) {
-          if (lane < n && ok) {
-            TX* to = static_cast<TX*>(g.hidden) + (int64_t)choice * 2 * g.d_pitch + i;
-            const TX hi = from_float<TX>(h);
-            to[0] = hi;
-            to[g.d_pitch] = from_float<TX>(isinf(to_float(hi)) ? 0.f : h - to_float(hi));  // what the rounding left
-          }
-        } else {
-          if (lane < n && ok) static_cast<float*>(g.hidden)[(int64_t)choice * g.d_pitch + i] = h;
-          const uint32_t top = __reduce_max_sync(0xffffffffu, lane < n ? abs_bits(h) : 0u);
-          if (lane == 0) atomicMax(g.top + choice, top);
-        }
-      }
-      meet();
-      p += n;
-    }
-    if (left > 0) release();
-
-    // The grid barrier.
-    __threadfence();
-    meet();
-    if (threadIdx.x == 0) {
-      asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(g.arrived) : "memory");
-      const uint64_t t0 = globaltimer();
-      for (uint32_t it = 1;; ++it) {
-        uint32_t n;
-        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(g.arrived) : "memory");
-        if (n >= (uint32_t)ctas) break;
-        if ((it & 63u) == 0u) {
-          if (!aborted(ctx.status) && globaltimer() - t0 <= ctx.timeout_ns) continue;
+  // A wait for all CTAs, by one thread; what they wrote before they arrived is
+  // visible after it.
+  auto wait_for_all = [&](const uint32_t* count) {
+    const uint64_t t0 = globaltimer();
+    for (uint32_t it = 1;; ++it) {
+      uint32_t n;
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(count) : "memory");
+      if (n >= gridDim.x) return true;
+      if ((it & 63u) == 0u) {
+        if (aborted(ctx.status)) return false;
+        if (globaltimer() - t0 > ctx.timeout_ns) {
           record_error(ctx.status, DEV_TIMEOUT, SITE_GRID);
-          s_count[1] = 1;
-          break;
+          return false;
         }
       }
-      __threadfence();
     }
-    meet();
-    if (s_count[1]) ok = false;
-    // What a choice's values are multiplied by before they are rounded, and its
-    // products after: the inverse, and the choice's weight.
-    for (int i = threadIdx.x; i < choices; i += 32 * WARPS) {
-      float inverse = 1.f;
-      if constexpr (I8) {
-        const RowScale code = row_scale(__ldcg(g.top + i));
-        s_scale[i] = code.inv;
-        inverse = code.scale;
-      } else if constexpr (!SPLIT) {
-        s_scale[i] = power_for(__ldcg(g.top + i), inverse);
-      }
-      s_factor[i] = s_weight[i] * inverse;
+  };
+  // 128 bytes of rows on any boundary, value by value, as TMA would place them:
+  // `rows` rows of `cols` values at a pitch (in values), from value k0 on; zeros
+  // past the ends. By a whole warp.
+  auto copy_rows = [&](uint8_t* dst, const void* src, int64_t pitch, int rows, int r8, int k0, int cols) {
+    for (int i = lane; i < r8 * EPB; i += 32) {
+      const int r = i / EPB, c = i % EPB, b = c * ES;
+      const bool is = r < rows && k0 + c < cols;
+      uint8_t* to = dst + r * 128 + ((b >> 4 ^ (r & 7)) << 4) + (b & 15);
+      if constexpr (I8) *to = is ? static_cast<const uint8_t*>(src)[r * pitch + k0 + c] : 0;
+      else *reinterpret_cast<uint16_t*>(to) = is ? static_cast<const uint16_t*>(src)[r * pitch + k0 + c] : 0;
     }
-    meet();
+  };
 
-    // Outputs. The hidden values are loaded a chunk ahead, too.
-    uint4 raw[STEPS][RAW];
-    auto load = [&](int a, int c, int n) {
-      const int len = down.length(c), col = n * 8 + gq;
-      const bool is = col < s_many[a];
-      const int who = is ? s_who[a * g.T + col] : 0, choice = (who >> 5) * g.k + (who & 31);
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int off = (warp + i * WARPS) * 64 + cq * 16;
-        const int64_t k0 = ((int64_t)c * down.chunk + off) / ES;
-        const uint4* from;
-        if constexpr (SPLIT) from = reinterpret_cast<const uint4*>(static_cast<const TX*>(g.hidden) + (int64_t)choice * 2 * g.d_pitch + k0);
-        else from = reinterpret_cast<const uint4*>(static_cast<const float*>(g.hidden) + (int64_t)choice * g.d_pitch + k0);
-        const int64_t step = SPLIT ? g.d_pitch / 8 : 1;
-#pragma unroll
-        for (int u = 0; u < RAW; ++u)
-          raw[i][u] = is && off < len ? __ldcg(from + u * step) : make_uint4(0, 0, 0, 0);
+  if (warp == 0 || warp == 3) {
+    // -------------------------------------------------- copies of weights
+    // Of the first product one warp copies the gate rows, the other the up rows;
+    // of the second every other K-block. The loops run with all lanes, so that
+    // addresses stay in uniform registers.
+    const int which = warp == 0 ? 0 : 1;
+    auto copy = [&](auto product, const RowBoxes& tm, const void* w, int per, int cols, int blocks) {
+      using P = decltype(product);
+      Passes p(active, per, P::MOST);
+      while (ok && p.next()) {
+        const Layout l(product, p.rows, slot_bytes);
+        const int e = __shfl_sync(0xffffffffu, s_active[p.a], 0);
+        const int row = P::kUp ? which * per + p.first : p.first;
+        const int low = min(l.r8, 64), high = l.r8 - low;
+        for (int kb = 0; kb < blocks; kb += l.units) {
+          ok = all_ok(mbar_wait(&empty[slot], phase ^ 1u, ctx, SITE_EMPTY));
+          if (!ok) break;
+          const int n = min(l.units, blocks - kb);
+          const int q0 = P::kUp ? 0 : which, step = P::kUp ? 1 : 2;
+          const int mine = P::kUp ? n : (n - which + 1) / 2;
+          uint8_t* dst = smem + slot * slot_bytes + (P::kUp ? which * l.r8 * 128 : which * l.bytes);
+          if (g.tma_w) {
+            if (elect_one()) mbar_arrive_expect_tx(&full[slot], mine * l.r8 * 128);
+            __syncwarp();
+            for (int q = q0; q < n; q += step, dst += step * l.bytes) {
+              const int k0 = (kb + q) * EPB;
+              if (elect_one()) {
+                tma_load_3d(dst, &tm.box[low / 8 - 1], &full[slot], k0, row, e);
+                if (high) tma_load_3d(dst + 64 * 128, &tm.box[high / 8 - 1], &full[slot], k0, row + 64, e);
+              }
+              __syncwarp();
+            }
+          } else {
+            const int64_t from = ((int64_t)e * P::MATRICES * per + row) * cols * ES;
+            for (int q = q0; q < n; q += step, dst += step * l.bytes)
+              copy_rows(dst, static_cast<const uint8_t*>(w) + from, cols, p.rows, l.r8, (kb + q) * EPB, cols);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[slot]);
+            __syncwarp();
+          }
+          advance();
+        }
       }
     };
-    auto convert = [&](int a, int n) {
-      if constexpr (SPLIT) {
+    copy(Up(), tmIn, g.w_in, g.D, g.H, up_blocks);
+    copy(Down(), tmOut, g.w_out, g.H, g.D, down_blocks);
+  } else if (warp == 2) {
+    // -------------------------------------------------- copies of columns
+    auto copy = [&](auto product, int per, int blocks) {
+      using P = decltype(product);
+      Passes p(active, per, P::MOST);
+      while (ok && p.next()) {
+        const Layout l(product, p.rows, slot_bytes);
+        const int base = __shfl_sync(0xffffffffu, (int)s_base[p.a], 0);
+        for (int kb = 0; kb < blocks; kb += l.units) {
+          ok = all_ok(mbar_wait(&empty[slot], phase ^ 1u, ctx, SITE_EMPTY));
+          if (!ok) break;
+          const int n = min(l.units, blocks - kb);
+          uint8_t* dst = smem + slot * slot_bytes + P::MATRICES * l.r8 * 128;
+          if (P::kUp && !g.tma_x) {
+            for (int q = 0; q < n; ++q, dst += l.bytes)
+              copy_rows(dst, g.x, g.ldx, g.T, box, (kb + q) * EPB, g.H);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[slot]);
+            __syncwarp();
+          } else {
+            if (elect_one()) mbar_arrive_expect_tx(&full[slot], n * P::OPERANDS * box * 128);
+            __syncwarp();
+            for (int q = 0; q < n; ++q, dst += l.bytes) {
+              const int k0 = (kb + q) * EPB;
+              if (elect_one()) {
+                if constexpr (P::kUp) {
+                  tma_load_2d(dst, &tmX, &full[slot], k0, 0);
+                } else {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i)
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            const uint4 v = raw[i][p];
-            uint32_t* to = b[i][n][p % PARTS];
-            to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
-          }
-      } else {
-        const int col = n * 8 + gq;
-        const bool is = col < s_many[a];
-        const int who = is ? s_who[a * g.T + col] : 0;
-        const float scale = is ? s_scale[(who >> 5) * g.k + (who & 31)] : 0.f;
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-          float v[RAW * 4];
-#pragma unroll
-          for (int u = 0; u < RAW; ++u) {
-            v[4 * u] = __uint_as_float(raw[i][u].x), v[4 * u + 1] = __uint_as_float(raw[i][u].y);
-            v[4 * u + 2] = __uint_as_float(raw[i][u].z), v[4 * u + 3] = __uint_as_float(raw[i][u].w);
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if constexpr (I8) {
-              uint32_t code[4];
-#pragma unroll
-              for (int u = 0; u < 4; ++u) code[u] = code_bits(v[4 * q + u], scale);
-              b[i][n][0][q] = scale == 0.f ? 0u : pack4(code[0], code[1], code[2], code[3]);
-            } else {
-              const float x0 = v[2 * q] * scale, x1 = v[2 * q + 1] * scale;
-              const __half2 hi = __floats2half2_rn(x0, x1);
-              const float2 h = __half22float2(hi);
-              // What the rounding left; of an infinity nothing.
-              const __half2 lo = __floats2half2_rn(isinf(x0) ? 0.f : x0 - h.x, isinf(x1) ? 0.f : x1 - h.y);
-              b[i][n][0][q] = *reinterpret_cast<const uint32_t*>(&hi);
-              b[i][n][PARTS - 1][q] = *reinterpret_cast<const uint32_t*>(&lo);
+                  for (int part = 0; part < PARTS; ++part)
+                    tma_load_3d(dst + part * COLUMNS, &tmH, &full[slot], k0, base, part);
+                }
+              }
+              __syncwarp();
             }
           }
+          advance();
         }
       }
     };
-    if (n0 < n1) load(0, 0, 0);
-    float* sums = reinterpret_cast<float*>(red) + warp * NT * 8 * RED;  // this warp's: token, then row
-    for (int r0 = n0; r0 < n1; r0 += ROWS) {
-      const int n = min(ROWS, n1 - r0);
-      for (int i = lane; i < NT * 8 * RED; i += 32) sums[i] = 0.f;
+    copy(Up(), g.D, up_blocks);
+    if (ok) {
+      // The hidden values of all CTAs, which wrote them as other memory than TMA's.
+      bool here = true;
+      if (lane == 0) here = wait_for_all(g.arrived + (SPLIT ? 0 : 1));
+      ok = all_ok(here);
+      fence_proxy_async_global();
       __syncwarp();
-      for (int a = 0; a < active; ++a) {
-        const bool wide = NT > 1 && s_many[a] > 8;
-        clear();
-        for (int c = 0; c < down.chunks; ++c) {
-          convert(a, 0);
-          if (wide) {
-            load(a, c, NT - 1);
-            convert(a, NT - 1);
-          }
-          if (c + 1 < down.chunks) load(a, c + 1, 0);
-          else load(a + 1 < active ? a + 1 : 0, 0, 0);
-          const int len = down.length(c);
+    }
+    copy(Down(), g.H, down_blocks);
+  } else if (warp == 1) {
+    // --------------------------------------------------------- MMA issuer
+    const uint32_t ring = smem_u32(smem), d0 = __shfl_sync(0xffffffffu, tmem, 0);
+    uint32_t pass = 0;
+    auto multiply = [&](auto product, int per, int blocks) {
+      using P = decltype(product);
+      constexpr int N = P::OPERANDS * 16;
+      constexpr uint32_t IDESC = I8 ? umma_idesc_i8(128, N) : umma_idesc_f16(128, N, ElemTraits<TX>::kBf16);
+      Passes p(active, per, P::MOST);
+      while (ok && p.next()) {
+        const Layout l(product, p.rows, slot_bytes);
+        const uint32_t set = pass & 1u, d_tmem = d0 + set * 32;
+        ok = all_ok(mbar_wait(&acc_empty[set], (pass >> 1 & 1u) ^ 1u, ctx, SITE_TMEM_EMPTY));
+        tc_fence_after();
+        for (int kb = 0; ok && kb < blocks; kb += l.units) {
+          ok = all_ok(mbar_wait(&full[slot], phase, ctx, SITE_FULL));
+          if (!ok) break;
+          tc_fence_after();
+          const int n = min(l.units, blocks - kb);
+          const uint32_t base = ring + slot * slot_bytes;
+          for (int q = 0; q < n; ++q) {
+            const uint64_t a = umma_desc_sw128(base + q * l.bytes);
+            const uint64_t b = umma_desc_sw128(base + q * l.bytes + P::MATRICES * l.r8 * 128);
+            const uint32_t first = kb + q == 0 ? 0u : 1u;
+            if (elect_one()) {
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
-            if (m * 16 < n) multiply(down, len, wide, All(), acc[m]);
-        }
-        // Onto the tokens' sums.
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int col = nt * 8 + 2 * cq + u;
-            if (col >= s_many[a]) continue;
-            const int who = s_who[a * g.T + col], t = who >> 5;
-            const float factor = s_factor[t * g.k + (who & 31)];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              if (m * 16 >= n) break;
-#pragma unroll
-              for (int v = 0; v < 2; ++v) {
-                float f = factor;
-                if constexpr (I8) {
-                  const int r = r0 + m * 16 + v * 8 + gq;
-                  f *= r < n1 ? g.out_scale[(int64_t)s_active[a] * g.H + r] : 0.f;
-                }
-                sums[t * RED + m * 16 + v * 8 + gq] += f * (float)acc[m][nt][2 * v + u];
+              for (int k = 0; k < 4; ++k) {
+                if constexpr (I8) umma_i8<1>(d_tmem, a + k * 2, b + k * 2, IDESC, k == 0 ? first : 1u);
+                else umma_f16_cg1(d_tmem, a + k * 2, b + k * 2, IDESC, k == 0 ? first : 1u);
               }
             }
+            __syncwarp();
           }
-        __syncwarp();  // another lane may have the token's column of the next expert
+          if (elect_one()) {
+            umma_commit_cg1(&empty[slot]);
+            if (kb + l.units >= blocks) umma_commit_cg1(&acc_full[set]);
+          }
+          __syncwarp();
+          advance();
+        }
+        ++pass;
       }
+    };
+    multiply(Up(), g.D, up_blocks);
+    multiply(Down(), g.H, down_blocks);
+  } else if (warp >= EPI_WARP) {
+    // ----------------------------------------------------------- epilogue
+    const int et = threadIdx.x - 32 * EPI_WARP;  // the thread's row of a pass
+    const uint32_t quarter = tmem + ((uint32_t)(warp % 4 * 32) << 16);
+    auto meet = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    auto number = [](uint32_t v) {
+      if constexpr (I8) return (float)(int)v;
+      else return __uint_as_float(v);
+    };
+    // Arrival at a grid barrier, after all that the CTA's threads wrote.
+    auto arrive = [&](uint32_t* count) {
+      __threadfence();
+      fence_proxy_async_global();
       meet();
-      for (int t = warp; t < g.T; t += WARPS) {
-        for (int r = lane; r < n; r += 32) {
-          const float* from = reinterpret_cast<const float*>(red) + t * RED + r;
-          float sum = 0.f;
+      if (et == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(count) : "memory");
+    };
+    uint32_t pass = 0;
+    // The accumulators of the next pass.
+    uint32_t v[32];
+    auto take = [&] {
+      const uint32_t set = pass & 1u;
+      if (ok) ok = all_ok(mbar_wait(&acc_full[set], pass >> 1 & 1u, ctx, SITE_TMEM_FULL));
+      tc_fence_after();
+      tmem_ld_32x32b_x32(quarter + set * 32, v);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[set]);
+      ++pass;
+    };
+
+    // Hidden values: silu(gate) * up.
+    {
+      Passes p(active, g.D, Up::MOST);
+      while (p.next()) {
+        const int i = p.first + et, r8 = (p.rows + 7) / 8 * 8;
+        const bool mine = et < p.rows;
+        float gate_scale = 1.f, up_scale = 1.f;
+        if constexpr (I8) {
+          const float* scale = g.in_scale + (int64_t)s_active[p.a] * 2 * g.D + i;
+          gate_scale = mine ? scale[0] : 0.f;
+          up_scale = mine ? scale[g.D] : 0.f;
+        }
+        const uint32_t who = s_who[p.a];
+        int place = s_base[p.a];
+        take();
+        // The up rows are the threads from r8 on. Through shared memory, and then
+        // token by token in a loop: unrolled, one token's values took 4 us, for
+        // the instructions that are fetched on the way.
+        meet();  // what was there has been read
 #pragma unroll
-          for (int w = 0; w < WARPS; ++w) sum += from[w * NT * 8 * RED];
-          if (ok) static_cast<TX*>(g.y)[t * g.ldy + r0 + r] = from_float<TX>(sum);
+        for (int t = 0; t < MAX_TOKENS; ++t)
+          if (who >> t & 1u) s_rows[et * (MAX_TOKENS + 1) + t] = v[t];
+        meet();
+        if (warp - EPI_WARP > (p.rows - 1) / 32) continue;
+#pragma unroll 1
+        for (uint32_t rest = who; rest; rest &= rest - 1) {
+          const int t = __ffs(rest) - 1;
+          float gate = mine ? number(s_rows[et * (MAX_TOKENS + 1) + t]) : 0.f;
+          float value = mine ? number(s_rows[(et + r8) * (MAX_TOKENS + 1) + t]) : 0.f;
+          if constexpr (I8) {
+            const float s = g.x_scale[t];
+            gate *= s * gate_scale;
+            value *= s * up_scale;
+          }
+          const float h = gate / (1.f + expf(-gate)) * value;
+          if constexpr (SPLIT) {
+            if (mine && ok) {
+              TX* to = reinterpret_cast<TX*>(g.operand + (int64_t)place * g.d_bytes) + i;
+              const TX hi = from_float<TX>(h);
+              // What the rounding left; of an infinity nothing.
+              const TX lo = from_float<TX>(isinf(to_float(hi)) ? 0.f : h - to_float(hi));
+              *to = hi;
+              *reinterpret_cast<TX*>(reinterpret_cast<uint8_t*>(to) + (int64_t)choices * g.d_bytes) = lo;
+            }
+          } else {
+            if (mine && ok) g.hidden[(int64_t)place * g.D + i] = h;
+            const uint32_t top = __reduce_max_sync(0xffffffffu, mine ? abs_bits(h) : 0u);
+            if (lane == 0) atomicMax(g.top + place, top);
+          }
+          ++place;
         }
       }
-      meet();
     }
-    if (left > 0) release();
+    arrive(g.arrived);
+    if constexpr (!SPLIT) {
+      // The largest values are known: this CTA's share in the operands' form.
+      bool here = true;
+      if (et == 0) here = wait_for_all(g.arrived);
+      if (!here) ok = false;
+      __threadfence();
+      meet();
+      for (int i = et; i < choices; i += 128) {
+        float inverse;
+        const uint32_t top = __ldcg(g.top + i);
+        if constexpr (I8) {
+          const RowScale code = row_scale(top);
+          s_scale[i] = code.inv;
+          inverse = code.scale;
+        } else {
+          s_scale[i] = power_for(top, inverse);
+        }
+        s_factor[i] *= inverse;
+      }
+      meet();
+      Passes p(active, g.D, Up::MOST);
+      while (p.next()) {
+        const int n = __popc((uint32_t)s_who[p.a]), i = p.first + et;
+        if (et >= p.rows) continue;
+        for (int place = s_base[p.a]; place < s_base[p.a] + n; ++place) {
+          const float h = __ldcg(g.hidden + (int64_t)place * g.D + i), scale = s_scale[place];
+          uint8_t* to = g.operand + (int64_t)place * g.d_bytes;
+          if constexpr (I8) {
+            to[i] = scale == 0.f ? 0 : (uint8_t)(code_bits(h, scale) & 0xffu);
+          } else {
+            const float x = h * scale;
+            const TX hi = from_float<TX>(x);
+            reinterpret_cast<TX*>(to)[i] = hi;
+            reinterpret_cast<TX*>(to + (int64_t)choices * g.d_bytes)[i] = from_float<TX>(isinf(x) ? 0.f : x - to_float(hi));
+          }
+        }
+      }
+      arrive(g.arrived + 1);
+    }
+
+    // Outputs of the choices, and sums of the blocks that they complete.
+    Passes p(active, g.H, Down::MOST);
+    while (p.next()) {
+      const int r = p.first + et, n = __popc((uint32_t)s_who[p.a]), base = s_base[p.a];
+      const bool mine = et < p.rows;
+      float scale = 1.f;
+      if constexpr (I8) scale = mine ? g.out_scale[(int64_t)s_active[p.a] * g.H + r] : 0.f;
+      take();
+#pragma unroll
+      for (int c = 0; c < MAX_TOKENS; ++c) {
+        if (c >= n) break;
+        float o = number(v[c]);
+        if constexpr (PARTS == 2) o += number(v[16 + c]);
+        if (mine) g.out[(int64_t)(base + c) * g.out_pitch + r] = s_factor[base + c] * scale * o;
+      }
+      __threadfence();
+      meet();
+      // The pass's rows lie in at most 5 blocks.
+      const int b0 = p.first / BLOCK, b1 = (p.first + p.rows - 1) / BLOCK;
+      if (et == 0) *s_last = 0;
+      meet();
+      if (et <= b1 - b0) {
+        const int b = b0 + et, begin = b * BLOCK, end = min(begin + BLOCK, g.H);
+        const uint32_t rows = min(end, p.first + p.rows) - max(begin, p.first);
+        const uint32_t all = (uint32_t)active * (uint32_t)(end - begin);
+        if (atomicAdd(g.done + b, rows) + rows == all) atomicOr(s_last, 1 << et);
+      }
+      __threadfence();
+      meet();
+      // Eight threads a block and token, four outputs each.
+      const int last = *s_last, blocks = __popc((uint32_t)last);
+      for (int i = et / 8; i < blocks * g.T; i += 16) {
+        const int t = i % g.T;
+        uint32_t rest = (uint32_t)last;
+        for (int skip = i / g.T; skip; --skip) rest &= rest - 1;
+        const int o = (b0 + __ffs(rest) - 1) * BLOCK + et % 8 * 4;
+        if (o >= g.H) continue;
+        const int* place = s_place + t * g.k;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int j0 = 0; j0 < g.k; j0 += 8) {
+          float4 u[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j0 + j < g.k) u[j] = __ldcg(reinterpret_cast<const float4*>(g.out + (int64_t)place[j0 + j] * g.out_pitch + o));
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j0 + j < g.k) sum.x += u[j].x, sum.y += u[j].y, sum.z += u[j].z, sum.w += u[j].w;
+        }
+        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (ok && o + u < g.H) static_cast<TX*>(g.y)[t * g.ldy + o + u] = from_float<TX>(f[u]);
+      }
+    }
   }
   // A wait ran out: what is in flight has to land before the CTA leaves.
+  __syncwarp();
+  tc_fence_before();
   if (__syncthreads_or(!ok)) settle();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem, TMEM_COLS);
+  }
 }
 
 // ---------------------------------------------------------------- host side
@@ -827,9 +827,30 @@ struct Sizes {
 
 int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
 
-// logits, hidden values, their largest, the tokens' scales, the barrier's count; the tokens' codes.
-int64_t words(const Sizes& s) { return up16(s.T * s.E * 4) + s.T * s.k * up16(s.D) * 4 + up16(s.T * s.k * 4) + 64 + 16; }
-int64_t bytes(const Sizes& s) { return words(s) + s.T * up16(s.H); }
+// Of T tokens: logits, hidden values, operands, their largest, outputs, blocks' counts, scales, barriers, codes.
+struct Workspace {
+  int64_t logits, hidden, operand, top, out, done, x_scale, arrived, x_codes, end;
+  explicit Workspace(const Sizes& s) {
+    int64_t at = 0;
+    auto take = [&](int64_t n) {
+      const int64_t here = at;
+      at += up16(n);
+      return here;
+    };
+    const int64_t n = s.T * s.k;
+    logits = take(s.T * s.E * 4);
+    hidden = take(n * s.D * 4);
+    operand = take(2 * n * up16(2 * s.D));
+    top = take(n * 4);
+    out = take(n * up16(s.H) * 4);
+    done = take((s.H + BLOCK - 1) / BLOCK * 4);
+    x_scale = take(64);
+    arrived = take(8);
+    x_codes = take(s.T * up16(s.H));
+    end = at;
+  }
+};
+int64_t bytes(const Sizes& s) { return Workspace(s).end; }
 
 int check(const char* what, int dtype, const void* x, int64_t ldx, const void* router, const void* w_in,
           const void* w_out, const void* y, int64_t ldy, const Sizes& s, void* ws, int64_t ws_bytes) {
@@ -851,33 +872,64 @@ int check(const char* what, int dtype, const void* x, int64_t ldx, const void* r
   return KEBAB_OK;
 }
 
-template <typename TX, bool I8, int NT>
-int launch(LayerArgs& g, cudaStream_t stream) {
+// Boxes of a stack of matrices' rows.
+int row_boxes(RowBoxes* m, const void* base, int type, int es, int64_t n, int64_t rows, int64_t cols) {
+  const uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, (uint64_t)n};
+  const uint64_t strides[2] = {(uint64_t)(cols * es), (uint64_t)(rows * cols * es)};
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t box[3] = {(uint32_t)(128 / es), 8u * (i + 1), 1};
+    const int rc = make_tmap(&m->box[i], base, type, 3, dims, strides, box, 128);
+    if (rc) return rc;
+  }
+  return KEBAB_OK;
+}
+
+template <typename TX, bool I8>
+int launch(int dtype, LayerArgs& g, cudaStream_t stream) {
+  constexpr int ES = I8 ? 1 : 2;
   int rc;
   DeviceInfo* dev = nullptr;
   if ((rc = device_info(&dev)) || (rc = wait_ctx(&g.ctx))) return rc;
   g.pdl = pdl_enabled();
-  auto kern = layer_kernel<TX, I8, NT>;
+  const int type = I8 ? TMAP_U8 : dtype;
+  RowBoxes in = {}, out = {};
+  CUtensorMap tx = {}, th = {};
+  if (g.tma_w && ((rc = row_boxes(&in, g.w_in, type, ES, g.E, 2 * (int64_t)g.D, g.H)) ||
+                  (rc = row_boxes(&out, g.w_out, type, ES, g.E, g.H, g.D))))
+    return rc;
+  const uint32_t columns = g.T <= 8 ? 8 : 16;
+  if (g.tma_x) {
+    const uint64_t dims[2] = {(uint64_t)(I8 ? g.x_pitch : g.H), (uint64_t)g.T};
+    const uint64_t strides[1] = {(uint64_t)(I8 ? g.x_pitch : g.ldx * 2)};
+    const uint32_t box[2] = {128 / ES, columns};
+    if ((rc = make_tmap(&tx, I8 ? (const void*)g.x_codes : g.x, type, 2, dims, strides, box, 128))) return rc;
+  }
+  {
+    const uint64_t n = (uint64_t)g.T * g.k;
+    const uint64_t dims[3] = {(uint64_t)g.D, n, I8 ? 1u : 2u}, strides[2] = {(uint64_t)g.d_bytes, n * g.d_bytes};
+    const uint32_t box[3] = {128 / ES, columns, 1};
+    if ((rc = make_tmap(&th, g.operand, type, 3, dims, strides, box, 128))) return rc;
+  }
+  auto kern = layer_kernel<TX, I8>;
   static std::once_flag once[64];
   static cudaError_t err[64];
   const int di = dev->device & 63;
   std::call_once(once[di], [&] {
     err[di] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   LayerSmem<NT>::MOST);
+                                   LayerSmem::bytes(MAX_TOKENS, MAX_K, kMaxExperts));
   });
   if (err[di] != cudaSuccess) return cuda_fail(err[di], "cudaFuncSetAttribute(max dynamic smem)");
   PdlLaunch first(dim3((unsigned)(g.E + (I8 ? g.T : 0))), dim3(256), 0, stream);
-  cudaError_t e = cudaLaunchKernelEx(&first.cfg, layer_logits_kernel<TX>, (const LayerArgs)g, (int)is_split<TX, I8>());
+  cudaError_t e = cudaLaunchKernelEx(&first.cfg, layer_logits_kernel<TX>, (const LayerArgs)g);
   if (e != cudaSuccess) return cuda_fail(e, "expert_layer: logits launch");
-  const int smem = LayerSmem<NT>::bytes(g.T, g.k, g.E);
-  PdlLaunch l(dim3((unsigned)dev->sm_count), dim3(THREADS), smem, stream);
+  PdlLaunch l(dim3((unsigned)dev->sm_count), dim3(THREADS), LayerSmem::bytes(g.T, g.k, g.E), stream);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeCooperative;
   attr[0].val.cooperative = 1;
   if (l.cfg.numAttrs) attr[1] = l.attr[0];
   l.cfg.attrs = attr;
   ++l.cfg.numAttrs;
-  e = cudaLaunchKernelEx(&l.cfg, kern, (const LayerArgs)g);
+  e = cudaLaunchKernelEx(&l.cfg, kern, in, out, tx, th, (const LayerArgs)g);
   return e == cudaSuccess ? KEBAB_OK : cuda_fail(e, "expert_layer launch");
 }
 
@@ -885,26 +937,26 @@ template <bool I8>
 int run(int dtype, LayerArgs g, const Sizes& s, void* ws, kebab_stream_t stream) {
   constexpr int ES = I8 ? 1 : 2;
   g.T = (int)s.T, g.E = (int)s.E, g.k = (int)s.k, g.H = (int)s.H, g.D = (int)s.D;
+  const Workspace w(s);
   uint8_t* at = static_cast<uint8_t*>(ws);
-  auto take = [&](int64_t n) {
-    uint8_t* p = at;
-    at += up16(n);
-    return p;
-  };
-  g.logits = reinterpret_cast<float*>(take(s.T * s.E * 4));
-  g.d_pitch = (int)up16(s.D);
-  g.hidden = take(s.T * s.k * g.d_pitch * 4);
-  g.top = reinterpret_cast<uint32_t*>(take(s.T * s.k * 4));
-  g.x_scale = reinterpret_cast<float*>(take(64));
-  g.arrived = reinterpret_cast<uint32_t*>(take(16));
-  g.x_codes = reinterpret_cast<int8_t*>(at);
+  g.logits = reinterpret_cast<float*>(at + w.logits);
+  g.hidden = reinterpret_cast<float*>(at + w.hidden);
+  g.operand = at + w.operand;
+  g.d_bytes = (int)up16(s.D * ES);
+  g.top = reinterpret_cast<uint32_t*>(at + w.top);
+  g.out = reinterpret_cast<float*>(at + w.out);
+  g.out_pitch = (int)up16(s.H);
+  g.done = reinterpret_cast<uint32_t*>(at + w.done);
+  g.x_scale = reinterpret_cast<float*>(at + w.x_scale);
+  g.arrived = reinterpret_cast<uint32_t*>(at + w.arrived);
+  g.x_codes = reinterpret_cast<int8_t*>(at + w.x_codes);
   g.x_pitch = (int)up16(s.H);
   auto on16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
-  g.fast = on16(g.w_in) && on16(g.w_out) && s.H * ES % 16 == 0 && s.D * ES % 16 == 0;
+  g.tma_w = on16(g.w_in) && on16(g.w_out) && s.H * ES % 16 == 0 && s.D * ES % 16 == 0;
   g.vec_x = on16(g.x) && g.ldx % 8 == 0;
+  g.tma_x = I8 || g.vec_x;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == KEBAB_F16) return s.T <= 8 ? launch<__half, I8, 1>(g, st) : launch<__half, I8, 2>(g, st);
-  return s.T <= 8 ? launch<__nv_bfloat16, I8, 1>(g, st) : launch<__nv_bfloat16, I8, 2>(g, st);
+  return dtype == KEBAB_F16 ? launch<__half, I8>(dtype, g, st) : launch<__nv_bfloat16, I8>(dtype, g, st);
 }
 }  // namespace
 }  // namespace kb
