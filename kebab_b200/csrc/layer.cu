@@ -274,19 +274,19 @@ static_assert(LayerSmem::bytes(MAX_TOKENS, MAX_K, kMaxExperts) <= 232448, "share
 // Made by whole warps; the shuffles tell the compiler that a warp's lanes have
 // the same values.
 struct Passes {
-  int64_t at, end;
-  int per, most;
+  int at, end, per, most;
   int a, first, rows;  // the expert (by its place among the chosen), the first row, rows
   int left;            // rows of the segment after this pass
   __device__ __forceinline__ Passes(int active, int per_expert, int most) : per(per_expert), most(most), rows(0), left(0) {
     const int ctas = gridDim.x, cta = blockIdx.x, each = ctas / active;
     if (each * active * 8 >= ctas * 7) {
-      const int64_t before = (int64_t)(cta / each) * per, i = cta % each;
-      at = cta < each * active ? before + per * i / each : 0;
-      end = cta < each * active ? before + per * (i + 1) / each : 0;
+      const int before = cta / each * per, i = cta % each, share = per / each, more = per % each;
+      at = cta < each * active ? before + share * i + min(i, more) : 0;
+      end = cta < each * active ? at + share + (i < more) : 0;
     } else {
-      at = (int64_t)active * per * cta / ctas;
-      end = (int64_t)active * per * (cta + 1) / ctas;
+      const int total = active * per, share = total / ctas, more = total % ctas;
+      at = share * cta + min(cta, more);
+      end = at + share + (cta < more);
     }
   }
   __device__ __forceinline__ bool next() {
@@ -294,9 +294,9 @@ struct Passes {
       first += rows;
     } else {
       if (at >= end) return false;
-      a = (int)(at / per);
-      first = (int)(at - (int64_t)a * per);
-      left = (int)min((int64_t)(per - first), end - at);
+      a = at / per;
+      first = at - a * per;
+      left = min(per - first, end - at);
       at += left;
     }
     const int passes = (left + most - 1) / most;
@@ -436,8 +436,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   auto longest = [&](auto product, int per) {
     using P = decltype(product);
     const int each = gridDim.x / active;  // CTAs of an expert (Passes)
-    const int64_t rows = each ? (per + each - 1) / each : ((int64_t)active * per + gridDim.x - 1) / gridDim.x;
-    const int share = (int)min((int64_t)P::MOST, rows);
+    const int rows = each ? (per + each - 1) / each : (active * per + (int)gridDim.x - 1) / (int)gridDim.x;
+    const int share = min(P::MOST, rows);
     return P::MATRICES * ((share + 7) / 8 * 8) * 128 + P::COLUMN_BYTES;
   };
   const int unit_bytes = max(longest(Up(), g.D), longest(Down(), g.H));
@@ -534,6 +534,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     copy(Down(), tmOut, g.w_out, g.H, g.D, down_blocks);
   } else if (warp == 2) {
     // -------------------------------------------------- copies of columns
+    bool met = false;  // past the grid barrier
     auto copy = [&](auto product, int per, int blocks) {
       using P = decltype(product);
       Passes p(active, per, P::MOST);
@@ -542,6 +543,17 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int base = __shfl_sync(0xffffffffu, (int)s_base[p.a], 0);
         for (int kb = 0; kb < blocks; kb += l.units) {
           ok = all_ok(mbar_wait(&empty[slot], phase ^ 1u, ctx, SITE_EMPTY));
+          if (!P::kUp && ok && !met) {
+            // The hidden values of all CTAs, which wrote them as other memory than
+            // TMA's. (Waited for here, with all of the way to the first copy done:
+            // between the products it cost 2.8 us more, for instructions that are
+            // fetched from a memory that is busy with the weights.)
+            if (lane == 0) ok = wait_for_all(g.arrived + (SPLIT ? 0 : 1));
+            ok = all_ok(ok);
+            fence_proxy_async_global();
+            __syncwarp();
+            met = true;
+          }
           if (!ok) break;
           const int n = min(l.units, blocks - kb);
           uint8_t* dst = smem + slot * slot_bytes + P::MATRICES * l.r8 * 128;
@@ -574,14 +586,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     };
     copy(Up(), g.D, up_blocks);
-    if (ok) {
-      // The hidden values of all CTAs, which wrote them as other memory than TMA's.
-      bool here = true;
-      if (lane == 0) here = wait_for_all(g.arrived + (SPLIT ? 0 : 1));
-      ok = all_ok(here);
-      fence_proxy_async_global();
-      __syncwarp();
-    }
     copy(Down(), g.H, down_blocks);
   } else if (warp == 1) {
     // --------------------------------------------------------- MMA issuer
@@ -639,10 +643,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     // Arrival at a grid barrier, after all that the CTA's threads wrote.
     auto arrive = [&](uint32_t* count) {
-      __threadfence();
       fence_proxy_async_global();
       meet();
-      if (et == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(count) : "memory");
+      if (et == 0) asm volatile("fence.acq_rel.gpu;\n\tred.relaxed.gpu.global.add.u32 [%0], 1;" ::"l"(count) : "memory");
     };
     uint32_t pass = 0;
     // The accumulators of the next pass.
@@ -733,20 +736,32 @@ __global__ void __launch_bounds__(THREADS, 1)
         s_factor[i] *= inverse;
       }
       meet();
-      Passes p(active, g.D, Up::MOST);
+      Passes p(active, g.D, 1 << 30);  // the expert's part of the share at once
       while (p.next()) {
-        const int n = __popc((uint32_t)s_who[p.a]), i = p.first + et;
-        if (et >= p.rows) continue;
-        for (int place = s_base[p.a]; place < s_base[p.a] + n; ++place) {
-          const float h = __ldcg(g.hidden + (int64_t)place * g.D + i), scale = s_scale[place];
-          uint8_t* to = g.operand + (int64_t)place * g.d_bytes;
-          if constexpr (I8) {
-            to[i] = scale == 0.f ? 0 : (uint8_t)(code_bits(h, scale) & 0xffu);
-          } else {
-            const float x = h * scale;
-            const TX hi = from_float<TX>(x);
-            reinterpret_cast<TX*>(to)[i] = hi;
-            reinterpret_cast<TX*>(to + (int64_t)choices * g.d_bytes)[i] = from_float<TX>(isinf(x) ? 0.f : x - to_float(hi));
+        const int base = s_base[p.a], values = __popc((uint32_t)s_who[p.a]) * p.rows;
+        // Eight loads in flight a thread: one by one, they took 10 us of 13 tokens
+        // of 6 choices, 1272 values each.
+        for (int i0 = et; i0 < values; i0 += 8 * 128) {
+          float h[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int i = i0 + u * 128, c = i / p.rows;
+            if (i < values) h[u] = __ldcg(g.hidden + (int64_t)(base + c) * g.D + p.first + i - c * p.rows);
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int i = i0 + u * 128, c = i / p.rows, at = p.first + i - c * p.rows;
+            if (i >= values) break;
+            const float scale = s_scale[base + c];
+            uint8_t* to = g.operand + (int64_t)(base + c) * g.d_bytes;
+            if constexpr (I8) {
+              to[at] = scale == 0.f ? 0 : (uint8_t)(code_bits(h[u], scale) & 0xffu);
+            } else {
+              const float x = h[u] * scale;
+              const TX hi = from_float<TX>(x);
+              reinterpret_cast<TX*>(to)[at] = hi;
+              reinterpret_cast<TX*>(to + (int64_t)choices * g.d_bytes)[at] = from_float<TX>(isinf(x) ? 0.f : x - to_float(hi));
+            }
           }
         }
       }
@@ -821,6 +836,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 // ---------------------------------------------------------------- host side
 
+constexpr int64_t kMaxWidth = 1 << 20;  // of H and D: the rows of 512 choices are counted in 32 bits
+
 struct Sizes {
   int64_t T, E, k, H, D;
 };
@@ -862,7 +879,7 @@ int check(const char* what, int dtype, const void* x, int64_t ldx, const void* r
     return fail(KEBAB_EINVAL, w + ": number of experts " + std::to_string(s.E) + " is not in 1.." + std::to_string(kMaxExperts));
   if (s.k < 1 || s.k > MAX_K || s.k > s.E)
     return fail(KEBAB_EINVAL, w + ": k = " + std::to_string(s.k) + " is not in 1..min(E, 32)");
-  if (s.H <= 0 || s.D <= 0 || s.H > (1 << 24) || s.D > (1 << 24))
+  if (s.H <= 0 || s.D <= 0 || s.H > kMaxWidth || s.D > kMaxWidth)
     return fail(KEBAB_EINVAL, w + ": invalid dimensions H=" + std::to_string(s.H) + " D=" + std::to_string(s.D));
   if (ldx < s.H || ldy < s.H) return fail(KEBAB_EINVAL, w + ": a row pitch is below the row length");
   if (s.T == 0) return KEBAB_OK;
@@ -967,7 +984,7 @@ extern "C" {
 
 int64_t kebab_expert_layer_workspace(int64_t T, int64_t E, int k, int64_t H, int64_t D) {
   if (T < 0 || T > KEBAB_FEW_TOKENS || E < 1 || E > kMaxExperts || k < 1 || k > MAX_K || H <= 0 || D <= 0 ||
-      H > (1 << 24) || D > (1 << 24))
+      H > kMaxWidth || D > kMaxWidth)
     return -KEBAB_EINVAL;
   return bytes({T, E, k, H, D});
 }
