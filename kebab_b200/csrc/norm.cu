@@ -247,12 +247,15 @@ struct GradArgs {
   int cols;
 };
 
-template <typename T, int W, int HELD, int THREADS>
-__global__ void __launch_bounds__(THREADS) norm_backward_kernel(const GradArgs g) {
+// AHEAD: the next row of the first slab is loaded before the sums of this one
+// are exchanged (where the registers hold two).
+template <typename T, int W, int HELD, int THREADS, bool AHEAD>
+__global__ void __launch_bounds__(THREADS, AHEAD ? 512 / THREADS : 1) norm_backward_kernel(const GradArgs g) {
   constexpr int SLAB = THREADS * W * HELD;
   __shared__ float part[2][THREADS / 32][2];
   pdl_wait();
   pdl_launch_dependents();
+  const bool add = g.ds && g.dx;
   int turn = 0;
   for (int base = 0; base < g.cols; base += SLAB) {
     const int c0 = base + threadIdx.x * W;
@@ -261,22 +264,31 @@ __global__ void __launch_bounds__(THREADS) norm_backward_kernel(const GradArgs g
     for (int h = 0; h < HELD; ++h)
 #pragma unroll
       for (int i = 0; i < W; ++i) acc[h][i] = 0.f;
-    for (int64_t row = blockIdx.x; row < g.rows; row += gridDim.x) {
-      const T* s = static_cast<const T*>(g.s) + row * g.lds;
-      const T* dy = static_cast<const T*>(g.dy) + row * g.lddy;
-      const T* ds = static_cast<const T*>(g.ds) + row * g.ldds;
-      Run<T, W> rs[HELD], rd[HELD], re[HELD];
+    Run<T, W> rs[HELD], rd[HELD], re[HELD], ns[HELD], nd[HELD], ne[HELD];
+    auto load = [&](int64_t row, Run<T, W> (&ls)[HELD], Run<T, W> (&ld)[HELD], Run<T, W> (&le)[HELD]) {
+      const T* s = static_cast<const T*>(g.s) + row * g.lds + c0;
+      const T* dy = static_cast<const T*>(g.dy) + row * g.lddy + c0;
+      const T* ds = static_cast<const T*>(g.ds) + row * g.ldds + c0;
 #pragma unroll
       for (int h = 0; h < HELD; ++h) {
-        const int c = c0 + h * THREADS * W;
-        if (c < g.cols) {
-          rs[h].load(s + c);
-          rd[h].load(dy + c);
-          if (g.ds && g.dx) re[h].load(ds + c);
+        if (c0 + h * THREADS * W < g.cols) {
+          ls[h].load(s + h * THREADS * W);
+          ld[h].load(dy + h * THREADS * W);
+          if (add) le[h].load(ds + h * THREADS * W);
         }
       }
+    };
+    if (AHEAD) load(blockIdx.x, ns, nd, ne);
+    for (int64_t row = blockIdx.x; row < g.rows; row += gridDim.x) {
+      if (AHEAD) {
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) rs[h] = ns[h], rd[h] = nd[h], re[h] = ne[h];
+        if (row + gridDim.x < g.rows) load(row + gridDim.x, ns, nd, ne);
+      } else {
+        load(row, rs, rd, re);
+      }
       float a[W], b[W], w[W], sum[2] = {0.f, 0.f};
-      auto add = [&](int c) {
+      auto count = [&](int c) {
         load_weight<T, W>(g.w, g.w_f32, c, w);
 #pragma unroll
         for (int i = 0; i < W; ++i) {
@@ -291,12 +303,12 @@ __global__ void __launch_bounds__(THREADS) norm_backward_kernel(const GradArgs g
           if (c >= g.cols) break;
           rs[h].values(a);
           rd[h].values(b);
-          add(c);
+          count(c);
         }
         for (int c = c0 + SLAB; c < g.cols; c += THREADS * W) {
-          load_row<W>(s + c, a);
-          load_row<W>(dy + c, b);
-          add(c);
+          load_row<W>(static_cast<const T*>(g.s) + row * g.lds + c, a);
+          load_row<W>(static_cast<const T*>(g.dy) + row * g.lddy + c, b);
+          count(c);
         }
         row_sum<THREADS, 2>(sum, part[turn]);  // two buffers in turn: one barrier a row
         turn ^= 1;
@@ -323,7 +335,7 @@ __global__ void __launch_bounds__(THREADS) norm_backward_kernel(const GradArgs g
           load_weight<T, W>(g.w, g.w_f32, c, w);
 #pragma unroll
           for (int i = 0; i < W; ++i) a[i] = rstd * (b[i] * w[i] - a[i] * k);
-          if (g.ds) {
+          if (add) {
             re[h].values(b);
 #pragma unroll
             for (int i = 0; i < W; ++i) a[i] += b[i];
@@ -345,40 +357,43 @@ __global__ void __launch_bounds__(THREADS) norm_backward_kernel(const GradArgs g
   }
 }
 
-// dweight[c] = the sum of the blocks' partial sums in their order: 8 warps take
-// every eighth of them, 32 columns a block.
+// dweight[c] = the sum of the blocks' partial sums in a fixed order: 32 warps
+// take every 32nd of them, 32 columns a block.
 template <typename TW>
-__global__ void __launch_bounds__(256) norm_dweight_kernel(const float* partial, int blocks, int cols, TW* dweight) {
-  __shared__ float sums[8][32];
+__global__ void __launch_bounds__(1024) norm_dweight_kernel(const float* partial, int blocks, int cols, TW* dweight) {
+  __shared__ float sums[32][33];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float sum = 0.f;
   if (c < cols) {
 #pragma unroll 8
-    for (int b = warp; b < blocks; b += 8) sum += partial[(int64_t)b * cols + c];
+    for (int b = warp; b < blocks; b += 32) sum += partial[(int64_t)b * cols + c];
   }
   sums[warp][lane] = sum;
   __syncthreads();
-  if (warp == 0 && c < cols) {
+  sum = sums[lane][warp];  // column `warp`, the sum of warp `lane`
 #pragma unroll
-    for (int i = 1; i < 8; ++i) sum += sums[i][lane];
-    dweight[c] = from_float<TW>(sum);
-  }
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0 && blockIdx.x * 32 + warp < cols) dweight[blockIdx.x * 32 + warp] = from_float<TW>(sum);
 }
 
 constexpr int kMaxBlocks = 1024;  // of the backward kernel, as the workspace is sized
 
+// Threads of a block by the runs of a row, and the blocks that an SM holds.
 template <typename T, int W>
-int launch_backward(const GradArgs& g, int blocks, cudaStream_t stream) {
+int launch_backward(const GradArgs& g, int sms, int* blocks, cudaStream_t stream) {
   const int64_t runs = (g.cols + W - 1) / W;
-  auto kern = norm_backward_kernel<T, W, 4, 512>;
+  // (F32 rows: registers for half as many runs, and not for the next row's.)
+  constexpr bool F32 = sizeof(T) == 4;
+  auto kern = norm_backward_kernel<T, W, F32 ? 2 : 4, 512, false>;
   int threads = 512;
-  if (runs <= 128) kern = norm_backward_kernel<T, W, 1, 128>, threads = 128;
-  else if (runs <= 256) kern = norm_backward_kernel<T, W, 1, 256>, threads = 256;
-  else if (runs <= 512) kern = norm_backward_kernel<T, W, 2, 256>, threads = 256;
-  else if (runs <= 1024) kern = norm_backward_kernel<T, W, 2, 512>;
-  PdlLaunch l(dim3(blocks), dim3(threads), 0, stream);
+  if (runs <= 128) kern = norm_backward_kernel<T, W, 1, 128, true>, threads = 128;
+  else if (runs <= 256) kern = norm_backward_kernel<T, W, 1, 256, true>, threads = 256;
+  else if (runs <= 512) kern = norm_backward_kernel<T, W, 2, 256, true>, threads = 256;
+  else if (runs <= 1024) kern = norm_backward_kernel<T, W, 2, 512, !F32>;
+  *blocks = (int)std::min<int64_t>({g.rows, kMaxBlocks, (int64_t)sms * (512 / threads)});
+  PdlLaunch l(dim3(*blocks), dim3(threads), 0, stream);
   const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, g);
   return e == cudaSuccess ? KEBAB_OK : cuda_fail(e, "rms_norm_backward launch");
 }
@@ -506,14 +521,14 @@ int kebab_rms_norm_backward(kebab_dtype dtype, kebab_dtype weight_dtype, const v
     const bool vec = cols % 8 == 0 && aligned(dy, lddy, es, 16) && aligned(s, lds, es, 16) &&
                      aligned(weight, 0, 1, 16) && (!ds || aligned(ds, ldds, es, 16)) &&
                      (!dx || aligned(dx, lddx, es, 16));
-    const int blocks = (int)std::min<int64_t>({rows, kMaxBlocks, (int64_t)dev->sm_count * 4});
+    int blocks = 0;
     auto run = [&](auto t) {
       using T = decltype(t);
-      return vec ? launch_backward<T, 8>(g, blocks, st) : launch_backward<T, 1>(g, blocks, st);
+      return vec ? launch_backward<T, 8>(g, dev->sm_count, &blocks, st) : launch_backward<T, 1>(g, dev->sm_count, &blocks, st);
     };
     rc = dtype == KEBAB_F16 ? run(__half()) : dtype == KEBAB_BF16 ? run(__nv_bfloat16()) : run(0.f);
     if (rc || !dweight) return rc;
-    PdlLaunch l(dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, st);
+    PdlLaunch l(dim3((unsigned)((cols + 31) / 32)), dim3(1024), 0, st);
     cudaError_t e;
     if (weight_dtype == KEBAB_F16) e = cudaLaunchKernelEx(&l.cfg, norm_dweight_kernel<__half>, (const float*)partial, blocks, (int)cols, static_cast<__half*>(dweight));
     else if (weight_dtype == KEBAB_BF16) e = cudaLaunchKernelEx(&l.cfg, norm_dweight_kernel<__nv_bfloat16>, (const float*)partial, blocks, (int)cols, static_cast<__nv_bfloat16*>(dweight));

@@ -48,59 +48,68 @@ struct QuantArgs {
   int64_t ldx, x_stride;
   uint8_t* codes;
   uint8_t* scales;
-  int64_t rows;     // of a matrix
-  int K, tiles;     // tiles: runs of 128 values
+  int64_t rows;  // of a matrix
+  int K, tiles;  // tiles: runs of 128 values
+  int spans;     // runs of 256 values that a warp takes
   int64_t entries;  // tokens: R + F4_SLACK
 };
 
-// A warp takes 256 values (two runs of 128) of a row; blockIdx.y is the matrix.
-// TOKENS picks the layout of the scales.
+// A warp takes spans of 256 values (two runs of 128) of a row, four of them in
+// flight; blockIdx.y is the part of the row, blockIdx.z the matrix. TOKENS picks
+// the layout of the scales.
 template <typename T, bool VEC, bool TOKENS>
 __global__ void __launch_bounds__(THREADS) quantize_f4_kernel(const QuantArgs g) {
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int spans = (g.tiles + 1) / 2;  // of 256 values
-  const int64_t at = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-  const int64_t padded = TOKENS ? g.rows : (g.rows + 127) / 128 * 128;
-  if (at >= padded * spans) return;
-  const int64_t row = at / spans;
-  const int k = (int)(at - row * spans) * 256 + lane * 8;
-  float v[8];
+  const int lane = threadIdx.x & 31, part = lane % 16;
+  const int64_t row = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
   const bool real = row < g.rows;
-  const T* x = static_cast<const T*>(g.X) + blockIdx.y * g.x_stride + row * g.ldx;
-  if (VEC && real && k + 8 <= g.K) {
-    load_row<8>(x + k, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = real && k + i < g.K ? to_float(x[k + i]) : 0.f;
-  }
-  uint32_t top = largest<8>(v, 0u);
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  const BlockScale s = block_scale(top);
-  uint32_t word = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float lo = s.byte == 255u ? 0.f : v[2 * i] * s.inv, hi = s.byte == 255u ? 0.f : v[2 * i + 1] * s.inv;
-    word |= codes2(lo, hi) << (8 * i);
-  }
+  const int64_t row_tiles = (g.rows + 127) / 128;
+  if (TOKENS ? !real : row >= row_tiles * 128) return;
+  const T* x = static_cast<const T*>(g.X) + blockIdx.z * g.x_stride + row * g.ldx;
   const int pitch = (int)f4_pitch(g.K);
-  if (real && k / 2 < pitch)
-    *reinterpret_cast<uint32_t*>(g.codes + (blockIdx.y * g.rows + row) * (int64_t)pitch + k / 2) = word;
-  // Of 16 lanes, the scales of blocks 0 .. 3.
-  uint32_t scales = s.byte << (lane / 4 % 4 * 8);
-  scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
-  scales |= __shfl_xor_sync(0xffffffffu, scales, 8);
-  const int tile = k / 128, part = lane % 16;
-  if (tile >= g.tiles) return;
-  if (TOKENS) {
-    const int64_t entry = row - 32 * part;
-    if (part < 4 && entry >= 0)
-      reinterpret_cast<uint32_t*>(g.scales)[(tile * g.entries + entry) * 4 + part] = scales;
-  } else if (part == 0) {
-    uint8_t* to = g.scales + ((blockIdx.y * (padded / 128) + row / 128) * g.tiles + tile) * 512;
-    *reinterpret_cast<uint32_t*>(to + row % 32 * 16 + row % 128 / 32 * 4) = scales;
+  uint8_t* codes = g.codes + (blockIdx.z * g.rows + row) * (int64_t)pitch;
+  const int64_t entry = row - 32 * part;
+  // Where this lane's words of scales go: the place of tile 0, and the next tile's.
+  uint32_t* to = reinterpret_cast<uint32_t*>(g.scales);
+  if (TOKENS) to += entry * 4 + part;
+  else to += (blockIdx.z * row_tiles + row / 128) * g.tiles * 128 + row % 32 * 4 + row % 128 / 32;
+  const int64_t step = TOKENS ? g.entries * 4 : 128;
+  const bool writes = TOKENS ? part < 4 && entry >= 0 : part == 0;
+  const int begin = (int)blockIdx.y * g.spans * 256, end = min(begin + g.spans * 256, g.tiles * 128);
+  constexpr int UNROLL = 4;
+  for (int k0 = begin + lane * 8; k0 - lane * 8 < end; k0 += UNROLL * 256) {
+    Run<T, 8> run[UNROLL];
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (VEC && real && k0 + u * 256 + 8 <= g.K && k0 + u * 256 < end) run[u].load(x + k0 + u * 256);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int k = k0 + u * 256;
+      if (k - lane * 8 >= end) break;
+      if (VEC && real && k + 8 <= g.K) {
+        run[u].values(v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = real && k + i < g.K ? to_float(x[k + i]) : 0.f;
+      }
+      uint32_t top = largest<8>(v, 0u);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const BlockScale s = block_scale(top);
+      uint32_t word = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) word |= codes2(v[2 * i] * s.inv, v[2 * i + 1] * s.inv) << (8 * i);
+      if (s.byte == 255u) word = 0;  // an infinity or NaN in the block
+      if (real && k / 2 < pitch) *reinterpret_cast<uint32_t*>(codes + k / 2) = word;
+      // Of 16 lanes, the scales of blocks 0 .. 3.
+      uint32_t scales = s.byte << (lane / 4 % 4 * 8);
+      scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
+      scales |= __shfl_xor_sync(0xffffffffu, scales, 8);
+      const int tile = k / 128;
+      if (writes && tile < g.tiles) to[tile * step] = scales;
+    }
   }
 }
 
@@ -109,13 +118,18 @@ struct DequantArgs {
   const uint8_t* scales;
   void* W;
   int64_t rows;
-  int K, tiles;
+  int K, tiles, spans;
 };
 
-// The value of a code's low nibble: 2^e times its magnitude, by a table of halves.
-__device__ __forceinline__ float value_of(uint32_t code, float scale) {
-  const float m = (float)(0xC8643210u >> (code & 7u) * 4 & 15u) * 0.5f;
-  return (code & 8u ? -m : m) * scale;
+// The values of a byte's two codes, the low nibble's first.
+__device__ __forceinline__ float2 values2(uint32_t byte) {
+  uint32_t h;
+  asm("{\n\t.reg .b8 c, x, y, z;\n\t"
+      "mov.b32 {c, x, y, z}, %1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, c;\n\t}"
+      : "=r"(h)
+      : "r"(byte));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
 __device__ __forceinline__ float scale_of(uint32_t byte) {
@@ -126,40 +140,64 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS) dequantize_f4_kernel(const DequantArgs g) {
   pdl_wait();
   pdl_launch_dependents();
-  const int runs = (g.K + 7) / 8;
-  const int64_t at = (int64_t)blockIdx.x * THREADS + threadIdx.x;
-  if (at >= g.rows * runs) return;
-  const int64_t row = at / runs;
-  const int k = (int)(at - row * runs) * 8;
-  const uint32_t word =
-      *reinterpret_cast<const uint32_t*>(g.codes + (blockIdx.y * g.rows + row) * f4_pitch(g.K) + k / 2);
-  const uint8_t* tile = g.scales + ((blockIdx.y * ((g.rows + 127) / 128) + row / 128) * g.tiles + k / 128) * 512;
-  const float scale = scale_of(tile[row % 32 * 16 + row % 128 / 32 * 4 + k / 32 % 4]);
-  float v[8];
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (row >= g.rows) return;
+  const int pitch = (int)f4_pitch(g.K);
+  const uint8_t* codes = g.codes + (blockIdx.z * g.rows + row) * (int64_t)pitch;
+  const uint8_t* scales = g.scales + (blockIdx.z * ((g.rows + 127) / 128) + row / 128) * g.tiles * 512 + row % 32 * 16 +
+                          row % 128 / 32 * 4;
+  T* w = static_cast<T*>(g.W) + (blockIdx.z * g.rows + row) * (int64_t)g.K;
+  const int begin = (int)blockIdx.y * g.spans * 256, end = min(begin + g.spans * 256, g.K);
+  constexpr int UNROLL = 4;
+  for (int k0 = begin + lane * 8; k0 < end; k0 += UNROLL * 256) {
+    uint32_t word[UNROLL], byte[UNROLL];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = value_of(word >> (4 * i), scale);
-  T* w = static_cast<T*>(g.W) + (blockIdx.y * g.rows + row) * (int64_t)g.K + k;
-  if (VEC) {
-    store_row<8>(w, v);
-  } else {
+    for (int u = 0; u < UNROLL; ++u) {
+      const int k = k0 + u * 256;
+      if (k < end) {
+        word[u] = *reinterpret_cast<const uint32_t*>(codes + k / 2);
+        byte[u] = scales[k / 128 * 512 + k / 32 % 4];
+      }
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (k + i < g.K) w[i] = from_float<T>(v[i]);
+    for (int u = 0; u < UNROLL; ++u) {
+      const int k = k0 + u * 256;
+      if (k >= end) break;
+      const float scale = scale_of(byte[u]);
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 two = values2(word[u] >> (8 * i));
+        v[2 * i] = two.x * scale, v[2 * i + 1] = two.y * scale;
+      }
+      if (VEC) {
+        store_row<8>(w + k, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (k + i < g.K) w[k + i] = from_float<T>(v[i]);
+      }
+    }
   }
 }
 
 constexpr int64_t kMaxDim = int64_t(1) << 30;
 
+// Spans of 256 values that a warp takes of a row: more than four only while
+// there are warps for every SM.
+int spans_of(int64_t rows, int64_t spans) { return rows * spans >= 148 * 64 * 8 ? 8 : rows * spans >= 148 * 64 * 4 ? 4 : 1; }
+
 template <typename T, bool TOKENS>
-int quantize(const QuantArgs& g, int64_t E, cudaStream_t stream) {
-  const int64_t rows = TOKENS ? g.rows : (g.rows + 127) / 128 * 128;
-  const int64_t blocks = (rows * ((g.tiles + 1) / 2) + WARPS - 1) / WARPS;
-  if (blocks > INT32_MAX) return fail(KEBAB_EINVAL, "quantize_f4: too many values");
+int quantize(QuantArgs g, int64_t E, cudaStream_t stream) {
+  const int64_t rows = TOKENS ? g.rows : (g.rows + 127) / 128 * 128, spans = (g.tiles + 1) / 2;
+  g.spans = std::max<int>(spans_of(rows * E, spans), (int)((spans + 65534) / 65535));
   const bool vec = (reinterpret_cast<uintptr_t>(g.X) & 15u) == 0 && (g.ldx * sizeof(T)) % 16 == 0 &&
                    (E == 1 || (g.x_stride * sizeof(T)) % 16 == 0);
-  PdlLaunch l(dim3((unsigned)blocks, (unsigned)E), dim3(THREADS), 0, stream);
+  PdlLaunch l(dim3((unsigned)((rows + WARPS - 1) / WARPS), (unsigned)((spans + g.spans - 1) / g.spans), (unsigned)E),
+              dim3(THREADS), 0, stream);
   const cudaError_t e = cudaLaunchKernelEx(
-      &l.cfg, vec ? quantize_f4_kernel<T, true, TOKENS> : quantize_f4_kernel<T, false, TOKENS>, g);
+      &l.cfg, vec ? quantize_f4_kernel<T, true, TOKENS> : quantize_f4_kernel<T, false, TOKENS>, (const QuantArgs)g);
   return e == cudaSuccess ? KEBAB_OK : cuda_fail(e, "quantize_f4 launch");
 }
 
@@ -171,13 +209,14 @@ int quantize_any(int dtype, const QuantArgs& g, int64_t E, cudaStream_t s) {
 }
 
 template <typename T>
-int dequantize(const DequantArgs& g, int64_t E, cudaStream_t stream) {
-  const int64_t blocks = (g.rows * ((g.K + 7) / 8) + THREADS - 1) / THREADS;
-  if (blocks > INT32_MAX) return fail(KEBAB_EINVAL, "dequantize_f4: too many values");
+int dequantize(DequantArgs g, int64_t E, cudaStream_t stream) {
+  const int64_t spans = (g.K + 255) / 256;
+  g.spans = std::max<int>(spans_of(g.rows * E, spans), (int)((spans + 65534) / 65535));
   const bool vec = (reinterpret_cast<uintptr_t>(g.W) & 15u) == 0 && g.K % 8 == 0;
-  PdlLaunch l(dim3((unsigned)blocks, (unsigned)E), dim3(THREADS), 0, stream);
+  PdlLaunch l(dim3((unsigned)((g.rows + WARPS - 1) / WARPS), (unsigned)((spans + g.spans - 1) / g.spans), (unsigned)E),
+              dim3(THREADS), 0, stream);
   const cudaError_t e =
-      cudaLaunchKernelEx(&l.cfg, vec ? dequantize_f4_kernel<T, true> : dequantize_f4_kernel<T, false>, g);
+      cudaLaunchKernelEx(&l.cfg, vec ? dequantize_f4_kernel<T, true> : dequantize_f4_kernel<T, false>, (const DequantArgs)g);
   return e == cudaSuccess ? KEBAB_OK : cuda_fail(e, "dequantize_f4 launch");
 }
 
@@ -225,7 +264,7 @@ int kebab_quantize_f4(kebab_dtype dtype, const void* W, int64_t ldw, int64_t w_s
     if (!W || !codes || !scales) return fail(KEBAB_EINVAL, "quantize_f4: null pointer");
     if (!on16(codes) || !on16(scales))
       return fail(KEBAB_EINVAL, "quantize_f4: codes and scales must be 16-byte aligned");
-    const QuantArgs g = {W, ldw, w_stride, codes, scales, N, (int)K, (int)((K + 127) / 128), 0};
+    const QuantArgs g = {W, ldw, w_stride, codes, scales, N, (int)K, (int)((K + 127) / 128), 0, 0};
     return quantize_any<false>(dtype, g, E, reinterpret_cast<cudaStream_t>(stream));
   });
 }
@@ -241,7 +280,7 @@ int kebab_quantize_f4_tokens(kebab_dtype dtype, const void* X, int64_t ldx, uint
     if (!X || !codes || !scales) return fail(KEBAB_EINVAL, "quantize_f4_tokens: null pointer");
     if (!on16(codes) || !on16(scales))
       return fail(KEBAB_EINVAL, "quantize_f4_tokens: codes and scales must be 16-byte aligned");
-    const QuantArgs g = {X, ldx, 0, codes, scales, R, (int)K, (int)((K + 127) / 128), R + F4_SLACK};
+    const QuantArgs g = {X, ldx, 0, codes, scales, R, (int)K, (int)((K + 127) / 128), 0, R + F4_SLACK};
     return quantize_any<true>(dtype, g, 1, reinterpret_cast<cudaStream_t>(stream));
   });
 }
@@ -254,7 +293,7 @@ int kebab_dequantize_f4(kebab_dtype dtype, const uint8_t* codes, const uint8_t* 
     if (!W || !codes || !scales) return fail(KEBAB_EINVAL, "dequantize_f4: null pointer");
     if (!on16(codes) || !on16(scales))
       return fail(KEBAB_EINVAL, "dequantize_f4: codes and scales must be 16-byte aligned");
-    const DequantArgs g = {codes, scales, W, N, (int)K, (int)((K + 127) / 128)};
+    const DequantArgs g = {codes, scales, W, N, (int)K, (int)((K + 127) / 128), 0};
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return dtype == KEBAB_F16 ? dequantize<__half>(g, E, s) : dtype == KEBAB_BF16 ? dequantize<__nv_bfloat16>(g, E, s) : dequantize<float>(g, E, s);
   });
