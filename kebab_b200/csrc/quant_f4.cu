@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "f4.h"
 #include "kebab/f4.h"
@@ -21,15 +22,40 @@ namespace kb {
 namespace {
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 
-// Codes of two values: `lo` in the low nibble. Nearest, ties to even, at most 6.
-__device__ __forceinline__ uint32_t codes2(float lo, float hi) {
+// Codes of eight values, the first in the lowest nibble. Nearest, ties to even.
+__device__ __forceinline__ uint32_t codes8(const float (&v)[8]) {
   uint32_t r;
-  asm("{\n\t.reg .b8 c, z;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 c, %2, %1;\n\t"
-      "mov.b32 %0, {c, 0, 0, 0};\n\t}"
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
       : "=r"(r)
-      : "f"(lo), "f"(hi));
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
+}
+
+// Bits of the largest magnitude of the 32 values of four neighbouring lanes.
+// Values of 16 bits are compared in pairs, as they are stored (their magnitudes
+// order as integers, a NaN above everything).
+template <typename T>
+__device__ __forceinline__ uint32_t block_top(const Run<T, 8>& run) {
+  if constexpr (sizeof(T) == 2) {
+    constexpr uint32_t M = 0x7fff7fffu;
+    const uint4 r = run.raw[0];
+    uint32_t m = __vmaxu2(__vmaxu2(r.x & M, r.y & M), __vmaxu2(r.z & M, r.w & M));
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const uint16_t h = (uint16_t)max(m >> 16, m & 0xffffu);
+    return __float_as_uint(to_float(*reinterpret_cast<const T*>(&h)));
+  } else {
+    float v[8];
+    run.values(v);
+    uint32_t top = largest<8>(v, 0u);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    return max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  }
 }
 
 // The scale's byte and 2^-e.
@@ -61,7 +87,7 @@ template <typename T, bool VEC, bool TOKENS>
 __global__ void __launch_bounds__(THREADS) quantize_f4_kernel(const QuantArgs g) {
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, part = lane % 16;
+  const int lane = threadIdx.x & 31, part = lane % 16, shift = lane / 4 % 4 * 8;
   const int64_t row = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
   const bool real = row < g.rows;
   const int64_t row_tiles = (g.rows + 127) / 128;
@@ -77,39 +103,47 @@ __global__ void __launch_bounds__(THREADS) quantize_f4_kernel(const QuantArgs g)
   const int64_t step = TOKENS ? g.entries * 4 : 128;
   const bool writes = TOKENS ? part < 4 && entry >= 0 : part == 0;
   const int begin = (int)blockIdx.y * g.spans * 256, end = min(begin + g.spans * 256, g.tiles * 128);
-  constexpr int UNROLL = 4;
-  for (int k0 = begin + lane * 8; k0 - lane * 8 < end; k0 += UNROLL * 256) {
-    Run<T, 8> run[UNROLL];
+  // The codes and scales of 8 values a lane from k on; INSIDE: all of the span is within the row.
+  auto span = [&](auto inside, Run<T, 8>& run, int k) {
+    constexpr bool INSIDE = decltype(inside)::value;
+    const BlockScale s = block_scale(block_top(run));
     float v[8];
+    run.values(v);
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-      if (VEC && real && k0 + u * 256 + 8 <= g.K && k0 + u * 256 < end) run[u].load(x + k0 + u * 256);
+    for (int i = 0; i < 8; ++i) v[i] *= s.inv;
+    const uint32_t word = s.byte == 255u ? 0u : codes8(v);  // 0: an infinity or NaN in the block
+    if (INSIDE || (real && k / 2 < pitch)) *reinterpret_cast<uint32_t*>(codes + k / 2) = word;
+    // Of 16 lanes, the scales of blocks 0 .. 3.
+    uint32_t scales = s.byte << shift;
+    scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
+    scales |= __shfl_xor_sync(0xffffffffu, scales, 8);
+    const int tile = k / 128;
+    if (writes && (INSIDE || tile < g.tiles)) to[tile * step] = scales;
+  };
+  constexpr int UNROLL = 4;
+  int k0 = begin;
+  if (VEC && real) {
+    const T* from = x + lane * 8;
+    for (; k0 + UNROLL * 256 <= min(end, g.K); k0 += UNROLL * 256) {
+      Run<T, 8> run[UNROLL];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int k = k0 + u * 256;
-      if (k - lane * 8 >= end) break;
-      if (VEC && real && k + 8 <= g.K) {
-        run[u].values(v);
-      } else {
+      for (int u = 0; u < UNROLL; ++u) run[u].load(from + k0 + u * 256);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = real && k + i < g.K ? to_float(x[k + i]) : 0.f;
-      }
-      uint32_t top = largest<8>(v, 0u);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const BlockScale s = block_scale(top);
-      uint32_t word = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) word |= codes2(v[2 * i] * s.inv, v[2 * i + 1] * s.inv) << (8 * i);
-      if (s.byte == 255u) word = 0;  // an infinity or NaN in the block
-      if (real && k / 2 < pitch) *reinterpret_cast<uint32_t*>(codes + k / 2) = word;
-      // Of 16 lanes, the scales of blocks 0 .. 3.
-      uint32_t scales = s.byte << (lane / 4 % 4 * 8);
-      scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
-      scales |= __shfl_xor_sync(0xffffffffu, scales, 8);
-      const int tile = k / 128;
-      if (writes && tile < g.tiles) to[tile * step] = scales;
+      for (int u = 0; u < UNROLL; ++u) span(std::true_type(), run[u], k0 + u * 256 + lane * 8);
     }
+  }
+  for (; k0 < end; k0 += 256) {
+    const int k = k0 + lane * 8;
+    Run<T, 8> run;
+    if (VEC && real && k + 8 <= g.K) {
+      run.load(x + k);
+    } else {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = real && k + i < g.K ? to_float(x[k + i]) : 0.f;
+      run.set(v);
+    }
+    span(std::false_type(), run, k);
   }
 }
 
