@@ -5,6 +5,11 @@ training and in serving.
     y, routing = layer(x)
     served = layer.quantize()                       # 8-bit integer experts, forward only
     y = served(x)
+    served = layer.serve(bits)                      # 16, 8 or 4 bits; a few tokens take two launches
+
+    block = Block(width, hidden, experts, k)        # the norm before the layer, on a residual stream
+    y, stream, routing = block(x, stream)           # stream: the sum x + stream that was normed
+    y, stream = block.serve(bits)(x, stream)
 
 The layer is y[t] = sum_j w[t, j] W2_e (silu(Wg_e x[t]) * Wu_e x[t]) over the k
 experts e = e[t, j] that its router picks. `route`, `dispatch`, `combine` and
@@ -85,6 +90,27 @@ class _GroupedLinear(torch.autograd.Function):
         return dx, dw, None
 
 
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        x = _rows(x)
+        y, s = kb.rms_norm(x, weight, eps, residual=None if residual is None else _rows(residual))
+        ctx.save_for_backward(s, weight)
+        ctx.eps, ctx.added = eps, residual is not None
+        ctx.set_materialize_grads(False)  # a stream that ends here has no gradient
+        return (y, s) if ctx.added else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds=None):
+        s, weight = ctx.saved_tensors
+        if dy is None:
+            dx, dweight = ds, None
+        else:
+            dx, dweight = kb.rms_norm_backward(_rows(dy), s, weight, ctx.eps, dresidual=None if ds is None else _rows(ds))
+        return dx, dweight, dx if ctx.added else None, None
+
+
 def _rows(t):
     """`t` with contiguous rows that do not overlap (gradients of a sum are
     expanded: rows of stride 0)."""
@@ -112,6 +138,12 @@ def grouped_linear(x, w, offsets):
     return _GroupedLinear.apply(x, w, offsets)
 
 
+def rms_norm(x, weight, residual=None, eps=1e-6):
+    """kb.rms_norm -> (y, s), differentiable in x, weight and the residual; s is x without a residual."""
+    out = _RmsNorm.apply(x, weight, residual, eps)
+    return (out, x) if residual is None else out
+
+
 def _gated(h):
     gate, up = h.chunk(2, dim=-1)
     return torch.nn.functional.silu(gate) * up
@@ -137,6 +169,9 @@ class MoE(torch.nn.Module):
     def quantize(self):
         return QuantizedMoE(self)
 
+    def serve(self, bits=8):
+        return ServedMoE(self, bits)
+
 
 class QuantizedMoE:
     """A trained MoE for serving, its experts' weights in 8-bit integers with a
@@ -151,6 +186,104 @@ class QuantizedMoE:
         r = kb.route(x.float() @ self.router.T, self.k, self.renormalize)
         h = _gated(kb.linear_grouped_i8(kb.dispatch(x, r.slots), *self.w_in, r.offsets))
         return kb.combine(kb.linear_grouped_i8(h, *self.w_out, r.offsets), r.slots, r.weights)
+
+
+class ServedMoE:
+    """A trained MoE for serving, its experts in 16 bits, in 8-bit integers or in
+    4-bit floating point. Up to kb.FEW_TOKENS tokens through experts of 16 or 8
+    bits take kb.expert_layer, more of them (and 4 bits) the separate operators."""
+
+    def __init__(self, layer, bits=8):
+        self.k, self.renormalize, self.bits = layer.k, layer.renormalize, bits
+        self.router = layer.router.detach()
+        make = {16: lambda w: (w,), 8: kb.quantize_i8, 4: lambda w: (kb.quantize_f4(w),)}.get(bits)
+        if make is None:
+            raise kb.KebabError(kb.EINVAL, "ServedMoE: bits = %s is not 16, 8 or 4" % (bits,))
+        self.w_in, self.w_out = make(layer.w_in.detach()), make(layer.w_out.detach())
+        self.linear = {16: kb.gemm_grouped, 8: kb.linear_grouped_i8, 4: kb.linear_grouped_f4}[bits]
+
+    def __call__(self, x):
+        if self.bits != 4 and len(x) <= kb.FEW_TOKENS:
+            few = kb.expert_layer if self.bits == 16 else kb.expert_layer_i8
+            return few(x, self.router, *self.w_in, *self.w_out, self.k, self.renormalize)
+        r = kb.route(x.float() @ self.router.T, self.k, self.renormalize)
+        h = _gated(self.linear(kb.dispatch(x, r.slots), *self.w_in, r.offsets))
+        return kb.combine(self.linear(h, *self.w_out, r.offsets), r.slots, r.weights)
+
+
+class Block(torch.nn.Module):
+    """The residual stream's addition and norm, and an MoE on the result."""
+
+    def __init__(self, width, hidden, experts, k, dtype=torch.bfloat16, renormalize=True, device="cuda", eps=1e-6):
+        super().__init__()
+        self.eps = eps
+        self.norm = torch.nn.Parameter(torch.ones(width, device=device))
+        self.moe = MoE(width, hidden, experts, k, dtype, renormalize, device)
+
+    def forward(self, x, stream=None):
+        y, stream = rms_norm(x, self.norm, stream, self.eps)
+        y, r = self.moe(y)
+        return y, stream, r
+
+    def serve(self, bits=8):
+        return ServedBlock(self, bits)
+
+
+class ServedBlock:
+    """A trained Block for serving; see ServedMoE."""
+
+    def __init__(self, block, bits=8):
+        self.norm, self.eps, self.moe = block.norm.detach(), block.eps, block.moe.serve(bits)
+
+    def __call__(self, x, stream=None):
+        y, stream = kb.rms_norm(x, self.norm, self.eps, residual=stream)
+        return self.moe(y), stream
+
+
+def _through(blocks, x):
+    """The residual stream after the blocks."""
+    stream = None
+    for b in blocks:
+        x, stream = b(x, stream)[:2]
+    return x + stream
+
+
+def demo_blocks(width=64, hidden=128, experts=8, k=2, tokens=2048, steps=40, lr=1e-2, seed=0):
+    """Trains two blocks to imitate two fixed random ones; returns the losses and,
+    by bits, the relative distance of the served blocks' output for single tokens."""
+    torch.manual_seed(seed)
+    target = [Block(width, hidden, experts, k) for _ in range(2)]
+    blocks = [Block(width, hidden, experts, k) for _ in range(2)]
+    with torch.no_grad():
+        for a, b in zip(blocks, target):
+            a.moe.router.copy_(b.moe.router)
+    params = [p for b in blocks for p in b.parameters()]
+    master = [p.detach().float().clone() for p in params]  # 32-bit copies for the optimiser
+    opt = torch.optim.Adam(master, lr=lr)
+    losses = []
+    for _ in range(steps):
+        x = torch.randn((tokens, width), device="cuda").bfloat16()
+        with torch.no_grad():
+            want = _through(target, x).float()
+        loss = (_through(blocks, x).float() - want).square().mean() / want.square().mean()
+        loss.backward()
+        for m, p in zip(master, params):
+            m.grad, p.grad = p.grad.float(), None
+        opt.step()
+        with torch.no_grad():
+            for m, p in zip(master, params):
+                p.copy_(m)
+        losses.append(loss.detach())
+    off = {}
+    with torch.no_grad():
+        for bits in (16, 8, 4):
+            served, d = [b.serve(bits) for b in blocks], []
+            for _ in range(16):
+                x = torch.randn((1, width), device="cuda").bfloat16()
+                a, b = _through(blocks, x).float(), _through(served, x).float()
+                d.append((a - b).norm() / a.norm())
+            off[bits] = float(torch.stack(d).mean())
+    return [float(v) for v in losses], off
 
 
 def demo(width=64, hidden=128, experts=8, k=2, tokens=2048, steps=60, lr=1e-2, seed=0):
@@ -197,6 +330,10 @@ def main(argv=None):
         print("step %3d  loss %.4f" % (i, losses[i]))
     print("step %3d  loss %.4f" % (len(losses) - 1, losses[-1]))
     print("single tokens, 8-bit experts against 16-bit: relative distance %.4f" % off)
+    losses, off = demo_blocks(steps=a.steps, tokens=a.tokens)
+    print("two blocks: loss %.4f -> %.4f" % (losses[0], losses[-1]))
+    for bits, d in off.items():
+        print("single tokens through the blocks, served in %d bits: relative distance %.4f" % (bits, d))
     return 0
 
 

@@ -43,6 +43,11 @@ def _like(what, name, t, x, dev):
             raise bad("%s: %s must be %s, got %s" % (what, name, tuple(x.shape), tuple(t.shape)))
 
 
+def _rows_like(x):
+    """A new contiguous tensor as x (empty_like takes 0.6 us less than new_empty)."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def _row_pitch(t):
     """(address, row pitch) of a matrix or of None."""
     return (None, 0) if t is None else (t.data_ptr(), pitch(t))
@@ -56,10 +61,13 @@ def rms_norm(x, weight, eps=1e-6, residual=None, stream=None):
         with on(dev, stream):
             return rms_norm(x, weight, eps, residual)
     T, H = x.shape
-    y = x.new_empty((T, H))
-    s = x if residual is None else x.new_empty((T, H))
-    call("kebab_rms_norm", dev, CODES[x.dtype], CODES[weight.dtype], x.data_ptr(), pitch(x), *_row_pitch(residual),
-         weight.data_ptr(), eps, s.data_ptr(), pitch(s), y.data_ptr(), H, T, H)
+    y = _rows_like(x)
+    if residual is None:
+        s, r, ldr = x, None, 0
+    else:
+        s, r, ldr = _rows_like(x), residual.data_ptr(), pitch(residual)
+    call("kebab_rms_norm", dev, CODES[x.dtype], CODES[weight.dtype], x.data_ptr(), pitch(x), r, ldr, weight.data_ptr(),
+         eps, s.data_ptr(), H, y.data_ptr(), H, T, H)
     return y, s
 
 
@@ -72,10 +80,10 @@ def rms_norm_i8(x, weight, eps=1e-6, residual=None, keep=False, stream=None):
             return rms_norm_i8(x, weight, eps, residual, keep)
     T, H = x.shape
     codes, scale = x.new_empty((T, H), dtype=torch.int8), x.new_empty((T,), dtype=torch.float32)
-    y = x.new_empty((T, H)) if keep else None
-    s = x if residual is None else x.new_empty((T, H))
+    y = _rows_like(x) if keep else None
+    s = x if residual is None else _rows_like(x)
     call("kebab_rms_norm_i8", dev, CODES[x.dtype], CODES[weight.dtype], x.data_ptr(), pitch(x), *_row_pitch(residual),
-         weight.data_ptr(), eps, s.data_ptr(), pitch(s), *_row_pitch(y), codes.data_ptr(), H, scale.data_ptr(), T, H)
+         weight.data_ptr(), eps, s.data_ptr(), H, y.data_ptr() if keep else None, H, codes.data_ptr(), H, scale.data_ptr(), T, H)
     return Normed8(codes, scale, s, y)
 
 
@@ -93,7 +101,7 @@ def rms_norm_backward(dy, s, weight, eps=1e-6, dresidual=None, stream=None):
         with on(dev, stream):
             return rms_norm_backward(dy, s, weight, eps, dresidual)
     T, H = s.shape
-    dx, dweight = s.new_empty((T, H)), torch.empty_like(weight)
+    dx, dweight = _rows_like(s), torch.empty_like(weight)
     size = (T * 8 + 15) // 16 * 16 + min(T, 1024) * H * 4  # kebab_rms_norm_backward_workspace
     ws = s.new_empty((size,), dtype=torch.uint8)
     call("kebab_rms_norm_backward", dev, CODES[s.dtype], CODES[weight.dtype], dy.data_ptr(), pitch(dy), s.data_ptr(),
