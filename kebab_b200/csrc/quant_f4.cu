@@ -170,7 +170,11 @@ __device__ __forceinline__ float scale_of(uint32_t byte) {
   return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255u ? 0x7fffffffu : byte << 23);
 }
 
-template <typename T, bool VEC>
+// A warp takes spans of 256 values of a row, four in flight; 8 values a lane, of
+// a 16-byte granule of W (SHIFT: rows that start `off` values into their first
+// granule; then the codes of the eight are cut from two words, and they may lie
+// in two blocks).
+template <typename T, bool SHIFT>
 __global__ void __launch_bounds__(THREADS) dequantize_f4_kernel(const DequantArgs g) {
   pdl_wait();
   pdl_launch_dependents();
@@ -178,39 +182,49 @@ __global__ void __launch_bounds__(THREADS) dequantize_f4_kernel(const DequantArg
   const int64_t row = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
   if (row >= g.rows) return;
   const int pitch = (int)f4_pitch(g.K);
-  const uint8_t* codes = g.codes + (blockIdx.z * g.rows + row) * (int64_t)pitch;
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>(g.codes + (blockIdx.z * g.rows + row) * (int64_t)pitch);
   const uint8_t* scales = g.scales + (blockIdx.z * ((g.rows + 127) / 128) + row / 128) * g.tiles * 512 + row % 32 * 16 +
                           row % 128 / 32 * 4;
   T* w = static_cast<T*>(g.W) + (blockIdx.z * g.rows + row) * (int64_t)g.K;
-  const int begin = (int)blockIdx.y * g.spans * 256, end = min(begin + g.spans * 256, g.K);
+  const int off = SHIFT ? (int)((reinterpret_cast<uintptr_t>(w) & 15u) / sizeof(T)) : 0;
+  const int begin = (int)blockIdx.y * g.spans * 256, end = min(begin + g.spans * 256, g.K + off);
+  auto scale_at = [&](int k) { return scale_of(scales[k / 128 * 512 + k / 32 % 4]); };
   constexpr int UNROLL = 4;
-  for (int k0 = begin + lane * 8; k0 < end; k0 += UNROLL * 256) {
-    uint32_t word[UNROLL], byte[UNROLL];
+  for (int k0 = begin + lane * 8 - off; k0 < end - off; k0 += UNROLL * 256) {
+    uint32_t word[UNROLL], next[UNROLL];
+    float first[UNROLL], second[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const int k = k0 + u * 256;
-      if (k < end) {
-        word[u] = *reinterpret_cast<const uint32_t*>(codes + k / 2);
-        byte[u] = scales[k / 128 * 512 + k / 32 % 4];
+      if (k < end - off) {
+        word[u] = k >= 0 ? codes[k >> 3] : 0u;
+        first[u] = k >= 0 ? scale_at(k) : 0.f;
+        if (SHIFT) {
+          const int last = min(k + 7, g.K - 1);
+          next[u] = codes[last >> 3];
+          second[u] = scale_at(last);
+        }
       }
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       const int k = k0 + u * 256;
-      if (k >= end) break;
-      const float scale = scale_of(byte[u]);
+      if (k >= end - off) break;
+      const uint32_t eight = SHIFT ? __funnelshift_r(word[u], next[u], (k & 7) * 4) : word[u];
       float v[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 two = values2(word[u] >> (8 * i));
-        v[2 * i] = two.x * scale, v[2 * i + 1] = two.y * scale;
+        const float2 two = values2(eight >> (8 * i));
+        v[2 * i] = two.x, v[2 * i + 1] = two.y;
       }
-      if (VEC) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= SHIFT && ((k + i) >> 5) != (k >> 5) ? second[u] : first[u];
+      if (!SHIFT || (k >= 0 && k + 8 <= g.K)) {
         store_row<8>(w + k, v);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (k + i < g.K) w[k + i] = from_float<T>(v[i]);
+          if (k + i >= 0 && k + i < g.K) w[k + i] = from_float<T>(v[i]);
       }
     }
   }
@@ -244,13 +258,13 @@ int quantize_any(int dtype, const QuantArgs& g, int64_t E, cudaStream_t s) {
 
 template <typename T>
 int dequantize(DequantArgs g, int64_t E, cudaStream_t stream) {
-  const int64_t spans = (g.K + 255) / 256;
+  const int64_t spans = (g.K + 7 + 255) / 256;  // a granule may begin before the row
   g.spans = std::max<int>(spans_of(g.rows * E, spans), (int)((spans + 65534) / 65535));
   const bool vec = (reinterpret_cast<uintptr_t>(g.W) & 15u) == 0 && g.K % 8 == 0;
   PdlLaunch l(dim3((unsigned)((g.rows + WARPS - 1) / WARPS), (unsigned)((spans + g.spans - 1) / g.spans), (unsigned)E),
               dim3(THREADS), 0, stream);
   const cudaError_t e =
-      cudaLaunchKernelEx(&l.cfg, vec ? dequantize_f4_kernel<T, true> : dequantize_f4_kernel<T, false>, (const DequantArgs)g);
+      cudaLaunchKernelEx(&l.cfg, vec ? dequantize_f4_kernel<T, false> : dequantize_f4_kernel<T, true>, (const DequantArgs)g);
   return e == cudaSuccess ? KEBAB_OK : cuda_fail(e, "dequantize_f4 launch");
 }
 

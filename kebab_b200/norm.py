@@ -19,8 +19,9 @@ _ANY = (torch.float16, torch.bfloat16, torch.float32)
 
 
 class Normed8(NamedTuple):
-    """codes [T, H] int8 and scale [T] float32 (operands of gemm_i8), the sum
-    that was normed, and y in x's type where it was asked for."""
+    """codes [T, H] int8 (rows at a pitch of whole 16 bytes) and scale [T] float32,
+    operands of gemm_i8; the sum that was normed; y in x's type where it was
+    asked for."""
     codes: torch.Tensor
     scale: torch.Tensor
     residual: torch.Tensor
@@ -79,11 +80,14 @@ def rms_norm_i8(x, weight, eps=1e-6, residual=None, keep=False, stream=None):
         with on(dev, stream):
             return rms_norm_i8(x, weight, eps, residual, keep)
     T, H = x.shape
-    codes, scale = x.new_empty((T, H), dtype=torch.int8), x.new_empty((T,), dtype=torch.float32)
+    # Rows of codes on 16 bytes, as the products' copies need them.
+    Hp = (H + 15) // 16 * 16
+    codes, scale = x.new_empty((T, Hp), dtype=torch.int8), x.new_empty((T,), dtype=torch.float32)
+    codes = codes if Hp == H else codes[:, :H]
     y = _rows_like(x) if keep else None
     s = x if residual is None else _rows_like(x)
     call("kebab_rms_norm_i8", dev, CODES[x.dtype], CODES[weight.dtype], x.data_ptr(), pitch(x), *_row_pitch(residual),
-         weight.data_ptr(), eps, s.data_ptr(), H, y.data_ptr() if keep else None, H, codes.data_ptr(), H, scale.data_ptr(), T, H)
+         weight.data_ptr(), eps, s.data_ptr(), H, y.data_ptr() if keep else None, H, codes.data_ptr(), Hp, scale.data_ptr(), T, H)
     return Normed8(codes, scale, s, y)
 
 
@@ -102,7 +106,7 @@ def rms_norm_backward(dy, s, weight, eps=1e-6, dresidual=None, stream=None):
             return rms_norm_backward(dy, s, weight, eps, dresidual)
     T, H = s.shape
     dx, dweight = _rows_like(s), torch.empty_like(weight)
-    size = (T * 8 + 15) // 16 * 16 + min(T, 1024) * H * 4  # kebab_rms_norm_backward_workspace
+    size = (T * 8 + 15) // 16 * 16 + min((T + 7) // 8 * 8, 1024) * H * 4  # kebab_rms_norm_backward_workspace
     ws = s.new_empty((size,), dtype=torch.uint8)
     call("kebab_rms_norm_backward", dev, CODES[s.dtype], CODES[weight.dtype], dy.data_ptr(), pitch(dy), s.data_ptr(),
          pitch(s), weight.data_ptr(), eps, *_row_pitch(dresidual), dx.data_ptr(), H, dweight.data_ptr(), ws.data_ptr(),

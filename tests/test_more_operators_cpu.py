@@ -45,7 +45,7 @@ def test_norm_refusals():
 
     assert back(dtype=7) == kb.ENOTSUP and back(wt=kb.BF16) == kb.ENOTSUP
     need = sizes("kebab_rms_norm_backward_workspace", 2, 8)
-    assert need == 16 + 2 * 8 * 4 and sizes("kebab_rms_norm_backward_workspace", 2, 0) == -kb.EINVAL
+    assert need == 16 + 8 * 8 * 4 and sizes("kebab_rms_norm_backward_workspace", 2, 0) == -kb.EINVAL
     for args in (dict(T=-1), dict(H=0), dict(lddy=7), dict(lds=7), dict(ldds=7), dict(lddx=7), dict(dy=None), dict(s=None), dict(w=None), dict(ws=None),
                  dict(ws=BAD), dict(size=need - 1), dict(eps=-1.0), dict(H=(1 << 32) + 8, lddy=1 << 40, lds=1 << 40, ldds=1 << 40, lddx=1 << 40)):
         assert back(**args) == kb.EINVAL, args
