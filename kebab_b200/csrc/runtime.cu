@@ -136,6 +136,17 @@ static int get_encoder() {
 
 
 namespace {
+// Encoding needs a current context, and a thread that has called nothing but
+// cudaGetDevice has none: setting the device that is current makes it.
+template <typename... A>
+CUresult encode(A... args) {
+  CUresult r = g_encode(args...);
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = g_encode(args...);
+  return r;
+}
+
 // Tensor maps are cached per (device, base pointer, dtype, shape, pitch, box,
 // swizzle): encoding one costs about a microsecond of host time, and a GEMM
 // needs three. Bounded: the map is cleared when it reaches kTmapCap entries
@@ -187,7 +198,7 @@ int make_tmap_2d_sw(CUtensorMap* out, const void* base, int dtype, uint64_t rows
   cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUtensorMapDataType t = dtype == KEBAB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUresult r = g_encode(out, t, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = encode(out, t, 2u, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
                         : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
                         : swizzle_bytes == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
@@ -212,7 +223,7 @@ int make_tmap(CUtensorMap* out, const void* base, int type, int rank, const uint
   cuuint32_t b[3];
   for (int i = 0; i < rank; ++i) d[i] = dims[i], b[i] = box[i];
   for (int i = 0; i + 1 < rank; ++i) s[i] = strides[i];
-  const CUresult r = g_encode(out, t, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, ones,
+  const CUresult r = encode(out, t, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, ones,
                               CU_TENSOR_MAP_INTERLEAVE_NONE,
                               swizzle_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
                               : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
