@@ -8,18 +8,18 @@
 
 namespace kb {
 
-int f4_maps(const F4Problem& p, F4Maps* m) {
-  const uint64_t pitch = f4_pitch(p.K), k_tiles = (p.K + 127) / 128, n_tiles = (p.N + 127) / 128;
-  const uint64_t w_dims[3] = {pitch, (uint64_t)p.N, (uint64_t)p.E}, w_strides[2] = {pitch, pitch * p.N};
-  const uint64_t ws_dims[2] = {256, p.E * n_tiles * k_tiles}, ws_strides[1] = {512};
-  const uint64_t xs_dims[2] = {(uint64_t)(p.R + F4_SLACK) * 8, k_tiles};
-  const uint64_t xs_strides[1] = {(uint64_t)(p.R + F4_SLACK) * 16};
-  const uint32_t w_box[3] = {128, 128, 1}, s_box[2] = {256, 2};
-  int rc;
-  if ((rc = make_tmap(&m->w, p.w_codes, TMAP_U8, 3, w_dims, w_strides, w_box, 128)) ||
-      (rc = make_tmap(&m->w_scales, p.w_scales, KEBAB_F16, 2, ws_dims, ws_strides, s_box, 0)))
-    return rc;
-  return make_tmap(&m->x_scales, p.x_scales, KEBAB_F16, 2, xs_dims, xs_strides, s_box, 0);
+int f4_weight_map(const F4Problem& p, int rows, CUtensorMap* m) {
+  const uint64_t pitch = f4_pitch(p.K);
+  const uint64_t dims[3] = {pitch, (uint64_t)p.N, (uint64_t)p.E}, strides[2] = {pitch, pitch * p.N};
+  const uint32_t box[3] = {128, (uint32_t)rows, 1};
+  return make_tmap(m, p.w_codes, TMAP_U8, 3, dims, strides, box, 128);
+}
+
+int f4_weight_scale_map(const F4Problem& p, int tiles, CUtensorMap* m) {
+  const uint64_t k_tiles = (p.K + 127) / 128, n_tiles = (p.N + 127) / 128;
+  const uint64_t dims[3] = {256, k_tiles, p.E * n_tiles}, strides[2] = {512, k_tiles * 512};
+  const uint32_t box[3] = {256, 2, (uint32_t)tiles};
+  return make_tmap(m, p.w_scales, KEBAB_F16, 3, dims, strides, box, 0);
 }
 
 int f4_token_map(const F4Problem& p, int rows, CUtensorMap* m) {
@@ -27,6 +27,13 @@ int f4_token_map(const F4Problem& p, int rows, CUtensorMap* m) {
   const uint64_t dims[2] = {pitch, (uint64_t)p.R}, strides[1] = {pitch};
   const uint32_t box[2] = {128, (uint32_t)rows};
   return make_tmap(m, p.x_codes, TMAP_U8, 2, dims, strides, box, 128);
+}
+
+int f4_token_scale_map(const F4Problem& p, CUtensorMap* m) {
+  const uint64_t dims[2] = {(uint64_t)(p.R + F4_SLACK) * 8, (uint64_t)((p.K + 127) / 128)};
+  const uint64_t strides[1] = {(uint64_t)(p.R + F4_SLACK) * 16};
+  const uint32_t box[2] = {256, 2};
+  return make_tmap(m, p.x_scales, KEBAB_F16, 2, dims, strides, box, 0);
 }
 
 namespace {
@@ -42,8 +49,8 @@ int run(const char* what, const F4Problem& p) {
     return fail(KEBAB_EINVAL, std::string(what) + ": invalid dimensions rows=" + std::to_string(p.R) +
                                   " N=" + std::to_string(p.N) + " K=" + std::to_string(p.K));
   // Coordinates of the scales' tensor maps are 32 bits.
-  if (p.R > F4_MAX_ROWS || p.E * ((p.N + 127) / 128) * ((p.K + 127) / 128) > (1 << 30))
-    return fail(KEBAB_EINVAL, std::string(what) + ": more than 2^27 rows, or than 2^30 runs of 128 x 128 weights");
+  if (p.R > F4_MAX_ROWS || p.E * ((p.N + 127) / 128) > (1 << 30))
+    return fail(KEBAB_EINVAL, std::string(what) + ": more than 2^27 rows, or than 2^30 runs of 128 weight rows");
   if (p.ldy < p.N)
     return fail(KEBAB_EINVAL, std::string(what) + ": row pitch of Y (" + std::to_string(p.ldy) +
                                   ") is below its row length (" + std::to_string(p.N) + ")");

@@ -40,7 +40,7 @@ struct F4SkinnyArgs {
   const int32_t* offsets;
   int E, R, N;
   int pitch;             // bytes of a row's codes
-  int k_tiles, n_tiles;  // runs of 128 values, of 128 weight rows
+  int n_tiles;  // runs of 128 weight rows
   int splits;
   int kps, stages, x_rows;  // K-blocks a stage, stages, rows of X that a stage has room for
   void* Y;
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(THREADS)
     // bytes are all announced by the first; those of X may land before that.
     const bool of_w = warp == 0;
     const uint32_t block_bytes = SUB + width * 128 + 2 * SCALES;
-    const int w_tile = (e * g.n_tiles + n0 / 128) * g.k_tiles;
+    const int w_tile = e * g.n_tiles + n0 / 128;
     if (early && !of_w) pdl_wait();
     int stage = 0;
     uint32_t phase = 1;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(THREADS)
           const int k0 = (kb + q) * 128;  // bytes
           if (of_w) {
             tma_load_3d(dst, &tmW, &full[stage], k0, n0, e);
-            tma_load_2d(sf, &tmWs, &full[stage], 0, w_tile + 2 * (kb + q));
+            tma_load_3d(sf, &tmWs, &full[stage], 0, 2 * (kb + q), w_tile);
             dst += SUB;
           } else {
             int r = 0;
@@ -391,15 +391,26 @@ int launch(const F4Problem& p) {
   g.offsets = p.offsets;
   g.E = (int)p.E, g.R = (int)p.R, g.N = (int)p.N;
   g.pitch = (int)f4_pitch(p.K);
-  g.k_tiles = (int)((p.K + 127) / 128), g.n_tiles = (int)((p.N + 127) / 128);
+  g.n_tiles = (int)((p.N + 127) / 128);
   g.Y = p.Y, g.ldy = p.ldy, g.bias = p.bias;
   g.pdl = pdl_enabled();
   g.early = p.early;
-  F4Maps m;
-  if ((rc = f4_maps(p, &m))) return rc;
+  CUtensorMap tW, tWs, tXs;
+  if ((rc = f4_weight_map(p, 128, &tW)) || (rc = f4_weight_scale_map(p, 1, &tWs)) || (rc = f4_token_scale_map(p, &tXs)))
+    return rc;
+  // The boxes that the shares' widths are made of; of groups, whose sizes the
+  // device knows, all.
+  int boxes = 64 | 32 | 16;
+  if (!p.offsets) {
+    const int64_t n = (p.R + MAX_WIDTH - 1) / MAX_WIDTH, share = (p.R + n - 1) / n, last = p.R - (n - 1) * share;
+    auto width = [](int64_t rows) { return (int)((rows + 15) / 16 * 16); };
+    boxes = width(share) | width(last) | (std::max(width(share), width(last)) == MAX_WIDTH ? 64 : 0);
+  }
   RowMaps tX;
-  for (int i = 0; i < 3; ++i)
-    if ((rc = f4_token_map(p, 64 >> i, &tX.box[i]))) return rc;
+  for (int i = 0; i < 3; ++i) {
+    tX.box[i] = tXs;  // not used
+    if ((boxes & (64 >> i)) && (rc = f4_token_map(p, 64 >> i, &tX.box[i]))) return rc;
+  }
   // Once per device and instantiation: the shared-memory opt-in, and how many
   // clusters of 2, 4 and 8 such CTAs the device holds at once (fewer than its
   // SMs would give: a cluster stays within a GPC).
@@ -439,7 +450,7 @@ int launch(const F4Problem& p) {
   const int64_t x = (int64_t)g.n_tiles * g.splits;
   if (x > INT32_MAX || shares > 65535) return fail(KEBAB_EINVAL, "gemm_f4: too many tiles");
   PdlLaunch l(dim3((unsigned)x, (unsigned)shares), dim3(THREADS), smem, p.stream, g.splits);
-  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, m.w, m.w_scales, tX, m.x_scales, (const F4SkinnyArgs)g);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, tW, tWs, tX, tXs, (const F4SkinnyArgs)g);
   return e == cudaSuccess ? KEBAB_OK : cuda_fail(e, "few-rows 4-bit launch");
 }
 }  // namespace

@@ -3,10 +3,10 @@
 //
 // The MMA's rows are weight rows n, so that a lane of TMEM is a column of the
 // row-major result, and its columns are rows of the group. A tile is a panel of
-// 512 rows (two MMAs of 256 that share the staged columns) or, where that would
-// leave the pairs few tiles each, of 256, by up to 240 columns. Its halves take
-// turns on two accumulators of 240 columns; the other 32 of TMEM's 512 hold
-// scales. With 512-row panels the second half runs one K-block behind the
+// 512 rows (two MMAs of 256 that share the staged columns; a CTA's rows of both
+// follow one another) or, where that would leave the pairs few tiles each, of
+// 256, by up to 240 columns. Its halves take turns on two accumulators of 240
+// columns; the other 32 of TMEM's 512 hold scales. With 512-row panels the second half runs one K-block behind the
 // first, so that an accumulator has two K-blocks' MMAs of the other half between
 // its last MMA and the next tile's first, in which 8 epilogue warps read it into
 // registers and hand it back; they store afterwards, by TMA.
@@ -22,6 +22,13 @@
 // multiple of 16; equal shares of a group), and no group is padded in memory. A
 // tile may read past its group's end: the columns are not stored, and a column
 // does not reach its neighbours.
+//
+// Copies: as few as there can be (the panel's codes, its scales, the columns'
+// codes, at most two of the columns' scales a K-block; ten smaller ones took
+// 4093 x 28672 x 8192 357 us, five 354). What bounds it is what an SM takes from
+// L2: 52 KB a K-block, whose MMAs take 912 cycles at 228 columns; 4093 x 28672 x
+// 8192 in 337 us alone, 5.7 PFLOP/s, 45 bytes a cycle and SM. (Without the copies
+// of scales into TMEM, 336 us: they cost nothing.)
 //
 // Ring: 4 stages of 51 KB a CTA (512-row panels) or 6 of 34 KB. Warps: TMA
 // producer, MMA issuer, 8 epilogue warps, and one that works out the tiles ahead
@@ -61,7 +68,7 @@ struct F4Args {
   const int32_t* offsets;
   int E, R, N;
   int pitch;             // bytes of a row's codes
-  int k_tiles, n_tiles;  // runs of 128 values, of 128 weight rows
+  int n_tiles;           // runs of 128 weight rows
   int vec_out;           // rows of Y on 16-byte boundaries
   void* Y;
   int64_t ldy;
@@ -70,9 +77,16 @@ struct F4Args {
   WaitCtx ctx;
 };
 
-// Boxes of 64, 32, 16 and 8 rows of X.
+// Boxes of rows of X: the least that holds a CTA's half of a tile's columns.
+constexpr int BOXES = 5;
 struct ColumnMaps {
-  CUtensorMap box[4];
+  CUtensorMap box[BOXES];
+};
+__host__ __device__ constexpr int box_rows(int i) { return i == 0 ? 120 : i == 1 ? 112 : i == 2 ? 96 : i == 3 ? 64 : 32; }
+
+// Boxes of a CTA's weight rows of a K-block: 128 (256-row panels), or 256.
+struct PanelMaps {
+  CUtensorMap codes[2], scales[2];
 };
 
 // Group i has the column blocks first[i] .. first[i + 1] - 1, each of `panels` tiles.
@@ -83,7 +97,7 @@ struct Table {
 
 struct alignas(16) Tile {
   int e, a0, b0, width;  // group (-1: no more tiles), first row and column of the tile, its columns (a multiple of 16)
-  int nsub;              // halves of the panel that exist here
+  int nsub;              // halves: 2 in 512-row panels
   int begin, rows;       // the group's rows
   int pad;
 };
@@ -125,7 +139,7 @@ __device__ __forceinline__ Tile tile_of(int64_t t, const F4Args& g, const Table&
   x.width = w.narrow + (cb < w.wider ? 16 : 0);
   x.b0 = cb * w.narrow + min(cb, w.wider) * 16;
   x.a0 = pa * 256 * tab.nsub;
-  x.nsub = min(tab.nsub, (g.N - x.a0 + 255) / 256);
+  x.nsub = min(tab.nsub, (g.N - x.a0 + 255) / 256);  // (a last panel of up to 256 rows is one)
   x.pad = 0;
   return x;
 }
@@ -211,9 +225,8 @@ __device__ __forceinline__ Table make_table(const F4Args& g, int pairs, int* fir
 
 template <typename TO>
 __global__ void __launch_bounds__(THREADS, 1)
-    f4_umma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmWs,
-                   const __grid_constant__ ColumnMaps tmX, const __grid_constant__ CUtensorMap tmXs,
-                   const __grid_constant__ CUtensorMap tmY, const F4Args g) {
+    f4_umma_kernel(const __grid_constant__ PanelMaps tmW, const __grid_constant__ ColumnMaps tmX,
+                   const __grid_constant__ CUtensorMap tmXs, const __grid_constant__ CUtensorMap tmY, const F4Args g) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + OFF_BAR);
@@ -238,8 +251,6 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   cluster_arrive_release();  // this CTA has started
   if (threadIdx.x == 0) {
-    tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmWs);
     tma_prefetch_desc(&tmXs);
     for (int s = 0; s < MAX_STAGES; ++s) {
       mbar_init(&full[s], 1);
@@ -307,10 +318,16 @@ __global__ void __launch_bounds__(THREADS, 1)
         break;
       }
       const int half = x.width / 2, atoms = x.width > 128 ? 2 : 1;
-      const int a0 = x.a0 + (int)rank * 128, row0 = x.begin + x.b0, b0 = row0 + (int)rank * half;
-      // Rows past N have no scales of their own: what is read there scales zeros.
-      const int w_tile = (x.e * g.n_tiles + a0 / 128) * g.k_tiles;
-      const uint32_t bytes = 2 * (x.nsub * (SUB + SCALES) + half * 128 + atoms * SCALES);
+      const int a0 = x.a0 + (int)rank * 128 * x.nsub, row0 = x.begin + x.b0, b0 = row0 + (int)rank * half;
+      const int w_tile = x.e * g.n_tiles + a0 / 128;  // (rows past N have no scales of their own: any, for zeros)
+      const CUtensorMap* codes = &tmW.codes[x.nsub - 1];
+      const CUtensorMap* scales = &tmW.scales[x.nsub - 1];
+      int box = BOXES - 1;
+#pragma unroll
+      for (int i = BOXES - 2; i >= 0; --i)
+        if (half > box_rows(i + 1)) box = i;
+      const CUtensorMap* columns = &tmX.box[box];
+      const uint32_t bytes = 2 * (x.nsub * (SUB + SCALES) + box_rows(box) * 128 + atoms * SCALES);
       for (int kb = 0; kb < blocks; ++kb) {
         ok = all_ok(mbar_wait(&empty[stage], phase ^ 1u, ctx, SITE_EMPTY));
         if (!ok) break;
@@ -318,22 +335,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         uint8_t* sA = smem + stage * stage_bytes;
         if (elect_one()) {
           if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
-          const int k0 = kb * 128;
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            if (s >= x.nsub) break;
-            tma_load_3d_pair(sA + s * SUB, &tmW, bar, k0, a0 + s * 256, x.e);
-            tma_load_2d_pair(sA + sf_off + s * SCALES, &tmWs, bar, 0, w_tile + s * 2 * g.k_tiles + 2 * kb);
-          }
-          uint8_t* sB = sA + a_bytes;
-          int r = 0;
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            if (half & (64 >> m)) {
-              tma_load_2d_pair(sB + r * 128, &tmX.box[m], bar, k0, b0 + r);
-              r += 64 >> m;
-            }
-          }
+          tma_load_3d_pair(sA, codes, bar, kb * 128, a0, x.e);
+          tma_load_3d_pair(sA + sf_off, scales, bar, 0, 2 * kb, w_tile);
+          tma_load_2d_pair(sA + a_bytes, columns, bar, kb * 128, b0);
           tma_load_2d_pair(sA + sfb_off, &tmXs, bar, row0 * 8, 2 * kb);
           if (atoms == 2) tma_load_2d_pair(sA + sfb_off + SCALES, &tmXs, bar, (row0 + 128) * 8, 2 * kb);
         }
@@ -449,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int s = 0; s < x.nsub; ++s) {
         const uint32_t slot = halves & 1u, use = halves >> 1;
         ++halves;
-        const int a_warp = x.a0 + s * 256 + (int)rank * 128 + q * 32;  // this warp's first row of the half
+        const int a_warp = x.a0 + ((int)rank * x.nsub + s) * 128 + q * 32;  // this warp's first row of the half
         const float bias =
             g.bias && a_warp + lane < g.N ? to_float(static_cast<const TO*>(g.bias)[a_warp + lane]) : 0.f;
         ok = all_ok(mbar_wait(&tmem_full[slot], use & 1u, ctx, SITE_TMEM_FULL));
@@ -565,18 +569,21 @@ int launch(const F4Problem& p) {
   g.offsets = p.offsets;
   g.E = (int)p.E, g.R = (int)p.R, g.N = (int)p.N;
   g.pitch = (int)f4_pitch(p.K);
-  g.k_tiles = (int)((p.K + 127) / 128), g.n_tiles = (int)((p.N + 127) / 128);
+  g.n_tiles = (int)((p.N + 127) / 128);
   g.Y = p.Y, g.ldy = p.ldy, g.bias = p.bias;
   g.pdl = pdl_enabled() ? 1 : 0;
-  F4Maps m;
+  PanelMaps tW;
   ColumnMaps tX;
-  if ((rc = f4_maps(p, &m))) return rc;
-  for (int i = 0; i < 4; ++i)
-    if ((rc = f4_token_map(p, 64 >> i, &tX.box[i]))) return rc;
+  CUtensorMap tXs;
+  for (int i = 0; i < 2; ++i)
+    if ((rc = f4_weight_map(p, 128 << i, &tW.codes[i])) || (rc = f4_weight_scale_map(p, 1 << i, &tW.scales[i]))) return rc;
+  for (int i = 0; i < BOXES; ++i)
+    if ((rc = f4_token_map(p, box_rows(i), &tX.box[i]))) return rc;
+  if ((rc = f4_token_scale_map(p, &tXs))) return rc;
   const int64_t tiles = (p.N + 255) / 256 * (p.R / 128 + std::min(p.E, p.R));  // at most
   if (tiles > INT32_MAX / 2) return fail(KEBAB_EINVAL, "gemm_f4: too many tiles");
   // Whole runs of 8 (N too: a run stays within its row).
-  CUtensorMap tY = m.w;  // not used unless vec_out
+  CUtensorMap tY = tXs;  // not used unless vec_out
   g.vec_out = (reinterpret_cast<uintptr_t>(p.Y) & 15u) == 0 && g.ldy % 8 == 0 && g.N % 8 == 0;
   if (g.vec_out) {
     const uint64_t dims[2] = {(uint64_t)p.N, (uint64_t)p.R}, strides[1] = {(uint64_t)p.ldy * 2};
@@ -605,7 +612,7 @@ int launch(const F4Problem& p) {
   if (err[di] != cudaSuccess) return cuda_fail(err[di], "cudaFuncSetAttribute(max dynamic smem)");
   const int pairs = (int)std::min<int64_t>(tiles, max_pairs[di]);
   PdlLaunch ln(dim3(2 * pairs), dim3(THREADS), smem, p.stream, 2);
-  const cudaError_t e = cudaLaunchKernelEx(&ln.cfg, kern, m.w, m.w_scales, tX, m.x_scales, tY, (const F4Args)g);
+  const cudaError_t e = cudaLaunchKernelEx(&ln.cfg, kern, tW, tX, tXs, tY, (const F4Args)g);
   return e == cudaSuccess ? KEBAB_OK : cuda_fail(e, "4-bit tcgen05 launch");
 }
 }  // namespace

@@ -83,14 +83,24 @@ def _check_weights(what, q, blocks, dim, dev):
     """Checks an F4 of `dim` dimensions whose rows have `blocks` blocks; returns (E, N)."""
     if not isinstance(q, F4):
         raise bad("%s: the weights must be what quantize_f4 returns" % what)
-    at = tensor(what, "the weights' codes", q.codes, dim, _U8, dev)
-    if q.codes.shape[-1] != blocks * 16:
+    codes, scales = q
+    # Everything at once first: a call has a few microseconds.
+    if isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.dim() == dim:
+        shape = codes.shape
+        N, at = shape[-2], codes.get_device()
+        E = 1 if dim == 2 else shape[0]
+        tiles = (N + 127) // 128, (blocks + 3) // 4, 512
+        if (at >= 0 and at == (at if dev is None else dev) == scales.get_device() and shape[-1] == blocks * 16 and
+                scales.shape == (tiles if dim == 2 else (E, *tiles)) and codes.dtype is scales.dtype is torch.uint8 and
+                codes.is_contiguous() and scales.is_contiguous()):
+            return E, N
+    at = tensor(what, "the weights' codes", codes, dim, _U8, dev)
+    if codes.shape[-1] != blocks * 16:
         raise bad("%s: inner dimensions differ: X has %d blocks of 32, the weights %d" %
-                  (what, blocks, q.codes.shape[-1] // 16))
-    N = q.codes.shape[-2]
-    dense(what, "the weights' codes", q.codes, q.codes.shape, _U8, at)
-    dense(what, "the weights' scales", q.scales, (*q.codes.shape[:-2], _up(N, 128), _up(blocks, 4), 512), _U8, at)
-    return (1 if dim == 2 else q.codes.shape[0]), N
+                  (what, blocks, codes.shape[-1] // 16))
+    dense(what, "the weights' codes", codes, codes.shape, _U8, at)
+    dense(what, "the weights' scales", scales, (*codes.shape[:-2], _up(codes.shape[-2], 128), _up(blocks, 4), 512), _U8, at)
+    raise bad("%s: the weights must not be empty" % what)
 
 
 def dequantize_f4(q, K, dtype=torch.float32, stream=None):
