@@ -55,6 +55,7 @@ constexpr int TAIL = 128 * 128;           // what an MMA may read past the ring:
 constexpr int RING = 200 * 1024;
 constexpr int SLOT = 40 * 1024;           // bytes of a slot, about
 constexpr int BLOCK = 32;                 // outputs that are added up together
+constexpr int COUNTING = 1 << 19;         // comparisons of keys, at most, to choose by counting
 constexpr int TMEM_COLS = 64;             // two sets of 32
 
 struct LayerArgs {
@@ -184,61 +185,64 @@ constexpr bool is_split() {
   return !I8 && std::is_same<TX, __nv_bfloat16>::value;
 }
 
-// The top-k choices of token t by one warp: as kebab_route.
+// The top-k choices of the tokens, as kebab_route.
 __device__ __forceinline__ uint32_t order_key(float x) {
   x += 0.f;  // -0 becomes +0: they are equal
   if (x != x) return 0xffffffffu;
   const uint32_t b = __float_as_uint(x);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-__device__ __forceinline__ float key_value(uint32_t key) {
-  return __uint_as_float((key & 0x80000000u) ? (key ^ 0x80000000u) : ~key);  // NaN's key gives a NaN
-}
-__device__ void choose(const LayerArgs& g, int t, float* weights, int* experts) {
-  constexpr int V = kMaxExperts / 32;
+// By one warp, choice after choice; `keys`: the token's E words in shared memory.
+__device__ __forceinline__ void choose(const LayerArgs& g, int* experts, uint32_t* keys) {
   const int lane = threadIdx.x & 31;
-  uint32_t key[V];
-#pragma unroll
-  for (int u = 0; u < V; ++u) {
-    if (u * 32 >= g.E) break;
-    const int e = u * 32 + lane;
-    key[u] = e < g.E ? order_key(__ldcg(g.logits + t * g.E + e)) : 0u;
-  }
-  float highest = 0.f, sum = 0.f, mine = 0.f;
+  // The lane's largest key (ties: the lower expert).
+  uint32_t top = 0;
+  int e_top = 0;
+  auto scan = [&] {
+    top = 0;
+#pragma unroll 1
+    for (int e = lane; e < g.E; e += 32) {
+      const uint32_t key = keys[e];
+      if (key > top) top = key, e_top = e;
+    }
+  };
+  scan();
+#pragma unroll 1
   for (int j = 0; j < g.k; ++j) {
-    uint32_t top = 0;
-    int e = 0;
-#pragma unroll
-    for (int u = 0; u < V; ++u) {
-      if (u * 32 >= g.E) break;
-      if (key[u] > top) top = key[u], e = u * 32 + lane;
-    }
     const uint32_t all = __reduce_max_sync(0xffffffffu, top);
-    e = (int)__reduce_min_sync(0xffffffffu, top == all ? (unsigned)e : 0xffffffffu);
-    const float v = key_value(all);
-    if (j == 0) {
-      highest = v;
-      if (!g.renormalize) {
-#pragma unroll
-        for (int u = 0; u < V; ++u) {
-          if (u * 32 >= g.E) break;
-          if (u * 32 + lane < g.E) sum += expf(key_value(key[u]) - highest);
-        }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      }
-    }
-    const float p = highest == -INFINITY ? 0.f : expf(v - highest);  // all logits -inf: nothing to weigh
-    if (g.renormalize) sum += p;
-    if (lane == j) mine = p;
+    const int e = (int)__reduce_min_sync(0xffffffffu, top == all ? (unsigned)e_top : 0xffffffffu);
     if (lane == 0) experts[j] = e;
-#pragma unroll
-    for (int u = 0; u < V; ++u) {
-      if (u * 32 >= g.E) break;
-      if (e == u * 32 + lane) key[u] = 0;
+    if (top == all && e_top == e) {  // the lane that had it
+      keys[e] = 0;
+      scan();
     }
+    __syncwarp();
   }
-  if (lane < g.k) weights[lane] = mine / (highest == -INFINITY ? 1.f : sum);
+}
+
+// All tokens' choices at once by the whole block: an expert's place is how many
+// stand before it (larger keys, or as large ones of lower experts). `parts`
+// neighbouring lanes share an expert's comparisons.
+__device__ __forceinline__ void choose_by_counting(const LayerArgs& g, int* experts, const uint32_t* keys) {
+  const int items = g.T * g.E;
+  int parts = 1;
+  while (parts < 32 && items * parts * 2 <= THREADS) parts *= 2;
+  const int part = threadIdx.x % parts;
+#pragma unroll 1
+  for (int i0 = 0; i0 < items; i0 += THREADS / parts) {
+    const int i = min(i0 + (int)threadIdx.x / parts, items - 1);
+    const int t = i / g.E, e = i - t * g.E;
+    const uint32_t* row = keys + t * g.E;
+    const uint32_t key = row[e];
+    int before = 0;
+#pragma unroll 4
+    for (int o = part; o < g.E; o += parts) {
+      const uint32_t other = row[o];
+      before += o < e ? other >= key : other > key;
+    }
+    for (int d = 1; d < parts; d *= 2) before += __shfl_xor_sync(0xffffffffu, before, d);
+    if (before < g.k) experts[t * g.k + before] = e;
+  }
 }
 
 // 2^n by which a choice's values are multiplied, for the bits of the largest
@@ -270,7 +274,8 @@ static_assert(LayerSmem::bytes(MAX_TOKENS, MAX_K, kMaxExperts) <= 232448, "share
 // The passes of a CTA: its share [at, end) of active x per rows, cut at the
 // experts' ends and then in equal parts of at most `most`. Where the CTAs divide
 // among the experts with at most an eighth of them left over, no share crosses
-// from one expert to the next, which costs a pass more (1 token, 8 experts: XXX).
+// from one expert to the next, which costs a pass more (1 token, 8 experts: such
+// CTAs were 12 us behind the others).
 // Made by whole warps; the shuffles tell the compiler that a warp's lanes have
 // the same values.
 struct Passes {
@@ -387,10 +392,41 @@ __global__ void __launch_bounds__(THREADS, 1)
   for (int i = threadIdx.x; i < g.E; i += THREADS) s_chose[i] = 0;
   if (g.pdl) pdl_wait();
   __syncthreads();
+  // Keys of the logits, in the ring. By counting where that is short: choice
+  // after choice, a token with 8 of them took 3.5 us, for the latency of each.
+  uint32_t* keys = reinterpret_cast<uint32_t*>(smem);
+  for (int i = threadIdx.x; i < g.T * g.E; i += THREADS) keys[i] = order_key(__ldcg(g.logits + i));
+  __syncthreads();
+  const bool counting = (int64_t)g.T * g.E * g.E <= COUNTING;
+  if (counting) {
+    choose_by_counting(g, s_place, keys);
+    __syncthreads();
+  }
   for (int t = warp; t < g.T; t += THREADS / 32) {
-    choose(g, t, s_weight + t * g.k, s_place + t * g.k);
-    __syncwarp();
-    if (lane < g.k) atomicOr(&s_chose[s_place[t * g.k + lane]], 1u << t);
+    if (!counting) {
+      // The softmax's sum needs the keys that `choose` takes away.
+      choose(g, s_place + t * g.k, keys + t * g.E);
+      __syncwarp();
+    }
+    const bool mine = lane < g.k;
+    const int e = mine ? s_place[t * g.k + lane] : 0;
+    const float* logits = g.logits + t * g.E;
+    const float v = mine ? __ldcg(logits + e) + 0.f : 0.f;
+    const float highest = __shfl_sync(0xffffffffu, v, 0);
+    // All logits -inf: nothing to weigh.
+    const float p = mine && highest != -INFINITY ? expf(v - highest) : 0.f;
+    float sum = p;
+    if (!g.renormalize) {
+      sum = 0.f;
+#pragma unroll 1
+      for (int i = lane; i < g.E; i += 32) sum += expf(__ldcg(logits + i) - highest);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (mine) {
+      s_weight[t * g.k + lane] = p / (highest == -INFINITY ? 1.f : sum);
+      atomicOr(&s_chose[e], 1u << t);
+    }
   }
   __syncthreads();
   if (warp == 0) {
@@ -416,19 +452,20 @@ __global__ void __launch_bounds__(THREADS, 1)
       before += __shfl_sync(0xffffffffu, sum, 31);
     }
     if (lane == 0) *s_count = n;
+    __syncwarp();
+    for (int i = lane; i < choices; i += 32) {
+      const uint32_t chose = s_chose[s_place[i]];  // and the place of the expert's first choice
+      const int place = (int)(chose >> 16) + __popc(chose & 0xffffu & ((1u << (i / g.k)) - 1u));
+      s_place[i] = place;
+      s_factor[place] = s_weight[i];
+    }
   }
-  __syncthreads();
-  const int active = __shfl_sync(0xffffffffu, *s_count, 0);
-  for (int i = threadIdx.x; i < choices; i += THREADS) {
-    const uint32_t chose = s_chose[s_place[i]];  // and the place of the expert's first choice
-    const int place = (int)(chose >> 16) + __popc(chose & 0xffffu & ((1u << (i / g.k)) - 1u));
-    s_place[i] = place;
-    s_factor[place] = s_weight[i];
-  }
+  fence_proxy_async_smem();  // the keys' reads and writes before the copies into the ring
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const int active = __shfl_sync(0xffffffffu, *s_count, 0);
 
   // The ring's slots, by the longest pass that there can be.
   using Up = Product<true, PARTS>;
@@ -443,6 +480,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int unit_bytes = max(longest(Up(), g.D), longest(Down(), g.H));
   const int slot_bytes = unit_bytes * max(1, min(MAX_UNITS, SLOT / unit_bytes));
   const int slots = min(MAX_SLOTS, RING / slot_bytes);
+  // The first pass: here, once for all warps. (The second product's are worked out
+  // by each warp while it has time.)
+  Passes first_up(active, g.D, Up::MOST);
+  const bool any_up = first_up.next();
   const int up_blocks = (g.H + EPB - 1) / EPB, down_blocks = (g.D + EPB - 1) / EPB;
   const int box = g.T <= 8 ? 8 : 16;  // columns that are loaded
   auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
@@ -491,10 +532,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     // of the second every other K-block. The loops run with all lanes, so that
     // addresses stay in uniform registers.
     const int which = warp == 0 ? 0 : 1;
-    auto copy = [&](auto product, const RowBoxes& tm, const void* w, int per, int cols, int blocks) {
+    // Weights are read once: they leave L2 first, and the rest (hidden values, the
+    // kernel's own instructions) stays (13 tokens 177 -> 166 us, 1 token 31.6 -> 30.3).
+    const uint64_t policy = l2_policy_evict_first();
+    auto copy = [&](auto product, Passes p, bool more, const RowBoxes& tm, const void* w, int per, int cols, int blocks) {
       using P = decltype(product);
-      Passes p(active, per, P::MOST);
-      while (ok && p.next()) {
+      for (; ok && more; more = p.next()) {
         const Layout l(product, p.rows, slot_bytes);
         const int e = __shfl_sync(0xffffffffu, s_active[p.a], 0);
         const int row = P::kUp ? which * per + p.first : p.first;
@@ -512,8 +555,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int q = q0; q < n; q += step, dst += step * l.bytes) {
               const int k0 = (kb + q) * EPB;
               if (elect_one()) {
-                tma_load_3d(dst, &tm.box[low / 8 - 1], &full[slot], k0, row, e);
-                if (high) tma_load_3d(dst + 64 * 128, &tm.box[high / 8 - 1], &full[slot], k0, row + 64, e);
+                tma_load_3d_hint(dst, &tm.box[low / 8 - 1], &full[slot], k0, row, e, policy);
+                if (high) tma_load_3d_hint(dst + 64 * 128, &tm.box[high / 8 - 1], &full[slot], k0, row + 64, e, policy);
               }
               __syncwarp();
             }
@@ -530,15 +573,16 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
     };
-    copy(Up(), tmIn, g.w_in, g.D, g.H, up_blocks);
-    copy(Down(), tmOut, g.w_out, g.H, g.D, down_blocks);
+    copy(Up(), first_up, any_up, tmIn, g.w_in, g.D, g.H, up_blocks);
+    Passes first_down(active, g.H, Down::MOST);
+    const bool any_down = first_down.next();
+    copy(Down(), first_down, any_down, tmOut, g.w_out, g.H, g.D, down_blocks);
   } else if (warp == 2) {
     // -------------------------------------------------- copies of columns
     bool met = false;  // past the grid barrier
-    auto copy = [&](auto product, int per, int blocks) {
+    auto copy = [&](auto product, Passes p, bool more, int blocks) {
       using P = decltype(product);
-      Passes p(active, per, P::MOST);
-      while (ok && p.next()) {
+      for (; ok && more; more = p.next()) {
         const Layout l(product, p.rows, slot_bytes);
         const int base = __shfl_sync(0xffffffffu, (int)s_base[p.a], 0);
         for (int kb = 0; kb < blocks; kb += l.units) {
@@ -585,18 +629,19 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
     };
-    copy(Up(), g.D, up_blocks);
-    copy(Down(), g.H, down_blocks);
+    copy(Up(), first_up, any_up, up_blocks);
+    Passes first_down(active, g.H, Down::MOST);
+    const bool any_down = first_down.next();
+    copy(Down(), first_down, any_down, down_blocks);
   } else if (warp == 1) {
     // --------------------------------------------------------- MMA issuer
     const uint32_t ring = smem_u32(smem), d0 = __shfl_sync(0xffffffffu, tmem, 0);
     uint32_t pass = 0;
-    auto multiply = [&](auto product, int per, int blocks) {
+    auto multiply = [&](auto product, Passes p, bool more, int blocks) {
       using P = decltype(product);
       constexpr int N = P::OPERANDS * 16;
       constexpr uint32_t IDESC = I8 ? umma_idesc_i8(128, N) : umma_idesc_f16(128, N, ElemTraits<TX>::kBf16);
-      Passes p(active, per, P::MOST);
-      while (ok && p.next()) {
+      for (; ok && more; more = p.next()) {
         const Layout l(product, p.rows, slot_bytes);
         const uint32_t set = pass & 1u, d_tmem = d0 + set * 32;
         ok = all_ok(mbar_wait(&acc_empty[set], (pass >> 1 & 1u) ^ 1u, ctx, SITE_TMEM_EMPTY));
@@ -630,8 +675,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         ++pass;
       }
     };
-    multiply(Up(), g.D, up_blocks);
-    multiply(Down(), g.H, down_blocks);
+    multiply(Up(), first_up, any_up, up_blocks);
+    Passes first_down(active, g.H, Down::MOST);
+    const bool any_down = first_down.next();
+    multiply(Down(), first_down, any_down, down_blocks);
   } else if (warp >= EPI_WARP) {
     // ----------------------------------------------------------- epilogue
     const int et = threadIdx.x - 32 * EPI_WARP;  // the thread's row of a pass
@@ -664,8 +711,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     // Hidden values: silu(gate) * up.
     {
-      Passes p(active, g.D, Up::MOST);
-      while (p.next()) {
+      Passes p = first_up;
+      for (bool more = any_up; more; more = p.next()) {
         const int i = p.first + et, r8 = (p.rows + 7) / 8 * 8;
         const bool mine = et < p.rows;
         float gate_scale = 1.f, up_scale = 1.f;
