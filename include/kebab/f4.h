@@ -23,7 +23,8 @@
  *
  * Plain C, device pointers, asynchronous on `stream`, status codes and
  * kebab_last_error() as in kebab.h. Codes and scales are 16-byte aligned; `ld*`
- * are row pitches in elements. Y is row-major, [M, N]. No counterpart in kebab.
+ * are row pitches in elements. Y is row-major, [M, N]. At most 2^27 token rows,
+ * 1024 matrices, 2^30 values a row. No counterpart in kebab.
  */
 #ifndef KEBAB_F4_H_
 #define KEBAB_F4_H_

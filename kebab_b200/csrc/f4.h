@@ -26,11 +26,11 @@ constexpr int F4_SLACK = 160;  // entries of token scales past the last row
 
 __host__ __device__ inline int64_t f4_pitch(int64_t K) { return (K + 31) / 32 * 16; }  // bytes of a row's codes
 
-// Tensor maps of the operands. Codes: bytes, boxes of 128 bytes of `rows` rows.
-// Scales: as pairs of bytes, boxes of two runs of 128 values, each 512 bytes (of
-// weights, for `tiles` runs of 128 rows).
-int f4_weight_map(const F4Problem& p, int rows, CUtensorMap* m);         // {byte, n, e}
-int f4_weight_scale_map(const F4Problem& p, int tiles, CUtensorMap* m);  // {0, run of values, run of rows of all matrices}
+// Tensor maps of the operands. Codes: bytes, boxes of 128 bytes of 128 weight
+// rows, or of `rows` token rows. Scales: as pairs of bytes, boxes of two runs of
+// 128 values, each 512 bytes, for 128 rows.
+int f4_weight_map(const F4Problem& p, CUtensorMap* m);         // {byte, n, e}
+int f4_weight_scale_map(const F4Problem& p, CUtensorMap* m);  // {0, run of values, run of rows of all matrices}
 int f4_token_map(const F4Problem& p, int rows, CUtensorMap* m);          // {byte, token}
 int f4_token_scale_map(const F4Problem& p, CUtensorMap* m);              // {8 * token, run of values}
 

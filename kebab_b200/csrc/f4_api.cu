@@ -8,17 +8,17 @@
 
 namespace kb {
 
-int f4_weight_map(const F4Problem& p, int rows, CUtensorMap* m) {
+int f4_weight_map(const F4Problem& p, CUtensorMap* m) {
   const uint64_t pitch = f4_pitch(p.K);
   const uint64_t dims[3] = {pitch, (uint64_t)p.N, (uint64_t)p.E}, strides[2] = {pitch, pitch * p.N};
-  const uint32_t box[3] = {128, (uint32_t)rows, 1};
+  const uint32_t box[3] = {128, 128, 1};
   return make_tmap(m, p.w_codes, TMAP_U8, 3, dims, strides, box, 128);
 }
 
-int f4_weight_scale_map(const F4Problem& p, int tiles, CUtensorMap* m) {
+int f4_weight_scale_map(const F4Problem& p, CUtensorMap* m) {
   const uint64_t k_tiles = (p.K + 127) / 128, n_tiles = (p.N + 127) / 128;
   const uint64_t dims[3] = {256, k_tiles, p.E * n_tiles}, strides[2] = {512, k_tiles * 512};
-  const uint32_t box[3] = {256, 2, (uint32_t)tiles};
+  const uint32_t box[3] = {256, 2, 1};
   return make_tmap(m, p.w_scales, KEBAB_F16, 3, dims, strides, box, 0);
 }
 
@@ -63,8 +63,11 @@ int run(const char* what, const F4Problem& p) {
   DeviceInfo* dev = nullptr;
   const int rc = device_info(&dev);
   if (rc) return rc;
-  // The few-rows kernel up to 128 rows, and where the persistent one would have
-  // tiles for less than half of its CTA pairs.
+  // The few-rows kernel up to 128 rows (28672 x 8192: 64 rows 37 us against 43, 128
+  // rows 39 against 43; from 144 on, two shares, 57 against 43), and where the
+  // persistent one would have tiles for less than half of its CTA pairs (4096 x
+  // 14336, 192 rows, 16 tiles: 25 us against 29; 512 rows, 48 tiles: 31 both; 8192
+  // x 8192, 384 rows, 64 tiles: 29 against 27).
   const int64_t tiles = (p.N + 255) / 256 * (p.offsets ? p.R / 240 + std::min(p.E, p.R) : (p.R + 239) / 240);
   return p.R <= 128 || tiles <= dev->sm_count / 4 ? launch_f4_skinny(p) : launch_f4_umma(p);
 }

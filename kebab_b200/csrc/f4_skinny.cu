@@ -8,7 +8,9 @@
 // every other CTA the 128 / S of its rows that that one finishes (st.async,
 // counted on the receiver's barrier), and adds up its own rows over the S
 // partials in rank order. No workspace, no atomics, and the same bits every
-// time.
+// time. With the quantisation, 1 row of 8192 x 8192 takes 10.8 us and 61 rows
+// 14.4 (3.3 and 2.6 TB/s): latency of the quantisation before it, of the first
+// copies and of the exchange. Several accumulators in turn gave nothing.
 //
 // A K-block is 256 values: 128 bytes of codes a row, and two runs of 128 whose
 // scales (512 bytes for 128 rows, as they are stored) the issuer copies into
@@ -396,7 +398,7 @@ int launch(const F4Problem& p) {
   g.pdl = pdl_enabled();
   g.early = p.early;
   CUtensorMap tW, tWs, tXs;
-  if ((rc = f4_weight_map(p, 128, &tW)) || (rc = f4_weight_scale_map(p, 1, &tWs)) || (rc = f4_token_scale_map(p, &tXs)))
+  if ((rc = f4_weight_map(p, &tW)) || (rc = f4_weight_scale_map(p, &tWs)) || (rc = f4_token_scale_map(p, &tXs)))
     return rc;
   // The boxes that the shares' widths are made of; of groups, whose sizes the
   // device knows, all.

@@ -3,13 +3,9 @@
 //
 // The MMA's rows are weight rows n, so that a lane of TMEM is a column of the
 // row-major result, and its columns are rows of the group. A tile is a panel of
-// 512 rows (two MMAs of 256 that share the staged columns; a CTA's rows of both
-// follow one another) or, where that would leave the pairs few tiles each, of
-// 256, by up to 240 columns. Its halves take turns on two accumulators of 240
-// columns; the other 32 of TMEM's 512 hold scales. With 512-row panels the second half runs one K-block behind the
-// first, so that an accumulator has two K-blocks' MMAs of the other half between
-// its last MMA and the next tile's first, in which 8 epilogue warps read it into
-// registers and hand it back; they store afterwards, by TMA.
+// 256 rows by up to 240 columns. Two accumulators of 240 columns take turns, so
+// that 8 epilogue warps read one tile while the next is multiplied; the other 32
+// of TMEM's 512 columns hold scales.
 //
 // A K-block is 256 values: 128 bytes of codes a row, and two runs of 128 values
 // whose scales (512 bytes for 128 rows, as they are stored) the issuer copies
@@ -24,15 +20,17 @@
 // does not reach its neighbours.
 //
 // Copies: as few as there can be (the panel's codes, its scales, the columns'
-// codes, at most two of the columns' scales a K-block; ten smaller ones took
-// 4093 x 28672 x 8192 357 us, five 354). What bounds it is what an SM takes from
-// L2: 52 KB a K-block, whose MMAs take 912 cycles at 228 columns; 4093 x 28672 x
-// 8192 in 337 us alone, 5.7 PFLOP/s, 45 bytes a cycle and SM. (Without the copies
-// of scales into TMEM, 336 us: they cost nothing.)
+// codes, at most two of the columns' scales a K-block; of ten smaller ones, 1 %
+// more). 4093 x 28672 x 8192 takes 295 us after a pause, 6.5 PFLOP/s (3.9 times the
+// 16-bit library product's rate), and 320 in a row, at the clock that the power
+// leaves. Panels of 512 rows, two MMAs to a stage's columns, copy a third less and
+// took 324: what they save is not what bounds it, and their halves had to wait for
+// one another's accumulators (8 matrices of 14336 x 4096, 4093 rows: 131 against
+// 104). 32 matrices of 4096 x 4096 and 1021 rows, bound by the weights: 55 us with
+// the quantisation, 5.1 TB/s.
 //
-// Ring: 4 stages of 51 KB a CTA (512-row panels) or 6 of 34 KB. Warps: TMA
-// producer, MMA issuer, 8 epilogue warps, and one that works out the tiles ahead
-// of them.
+// Ring: 6 stages of 34 KB a CTA. Warps: TMA producer, MMA issuer, 8 epilogue
+// warps, and one that works out the tiles ahead of them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -51,14 +49,14 @@ constexpr int CAP = 240;             // columns of a tile, at most
 constexpr int SUB = 128 * 128;       // 128 rows of 128 bytes of codes
 constexpr int B_BYTES = CAP / 2 * 128;
 constexpr int SCALES = 2 * 512;      // of 128 rows and 256 values
-constexpr int RING = 4 * (2 * SUB + B_BYTES + 4 * SCALES);
-static_assert(RING == 6 * (SUB + B_BYTES + 3 * SCALES), "both stage sizes fill the ring");
-constexpr int MAX_STAGES = 6, TILES = 4;
+// A stage: codes of the panel and the columns, scales of the panel and the columns.
+constexpr int OFF_SFA = SUB + B_BYTES, OFF_SFB = OFF_SFA + SCALES, STAGE_BYTES = OFF_SFB + 2 * SCALES;
+constexpr int STAGES = 6, TILES = 4;
 constexpr int SF_COL = 2 * CAP;      // twice 16 columns: 8 of the columns' scales, 4 of the rows'
 constexpr int RUN = 32;              // columns that an epilogue warp stores at a time
-constexpr int OFF_C = RING;
+constexpr int OFF_C = STAGES * STAGE_BYTES;
 constexpr int OFF_BAR = OFF_C + EPILOGUE * RUN * 32 * 2;
-constexpr int NUM_BARS = 2 * MAX_STAGES + 4 + 2 * TILES;
+constexpr int NUM_BARS = 2 * STAGES + 4 + 2 * TILES;
 constexpr int OFF_TILES = (OFF_BAR + NUM_BARS * 8 + 8 + 15) / 16 * 16;  // after the TMEM address, abort
 constexpr int OFF_TABLE = OFF_TILES + TILES * 32;
 constexpr int smem_bytes(int E) { return OFF_TABLE + (E + 1) * 4 + 1024; }
@@ -84,22 +82,15 @@ struct ColumnMaps {
 };
 __host__ __device__ constexpr int box_rows(int i) { return i == 0 ? 120 : i == 1 ? 112 : i == 2 ? 96 : i == 3 ? 64 : 32; }
 
-// Boxes of a CTA's weight rows of a K-block: 128 (256-row panels), or 256.
-struct PanelMaps {
-  CUtensorMap codes[2], scales[2];
-};
-
 // Group i has the column blocks first[i] .. first[i + 1] - 1, each of `panels` tiles.
 struct Table {
   const int* first;
-  int panels, nsub, cap;
+  int panels, cap;
 };
 
 struct alignas(16) Tile {
   int e, a0, b0, width;  // group (-1: no more tiles), first row and column of the tile, its columns (a multiple of 16)
-  int nsub;              // halves: 2 in 512-row panels
   int begin, rows;       // the group's rows
-  int pad;
 };
 
 // Columns of a group's tiles: equal shares of at most `cap`, in runs of 16, the wider ones first.
@@ -138,16 +129,14 @@ __device__ __forceinline__ Tile tile_of(int64_t t, const F4Args& g, const Table&
   raster((int)(t - (int64_t)tab.first[lo] * tab.panels), tab.panels, w.count, pa, cb);
   x.width = w.narrow + (cb < w.wider ? 16 : 0);
   x.b0 = cb * w.narrow + min(cb, w.wider) * 16;
-  x.a0 = pa * 256 * tab.nsub;
-  x.nsub = min(tab.nsub, (g.N - x.a0 + 255) / 256);  // (a last panel of up to 256 rows is one)
-  x.pad = 0;
+  x.a0 = pa * 256;
   return x;
 }
 
 // The same from lane 0, for code of a whole warp.
 __device__ __forceinline__ Tile uniform(const Tile& x) {
   auto u = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
-  return {u(x.e), u(x.a0), u(x.b0), u(x.width), u(x.nsub), u(x.begin), u(x.rows), 0};
+  return {u(x.e), u(x.a0), u(x.b0), u(x.width), u(x.begin), u(x.rows)};
 }
 
 // Block-wide sums of three values a thread.
@@ -171,11 +160,11 @@ __device__ __forceinline__ void block_sums(int (&v)[3], int (*sums)[3]) {
 __device__ __forceinline__ Table make_table(const F4Args& g, int pairs, int* first) {
   __shared__ int sums[THREADS / 32][3];
   __shared__ int totals[THREADS / 32];
-  // 512-row panels from this many 256-row tiles a pair.
-  constexpr int WIDE_FROM = 8;
   const int panels = (g.N + 255) / 256;
   // The widest tile of 240, 192 or 128 columns, by the waves over the pairs and
-  // the rows that a tile's K-block copies (256 of the panel and its columns).
+  // the rows that a tile's K-block copies (256 of the panel and its columns). (Of
+  // a cost that counts the columns more, 64 + width, 4096 x 14336 x 4093 took 103 us,
+  // not 84; five widths to choose from gave nothing.)
   int c[3] = {0, 0, 0};
   for (int i = threadIdx.x; i < g.E; i += THREADS) {
     int begin, rows;
@@ -218,20 +207,20 @@ __device__ __forceinline__ Table make_table(const F4Args& g, int pairs, int* fir
   }
   if (threadIdx.x == 0) first[g.E] = total;
   tab.first = first;
-  tab.nsub = (int64_t)total * panels >= (int64_t)WIDE_FROM * pairs ? 2 : 1;
-  tab.panels = tab.nsub == 2 ? (g.N + 511) / 512 : panels;
+  tab.panels = panels;
   return tab;
 }
 
 template <typename TO>
 __global__ void __launch_bounds__(THREADS, 1)
-    f4_umma_kernel(const __grid_constant__ PanelMaps tmW, const __grid_constant__ ColumnMaps tmX,
-                   const __grid_constant__ CUtensorMap tmXs, const __grid_constant__ CUtensorMap tmY, const F4Args g) {
+    f4_umma_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmWs,
+                   const __grid_constant__ ColumnMaps tmX, const __grid_constant__ CUtensorMap tmXs,
+                   const __grid_constant__ CUtensorMap tmY, const F4Args g) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + OFF_BAR);
-  uint64_t* empty = full + MAX_STAGES;
-  uint64_t* tmem_full = empty + MAX_STAGES;
+  uint64_t* empty = full + STAGES;
+  uint64_t* tmem_full = empty + STAGES;
   uint64_t* tmem_empty = tmem_full + 2;
   uint64_t* tile_full = tmem_empty + 2;
   uint64_t* tile_empty = tile_full + TILES;
@@ -251,8 +240,10 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   cluster_arrive_release();  // this CTA has started
   if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmWs);
     tma_prefetch_desc(&tmXs);
-    for (int s = 0; s < MAX_STAGES; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -287,10 +278,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   cluster_wait_acquire();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int stages = tab.nsub == 2 ? 4 : 6;
-  // A stage: codes of the panel and the columns, scales of the panel and the columns.
-  const int a_bytes = tab.nsub * SUB, sf_off = a_bytes + B_BYTES, sfb_off = sf_off + tab.nsub * SCALES;
-  const int stage_bytes = sfb_off + 2 * SCALES;
   const int blocks = (g.pitch + 127) / 128;  // K-blocks
   // The i-th tile of this pair, for a whole warp; e is -1 after the last, and -2
   // where the wait for it ran out.
@@ -318,31 +305,29 @@ __global__ void __launch_bounds__(THREADS, 1)
         break;
       }
       const int half = x.width / 2, atoms = x.width > 128 ? 2 : 1;
-      const int a0 = x.a0 + (int)rank * 128 * x.nsub, row0 = x.begin + x.b0, b0 = row0 + (int)rank * half;
+      const int a0 = x.a0 + (int)rank * 128, row0 = x.begin + x.b0, b0 = row0 + (int)rank * half;
       const int w_tile = x.e * g.n_tiles + a0 / 128;  // (rows past N have no scales of their own: any, for zeros)
-      const CUtensorMap* codes = &tmW.codes[x.nsub - 1];
-      const CUtensorMap* scales = &tmW.scales[x.nsub - 1];
       int box = BOXES - 1;
 #pragma unroll
       for (int i = BOXES - 2; i >= 0; --i)
         if (half > box_rows(i + 1)) box = i;
       const CUtensorMap* columns = &tmX.box[box];
-      const uint32_t bytes = 2 * (x.nsub * (SUB + SCALES) + box_rows(box) * 128 + atoms * SCALES);
+      const uint32_t bytes = 2 * (SUB + SCALES + box_rows(box) * 128 + atoms * SCALES);
       for (int kb = 0; kb < blocks; ++kb) {
         ok = all_ok(mbar_wait(&empty[stage], phase ^ 1u, ctx, SITE_EMPTY));
         if (!ok) break;
         const uint32_t bar = full_leader0 + stage * 8u;
-        uint8_t* sA = smem + stage * stage_bytes;
+        uint8_t* sA = smem + stage * STAGE_BYTES;
         if (elect_one()) {
           if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
-          tma_load_3d_pair(sA, codes, bar, kb * 128, a0, x.e);
-          tma_load_3d_pair(sA + sf_off, scales, bar, 0, 2 * kb, w_tile);
-          tma_load_2d_pair(sA + a_bytes, columns, bar, kb * 128, b0);
-          tma_load_2d_pair(sA + sfb_off, &tmXs, bar, row0 * 8, 2 * kb);
-          if (atoms == 2) tma_load_2d_pair(sA + sfb_off + SCALES, &tmXs, bar, (row0 + 128) * 8, 2 * kb);
+          tma_load_3d_pair(sA, &tmW, bar, kb * 128, a0, x.e);
+          tma_load_3d_pair(sA + OFF_SFA, &tmWs, bar, 0, 2 * kb, w_tile);
+          tma_load_2d_pair(sA + SUB, columns, bar, kb * 128, b0);
+          tma_load_2d_pair(sA + OFF_SFB, &tmXs, bar, row0 * 8, 2 * kb);
+          if (atoms == 2) tma_load_2d_pair(sA + OFF_SFB + SCALES, &tmXs, bar, (row0 + 128) * 8, 2 * kb);
         }
         __syncwarp();
-        if (++stage == stages) {
+        if (++stage == STAGES) {
           stage = 0;
           phase ^= 1u;
         }
@@ -353,65 +338,48 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (leader) {
       int stage = 0;
       uint32_t phase = 0;
-      uint32_t halves = 0;  // accumulators used so far: slot = bit 0, phase = bit 1
       const uint32_t ring = smem_u32(smem);
       const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
-      // The MMAs of half `s` over the stage `at`, K-block kb.
-      auto issue = [&](const Tile& x, int s, int at, int kb, bool last) {
-        const uint32_t slot = (halves + s) & 1u;
-        if (kb == 0) {
-          if (!all_ok(mbar_wait(&tmem_empty[slot], ((halves + s) >> 1 & 1u) ^ 1u, ctx, SITE_TMEM_EMPTY))) return false;
-          tc_fence_after();
-        }
-        const uint32_t base = ring + at * stage_bytes;
-        const uint32_t d_tmem = tmem_u + slot * CAP;
-        const uint64_t a0 = umma_desc_sw128(base + s * SUB), b0 = umma_desc_sw128(base + a_bytes);
-        const uint64_t sfa0 = umma_desc(base + sf_off + s * SCALES, 16, 128, 0);
-        const uint64_t sfb0 = umma_desc(base + sfb_off, 16, 128, 0);
-        const uint32_t n_bits = (uint32_t)(x.width >> 3) << 17;
-        const uint32_t idesc0 = umma_idesc_mxf4(256, 0, 0) | n_bits, idesc2 = umma_idesc_mxf4(256, 0, 2) | n_bits;
-        const int bytes = g.pitch - kb * 128;  // of codes from here on
-        if (elect_one()) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (h * 64 >= bytes) break;  // no such run of 128 values
-            const uint32_t sfb = tmem_u + SF_COL + h * 16, sfa = sfb + 8;
-            tmem_cp_scales<2>(sfb, sfb0 + h * 32);  // 512 bytes on
-            if (x.width > 128) tmem_cp_scales<2>(sfb + 4, sfb0 + 64 + h * 32);
-            tmem_cp_scales<2>(sfa, sfa0 + h * 32);
-            umma_mxf4<2>(d_tmem, a0 + 4 * h, b0 + 4 * h, idesc0, sfa, sfb, h == 0 && kb == 0 ? 0u : 1u);
-            if (h * 64 + 32 < bytes) umma_mxf4<2>(d_tmem, a0 + 4 * h + 2, b0 + 4 * h + 2, idesc2, sfa, sfb, 1u);
-          }
-          if (s + 1 == x.nsub) umma_commit_cg2_mc(&empty[at], 0x3);  // the stage's last reader
-          if (last) umma_commit_cg2_mc(&tmem_full[slot], 0x3);
-        }
-        __syncwarp();
-        return true;
-      };
       for (int i = 0; ok; ++i) {
         const Tile x = next_tile(i);
         if (x.e < 0) {
           ok = x.e == -1;
           break;
         }
-        int before = 0;  // the stage of the K-block before
+        const uint32_t slot = i & 1, d_tmem = tmem_u + slot * CAP;
+        const uint32_t n_bits = (uint32_t)(x.width >> 3) << 17;
+        const uint32_t idesc0 = umma_idesc_mxf4(256, 0, 0) | n_bits, idesc2 = umma_idesc_mxf4(256, 0, 2) | n_bits;
+        ok = all_ok(mbar_wait(&tmem_empty[slot], (i >> 1 & 1) ^ 1u, ctx, SITE_TMEM_EMPTY));
+        if (!ok) break;
+        tc_fence_after();
         for (int kb = 0; kb < blocks; ++kb) {
           ok = all_ok(mbar_wait(&full[stage], phase, ctx, SITE_FULL));
           if (!ok) break;
           tc_fence_after();
-          const bool last = kb + 1 == blocks;
-          ok = issue(x, 0, stage, kb, last);
-          if (ok && x.nsub == 2 && kb > 0) ok = issue(x, 1, before, kb - 1, false);
-          if (ok && x.nsub == 2 && last) ok = issue(x, 1, stage, kb, true);
-          if (!ok) break;
-          before = stage;
+          const uint32_t base = ring + stage * STAGE_BYTES;
+          const uint64_t a0 = umma_desc_sw128(base), b0 = umma_desc_sw128(base + SUB);
+          const uint64_t sfa0 = umma_desc(base + OFF_SFA, 16, 128, 0), sfb0 = umma_desc(base + OFF_SFB, 16, 128, 0);
+          const int bytes = g.pitch - kb * 128;  // of codes from here on
+          if (elect_one()) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (h * 64 >= bytes) break;  // no such run of 128 values
+              const uint32_t sfb = tmem_u + SF_COL + h * 16, sfa = sfb + 8;
+              tmem_cp_scales<2>(sfb, sfb0 + h * 32);  // 512 bytes on
+              if (x.width > 128) tmem_cp_scales<2>(sfb + 4, sfb0 + 64 + h * 32);
+              tmem_cp_scales<2>(sfa, sfa0 + h * 32);
+              umma_mxf4<2>(d_tmem, a0 + 4 * h, b0 + 4 * h, idesc0, sfa, sfb, h == 0 && kb == 0 ? 0u : 1u);
+              if (h * 64 + 32 < bytes) umma_mxf4<2>(d_tmem, a0 + 4 * h + 2, b0 + 4 * h + 2, idesc2, sfa, sfb, 1u);
+            }
+            umma_commit_cg2_mc(&empty[stage], 0x3);
+            if (kb + 1 == blocks) umma_commit_cg2_mc(&tmem_full[slot], 0x3);
+          }
           __syncwarp();
-          if (++stage == stages) {
+          if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        halves += x.nsub;
       }
     }
   } else if (warp == EPILOGUE + 2) {
@@ -440,7 +408,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t* stage_c = reinterpret_cast<uint32_t*>(smem + OFF_C + (warp - 2) * RUN * 32 * 2);  // [RUN / 2 pairs][32]
     const uint32_t tmem_empty_leader0 = mapa_shared(smem_u32(&tmem_empty[0]), 0);
     const uint32_t t_quarter = tmem_base + ((uint32_t)(q * 32) << 16);
-    uint32_t halves = 0;
     for (int i = 0; ok; ++i) {
       const Tile x = next_tile(i);
       if (x.e < 0) {
@@ -449,94 +416,90 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       const int cols = x.width / 2;  // of this warp, a multiple of 8
       const int d0 = side * cols;    // its first column in the tile
-#pragma unroll 1
-      for (int s = 0; s < x.nsub; ++s) {
-        const uint32_t slot = halves & 1u, use = halves >> 1;
-        ++halves;
-        const int a_warp = x.a0 + ((int)rank * x.nsub + s) * 128 + q * 32;  // this warp's first row of the half
-        const float bias =
-            g.bias && a_warp + lane < g.N ? to_float(static_cast<const TO*>(g.bias)[a_warp + lane]) : 0.f;
-        ok = all_ok(mbar_wait(&tmem_full[slot], use & 1u, ctx, SITE_TMEM_FULL));
-        if (!ok) break;
-        tc_fence_after();
-        // Columns RUN c + 2 j and the next of this thread's row, as outputs (a
-        // last run is read whole; what is past it is not used).
-        uint32_t out[4][RUN / 2];
+      const uint32_t slot = i & 1;
+      const int a_warp = x.a0 + (int)rank * 128 + q * 32;  // this warp's first row
+      const float bias =
+          g.bias && a_warp + lane < g.N ? to_float(static_cast<const TO*>(g.bias)[a_warp + lane]) : 0.f;
+      ok = all_ok(mbar_wait(&tmem_full[slot], i >> 1 & 1, ctx, SITE_TMEM_FULL));
+      if (!ok) break;
+      tc_fence_after();
+      // Columns RUN c + 2 j and the next of this thread's row, as outputs (a
+      // last run is read whole; what is past it is not used).
+      uint32_t out[4][RUN / 2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c * RUN >= cols) break;
-          uint32_t v[RUN];
-          tmem_ld_32x32b_x32(t_quarter + slot * CAP + (uint32_t)(d0 + c * RUN), v);
-          tmem_ld_wait();
+      for (int c = 0; c < 4; ++c) {
+        if (c * RUN >= cols) break;
+        uint32_t v[RUN];
+        tmem_ld_32x32b_x32(t_quarter + slot * CAP + (uint32_t)(d0 + c * RUN), v);
+        tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < RUN / 2; ++j)
-            out[c][j] = pack2(TO(), __uint_as_float(v[2 * j]) + bias, __uint_as_float(v[2 * j + 1]) + bias);
-        }
-        // This warp's share read: hand it back to the MMA issuer.
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(tmem_empty_leader0 + slot * 8u);
-        if (a_warp >= g.N) continue;
+        for (int j = 0; j < RUN / 2; ++j)
+          out[c][j] = pack2(TO(), __uint_as_float(v[2 * j]) + bias, __uint_as_float(v[2 * j + 1]) + bias);
+      }
+      // This warp's share read: hand it back to the MMA issuer.
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tmem_empty_leader0 + slot * 8u);
+      if (a_warp >= g.N) continue;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int b = x.b0 + d0 + c * RUN;
-          const int n = min(min(RUN, cols - c * RUN), x.rows - b);  // columns to store
-          if (n <= 0) break;
-          uint16_t* y = static_cast<uint16_t*>(g.Y) + ((int64_t)x.begin + b) * g.ldy + a_warp;
-          if (g.vec_out && n == RUN) {
-            // Half a run at a time by TMA, staged in two buffers in turn.
-            uint16_t* b16 = reinterpret_cast<uint16_t*>(stage_c);
+      for (int c = 0; c < 4; ++c) {
+        const int b = x.b0 + d0 + c * RUN;
+        const int n = min(min(RUN, cols - c * RUN), x.rows - b);  // columns to store
+        if (n <= 0) break;
+        uint16_t* y = static_cast<uint16_t*>(g.Y) + ((int64_t)x.begin + b) * g.ldy + a_warp;
+        if (g.vec_out && n == RUN) {
+          // Half a run at a time by TMA, staged in two buffers in turn.
+          uint16_t* b16 = reinterpret_cast<uint16_t*>(stage_c);
 #pragma unroll
-            for (int u = 0; u < 2; ++u, b16 += RUN / 2 * 32) {
-              if (lane == 0) tma_store_wait_read<1>();  // the store that used this buffer has read it
-              __syncwarp();
-#pragma unroll
-              for (int j = 0; j < RUN / 4; ++j) {
-                const uint32_t two = out[c][u * (RUN / 4) + j];
-                b16[(2 * j) * 32 + lane] = (uint16_t)(two & 0xFFFFu);
-                b16[(2 * j + 1) * 32 + lane] = (uint16_t)(two >> 16);
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                tma_store_2d(&tmY, b16, a_warp, x.begin + b + u * (RUN / 2));
-                tma_store_commit();
-              }
-            }
-          } else if (g.vec_out) {
-            if (lane == 0) tma_store_wait_read<0>();
-            // Transposed through shared memory as pairs of columns: a lane reads 8
-            // rows of a pair and stores 16 bytes of each column.
-            __syncwarp();  // the run before has been read
-#pragma unroll
-            for (int j = 0; j < RUN / 2; ++j) stage_c[j * 32 + lane] = out[c][j];
+          for (int u = 0; u < 2; ++u, b16 += RUN / 2 * 32) {
+            if (lane == 0) tma_store_wait_read<1>();  // the store that used this buffer has read it
             __syncwarp();
-            const int a = lane % 4 * 8;
 #pragma unroll
-            for (int u = 0; u < RUN / 16; ++u) {
-              const int two = u * 8 + lane / 4;
-              const uint4 l = *reinterpret_cast<const uint4*>(stage_c + two * 32 + a);
-              const uint4 h = *reinterpret_cast<const uint4*>(stage_c + two * 32 + a + 4);
-              uint16_t* to = y + (2 * two) * g.ldy + a;
-              if (a_warp + a < g.N) {
-                if (2 * two < n)
-                  *reinterpret_cast<uint4*>(to) =
-                      make_uint4(__byte_perm(l.x, l.y, 0x5410), __byte_perm(l.z, l.w, 0x5410),
-                                 __byte_perm(h.x, h.y, 0x5410), __byte_perm(h.z, h.w, 0x5410));
-                if (2 * two + 1 < n)
-                  *reinterpret_cast<uint4*>(to + g.ldy) =
-                      make_uint4(__byte_perm(l.x, l.y, 0x7632), __byte_perm(l.z, l.w, 0x7632),
-                                 __byte_perm(h.x, h.y, 0x7632), __byte_perm(h.z, h.w, 0x7632));
-              }
+            for (int j = 0; j < RUN / 4; ++j) {
+              const uint32_t two = out[c][u * (RUN / 4) + j];
+              b16[(2 * j) * 32 + lane] = (uint16_t)(two & 0xFFFFu);
+              b16[(2 * j + 1) * 32 + lane] = (uint16_t)(two >> 16);
             }
-          } else if (a_warp + lane < g.N) {
-            // Rows of Y on odd boundaries: 64 bytes a column and warp.
-            y += lane;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmY, b16, a_warp, x.begin + b + u * (RUN / 2));
+              tma_store_commit();
+            }
+          }
+        } else if (g.vec_out) {
+          if (lane == 0) tma_store_wait_read<0>();
+          // Transposed through shared memory as pairs of columns: a lane reads 8
+          // rows of a pair and stores 16 bytes of each column.
+          __syncwarp();  // the run before has been read
 #pragma unroll
-            for (int j = 0; j < RUN / 2; ++j) {
-              if (2 * j < n) y[(2 * j) * g.ldy] = (uint16_t)(out[c][j] & 0xFFFFu);
-              if (2 * j + 1 < n) y[(2 * j + 1) * g.ldy] = (uint16_t)(out[c][j] >> 16);
+          for (int j = 0; j < RUN / 2; ++j) stage_c[j * 32 + lane] = out[c][j];
+          __syncwarp();
+          const int a = lane % 4 * 8;
+#pragma unroll
+          for (int u = 0; u < RUN / 16; ++u) {
+            const int two = u * 8 + lane / 4;
+            const uint4 l = *reinterpret_cast<const uint4*>(stage_c + two * 32 + a);
+            const uint4 h = *reinterpret_cast<const uint4*>(stage_c + two * 32 + a + 4);
+            uint16_t* to = y + (2 * two) * g.ldy + a;
+            if (a_warp + a < g.N) {
+              if (2 * two < n)
+                *reinterpret_cast<uint4*>(to) =
+                    make_uint4(__byte_perm(l.x, l.y, 0x5410), __byte_perm(l.z, l.w, 0x5410),
+                               __byte_perm(h.x, h.y, 0x5410), __byte_perm(h.z, h.w, 0x5410));
+              if (2 * two + 1 < n)
+                *reinterpret_cast<uint4*>(to + g.ldy) =
+                    make_uint4(__byte_perm(l.x, l.y, 0x7632), __byte_perm(l.z, l.w, 0x7632),
+                               __byte_perm(h.x, h.y, 0x7632), __byte_perm(h.z, h.w, 0x7632));
             }
+          }
+        } else if (a_warp + lane < g.N) {
+          // Rows of Y on odd boundaries: 64 bytes a column and warp.
+          y += lane;
+#pragma unroll
+          for (int j = 0; j < RUN / 2; ++j) {
+            if (2 * j < n) y[(2 * j) * g.ldy] = (uint16_t)(out[c][j] & 0xFFFFu);
+            if (2 * j + 1 < n) y[(2 * j + 1) * g.ldy] = (uint16_t)(out[c][j] >> 16);
           }
         }
       }
@@ -572,11 +535,9 @@ int launch(const F4Problem& p) {
   g.n_tiles = (int)((p.N + 127) / 128);
   g.Y = p.Y, g.ldy = p.ldy, g.bias = p.bias;
   g.pdl = pdl_enabled() ? 1 : 0;
-  PanelMaps tW;
   ColumnMaps tX;
-  CUtensorMap tXs;
-  for (int i = 0; i < 2; ++i)
-    if ((rc = f4_weight_map(p, 128 << i, &tW.codes[i])) || (rc = f4_weight_scale_map(p, 1 << i, &tW.scales[i]))) return rc;
+  CUtensorMap tW, tWs, tXs;
+  if ((rc = f4_weight_map(p, &tW)) || (rc = f4_weight_scale_map(p, &tWs))) return rc;
   for (int i = 0; i < BOXES; ++i)
     if ((rc = f4_token_map(p, box_rows(i), &tX.box[i]))) return rc;
   if ((rc = f4_token_scale_map(p, &tXs))) return rc;
@@ -612,7 +573,7 @@ int launch(const F4Problem& p) {
   if (err[di] != cudaSuccess) return cuda_fail(err[di], "cudaFuncSetAttribute(max dynamic smem)");
   const int pairs = (int)std::min<int64_t>(tiles, max_pairs[di]);
   PdlLaunch ln(dim3(2 * pairs), dim3(THREADS), smem, p.stream, 2);
-  const cudaError_t e = cudaLaunchKernelEx(&ln.cfg, kern, tW, tX, tXs, tY, (const F4Args)g);
+  const cudaError_t e = cudaLaunchKernelEx(&ln.cfg, kern, tW, tWs, tX, tXs, tY, (const F4Args)g);
   return e == cudaSuccess ? KEBAB_OK : cuda_fail(e, "4-bit tcgen05 launch");
 }
 }  // namespace
