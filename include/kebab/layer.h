@@ -7,9 +7,10 @@
  *   a[t, j, i] = g_i / (1 + exp(-g_i)) * u_i
  *   y[t, n] = sum_j w[t, j] sum_i w_out[e][n, i] a[t, j, i]
  *
- * for T <= KEBAB_FEW_TOKENS tokens of H values, E experts of D hidden values
- * and k choices a token. Logits, a and every sum are in FP32 (products with a
- * keep at least 16 bits of it), with one rounding to the output type.
+ * for T <= KEBAB_FEW_TOKENS tokens of H values, E <= 1024 experts of D hidden
+ * values and k <= 32 choices a token, H and D <= 2^20. Logits, a and every sum
+ * are in FP32 (products with a keep at least 16 bits of it), with one rounding
+ * to the output type.
  *
  * With experts in 8-bit integers (the codes and row scales of
  * kebab_quantize_i8, kebab/int8.h) x[t] and every a[t, j] are quantised by row
@@ -21,7 +22,9 @@
  * kebab_last_error() as in kebab.h. x and y are rows at a pitch; router [E, H]
  * (F32), w_in [E, 2 D, H] (gate rows, then up rows) and w_out [E, H, D] are
  * contiguous. An expert that no token chooses is not read, and what an expert
- * holds reaches the tokens that choose it only. T = 0 is a no-op. `workspace`
+ * holds reaches the tokens that choose it only. A call is two launches; all of
+ * the second's blocks (one a multiprocessor) are on the device at once, so it
+ * waits for room among kernels of other streams. T = 0 is a no-op. `workspace`
  * (16-byte aligned) holds kebab_expert_layer_workspace(T, E, k, H, D) bytes.
  * No counterpart in kebab.
  */

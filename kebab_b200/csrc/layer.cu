@@ -17,6 +17,10 @@
 // not used). The tokens, or the hidden values of the tokens that chose the
 // expert, are the 16 columns. A warp of its own copies the columns: at the grid
 // barrier only it waits, while the second matrices' rows arrive in the ring.
+// 1 token, 8 experts of H 2048 and D 1024 in BF16: 30 us (3.3 TB/s; 8 of them are
+// the logits and the second kernel's start, which cooperative launches do not
+// overlap); 13 tokens, 6 of 64 experts each, D 1272, F16: 162 us (4.5 TB/s); 5
+// tokens, 2 of 8 experts each, H 4096, D 8192, BF16: 222 us (5.5 TB/s).
 //
 // A token takes the products of its own experts only, from columns of its own:
 // what other experts or tokens hold (infinities, NaN) does not reach it.
@@ -55,7 +59,7 @@ constexpr int TAIL = 128 * 128;           // what an MMA may read past the ring:
 constexpr int RING = 200 * 1024;
 constexpr int SLOT = 40 * 1024;           // bytes of a slot, about
 constexpr int BLOCK = 32;                 // outputs that are added up together
-constexpr int COUNTING = 1 << 19;         // comparisons of keys, at most, to choose by counting
+constexpr int COUNTING = 2048;            // comparisons of keys a choice, at most, to choose by counting
 constexpr int TMEM_COLS = 64;             // two sets of 32
 
 struct LayerArgs {
@@ -70,7 +74,7 @@ struct LayerArgs {
   int T, E, k, H, D;
   int renormalize;
   int tma_w, tma_x;  // whether TMA can address the weights, x
-  int vec_x;         // rows of x on 16-byte boundaries
+  int vec_x;         // whether rows of x start on 16-byte boundaries
   const float* router;
   // The workspace.
   float* logits;      // [T][E]
@@ -274,8 +278,9 @@ static_assert(LayerSmem::bytes(MAX_TOKENS, MAX_K, kMaxExperts) <= 232448, "share
 // The passes of a CTA: its share [at, end) of active x per rows, cut at the
 // experts' ends and then in equal parts of at most `most`. Where the CTAs divide
 // among the experts with at most an eighth of them left over, no share crosses
-// from one expert to the next, which costs a pass more (1 token, 8 experts: such
-// CTAs were 12 us behind the others).
+// from one expert to the next, which costs a pass more: 2 experts of 4096 x 2048
+// 49 us, 43 without such shares, 8 98 and 94; from an eighth on what is left over
+// costs as much (26 experts, 0.12 of the CTAs: 248 and 249 us).
 // Made by whole warps; the shuffles tell the compiler that a warp's lanes have
 // the same values.
 struct Passes {
@@ -392,12 +397,15 @@ __global__ void __launch_bounds__(THREADS, 1)
   for (int i = threadIdx.x; i < g.E; i += THREADS) s_chose[i] = 0;
   if (g.pdl) pdl_wait();
   __syncthreads();
-  // Keys of the logits, in the ring. By counting where that is short: choice
-  // after choice, a token with 8 of them took 3.5 us, for the latency of each.
+  // Keys of the logits, in the ring. Choice after choice costs each one's latency,
+  // counting the comparisons of all pairs of experts (a whole call of 1 token, 64
+  // experts: of 16 choices 18.2 us against 16.2, of 8 16.0 against 15.2, of 2 15.1
+  // against 15.4; 256 experts, 8 choices: 19.3 against 21.2; 16 tokens, 128
+  // experts, 8 choices: 33.5 against 50.0).
   uint32_t* keys = reinterpret_cast<uint32_t*>(smem);
   for (int i = threadIdx.x; i < g.T * g.E; i += THREADS) keys[i] = order_key(__ldcg(g.logits + i));
   __syncthreads();
-  const bool counting = (int64_t)g.T * g.E * g.E <= COUNTING;
+  const bool counting = g.k >= 4 && g.T * g.E * g.E <= COUNTING * g.k;
   if (counting) {
     choose_by_counting(g, s_place, keys);
     __syncthreads();

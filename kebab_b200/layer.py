@@ -9,8 +9,11 @@ to FEW_TOKENS tokens that a serving step or a draft has. Nothing is copied to
 the host. All calls are asynchronous on `stream` (default: torch's current
 stream) and raise KebabError on a refusal.
 """
+import ctypes as c
+
 import torch
 
+from . import lib
 from ._call import CODES, bad, call, dense, elsewhere, on, pitch, tensor
 
 FEW_TOKENS = 16  # KEBAB_FEW_TOKENS
@@ -38,10 +41,10 @@ def _layer(what, x, router, w_in, in_scale, w_out, out_scale, k, renormalize, st
     if elsewhere(dev, stream):
         with on(dev, stream):
             return _layer(what, x, router, w_in, in_scale, w_out, out_scale, k, renormalize, None)
-    y = x.new_empty((T, H))
     size = workspace(T, E, k, H, D)
     if size < 0:
-        raise bad("%s: invalid dimensions H=%d D=%d" % (what, H, D))
+        raise bad("%s: invalid dimensions E=%d H=%d D=%d" % (what, E, H, D))
+    y = x.new_empty((T, H))
     ws = x.new_empty((size,), dtype=torch.uint8)
     weights = ((w_in.data_ptr(), in_scale.data_ptr(), w_out.data_ptr(), out_scale.data_ptr()) if i8 else
                (w_in.data_ptr(), w_out.data_ptr()))
@@ -50,12 +53,17 @@ def _layer(what, x, router, w_in, in_scale, w_out, out_scale, k, renormalize, st
     return y
 
 
+_workspace = None
+
+
 def workspace(T, E, k, H, D):
-    from . import lib
-    f = lib().kebab_expert_layer_workspace
-    import ctypes as c
-    f.argtypes, f.restype = [c.c_int64, c.c_int64, c.c_int, c.c_int64, c.c_int64], c.c_int64
-    return f(T, E, k, H, D)
+    """kebab_expert_layer_workspace: negative for sizes that a call refuses."""
+    global _workspace
+    if _workspace is None:
+        f = lib().kebab_expert_layer_workspace
+        f.argtypes, f.restype = [c.c_int64, c.c_int64, c.c_int, c.c_int64, c.c_int64], c.c_int64
+        _workspace = f
+    return _workspace(T, E, k, H, D)
 
 
 def expert_layer(x, router, w_in, w_out, k, renormalize=True, stream=None):
