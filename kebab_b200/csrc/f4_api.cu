@@ -54,7 +54,7 @@ int run(const char* what, const F4Problem& p) {
   if (p.ldy < p.N)
     return fail(KEBAB_EINVAL, std::string(what) + ": row pitch of Y (" + std::to_string(p.ldy) +
                                   ") is below its row length (" + std::to_string(p.N) + ")");
-  if (!p.w_codes || !p.w_scales || (p.R > 0 && (!p.x_codes || !p.x_scales || !p.Y)))
+  if (!p.w_codes || !p.w_scales || (p.R > 0 && ((!p.x && (!p.x_codes || !p.x_scales)) || !p.Y)))
     return fail(KEBAB_EINVAL, std::string(what) + ": null pointer");
   auto off16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) != 0; };
   if (off16(p.w_codes) || off16(p.w_scales) || off16(p.x_codes) || off16(p.x_scales))
@@ -122,6 +122,10 @@ int kebab_linear_f4(kebab_dtype dtype, const void* X, int64_t ldx, const uint8_t
     if (!workspace || workspace_bytes < kebab_linear_f4_workspace(M, K) ||
         (reinterpret_cast<uintptr_t>(workspace) & 15u))
       return fail(KEBAB_EINVAL, "linear_f4: the workspace is null, too small or not 16-byte aligned");
+    if (M <= F4_FUSED_ROWS) {
+      p.x = X, p.ldx = ldx, p.R = M;
+      return run(what, p);
+    }
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     uint8_t* scales = codes + kebab_f4_code_bytes(M, K);
     if ((rc = kebab_quantize_f4_tokens(dtype, X, ldx, codes, scales, M, K, stream))) return rc;

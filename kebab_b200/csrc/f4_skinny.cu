@@ -8,9 +8,9 @@
 // every other CTA the 128 / S of its rows that that one finishes (st.async,
 // counted on the receiver's barrier), and adds up its own rows over the S
 // partials in rank order. No workspace, no atomics, and the same bits every
-// time. With the quantisation, 1 row of 8192 x 8192 takes 10.8 us and 61 rows
-// 14.4 (3.3 and 2.6 TB/s): latency of the quantisation before it, of the first
-// copies and of the exchange. Several accumulators in turn gave nothing.
+// time. With the quantisation, 1 row of 8192 x 8192 takes 9.1 us and 61 rows
+// 14.4 (3.9 and 2.6 TB/s): latency of the quantisation, of the first copies and
+// of the exchange. Several accumulators in turn gave nothing.
 //
 // A K-block is 256 values: 128 bytes of codes a row, and two runs of 128 whose
 // scales (512 bytes for 128 rows, as they are stored) the issuer copies into
@@ -19,6 +19,8 @@
 //
 // In linear_f4 the kernel before this one only makes the codes and scales of X
 // (`early`): the first weights are fetched while it still runs.
+// Of up to 6 rows this kernel makes them itself (FUSED): 8 values a lane, eight
+// warps, some 300 cycles a row and K-block of a warp, while the weights arrive.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -27,7 +29,7 @@
 
 #include "f4.h"
 #include "gemm_umma.cuh"
-#include "vec.cuh"
+#include "quant_f4.cuh"
 
 namespace kb {
 namespace {
@@ -49,6 +51,9 @@ struct F4SkinnyArgs {
   int64_t ldy;
   const void* bias;
   int early, pdl;
+  const void* x;  // FUSED
+  int64_t ldx;
+  int K, vec_x;   // whether rows of x start on 16-byte boundaries
   WaitCtx ctx;
 };
 
@@ -120,7 +125,9 @@ __device__ bool nth_share(const F4SkinnyArgs& g, int nth, int& e, int& begin, in
   return rows > 0;
 }
 
-template <typename TO>
+// FUSED: the epilogue's warps, which have nothing else to do before the end, make
+// the codes and scales of X (of the output type) where TMA would place them.
+template <typename TO, bool FUSED>
 __global__ void __launch_bounds__(THREADS)
     f4_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmWs,
                      const __grid_constant__ RowMaps tmX, const __grid_constant__ CUtensorMap tmXs,
@@ -130,8 +137,9 @@ __global__ void __launch_bounds__(THREADS)
   // its successor start. The successor of others may start before this CTA has
   // allocated TMEM: beside its shared memory (launch) only another CTA of this
   // kernel fits, and their 256 columns each.
+  const bool late = FUSED && !g.offsets;  // nothing is read before the loads
   if (!early && g.pdl) {
-    pdl_wait();
+    if (!late) pdl_wait();
     pdl_launch_dependents();
   }
   int e, begin, rows;
@@ -145,7 +153,7 @@ __global__ void __launch_bounds__(THREADS)
   __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full, recv_full;
   __shared__ uint32_t tmem_slot;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int S = g.splits, kps = g.kps, stages = g.stages;
+  const int S = g.splits, kps = FUSED ? 2 : g.kps, stages = g.stages;  // (FUSED: at most 16 rows)
   const int width = (rows + 15) / 16 * 16;  // columns of the MMA
   // A stage: codes of W and X, scales of W and X, each kps K-blocks.
   const int w_bytes = kps * SUB, x_block = g.x_rows * 128, sf_bytes = w_bytes + kps * x_block;
@@ -159,7 +167,7 @@ __global__ void __launch_bounds__(THREADS)
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmW);
     for (int s = 0; s < stages; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], FUSED ? 1 + EPI : 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(&acc_full, 1);
@@ -177,6 +185,7 @@ __global__ void __launch_bounds__(THREADS)
   if (S > 1) cluster_arrive_release();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  if (late && g.pdl) pdl_wait();
 
   // This CTA's K-blocks, a multiple of kps but at the end.
   const int total = (g.pitch + 127) / 128;
@@ -185,12 +194,14 @@ __global__ void __launch_bounds__(THREADS)
   auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
   bool ok = true;  // of every wait of this warp
 
-  if (warp == 0 || warp == X_WARP) {
+  if (FUSED && warp == X_WARP) {
+    // (nothing to copy)
+  } else if (warp == 0 || warp == X_WARP) {
     // ---------------------------------------- producers: of W (warp 0), of X
     // (the last warp). One warp for both took 1.2 us longer to fill the ring. A stage's
     // bytes are all announced by the first; those of X may land before that.
     const bool of_w = warp == 0;
-    const uint32_t block_bytes = SUB + width * 128 + 2 * SCALES;
+    const uint32_t block_bytes = FUSED ? SUB + SCALES : SUB + width * 128 + 2 * SCALES;
     const int w_tile = e * g.n_tiles + n0 / 128;
     if (early && !of_w) pdl_wait();
     int stage = 0;
@@ -284,6 +295,65 @@ __global__ void __launch_bounds__(THREADS)
     const int et = threadIdx.x - 64;
     // Y may be what a kernel before the one that makes X's codes still reads.
     if (early) pdl_wait();
+    if constexpr (FUSED) {
+      // Rows and K-blocks of a stage in turn, 8 values a lane; four loads ahead.
+      const TO* x = static_cast<const TO*>(g.x) + (int64_t)begin * g.ldx;
+      const int w = warp - 2, steps = rows * kps;  // of a stage
+      int load_kb = kb0, load_i = w;
+      auto load = [&] {
+        Run<TO, 8> run = {};
+        if (load_kb >= kb1 || load_i >= steps) return run;
+        const int k = (load_kb + load_i % kps) * 256 + lane * 8;
+        const TO* from = x + (int64_t)(load_i / kps) * g.ldx;
+        if (g.vec_x && k + 8 <= g.K) {
+          run.load(from + k);
+        } else {
+          float v[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) v[u] = k + u < g.K ? to_float(from[k + u]) : 0.f;
+          run.set(v);
+        }
+        if ((load_i += EPI) >= steps) load_i = w, load_kb += kps;
+        return run;
+      };
+      constexpr int AHEAD = 4;
+      Run<TO, 8> next[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) next[u] = load();
+      int stage = 0, kb = kb0, i = w;
+      uint32_t phase = 1;
+      while (kb < kb1) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          if (kb >= kb1) break;
+          if (i == w) ok = all_ok(mbar_wait(&empty[stage], phase, ctx, SITE_EMPTY));
+          if (!ok) break;
+          uint8_t* base = smem + stage * stage_bytes;
+          const Run<TO, 8> run = next[u];
+          next[u] = load();
+          const EightCodes r = eight_codes(run, lane);
+          const int at = i / kps, q = i % kps;  // (of a last stage with less than kps: zeros that nothing reads)
+          if (i < steps) {
+            *reinterpret_cast<uint32_t*>(base + w_bytes + q * x_block + at * 128 + ((lane / 4 ^ (at & 7)) << 4) +
+                                         lane % 4 * 4) = r.codes;
+            if (lane % 16 == 0)
+              *reinterpret_cast<uint32_t*>(base + sf_bytes + (kps + q) * SCALES + lane / 16 * 512 + at * 16) = r.scales;
+          }
+          if ((i += EPI) < steps) continue;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[stage]);
+          __syncwarp();
+          i = w;
+          kb += kps;
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+      }
+    }
     if (S > 1) {
       // The barrier completes once every peer's rows have landed.
       if (threadIdx.x == 64) mbar_arrive_expect_tx(&recv_full, (uint32_t)((S - 1) * share * width * 4));
@@ -291,7 +361,7 @@ __global__ void __launch_bounds__(THREADS)
       cluster_wait_acquire();  // second half: the peers' barriers are set up
     }
     const bool some = kb1 > kb0;
-    ok = all_ok(!some || mbar_wait(&acc_full, 0, ctx, SITE_TMEM_FULL));
+    ok = all_ok(!some || mbar_wait(&acc_full, 0, ctx, SITE_TMEM_FULL)) && ok;
     tc_fence_after();
     if (S == 1) {
       const int n = n0 + row;
@@ -383,7 +453,7 @@ __global__ void __launch_bounds__(THREADS)
   }
 }
 
-template <typename TO>
+template <typename TO, bool FUSED>
 int launch(const F4Problem& p) {
   int rc;
   DeviceInfo* dev = nullptr;
@@ -397,9 +467,14 @@ int launch(const F4Problem& p) {
   g.Y = p.Y, g.ldy = p.ldy, g.bias = p.bias;
   g.pdl = pdl_enabled();
   g.early = p.early;
+  if (FUSED) {
+    g.x = p.x, g.ldx = p.ldx, g.K = (int)p.K;
+    g.vec_x = (reinterpret_cast<uintptr_t>(p.x) & 15u) == 0 && p.ldx % 8 == 0;
+  }
   CUtensorMap tW, tWs, tXs;
-  if ((rc = f4_weight_map(p, &tW)) || (rc = f4_weight_scale_map(p, &tWs)) || (rc = f4_token_scale_map(p, &tXs)))
-    return rc;
+  if ((rc = f4_weight_map(p, &tW)) || (rc = f4_weight_scale_map(p, &tWs))) return rc;
+  tXs = tW;  // not used if FUSED
+  if (!FUSED && (rc = f4_token_scale_map(p, &tXs))) return rc;
   // The boxes that the shares' widths are made of; of groups, whose sizes the
   // device knows, all.
   int boxes = 64 | 32 | 16;
@@ -411,12 +486,12 @@ int launch(const F4Problem& p) {
   RowMaps tX;
   for (int i = 0; i < 3; ++i) {
     tX.box[i] = tXs;  // not used
-    if ((boxes & (64 >> i)) && (rc = f4_token_map(p, 64 >> i, &tX.box[i]))) return rc;
+    if (!FUSED && (boxes & (64 >> i)) && (rc = f4_token_map(p, 64 >> i, &tX.box[i]))) return rc;
   }
   // Once per device and instantiation: the shared-memory opt-in, and how many
   // clusters of 2, 4 and 8 such CTAs the device holds at once (fewer than its
   // SMs would give: a cluster stays within a GPC).
-  auto kern = f4_skinny_kernel<TO>;
+  auto kern = f4_skinny_kernel<TO, FUSED>;
   constexpr int ONE_CTA = 221 * 1024;
   static std::once_flag once[64];
   static cudaError_t err[64];
@@ -458,7 +533,8 @@ int launch(const F4Problem& p) {
 }  // namespace
 
 int launch_f4_skinny(const F4Problem& p) {
-  return p.out == KEBAB_F16 ? launch<__half>(p) : launch<__nv_bfloat16>(p);
+  if (p.x) return p.out == KEBAB_F16 ? launch<__half, true>(p) : launch<__nv_bfloat16, true>(p);
+  return p.out == KEBAB_F16 ? launch<__half, false>(p) : launch<__nv_bfloat16, false>(p);
 }
 
 }  // namespace kb
