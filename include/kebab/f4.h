@@ -68,8 +68,8 @@ int kebab_gemm_grouped_f4(kebab_dtype out, const uint8_t* x_codes, const uint8_t
 
 /* Quantises X (M x K, F16 or BF16) and multiplies, Y of X's type. offsets NULL
  * (then E = 1): one weight matrix, bias optional; else grouped by expert, no
- * bias. `workspace` (16-byte aligned) holds the codes and scales of X:
- * kebab_linear_f4_workspace(M, K) bytes. */
+ * bias. Y may lie on X. `workspace` (16-byte aligned) holds the codes and scales
+ * of X: kebab_linear_f4_workspace(M, K) bytes. */
 int64_t kebab_linear_f4_workspace(int64_t M, int64_t K);
 int kebab_linear_f4(kebab_dtype dtype, const void* X, int64_t ldx, const uint8_t* w_codes, const uint8_t* w_scales,
                     const void* bias, void* Y, int64_t ldy, const int32_t* offsets, int64_t E, int64_t M, int64_t N,

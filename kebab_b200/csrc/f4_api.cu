@@ -122,7 +122,10 @@ int kebab_linear_f4(kebab_dtype dtype, const void* X, int64_t ldx, const uint8_t
     if (!workspace || workspace_bytes < kebab_linear_f4_workspace(M, K) ||
         (reinterpret_cast<uintptr_t>(workspace) & 15u))
       return fail(KEBAB_EINVAL, "linear_f4: the workspace is null, too small or not 16-byte aligned");
-    if (M <= F4_FUSED_ROWS) {
+    // (Where Y may lie on X, X is quantised before the product writes.)
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(X), y0 = reinterpret_cast<uintptr_t>(Y);
+    const bool apart = x0 >= y0 + 2 * ((M - 1) * ldy + N) || y0 >= x0 + 2 * ((M - 1) * ldx + K);
+    if (M <= F4_FUSED_ROWS && apart) {
       p.x = X, p.ldx = ldx, p.R = M;
       return run(what, p);
     }

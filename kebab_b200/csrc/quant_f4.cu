@@ -205,9 +205,9 @@ int quantize_any(int dtype, const QuantArgs& g, int64_t E, cudaStream_t s) {
 
 template <typename T>
 int dequantize(DequantArgs g, int64_t E, cudaStream_t stream) {
-  const int64_t spans = (g.K + 7 + 255) / 256;  // a granule may begin before the row
-  g.spans = std::max<int>(spans_of(g.rows * E, spans), (int)((spans + 65534) / 65535));
   const bool vec = (reinterpret_cast<uintptr_t>(g.W) & 15u) == 0 && g.K % 8 == 0;
+  const int64_t spans = (g.K + (vec ? 0 : 7) + 255) / 256;  // a granule may begin before the row
+  g.spans = std::max<int>(spans_of(g.rows * E, spans), (int)((spans + 65534) / 65535));
   PdlLaunch l(dim3((unsigned)((g.rows + WARPS - 1) / WARPS), (unsigned)((spans + g.spans - 1) / g.spans), (unsigned)E),
               dim3(THREADS), 0, stream);
   const cudaError_t e =

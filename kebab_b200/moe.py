@@ -16,9 +16,14 @@ experts e = e[t, j] that its router picks. `route`, `dispatch`, `combine` and
 `grouped_linear` below are the operators as functions with a first gradient; a
 second one raises (their backwards are calls that autograd does not see).
 Nothing is copied to the host in a step: the ragged sizes stay on the device.
+To capture a training step into a CUDA graph, warm up on a side stream and let go
+of every eager output and loss of the same parameters first: their accumulation
+nodes belong to the eager stream, and a captured backward pass that reaches them
+ends the process.
 
 `python -m kebab_b200.moe` trains a small layer on a synthetic task and then
-serves single tokens with its experts quantised.
+serves single tokens with its experts quantised; then two blocks, served in 16,
+8 and 4 bits.
 """
 import argparse
 import sys

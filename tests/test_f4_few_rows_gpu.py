@@ -57,6 +57,23 @@ def test_grouped(cuda, counts):
     assert torch.equal(Y[:rows], want[:rows]) and (Y[rows:] == 3).all()
 
 
+@pytest.mark.parametrize("M", [1, 4, 6, 7, 40])
+def test_output_on_the_input(cuda, M):
+    """Y in X's place, and beside X in the rows of one buffer."""
+    import torch
+    import kebab_b200 as kb
+    H = 1024
+    W = kb.quantize_f4(randn((H, H), torch.bfloat16, 1))
+    X = randn((M, H), torch.bfloat16, 2)
+    want = kb.linear_f4(X, W)
+    for _ in range(20):
+        Y = X.clone()
+        assert torch.equal(kb.linear_f4(Y, W, Y=Y), want)
+    both = torch.cat([X, X], 1)
+    kb.linear_f4(both[:, :H], W, Y=both[:, H:])
+    assert torch.equal(both[:, H:], want) and torch.equal(both[:, :H], X)
+
+
 def test_a_chain_of_layers(cuda):
     """Each call reads what the one before wrote, captured too: nothing starts on old rows."""
     import torch
