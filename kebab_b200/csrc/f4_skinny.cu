@@ -175,6 +175,8 @@ __global__ void __launch_bounds__(THREADS)
     fence_barrier_init();
   }
   __syncwarp();
+  // TMEM is not held while another kernel, which may share the SM, still needs some.
+  if (late && g.pdl) pdl_wait();
   if (warp == 1) {
     tmem_alloc<1>(&tmem_slot, TMEM_COLS);
     tmem_relinquish<1>();
@@ -185,7 +187,6 @@ __global__ void __launch_bounds__(THREADS)
   if (S > 1) cluster_arrive_release();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  if (late && g.pdl) pdl_wait();
 
   // This CTA's K-blocks, a multiple of kps but at the end.
   const int total = (g.pitch + 127) / 128;
