@@ -42,10 +42,11 @@ __device__ __forceinline__ void group_range(const int32_t* offsets, int e, int R
   count = max(hi - lo, 0);
 }
 
-int launch_grouped_simt(const GroupedProblem& p);
+int launch_grouped_simt(const GroupedProblem& p);    // 16 bits
+int launch_grouped_i8_any(const GroupedProblem& p);  // IN_I8, forward
 int launch_grouped_umma(const GroupedProblem& p);
 int launch_grouped_skinny(const GroupedProblem& p);
-// Whether TMA can address X and W (and dY): the others take the CUDA cores.
+// Whether TMA can address X and W (and dY).
 bool grouped_tma_ok(const GroupedProblem& p);
 
 // Runs the body of a C entry point; an exception (host memory) becomes a status.

@@ -54,7 +54,7 @@ int parse_mode(const char* what, const char* opmode, bool* kn) {
 // 100 rows of 64 experts 1024 x 1024 27.3 and 26.9.
 int run(const GroupedProblem& p) {
   // dw without rows has no operand for a tensor map; it only writes zeros.
-  if (p.R == 0 || !grouped_tma_ok(p)) return launch_grouped_simt(p);
+  if (p.R == 0 || !grouped_tma_ok(p)) return p.in == IN_I8 ? launch_grouped_i8_any(p) : launch_grouped_simt(p);
   if (p.dw) return launch_grouped_umma(p);
   DeviceInfo* dev = nullptr;
   const int rc = device_info(&dev);
@@ -69,6 +69,7 @@ int run_i8(int out, const int8_t* q, int64_t ldq, const float* scale, const int8
   GroupedProblem p = {};
   p.early = early;
   p.in = IN_I8, p.out = out;
+  if (R == 1) ldq = (K + 15) / 16 * 16;  // one row's pitch is not used
   p.X = q, p.ldx = ldq, p.W = Wq, p.ldw = ldw, p.w_stride = w_stride, p.Y = Y, p.ldy = ldy;
   p.offsets = offsets, p.E = E, p.R = R, p.N = N, p.K = K;
   p.scale = scale, p.w_scale = w_scale, p.bias = bias;

@@ -105,3 +105,36 @@ def test_waits_that_run_out(cuda, M, N, K):
     X, W = randn((M, K), torch.bfloat16, 1), kb.quantize_f4(randn((N, K), torch.bfloat16, 2))
     check_aborts(lambda: kb.linear_f4(X, W))
     check_aborts(lambda: kb.linear_grouped_f4(X, kb.F4(W.codes[None], W.scales[None]), offsets_of([M])))
+
+
+def test_several_streams(cuda):
+    """Few rows on four streams at once, between layers and norms: the same bits as alone."""
+    import torch
+    import kebab_b200 as kb
+    H, D, E = 1024, 512, 8
+    W = kb.quantize_f4(randn((H, H), torch.bfloat16, 1) * H ** -0.5)
+    stack = kb.quantize_f4(randn((3, H, H), torch.bfloat16, 2) * H ** -0.5)
+    router, w_in, w_out = randn((E, H), torch.float32, 3), randn((E, 2 * D, H), torch.bfloat16, 4) * 0.03, randn((E, H, D), torch.bfloat16, 5) * 0.04
+    w = torch.ones(H, device="cuda")
+    offsets = [offsets_of([0, M - M // 2, M // 2]) for M in range(7)]
+
+    def steps(x):
+        for _ in range(6):
+            x = kb.linear_f4(x, W)
+            x = kb.linear_grouped_f4(x, stack, offsets[len(x)])
+            x = kb.expert_layer(x, router, w_in, w_out, 2)
+            x = kb.rms_norm(x, w)[0]
+        return x
+
+    xs = [randn((M, H), torch.bfloat16, M) for M in (1, 2, 5, 6)]
+    want = [steps(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(5):
+        got = []
+        for x, s in zip(xs, streams):
+            with torch.cuda.stream(s):
+                got.append(steps(x))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
