@@ -35,7 +35,7 @@ def check_norm(x, w, r, y, s):
 
 
 SHAPES = [(1, 1), (1, 8192), (3, 7), (5, 64), (2, 4097), (300, 8192), (2000, 256), (1500, 1000), (1030, 1024), (700, 2048), (2, 20000),
-          (400, 16384), (400, 9000), (1100, 129), (301, 257)]
+          (400, 16384), (400, 9000), (1100, 129), (301, 257), (300, 8193), (300, 8200), (310, 8191), (300, 10239), (300, 10248)]
 
 
 @pytest.mark.parametrize("T,H", SHAPES)
@@ -49,7 +49,8 @@ def test_norm(cuda, T, H, dtype, weight, residual):
     check_norm(x, w, r, y, s)
 
 
-@pytest.mark.parametrize("T,H", [(1, 8192), (5, 64), (2, 4097), (300, 8192), (2000, 256), (1500, 1000), (2, 20000), (1100, 129)])
+@pytest.mark.parametrize("T,H", [(1, 8192), (5, 64), (2, 4097), (300, 8192), (2000, 256), (1500, 1000), (2, 20000), (1100, 129),
+                                 (300, 8200), (300, 8191), (300, 10240), (300, 10248), (300, 2501)])
 @pytest.mark.parametrize("dtype,weight", [("float16", "float32"), ("bfloat16", "bfloat16"), ("float32", "float32")])
 @pytest.mark.parametrize("residual,keep", [(False, False), (True, True)])
 def test_norm_i8(cuda, T, H, dtype, weight, residual, keep):
@@ -109,7 +110,7 @@ def check_backward(T, H, dtype, weight, with_ds, make=lambda t: t, seed=7):
 
 
 @pytest.mark.parametrize("T,H", [(1, 1), (1, 4096), (3, 7), (700, 1024), (1300, 2048), (200, 4096), (200, 8192), (40, 16384), (37, 20000),
-                                 (5, 40000), (200, 1001), (30, 4097), (9, 2049)])
+                                 (5, 40000), (200, 1001), (30, 4097), (9, 2049), (200, 8200), (200, 8191), (50, 12288), (50, 12281), (50, 12289)])
 @pytest.mark.parametrize("dtype,weight", [("float16", "float16"), ("bfloat16", "float32"), ("float32", "float32")])
 @pytest.mark.parametrize("with_ds", [False, True])
 def test_backward(cuda, T, H, dtype, weight, with_ds):
