@@ -15,7 +15,7 @@
 // the row side of tcgen05.mma (up to 128 rows; rows that the CTA does not own
 // are not loaded, and what the MMA reads in their place ends in rows that are
 // not used). The tokens, or the hidden values of the tokens that chose the
-// expert, are the 16 columns. A warp of its own copies the columns: at the grid
+// expert, are the columns, 8 or 16. A warp of its own copies the columns: at the grid
 // barrier only it waits, while the second matrices' rows arrive in the ring.
 // 1 token, 8 experts of H 2048 and D 1024 in BF16: 30 us (3.3 TB/s; 8 of them are
 // the logits and the second kernel's start, which cooperative launches do not
@@ -25,13 +25,15 @@
 // A token takes the products of its own experts only, from columns of its own:
 // what other experts or tokens hold (infinities, NaN) does not reach it.
 //
-// For 16-bit weights the hidden values enter the second product as the sum of
-// two 16-bit numbers, 16 columns each (at least 16 bits of them); F16 ones scaled
-// by the power of two that brings the largest of a choice's values to [2^13,
-// 2^14). For 8-bit weights they are codes of that largest value / 127. The
-// largest is found with atomic maxima, which do not depend on their order; it is
-// known at the grid barrier, after which every CTA converts its share, and all
-// meet once more. BF16 has FP32's range: its values are split as they are made.
+// For 16-bit weights the hidden values enter the second product as a sum of
+// 16-bit numbers, each with columns of its own. BF16 has FP32's range: its values are split as
+// they are made, into three numbers of 8 bits, which are all of FP32's 24. F16 ones
+// are scaled by the power of two that brings the largest of a choice's values to
+// [2^13, 2^14), and are sums of two numbers (22 bits, or 2^-38 of that largest; a
+// rounding that F16 outputs, of 11 bits, do not show). For 8-bit weights they are
+// codes of the largest value / 127. The largest is found with atomic maxima, which
+// do not depend on their order; it is known at the grid barrier, after which every
+// CTA converts its share, and all meet once more.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -53,14 +55,12 @@ constexpr int MAX_TOKENS = KEBAB_FEW_TOKENS, MAX_K = 32;
 // four for the epilogue.
 constexpr int THREADS = 256, EPI_WARP = 4;
 constexpr int ROWS = 128;                 // weight rows of a pass
-constexpr int COLUMNS = 16 * 128;         // bytes of 16 columns of a K-block
 constexpr int MAX_SLOTS = 16, MAX_UNITS = 8;
 constexpr int TAIL = 128 * 128;           // what an MMA may read past the ring: the tables lie there
 constexpr int RING = 200 * 1024;
 constexpr int SLOT = 40 * 1024;           // bytes of a slot, about
 constexpr int BLOCK = 32;                 // outputs that are added up together
 constexpr int COUNTING = 2048;            // comparisons of keys a choice, at most, to choose by counting
-constexpr int TMEM_COLS = 64;             // two sets of 32
 
 struct LayerArgs {
   const void* x;
@@ -79,7 +79,7 @@ struct LayerArgs {
   // The workspace.
   float* logits;      // [T][E]
   float* hidden;      // [T k][D] by expert and token, not BF16
-  uint8_t* operand;   // [2][T k][d_bytes]: the rounded values, the rest; or [T k][d_bytes] codes
+  uint8_t* operand;   // [parts][T k][d_bytes]: the numbers that add up to the values; or their codes
   int d_bytes;
   uint32_t* top;      // [T k]: bits of the largest |hidden|, not BF16
   float* out;         // [T k][out_pitch]: weighted outputs of the choices
@@ -182,7 +182,12 @@ __global__ void __launch_bounds__(256) layer_logits_kernel(const LayerArgs g) {
 
 // -------------------------------------------------------------------- layer
 
-// Whether hidden values are stored as two numbers of the weights' type: BF16 has
+// How many operands a hidden value makes.
+template <typename TX, bool I8>
+constexpr int parts_of() {
+  return I8 ? 1 : std::is_same<TX, __nv_bfloat16>::value ? 3 : 2;
+}
+// Whether hidden values are stored as numbers of the weights' type: BF16 has
 // FP32's range, F16 needs a scale that is known only when all of them are.
 template <typename TX, bool I8>
 constexpr bool is_split() {
@@ -328,7 +333,8 @@ struct Product {
   static constexpr bool kUp = UP;
   static constexpr int MATRICES = UP ? 2 : 1, MOST = ROWS / MATRICES;
   static constexpr int OPERANDS = UP ? 1 : PARTS;
-  static constexpr int COLUMN_BYTES = OPERANDS * COLUMNS;
+  // Columns of the MMA, a multiple of 16, of operands of `box` each.
+  static __device__ __forceinline__ int columns(int box) { return (OPERANDS * box + 15) / 16 * 16; }
 };
 
 // How a pass lies in the ring: units of `bytes` (the matrices' rows, r8 each, then
@@ -336,9 +342,9 @@ struct Product {
 struct Layout {
   int r8, bytes, units;
   template <typename P>
-  __device__ __forceinline__ Layout(P, int rows, int slot) {
+  __device__ __forceinline__ Layout(P, int rows, int box, int slot) {
     r8 = (rows + 7) / 8 * 8;
-    bytes = P::MATRICES * r8 * 128 + P::COLUMN_BYTES;
+    bytes = (P::MATRICES * r8 + P::columns(box)) * 128;
     units = min(MAX_UNITS, slot / bytes);
   }
 };
@@ -349,7 +355,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                  const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmH, const LayerArgs g) {
   constexpr int ES = I8 ? 1 : 2;              // bytes of a weight
   constexpr int EPB = 128 / ES;               // values of a K-block
-  constexpr int PARTS = I8 ? 1 : 2;           // operands that a hidden value makes
+  constexpr int PARTS = parts_of<TX, I8>();
+  constexpr int SET_COLS = PARTS == 3 ? 64 : 32, TMEM_COLS = 2 * SET_COLS;  // two sets of accumulators
   constexpr bool SPLIT = is_split<TX, I8>();  // made in the first product's epilogue
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -475,6 +482,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem = *tmem_slot;
   const int active = __shfl_sync(0xffffffffu, *s_count, 0);
 
+  const int box = g.T <= 8 ? 8 : 16;  // columns of an operand
   // The ring's slots, by the longest pass that there can be.
   using Up = Product<true, PARTS>;
   using Down = Product<false, PARTS>;
@@ -483,7 +491,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int each = gridDim.x / active;  // CTAs of an expert (Passes)
     const int rows = each ? (per + each - 1) / each : (active * per + (int)gridDim.x - 1) / (int)gridDim.x;
     const int share = min(P::MOST, rows);
-    return P::MATRICES * ((share + 7) / 8 * 8) * 128 + P::COLUMN_BYTES;
+    return (P::MATRICES * ((share + 7) / 8 * 8) + P::columns(box)) * 128;
   };
   const int unit_bytes = max(longest(Up(), g.D), longest(Down(), g.H));
   const int slot_bytes = unit_bytes * max(1, min(MAX_UNITS, SLOT / unit_bytes));
@@ -493,7 +501,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   Passes first_up(active, g.D, Up::MOST);
   const bool any_up = first_up.next();
   const int up_blocks = (g.H + EPB - 1) / EPB, down_blocks = (g.D + EPB - 1) / EPB;
-  const int box = g.T <= 8 ? 8 : 16;  // columns that are loaded
   auto all_ok = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
   bool ok = true;
   int slot = 0;
@@ -546,7 +553,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto copy = [&](auto product, Passes p, bool more, const RowBoxes& tm, const void* w, int per, int cols, int blocks) {
       using P = decltype(product);
       for (; ok && more; more = p.next()) {
-        const Layout l(product, p.rows, slot_bytes);
+        const Layout l(product, p.rows, box, slot_bytes);
         const int e = __shfl_sync(0xffffffffu, s_active[p.a], 0);
         const int row = P::kUp ? which * per + p.first : p.first;
         const int low = min(l.r8, 64), high = l.r8 - low;
@@ -591,7 +598,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto copy = [&](auto product, Passes p, bool more, int blocks) {
       using P = decltype(product);
       for (; ok && more; more = p.next()) {
-        const Layout l(product, p.rows, slot_bytes);
+        const Layout l(product, p.rows, box, slot_bytes);
         const int base = __shfl_sync(0xffffffffu, (int)s_base[p.a], 0);
         for (int kb = 0; kb < blocks; kb += l.units) {
           ok = all_ok(mbar_wait(&empty[slot], phase ^ 1u, ctx, SITE_EMPTY));
@@ -622,13 +629,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int q = 0; q < n; ++q, dst += l.bytes) {
               const int k0 = (kb + q) * EPB;
               if (elect_one()) {
-                if constexpr (P::kUp) {
-                  tma_load_2d(dst, &tmX, &full[slot], k0, 0);
-                } else {
-#pragma unroll
-                  for (int part = 0; part < PARTS; ++part)
-                    tma_load_3d(dst + part * COLUMNS, &tmH, &full[slot], k0, base, part);
-                }
+                if constexpr (P::kUp) tma_load_2d(dst, &tmX, &full[slot], k0, 0);
+                else tma_load_3d(dst, &tmH, &full[slot], k0, base, 0);
               }
               __syncwarp();
             }
@@ -647,11 +649,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t pass = 0;
     auto multiply = [&](auto product, Passes p, bool more, int blocks) {
       using P = decltype(product);
-      constexpr int N = P::OPERANDS * 16;
-      constexpr uint32_t IDESC = I8 ? umma_idesc_i8(128, N) : umma_idesc_f16(128, N, ElemTraits<TX>::kBf16);
+      const uint32_t idesc = (I8 ? umma_idesc_i8(128, 0) : umma_idesc_f16(128, 0, ElemTraits<TX>::kBf16)) |
+                             (uint32_t)(P::columns(box) >> 3) << 17;
       for (; ok && more; more = p.next()) {
-        const Layout l(product, p.rows, slot_bytes);
-        const uint32_t set = pass & 1u, d_tmem = d0 + set * 32;
+        const Layout l(product, p.rows, box, slot_bytes);
+        const uint32_t set = pass & 1u, d_tmem = d0 + set * SET_COLS;
         ok = all_ok(mbar_wait(&acc_empty[set], (pass >> 1 & 1u) ^ 1u, ctx, SITE_TMEM_EMPTY));
         tc_fence_after();
         for (int kb = 0; ok && kb < blocks; kb += l.units) {
@@ -667,8 +669,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                if constexpr (I8) umma_i8<1>(d_tmem, a + k * 2, b + k * 2, IDESC, k == 0 ? first : 1u);
-                else umma_f16_cg1(d_tmem, a + k * 2, b + k * 2, IDESC, k == 0 ? first : 1u);
+                if constexpr (I8) umma_i8<1>(d_tmem, a + k * 2, b + k * 2, idesc, k == 0 ? first : 1u);
+                else umma_f16_cg1(d_tmem, a + k * 2, b + k * 2, idesc, k == 0 ? first : 1u);
               }
             }
             __syncwarp();
@@ -703,13 +705,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (et == 0) asm volatile("fence.acq_rel.gpu;\n\tred.relaxed.gpu.global.add.u32 [%0], 1;" ::"l"(count) : "memory");
     };
     uint32_t pass = 0;
-    // The accumulators of the next pass.
-    uint32_t v[32];
-    auto take = [&] {
+    // The accumulators of the next pass: of the first 32 columns, and `more`, of the third 16.
+    uint32_t v[32], v3[16];
+    auto take = [&](bool more) {
       const uint32_t set = pass & 1u;
       if (ok) ok = all_ok(mbar_wait(&acc_full[set], pass >> 1 & 1u, ctx, SITE_TMEM_FULL));
       tc_fence_after();
-      tmem_ld_32x32b_x32(quarter + set * 32, v);
+      tmem_ld_32x32b_x32(quarter + set * SET_COLS, v);
+      if (PARTS == 3 && more) tmem_ld_32x32b_x16(quarter + set * SET_COLS + 32, v3);
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
@@ -731,7 +734,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         const uint32_t who = s_who[p.a];
         int place = s_base[p.a];
-        take();
+        take(false);
         // The up rows are the threads from r8 on. Through shared memory, and then
         // token by token in a loop: unrolled, one token's values took 4 us, for
         // the instructions that are fetched on the way.
@@ -754,12 +757,17 @@ __global__ void __launch_bounds__(THREADS, 1)
           const float h = gate / (1.f + expf(-gate)) * value;
           if constexpr (SPLIT) {
             if (mine && ok) {
-              TX* to = reinterpret_cast<TX*>(g.operand + (int64_t)place * g.d_bytes) + i;
-              const TX hi = from_float<TX>(h);
-              // What the rounding left; of an infinity nothing.
-              const TX lo = from_float<TX>(isinf(to_float(hi)) ? 0.f : h - to_float(hi));
-              *to = hi;
-              *reinterpret_cast<TX*>(reinterpret_cast<uint8_t*>(to) + (int64_t)choices * g.d_bytes) = lo;
+              // Cut after eight bits, not rounded: what is left is exact, and the largest
+              // values stay finite. Of an infinity or a NaN nothing is left.
+              uint8_t* to = g.operand + (int64_t)place * g.d_bytes + (int64_t)i * 2;
+              const bool finite = abs_bits(h) < 0x7f800000u;
+              float rest = h;
+#pragma unroll
+              for (int part = 0; part < PARTS; ++part, to += (int64_t)choices * g.d_bytes) {
+                const float cut = finite ? __uint_as_float(__float_as_uint(rest) & 0xffff0000u) : rest;
+                *reinterpret_cast<TX*>(to) = from_float<TX>(cut);
+                rest = finite ? rest - cut : 0.f;
+              }
             }
           } else {
             if (mine && ok) g.hidden[(int64_t)place * g.D + i] = h;
@@ -830,12 +838,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool mine = et < p.rows;
       float scale = 1.f;
       if constexpr (I8) scale = mine ? g.out_scale[(int64_t)s_active[p.a] * g.H + r] : 0.f;
-      take();
+      take(box == 16);
 #pragma unroll
       for (int c = 0; c < MAX_TOKENS; ++c) {
         if (c >= n) break;
         float o = number(v[c]);
-        if constexpr (PARTS == 2) o += number(v[16 + c]);
+        if constexpr (PARTS == 2) o += number(box == 16 ? v[16 + c] : v[8 + c % 8]);
+        if constexpr (PARTS == 3) o += box == 16 ? number(v3[c]) + number(v[16 + c]) : number(v[16 + c % 8]) + number(v[8 + c % 8]);
         if (mine) g.out[(int64_t)(base + c) * g.out_pitch + r] = s_factor[base + c] * scale * o;
       }
       __threadfence();
@@ -912,7 +921,7 @@ struct Workspace {
     const int64_t n = s.T * s.k;
     logits = take(s.T * s.E * 4);
     hidden = take(n * s.D * 4);
-    operand = take(2 * n * up16(2 * s.D));
+    operand = take(3 * n * up16(2 * s.D));
     top = take(n * 4);
     out = take(n * up16(s.H) * 4);
     done = take((s.H + BLOCK - 1) / BLOCK * 4);
@@ -978,8 +987,8 @@ int launch(int dtype, LayerArgs& g, cudaStream_t stream) {
   }
   {
     const uint64_t n = (uint64_t)g.T * g.k;
-    const uint64_t dims[3] = {(uint64_t)g.D, n, I8 ? 1u : 2u}, strides[2] = {(uint64_t)g.d_bytes, n * g.d_bytes};
-    const uint32_t box[3] = {128 / ES, columns, 1};
+    const uint64_t dims[3] = {(uint64_t)g.D, n, (uint64_t)parts_of<TX, I8>()}, strides[2] = {(uint64_t)g.d_bytes, n * g.d_bytes};
+    const uint32_t box[3] = {128 / ES, columns, (uint32_t)parts_of<TX, I8>()};
     if ((rc = make_tmap(&th, g.operand, type, 3, dims, strides, box, 128))) return rc;
   }
   auto kern = layer_kernel<TX, I8>;

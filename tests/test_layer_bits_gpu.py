@@ -1,0 +1,48 @@
+"""How much of a hidden value few-token layers keep, on whole numbers whose sums are exact."""
+import pytest
+
+from operator_util import dtype_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("T", [1, 5, 16])
+def test_hidden_values_keep_their_bits(cuda, T, dtype):
+    """Hidden values of 21 bits, pairs of which differ in the last seven: their differences are the outputs. Every
+    product, sum and difference is a whole number of 2^-14 below 2^21 of them, exact in FP32 and (seven bits) in the
+    output's type; silu(32) is 32 in FP32."""
+    import torch
+    import kebab_b200 as kb
+    H, D, dt = 64, 96, dtype_of(dtype)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(T)
+    digits = torch.randint(64, 128, (D, 3), generator=g, device="cuda").double()
+    digits[1::2, :2] = digits[::2, :2]  # a pair differs in the last digit
+    x = torch.zeros((T, H), device="cuda")
+    x[:, 0], x[:, 1], x[:, 2] = 1, 2.0 ** -7, 2.0 ** -14
+    w_in = torch.zeros((1, 2 * D, H), device="cuda")
+    w_in[0, :D, 0] = 32
+    w_in[0, D:, :3] = digits.float()
+    w_out = torch.zeros((1, H, D), device="cuda")
+    n = torch.arange(H, device="cuda") % (D // 2)
+    w_out[0, torch.arange(H), 2 * n], w_out[0, torch.arange(H), 2 * n + 1] = 1, -1
+    y = kb.expert_layer(x.to(dt), torch.zeros((1, H), device="cuda"), w_in.to(dt), w_out.to(dt), 1)
+    want = 32 * 2.0 ** -14 * (digits[::2, 2] - digits[1::2, 2])[n].expand(T, H)
+    assert torch.equal(y.double(), want)
+
+
+def test_hidden_values_up_to_the_largest(cuda):
+    """A hidden value between the largest of BF16 and that of FP32, brought back by a small weight: 2^128 (1 - 2^-11)
+    times 2^-120, rounded once."""
+    import torch
+    import kebab_b200 as kb
+    x = torch.zeros((2, 64), device="cuda")
+    x[:, :2] = 2.0 ** 32
+    w_in = torch.zeros((1, 16, 64), device="cuda")
+    w_in[0, 0, 0] = 2.0 ** 32
+    w_in[0, 8, 0], w_in[0, 8, 1] = 2.0 ** 32, -2.0 ** 21
+    w_out = torch.zeros((1, 64, 8), device="cuda")
+    w_out[0, :, 0] = 2.0 ** -120
+    y = kb.expert_layer(x.bfloat16(), torch.zeros((1, 64), device="cuda"), w_in.bfloat16(), w_out.bfloat16(), 1)
+    assert torch.equal(y, torch.full_like(y, 256.0))
