@@ -11,6 +11,8 @@
  * values and k <= 32 choices a token, H and D <= 2^20. Logits, a and every sum
  * are in FP32, with one rounding to the output type. Products with a take all of
  * its 24 bits (F16: 22, or 2^-38 of the largest a[t, j, i] of a choice).
+ * The matrix units add up to 512 terms of a sum (their additions cut off bits),
+ * the rest is added to nearest.
  *
  * With experts in 8-bit integers (the codes and row scales of
  * kebab_quantize_i8, kebab/int8.h) x[t] and every a[t, j] are quantised by row
