@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(256) layer_logits_kernel(const LayerArgs g) {
   const T* x = static_cast<const T*>(g.x);
   if (blockIdx.x >= g.E) {
     // Codes of a token, nearest to 127 x / amax, ties to even. Of 16-bit values
-    // the product is exact and the quotient distinguishes ties from others.
+    // the product is exact and the quotient distinguishes ties from others. (Both
+    // by 2^-8 for rows that the product by 127 would bring beyond FP32.)
     const int t = blockIdx.x - g.E;
     x += t * g.ldx;
     uint32_t top = 0;
@@ -129,10 +130,10 @@ __global__ void __launch_bounds__(256) layer_logits_kernel(const LayerArgs g) {
 #pragma unroll
     for (int w = 0; w < 8; ++w) top = max(top, tops[w]);
     const RowScale s = row_scale(top);
-    const float amax = __uint_as_float(top);
+    const float down = __uint_as_float(top) > 0x1p100f ? 0x1p-8f : 1.f, amax = __uint_as_float(top) * down;
     int8_t* q = g.x_codes + (int64_t)t * g.x_pitch;
     for (int h = threadIdx.x; h < g.x_pitch; h += 256)
-      q[h] = h < g.H && s.inv != 0.f ? (int8_t)__float2int_rn(to_float(x[h]) * 127.f / amax) : 0;
+      q[h] = h < g.H && s.inv != 0.f ? (int8_t)__float2int_rn(to_float(x[h]) * down * 127.f / amax) : 0;
     if (threadIdx.x == 0) g.x_scale[t] = s.scale;
     return;
   }

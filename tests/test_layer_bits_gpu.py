@@ -108,3 +108,21 @@ def test_long_sums_of_the_second_product(cuda, T, dtype):
     want = (S + out[:, 0]).expand(T, H)
     # The run with the first number loses of S, the others of their own sums.
     assert_within(y, want, 2 * LOST * S + UNIT[dtype] * (want.abs() + 2 * LOST * S))
+
+
+def test_codes_of_the_largest_tokens(cuda):
+    """Rows of x whose largest value times 127 is beyond FP32, against 64 bits; the weights' scales bring the hidden
+    values back to ordinary ones."""
+    import torch
+    import kebab_b200 as kb
+    from test_layer_gpu import make, reference
+    x, router, w_in, w_out = make(6, 1, 256, 64, "bfloat16", 9)
+    top = torch.tensor([torch.finfo(torch.bfloat16).max, 2.0 ** 127, 2.8e36, 2.6e36, 2.0 ** 100, 2.0 ** 121], device="cuda")
+    x = (x.float() / x.float().abs().amax(1, keepdim=True) * top[:, None]).clamp(-top[0], top[0]).bfloat16()
+    assert torch.isfinite(x).all()
+    (qi, si), (qo, so) = kb.quantize_i8(w_in), kb.quantize_i8(w_out)
+    si = si * 2.0 ** -120
+    y = kb.expert_layer_i8(x, router * 0, qi, si, qo, so, 1)
+    want, bound = reference(x, router * 0, qi, qo, 1, True, (si, so))
+    assert (want.abs().amax(1)[:4] > 2.0 ** -12).all()
+    assert_within(y, want, bound)
