@@ -6,11 +6,14 @@
 // a row are cut from two aligned granules (selects and four funnel shifts) and
 // stored where TMA would place them; the next K-block's are in flight while this
 // one's are multiplied. Pieces whose granules reach past an operand's ends are
-// copied byte by byte, and bytes past K are zeros. Sums are exact in 32 bits, so that the results are those
-// of the other 8-bit kernels. Bound by the copies' instructions, with few warps to
-// hide their latency: 1 row of 4096 x 4100 38 us, 4096 rows 205, 4093 x 1024 x 1000
-// 26; rows on 16 bytes, by TMA, take 6, 64 and 11. (Pieces away from an operand's
-// ends take a path without conditions: with one for each, 68, 327 and 30.)
+// copied byte by byte, and bytes past K are zeros. Sums are exact in 32 bits, so
+// that the results are those of the other 8-bit kernels. Bound by the copies'
+// instructions, with few warps to hide their latency: 1 row of 4096 x 4100 38 us,
+// 4096 rows 205, 4093 x 1024 x 1000 26; rows on 16 bytes, by TMA, take 6, 64 and
+// 11. (Pieces away from an operand's ends take a path without conditions: with one
+// for each, 68, 327 and 30.) All threads look for the block's group together: 1021
+// rows of 1024 experts, 512 x 301, 111 us (one after the other 1637), of 256
+// experts, 1024 x 1001, 112 (255).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -18,6 +21,7 @@
 #include <mutex>
 
 #include "gemm_umma.cuh"
+#include "group_search.cuh"
 #include "grouped.h"
 #include "vec.cuh"
 
@@ -72,16 +76,8 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_i8_any_kernel(const AnyArg
     pdl_launch_dependents();
   }
   const int n0 = (int)(blockIdx.x % g.n_tiles) * TILE;
-  int tile = blockIdx.x / g.n_tiles, e = 0, begin, rows;
-  for (;; ++e) {
-    if (e >= g.E) return;
-    group_range(g.offsets, e, g.R, begin, rows);
-    const int t = (rows + TILE - 1) / TILE;
-    if (tile < t) break;
-    tile -= t;
-  }
-  begin += tile * TILE;
-  rows = min(TILE, rows - tile * TILE);
+  int e, begin, rows;
+  if (!nth_share<THREADS, TILE>(g.offsets, g.E, g.R, (int)(blockIdx.x / g.n_tiles), e, begin, rows)) return;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);

@@ -23,6 +23,7 @@
 #include <mutex>
 
 #include "gemm_umma.cuh"
+#include "group_search.cuh"
 #include "grouped.h"
 #include "vec.cuh"
 
@@ -54,69 +55,6 @@ struct RowMaps {
   CUtensorMap box[3];
 };
 
-// 16 bytes into a peer's shared memory; the bytes count towards the peer's
-// mbarrier (both given as shared::cluster addresses).
-__device__ __forceinline__ void send16(uint32_t dst, uint32_t bar, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(dst),
-               "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar)
-               : "memory");
-}
-
-// Rows begin .. begin + rows - 1 of group e: the `nth` of the shares (of at most
-// MAX_WIDTH rows) of all groups, by all threads of the block; false if there
-// are fewer.
-__device__ bool nth_share(const SkinnyArgs& g, int nth, int& e, int& begin, int& rows) {
-  __shared__ int s_count[THREADS / 32], s_found[4];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int at = nth;  // the share within its group
-  if (g.offsets == nullptr) {
-    e = 0;
-    begin = 0;
-    rows = g.R;
-  } else {
-    if (threadIdx.x == 0) s_found[0] = -1;
-    int before = 0;
-    for (int e0 = 0; e0 < g.E; e0 += THREADS) {
-      int b = 0, n = 0;
-      if (e0 + (int)threadIdx.x < g.E) group_range(g.offsets, e0 + threadIdx.x, g.R, b, n);
-      const int shares = (n + MAX_WIDTH - 1) / MAX_WIDTH;
-      int sum = shares;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, sum, d);
-        if (lane >= d) sum += up;
-      }
-      if (lane == 31) s_count[warp] = sum;
-      __syncthreads();
-      int first = before + sum - shares;
-#pragma unroll
-      for (int w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) first += s_count[w];
-        before += s_count[w];
-      }
-      if (first <= nth && nth < first + shares) {
-        s_found[0] = e0 + threadIdx.x;
-        s_found[1] = b;
-        s_found[2] = n;
-        s_found[3] = nth - first;
-      }
-      __syncthreads();
-      if (before > nth) break;
-    }
-    e = s_found[0];
-    if (e < 0) return false;
-    begin = s_found[1];
-    rows = s_found[2];
-    at = s_found[3];
-  }
-  const int shares = (rows + MAX_WIDTH - 1) / MAX_WIDTH;
-  if (at >= shares) return false;
-  const int share = (rows + shares - 1) / shares;
-  begin += at * share;
-  rows = min(share, rows - at * share);
-  return rows > 0;
-}
-
 template <typename TO, bool I8, bool RR>
 __global__ void __launch_bounds__(THREADS)
     grouped_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ RowMaps tmX,
@@ -134,7 +72,7 @@ __global__ void __launch_bounds__(THREADS)
     pdl_launch_dependents();
   }
   int e, begin, rows;
-  if (!nth_share(g, blockIdx.y, e, begin, rows)) {  // the whole cluster leaves
+  if (!nth_share<THREADS, MAX_WIDTH>(g.offsets, g.E, g.R, blockIdx.y, e, begin, rows)) {  // the whole cluster leaves
     if (early) pdl_wait();
     return;
   }
