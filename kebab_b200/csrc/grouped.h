@@ -42,7 +42,7 @@ __device__ __forceinline__ void group_range(const int32_t* offsets, int e, int R
   count = max(hi - lo, 0);
 }
 
-int launch_grouped_simt(const GroupedProblem& p);    // 16 bits
+int launch_grouped_simt(const GroupedProblem& p);
 int launch_grouped_i8_any(const GroupedProblem& p);  // IN_I8, forward
 int launch_grouped_umma(const GroupedProblem& p);
 int launch_grouped_skinny(const GroupedProblem& p);

@@ -46,6 +46,16 @@ int parse_mode(const char* what, const char* opmode, bool* kn) {
   return fail(KEBAB_EINVAL, std::string(what) + ": opmode must be RC or RR, got " + m);
 }
 
+// 8-bit products that TMA does not take, on the CUDA cores: of short rows, where
+// the tensor cores' kernel is its set-up. us, CUDA cores against tensor cores: 1 x
+// 64 of K = 9 3.4 and 9.2, of 49 7.4 and 9.3, of 65 9.0 and 9.3; 65536 x 64 (1024
+// tiles) of 31 18.7 and 24.9, of 49 31.0 and 26.5; 300000 x 8 of 31 73.8 and 103, of
+// 49 127 and 107; 4093 x 4096 (4096 tiles) of 9 41.5 and 40.0, of 31 66 and 41.
+bool few_terms(const GroupedProblem& p, int sms) {
+  const int64_t tiles = (p.N + 63) / 64 * (p.offsets ? p.R / 64 + std::min(p.E, p.R) : (p.R + 63) / 64);
+  return (p.K <= 32 && (p.N <= 64 || tiles <= 8 * sms)) || (p.K <= 64 && tiles <= 2 * sms);
+}
+
 // The skinny kernel up to 128 rows, and where the persistent one would have
 // tiles for less than half of its CTA pairs. us, skinny against persistent:
 // int8 64 x 8192 x 8192 19.4 and 23.1, 128 rows 24.2 and 25.8, 256 rows (32
@@ -53,12 +63,13 @@ int parse_mode(const char* what, const char* opmode, bool* kn) {
 // tiles) 24.3 and 35.4; 16-bit 200 rows of 16 experts 2048 x 2048 25.1 and 27.2,
 // 100 rows of 64 experts 1024 x 1024 27.3 and 26.9.
 int run(const GroupedProblem& p) {
-  // dw without rows has no operand for a tensor map; it only writes zeros.
-  if (p.R == 0 || !grouped_tma_ok(p)) return p.in == IN_I8 ? launch_grouped_i8_any(p) : launch_grouped_simt(p);
-  if (p.dw) return launch_grouped_umma(p);
   DeviceInfo* dev = nullptr;
   const int rc = device_info(&dev);
   if (rc) return rc;
+  // dw without rows has no operand for a tensor map; it only writes zeros.
+  if (p.R == 0 || !grouped_tma_ok(p))
+    return p.in == IN_I8 && !few_terms(p, dev->sm_count) ? launch_grouped_i8_any(p) : launch_grouped_simt(p);
+  if (p.dw) return launch_grouped_umma(p);
   const int64_t tiles = (p.N + 255) / 256 * (p.offsets ? p.R / 256 + std::min(p.E, p.R) : (p.R + 255) / 256);
   return p.R <= 128 || tiles <= dev->sm_count / 4 ? launch_grouped_skinny(p) : launch_grouped_umma(p);
 }
