@@ -23,8 +23,10 @@
  * Plain C, device pointers, asynchronous on `stream`, status codes and
  * kebab_last_error() as in kebab.h. x and y are rows at a pitch; router [E, H]
  * (F32), w_in [E, 2 D, H] (gate rows, then up rows) and w_out [E, H, D] are
- * contiguous. An expert that no token chooses is not read, and what an expert
- * holds reaches the tokens that choose it only. A call is two launches; all of
+ * contiguous; weights whose rows do not start on 16 bytes are copied value by
+ * value, which for large ones takes longer than the separate operators. An
+ * expert that no token chooses is not read, and what an expert holds reaches the
+ * tokens that choose it only. A call is two launches; all of
  * the second's blocks (one a multiprocessor) are on the device at once, so it
  * waits for room among kernels of other streams. T = 0 is a no-op. `workspace`
  * (16-byte aligned) holds kebab_expert_layer_workspace(T, E, k, H, D) bytes.

@@ -32,6 +32,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 import kebab_b200 as kb
+from kebab_b200.layer import workspace
 
 
 class _Route(torch.autograd.Function):
@@ -196,7 +197,13 @@ class QuantizedMoE:
 class ServedMoE:
     """A trained MoE for serving, its experts in 16 bits, in 8-bit integers or in
     4-bit floating point. Up to kb.FEW_TOKENS tokens through experts of 16 or 8
-    bits take kb.expert_layer, more of them (and 4 bits) the separate operators."""
+    bits take kb.expert_layer; more of them, 4 bits, what that does not take and
+    large weights that it copies value by value take the separate operators."""
+
+    # Values of the chosen experts' second matrices, at most, whose rows do not start on 16 bytes. us, the layer against
+    # the separate operators: 8 bits, 2.1 million 53 and 58, 3.2 million 87 and 57, 131 million (D = 1000) 4654 and 165;
+    # 16 bits, 8.4 million 73 and 129, 12.6 million 429 and 318, 134 million 4210 and 2548.
+    _UNALIGNED = {16: 10_000_000, 8: 3_000_000}
 
     def __init__(self, layer, bits=8):
         self.k, self.renormalize, self.bits = layer.k, layer.renormalize, bits
@@ -206,9 +213,20 @@ class ServedMoE:
             raise kb.KebabError(kb.EINVAL, "ServedMoE: bits = %s is not 16, 8 or 4" % (bits,))
         self.w_in, self.w_out = make(layer.w_in.detach()), make(layer.w_out.detach())
         self.linear = {16: kb.gemm_grouped, 8: kb.linear_grouped_i8, 4: kb.linear_grouped_f4}[bits]
+        if bits != 4:
+            weights = self.w_in[0], self.w_out[0]
+            E, H, D = weights[1].shape
+            self.takes = all(t.is_contiguous() for t in weights) and workspace(1, E, self.k, H, D) > 0
+            aligned = all(t.data_ptr() % 16 == 0 and t.shape[2] * t.element_size() % 16 == 0 for t in weights)
+            self.unaligned = 0 if aligned else H * D  # values an expert
+
+    def _few(self, tokens):
+        """Whether kb.expert_layer takes a step of so many tokens."""
+        return (self.bits != 4 and tokens <= kb.FEW_TOKENS and self.takes and
+                min(tokens * self.k, len(self.router)) * self.unaligned <= self._UNALIGNED[self.bits])
 
     def __call__(self, x):
-        if self.bits != 4 and len(x) <= kb.FEW_TOKENS:
+        if self._few(len(x)):
             few = kb.expert_layer if self.bits == 16 else kb.expert_layer_i8
             return few(x, self.router, *self.w_in, *self.w_out, self.k, self.renormalize)
         r = kb.route(x.float() @ self.router.T, self.k, self.renormalize)
