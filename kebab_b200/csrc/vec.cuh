@@ -87,14 +87,6 @@ struct Run {
       raw[0].x = __float_as_uint(to_float(*p));
     }
   }
-  __device__ __forceinline__ void store(T* p) const {
-    if constexpr (W == 8) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
-    } else {
-      *p = from_float<T>(__uint_as_float(raw[0].x));
-    }
-  }
   __device__ __forceinline__ void values(float (&v)[W]) const {
     if constexpr (W == 8 && sizeof(T) == 2) {
       unpack((const T*)nullptr, raw[0], v);
