@@ -113,7 +113,9 @@ class _RmsNorm(torch.autograd.Function):
         if dy is None:
             dx, dweight = ds, None
         else:
-            dx, dweight = kb.rms_norm_backward(_rows(dy), s, weight, ctx.eps, dresidual=None if ds is None else _rows(ds))
+            x, w, residual = ctx.needs_input_grad[:3]
+            dx, dweight = kb.rms_norm_backward(_rows(dy), s, weight, ctx.eps, dresidual=None if ds is None else _rows(ds),
+                                               need=(x or residual, w))
         return dx, dweight, dx if ctx.added else None, None
 
 

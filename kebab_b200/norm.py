@@ -91,10 +91,11 @@ def rms_norm_i8(x, weight, eps=1e-6, residual=None, keep=False, stream=None):
     return Normed8(codes, scale, s, y)
 
 
-def rms_norm_backward(dy, s, weight, eps=1e-6, dresidual=None, stream=None):
+def rms_norm_backward(dy, s, weight, eps=1e-6, dresidual=None, stream=None, need=(True, True)):
     """Gradients of rms_norm from that of y, and `dresidual`, that of s where it
     is used past the norm -> (dx, dweight): dx [T, H] is the gradient of x and
-    of the residual; dweight [H] has weight's type."""
+    of the residual; dweight [H] has weight's type. `need`: whether to compute
+    each of the two, None in place of one that is not."""
     what = "rms_norm_backward"
     dev = _check(what, s, weight, None, "s")
     if dy is None:
@@ -103,12 +104,12 @@ def rms_norm_backward(dy, s, weight, eps=1e-6, dresidual=None, stream=None):
     _like(what, "dresidual", dresidual, s, dev)
     if elsewhere(dev, stream):
         with on(dev, stream):
-            return rms_norm_backward(dy, s, weight, eps, dresidual)
+            return rms_norm_backward(dy, s, weight, eps, dresidual, need=need)
     T, H = s.shape
-    dx, dweight = _rows_like(s), torch.empty_like(weight)
+    dx, dweight = _rows_like(s) if need[0] else None, torch.empty_like(weight) if need[1] else None
     size = (T * 8 + 15) // 16 * 16 + min((T + 7) // 8 * 8, 1024) * H * 4  # kebab_rms_norm_backward_workspace
     ws = s.new_empty((size,), dtype=torch.uint8)
     call("kebab_rms_norm_backward", dev, CODES[s.dtype], CODES[weight.dtype], dy.data_ptr(), pitch(dy), s.data_ptr(),
-         pitch(s), weight.data_ptr(), eps, *_row_pitch(dresidual), dx.data_ptr(), H, dweight.data_ptr(), ws.data_ptr(),
-         size, T, H)
+         pitch(s), weight.data_ptr(), eps, *_row_pitch(dresidual), dx.data_ptr() if need[0] else None, H,
+         dweight.data_ptr() if need[1] else None, ws.data_ptr(), size, T, H)
     return dx, dweight
