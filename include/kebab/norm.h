@@ -32,7 +32,8 @@ int kebab_rms_norm(kebab_dtype dtype, kebab_dtype weight_dtype, const void* x, i
                    int64_t rows, int64_t cols, kebab_stream_t stream);
 
 /* The same with y quantised by row as kebab_quantize_i8 does (kebab/int8.h),
- * from the FP32 values: codes q and scales, operands of kebab_gemm_i8. y, in
+ * from the FP32 values: codes q and scales, operands of kebab_gemm_i8 (zeros, with
+ * scale 0, for a row whose largest |s * weight| is under 1e-30). y, in
  * `dtype`, is written too unless it is NULL. */
 int kebab_rms_norm_i8(kebab_dtype dtype, kebab_dtype weight_dtype, const void* x, int64_t ldx, const void* residual,
                       int64_t ldr, const void* weight, float eps, void* s, int64_t lds, void* y, int64_t ldy,
