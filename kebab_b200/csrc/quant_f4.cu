@@ -181,12 +181,17 @@ constexpr int64_t kMaxDim = int64_t(1) << 30;
 // Spans of 256 values that a warp takes of a row: as many as leave every SM its
 // 64 warps. (8192 x 8192 of 8, 4, 1: 37, 39, 74 us; 4096 x 4096 18, 16, 22; 16
 // rows of 8192 10, 8, 6, flushed and with the launch.)
-int spans_of(int64_t rows, int64_t spans) { return rows * spans >= 148 * 64 * 8 ? 8 : rows * spans >= 148 * 64 * 4 ? 4 : 1; }
+int spans_of(int64_t rows, int64_t spans, int sms) {
+  const int64_t warps = (int64_t)sms * 64;
+  return rows * spans >= warps * 8 ? 8 : rows * spans >= warps * 4 ? 4 : 1;
+}
 
 template <typename T, bool TOKENS>
 int quantize(QuantArgs g, int64_t E, cudaStream_t stream) {
+  DeviceInfo* dev = nullptr;
+  if (const int rc = device_info(&dev)) return rc;
   const int64_t rows = TOKENS ? g.rows : (g.rows + 127) / 128 * 128, spans = (g.tiles + 1) / 2;
-  g.spans = std::max<int>(spans_of(rows * E, spans), (int)((spans + 65534) / 65535));
+  g.spans = std::max<int>(spans_of(rows * E, spans, dev->sm_count), (int)((spans + 65534) / 65535));
   const bool vec = (reinterpret_cast<uintptr_t>(g.X) & 15u) == 0 && (g.ldx * sizeof(T)) % 16 == 0 &&
                    (E == 1 || (g.x_stride * sizeof(T)) % 16 == 0);
   PdlLaunch l(dim3((unsigned)((rows + WARPS - 1) / WARPS), (unsigned)((spans + g.spans - 1) / g.spans), (unsigned)E),
@@ -205,9 +210,11 @@ int quantize_any(int dtype, const QuantArgs& g, int64_t E, cudaStream_t s) {
 
 template <typename T>
 int dequantize(DequantArgs g, int64_t E, cudaStream_t stream) {
+  DeviceInfo* dev = nullptr;
+  if (const int rc = device_info(&dev)) return rc;
   const bool vec = (reinterpret_cast<uintptr_t>(g.W) & 15u) == 0 && g.K % 8 == 0;
   const int64_t spans = (g.K + (vec ? 0 : 7) + 255) / 256;  // a granule may begin before the row
-  g.spans = std::max<int>(spans_of(g.rows * E, spans), (int)((spans + 65534) / 65535));
+  g.spans = std::max<int>(spans_of(g.rows * E, spans, dev->sm_count), (int)((spans + 65534) / 65535));
   PdlLaunch l(dim3((unsigned)((g.rows + WARPS - 1) / WARPS), (unsigned)((spans + g.spans - 1) / g.spans), (unsigned)E),
               dim3(THREADS), 0, stream);
   const cudaError_t e =
