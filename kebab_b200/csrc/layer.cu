@@ -812,7 +812,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // The largest values are known: this CTA's share in the operands' form.
       bool here = true;
       if (et == 0) here = wait_for_all(g.arrived);
-      if (!here) ok = false;
+      ok = all_ok(here && ok);  // of the whole warp, which goes on together
       __threadfence();
       meet();
       for (int i = et; i < choices; i += 128) {
