@@ -721,9 +721,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (et == 0) asm volatile("fence.acq_rel.gpu;\n\tred.relaxed.gpu.global.add.u32 [%0], 1;" ::"l"(count) : "memory");
     };
     uint32_t run = 0;
-    // The sums of a pass, column by column, its runs of K-blocks one after the other.
+    // The sums of a pass for the first `n` columns, its runs of K-blocks one after the other.
     float sum[MAX_TOKENS];
-    auto take = [&](auto product, int blocks) {
+    auto take = [&](auto product, int blocks, int n) {
       constexpr int OPERANDS = decltype(product)::OPERANDS;
       const int runs = I8 ? 1 : (blocks + CHUNK - 1) / CHUNK;
 #pragma unroll 1
@@ -740,6 +740,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane == 0) mbar_arrive(&acc_empty[set]);
 #pragma unroll
         for (int c = 0; c < MAX_TOKENS; ++c) {
+          if (c >= n) break;
           float o = number(v[c]);
           if constexpr (OPERANDS == 2) o += number(box == 16 ? v[16 + c] : v[8 + c % 8]);
           if constexpr (OPERANDS == 3)
@@ -763,7 +764,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         const uint32_t who = s_who[p.a];
         int place = s_base[p.a];
-        take(Up(), up_blocks);
+        take(Up(), up_blocks, g.T);
         // The up rows are the threads from r8 on. Through shared memory, and then
         // token by token in a loop: unrolled, one token's values took 4 us, for
         // the instructions that are fetched on the way.
@@ -867,7 +868,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool mine = et < p.rows;
       float scale = 1.f;
       if constexpr (I8) scale = mine ? g.out_scale[(int64_t)s_active[p.a] * g.H + r] : 0.f;
-      take(Down(), down_blocks);
+      take(Down(), down_blocks, n);
 #pragma unroll
       for (int c = 0; c < MAX_TOKENS; ++c) {
         if (c >= n) break;
