@@ -43,8 +43,9 @@ int kebab_rms_norm_i8(kebab_dtype dtype, kebab_dtype weight_dtype, const void* x
  *   dx[t, h] = ds[t, h] + rstd[t] (g[t, h] - s[t, h] rstd[t]^2 mean_h(g s)[t])
  *   dweight[h] = sum_t dy[t, h] s[t, h] rstd[t]
  * dx is the gradient of x and of the residual; ds (NULL: none) is what reaches
- * s past the norm. dx and dweight may be NULL. The sums over t have a fixed
- * order: the same inputs give the same bits on devices with as many SMs.
+ * s past the norm. dx and dweight may be NULL. The sums have a fixed order: the
+ * same call gives the same bits on devices with as many SMs (another boundary of
+ * the rows, or dx left out, may choose another order).
  * `workspace` (16-byte aligned) holds
  * kebab_rms_norm_backward_workspace(rows, cols) bytes. rows = 0 gives a
  * dweight of zeros. */

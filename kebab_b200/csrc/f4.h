@@ -27,7 +27,8 @@ constexpr int64_t F4_MAX_ROWS = int64_t(1) << 27;  // of tokens
 // Rows that a product quantises itself, at most: every CTA does it for its k
 // range, and saves the launch before (8192 x 8192, back to back: 1 row 7.4 us
 // against 9.0, 4 rows 7.6 against 8.9, 8 rows 9.9 against 8.5; 2048 x 2048 3.9
-// against 5.6, 4.0 against 5.7, 4.8 against 5.7).
+// against 5.6, 4.0 against 5.7, 4.8 against 5.7; weights from memory: 6 rows 12.1
+// and 14.1 a call, 7 rows, in two launches, 11.6 and 16.9).
 constexpr int F4_FUSED_ROWS = 6;
 constexpr int F4_SLACK = 160;  // entries of token scales past the last row
 

@@ -8,9 +8,9 @@
 // every other CTA the 128 / S of its rows that that one finishes (st.async,
 // counted on the receiver's barrier), and adds up its own rows over the S
 // partials in rank order. No workspace, no atomics, and the same bits every
-// time. With the quantisation, 1 row of 8192 x 8192 takes 9.1 us and 61 rows
-// 14.4 (3.9 and 2.6 TB/s): latency of the quantisation, of the first copies and
-// of the exchange. Several accumulators in turn gave nothing.
+// time. With the quantisation, 1 row of 8192 x 8192 takes 9.6 us and 61 rows
+// 14.4 (3.7 and 2.6 TB/s; with codes at hand 61 rows 13.0): latency of the first
+// copies and of the exchange. Several accumulators in turn gave nothing.
 //
 // A K-block is 256 values: 128 bytes of codes a row, and two runs of 128 whose
 // scales (512 bytes for 128 rows, as they are stored) the issuer copies into

@@ -17,10 +17,10 @@
 // not used). The tokens, or the hidden values of the tokens that chose the
 // expert, are the columns, 8 or 16. A warp of its own copies the columns: at the grid
 // barrier only it waits, while the second matrices' rows arrive in the ring.
-// 1 token, 8 experts of H 2048 and D 1024 in BF16: 30 us (3.3 TB/s; 8 of them are
+// 1 token, 8 experts of H 2048 and D 1024 in BF16: 31 us (3.3 TB/s; 8 of them are
 // the logits and the second kernel's start, which cooperative launches do not
-// overlap); 13 tokens, 6 of 64 experts each, D 1272, F16: 162 us (4.5 TB/s); 5
-// tokens, 2 of 8 experts each, H 4096, D 8192, BF16: 222 us (5.5 TB/s).
+// overlap); 13 tokens, 6 of 64 experts each, D 1272, F16: 165 us (4.4 TB/s); 5
+// tokens, 2 of 8 experts each, H 4096, D 8192, BF16: 225 us (5.5 TB/s).
 //
 // A token takes the products of its own experts only, from columns of its own:
 // what other experts or tokens hold (infinities, NaN) does not reach it.
