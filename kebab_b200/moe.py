@@ -5,7 +5,7 @@ training and in serving.
     y, routing = layer(x)
     served = layer.quantize()                       # 8-bit integer experts, forward only
     y = served(x)
-    served = layer.serve(bits)                      # 16, 8 or 4 bits; a few tokens take two launches
+    served = layer.serve(bits)                      # 16, 8 or 4 bits; in 16 and 8 a few tokens take two launches
 
     block = Block(width, hidden, experts, k)        # the norm before the layer, on a residual stream
     y, stream, routing = block(x, stream)           # stream: the sum x + stream that was normed
