@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(SparseCfg<T, CG, STAGES, MT, BN>::THREADS, 1)
       tile_coords(tile, args.tiles_m, args.tiles_n, args.group_m, mb, nb);
       const int m_rows = mb * BM_T + t * BM_MMA + (int)rank * 128 + q * 32;
       const int n0 = nb * BN;
-      if (!mbar_wait(&tmem_full[acc], acc_phase, ctx, SITE_TMEM_FULL)) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[acc], acc_phase, ctx, SITE_TMEM_FULL))) break;  // the warp together
       const int tslot = (tile - cluster_id) / num_clusters;
       if (ew == 0 && lane == 0 && tslot < 8) SP_TRACE(tslot, 4);
       tc_fence_after();

@@ -549,7 +549,9 @@ __global__ void __launch_bounds__(UmmaEpi<BN>::THREADS, 1)
       tile_coords(u.tile, args.tiles_m, args.tiles_n, args.group_m, mb, nb);
       const int m_rows = mb * BM_T + (int)rank * 128 + q * 32;
       const int n0 = nb * BN;
-      if (!mbar_wait_backoff(&tmem_full[acc], acc_phase, ctx, SITE_TMEM_FULL, args.epi_backoff_ns)) break;
+      // The warp goes on, or not, together: what follows needs all of its lanes.
+      if (!__all_sync(0xffffffffu, mbar_wait_backoff(&tmem_full[acc], acc_phase, ctx, SITE_TMEM_FULL, args.epi_backoff_ns)))
+        break;
       if (q == 0 && lane == 0) SK_TRACE(uidx & 7, 2);
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
