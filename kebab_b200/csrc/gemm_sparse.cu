@@ -219,6 +219,7 @@ __global__ void __launch_bounds__(SparseCfg<T, CG, STAGES, MT, BN>::THREADS, 1)
           }
         }
       }
+      if (!ok) settle();  // copies in flight land before the CTA exits
     }
   } else if (warp == 1) {
     if (leader && lane == 0) {
@@ -288,8 +289,7 @@ __global__ void __launch_bounds__(SparseCfg<T, CG, STAGES, MT, BN>::THREADS, 1)
       if (!ok && any) {
         if constexpr (CG == 1) umma_commit_cg1(drain);
         else umma_commit_cg2_mc(drain, 0x1);
-        WaitCtx d{ctx.status, 50000000ull};
-        mbar_wait(drain, 0, d, SITE_DRAIN);
+        mbar_drain(drain, 0, DRAIN_NS);
       }
     }
   } else {

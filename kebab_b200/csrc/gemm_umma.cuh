@@ -451,9 +451,8 @@ __global__ void __launch_bounds__(UmmaEpi<BN>::THREADS, 1)
       }
       if (!ok && (CG == 1 || leader)) {
         // Abort: let our own copies still in flight land before the CTA exits.
-        WaitCtx drain_ctx{ctx.status, 50000000ull};
         for (int s = 0; s < STAGES; ++s)
-          if (issued[s]) mbar_wait(&full[s], issued_parity[s], drain_ctx, SITE_DRAIN);
+          if (issued[s]) mbar_drain(&full[s], issued_parity[s], DRAIN_NS);
       }
     }
   } else if (warp == 1) {
@@ -524,8 +523,7 @@ __global__ void __launch_bounds__(UmmaEpi<BN>::THREADS, 1)
         // Abort: wait for the MMAs already issued before TMEM is freed.
         if constexpr (CG == 1) umma_commit_cg1(drain);
         else umma_commit_cg2_mc(drain, 0x1);
-        WaitCtx drain_ctx{ctx.status, 50000000ull};
-        mbar_wait(drain, 0, drain_ctx, SITE_DRAIN);
+        mbar_drain(drain, 0, DRAIN_NS);
       }
     }
   } else {

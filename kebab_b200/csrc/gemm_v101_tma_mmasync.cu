@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(256, 1)
       for (int r = 0; r < 4; ++r) acc[i][j][r] = 0.f;
 
   bool ok = true;
-  for (int kb = 0; kb < nkb; ++kb) {
+  int kb = 0;
+  for (; kb < nkb; ++kb) {
     // Stage (kb+1)%2 was released by the __syncthreads at the end of kb-1.
     if (threadIdx.x == 0 && kb + 1 < nkb) issue(kb + 1);
     const int s = kb % STAGES;
@@ -127,10 +128,9 @@ __global__ void __launch_bounds__(256, 1)
     __syncthreads();
   }
   if (!ok) {
-    // Let the copy that may still be in flight land before the CTA exits.
+    // Let the copies that may still be in flight (this K-block's, the next one's) land before the CTA exits.
     if (threadIdx.x == 0) {
-      WaitCtx d{ctx.status, 50000000ull};
-      for (int kb = 0; kb < nkb && kb < STAGES; ++kb) mbar_wait(&full[kb], 0, d, SITE_DRAIN);
+      for (int i = kb; i < nkb && i < kb + 2; ++i) mbar_drain(&full[i % STAGES], (uint32_t)((i / STAGES) & 1), DRAIN_NS);
     }
     return;
   }

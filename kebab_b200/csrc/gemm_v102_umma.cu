@@ -61,8 +61,7 @@ __global__ void __launch_bounds__(128, 1)
       tma_load_2d(sA, &tmA, tma_bar, kb * BK, m0);
       tma_load_2d(sB, &tmB, tma_bar, kb * BK, n0);
       if (!mbar_wait(tma_bar, phase, ctx, SITE_TMA_DONE)) {
-        WaitCtx d{ctx.status, 50000000ull};
-        mbar_wait(tma_bar, phase, d, SITE_DRAIN);
+        mbar_drain(tma_bar, phase, DRAIN_NS);
         *ok_flag = 0;
         break;
       }
@@ -73,8 +72,7 @@ __global__ void __launch_bounds__(128, 1)
                      (kb | k) != 0 ? 1u : 0u);
       umma_commit_cg1(mma_bar);
       if (!mbar_wait(mma_bar, phase, ctx, SITE_MMA_DONE)) {
-        WaitCtx d{ctx.status, 50000000ull};
-        mbar_wait(mma_bar, phase, d, SITE_DRAIN);
+        mbar_drain(mma_bar, phase, DRAIN_NS);
         *ok_flag = 0;
         break;
       }

@@ -28,7 +28,6 @@ enum WaitSite : uint32_t {
   SITE_MMA_DONE = 5,    // single-stage kernels waiting for their MMA
   SITE_TMA_DONE = 6,    // single-stage kernels waiting for their TMA
   SITE_PROBE = 7,       // the deliberate-timeout probe kernel
-  SITE_DRAIN = 8,       // teardown drain after an abort
   SITE_PARTIAL = 9,     // stream-K owner waiting for a contributor's partial
   SITE_BCHUNK = 10,     // gated GEMM producer waiting for a chunk of B to arrive
   SITE_TILE = 11,       // grouped product: a tile's description, or a free place for one
@@ -176,6 +175,7 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
 // After a wait that ran out, before the CTA gives up the memory that is still
 // in use: a wait for the phase that does not stop for a recorded error, bounded
 // by `limit_ns`; and time for copies and MMAs in flight, which take microseconds.
+constexpr uint64_t DRAIN_NS = 50000000ull;  // for copies and MMAs of one CTA or pair
 __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
   const uint64_t t0 = globaltimer();
   while (!mbar_try_wait(smem_u32(bar), parity) && globaltimer() - t0 < limit_ns) {
